@@ -275,6 +275,100 @@ int q8mi_get_row_from_argmax(const uint8_t *weight, const q8mi_argmax_pair *argm
 int q8mi_get_rows(const uint8_t *weight, const uint64_t *row_ids, uint32_t batch, uint64_t rows,
                   uint64_t cols, void *out, int out_is_bf16, void *stream);
 
+/* ---- paged key / value cache --------------------------------------------- */
+/* One layer's cache: two pools of `pages` pages of page_size token rows.  The row of token t of page p
+ * and head h begins p*stride_page + h*stride_head + t*stride_token ELEMENTS behind k (or v) and holds
+ * head_dim elements.  The struct is host memory, read during the call only.
+ *   dtype       Q8MI_KV_BF16, Q8MI_KV_F16 or Q8MI_KV_E4M3 (OCP e4m3: an element stands for itself times
+ *               k_scale / v_scale; the two scales are used by this type alone)
+ *   head_dim    64, 128 or 256;  page_size 1..65536, any number
+ * k, v and every stride in bytes must be multiples of 16, stride_token >= head_dim, the scales finite
+ * and above zero: anything else is Q8MI_REJECTED by both operators below. */
+#define Q8MI_KV_BF16 0
+#define Q8MI_KV_F16 1
+#define Q8MI_KV_E4M3 2
+typedef struct q8mi_kv_cache {
+    void *k, *v;
+    int32_t dtype;
+    uint32_t pages, page_size, kv_heads, head_dim;
+    uint64_t stride_page, stride_head, stride_token;
+    float k_scale, v_scale;
+} q8mi_kv_cache;
+
+/* What lies between the Q/K/V projections and the attention, in one launch: RMS norm of every query and key
+ * head, position rotation of the normalised heads, and the append of keys and values to the cache.
+ *   norm      y[i] = x[i] / sqrt(mean_i x[i]^2 + eps) * weight[i] over a head's head_dim elements;
+ *             q_norm_weight / k_norm_weight (head_dim floats) may be NULL: those heads are not normalised
+ *   rotation  of the first rotary_dim elements (a multiple of 8, at most head_dim; 0 = none):
+ *             (a, b) -> (a cos t - b sin t, b cos t + a sin t), t = positions[token] * freqs[i] radians,
+ *             for pair i = elements (i, i + rotary_dim/2), or (2i, 2i + 1) when interleaved != 0.  freqs:
+ *             rotary_dim/2 doubles; the angle is taken in 64 bits, so that far positions keep theirs
+ *   append    key and value rows of token j go to slot slots[j] = page * page_size + row of the cache,
+ *             rounded to nearest even (e4m3: divided by the scale and clamped to +-448).  A slot below zero
+ *             or beyond the pools is skipped (padding); its query rows are written all the same.  Two tokens
+ *             of one call must not name the same slot.
+ * Activations (q, k, v, q_out) are fp32, or bf16 when is_bf16 != 0.  Head h of token j of q begins at
+ * j*stride_q_row + h*stride_q_head (queries may lie between other things, e.g. their gates); heads of k, v and
+ * q_out follow one another, rows stride_k_row, stride_v_row and stride_q_out_row elements apart.  q_out may be
+ * q when the strides agree (stride_q_head == head_dim), and must not overlap it otherwise.  All array
+ * arguments are device memory; any alignment, 16-byte aligned rows take vector accesses. */
+int q8mi_qk_norm_rope_append(const void *q, const void *k, const void *v, void *q_out, int is_bf16, uint32_t tokens,
+                             uint32_t q_heads, uint32_t stride_q_row, uint32_t stride_q_head, uint32_t stride_k_row,
+                             uint32_t stride_v_row, uint32_t stride_q_out_row, const float *q_norm_weight,
+                             const float *k_norm_weight, float eps, const double *freqs, uint32_t rotary_dim,
+                             int interleaved, const int32_t *positions, const int64_t *slots,
+                             const q8mi_kv_cache *cache, void *stream);
+
+/* Attention of each sequence's newest rows over its cached keys and values (decode: one row a sequence;
+ * verification: the accepted token and its drafts), after their keys have been appended.
+ * Sequence s has kv_lens[s] cached tokens (the new rows' own among them); token t lies in row t % page_size
+ * of page page_table[s*stride_page_table + t / page_size].  Its new rows are rows q_starts[s] ..
+ * q_starts[s+1]-1 of q, or, when q_starts is NULL, rows s*max_q_len .. s*max_q_len + max_q_len-1.  Row i of
+ * n sees the tokens up to kv_lens[s] - n + i:
+ *   out = sum_t p_t v_t,  p = softmax_t(scale * q . k_t)
+ * for every query head h with the keys and values of head h / (q_heads / kv_heads).  What a row does not see
+ * has no influence on it, whatever it holds; a row that sees nothing is zero; rows of q outside every
+ * sequence leave out as it was.
+ * q and out: rows stride_q_row / stride_out_row elements apart, heads dense; fp32, or bf16 per *_is_bf16.
+ * kv_lens, q_starts and page_table are device memory and may change between replays of a captured call;
+ * the host gives their bounds: n_seqs, q_rows (rows of q and out), max_q_len (1..16) and max_kv_len (at most
+ * stride_page_table * page_size).  Tokens from max_kv_len on are not read, rows of a sequence from
+ * max_q_len on and rows from q_rows on not computed, and a page id outside the pool hides its tokens.
+ * scratch: q8mi_paged_attention_scratch_bytes() device bytes, 16-byte aligned; calls that may overlap need
+ * one each.  Nothing in it needs clearing.  Q8MI_REJECTED: q_heads not a multiple of kv_heads, the bounds
+ * above, q or out or their strides in bytes not multiples of 16, a scale that is not finite. */
+size_t q8mi_paged_attention_scratch_bytes(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads,
+                                          uint32_t head_dim, uint32_t max_kv_len);
+int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_rows, uint32_t stride_q_row,
+                         const q8mi_kv_cache *cache, const int32_t *page_table, uint32_t stride_page_table,
+                         const int32_t *kv_lens, const int32_t *q_starts, uint32_t n_seqs, uint32_t max_q_len,
+                         uint32_t q_heads, uint32_t max_kv_len, float scale, void *out, int out_is_bf16,
+                         uint32_t stride_out_row, void *scratch, void *stream);
+
+/* ---- sampling ------------------------------------------------------------- */
+/* One token per row of logits ([batch][stride], `vocab` of them used) by temperature, top-k, top-p and min-p,
+ * from a given uniform number per row.  With the ranks of a row by logit, larger first, equal ones by lower
+ * index first, and p_i = exp((logit_i - max) / temperature):
+ *   top_k   keeps the first top_k ranks (<= 0: all);
+ *   top_p   keeps of those a rank when the p of the ranks before it sum to less than top_p times the p of all
+ *           that top_k kept (>= 1: all; the first rank always stays);
+ *   min_p   keeps of those the ranks with p_i >= min_p (<= 0: all, above 1 counts as 1);
+ *   token   the lowest index at which the sum of the kept p, in the order of the indices, exceeds uniform
+ *           times their whole sum.
+ * A temperature that is not above zero takes rank 0 (the row's argmax).  The five parameter arrays are device
+ * memory, one element a row; temperature (1), top_k, top_p and min_p (off) may be NULL.  Each p is rounded to
+ * a multiple of 2^-42 and all sums are integers, so that their order never changes a token; a logit more than
+ * about 30 temperatures below the maximum counts as 0 and is never drawn.  NaN and -inf logits are never
+ * drawn either; +inf logits share the whole mass.  uniform is clamped to [0, 1), NaN counts as 0.
+ *   out[j] = {the token's logit, the token}: what q8mi_get_row_from_argmax reads; {-inf, -1} when every
+ *            logit of the row is NaN or -inf.
+ * vocab: 1 .. 2^20.  scratch: q8mi_sample_scratch_bytes() device bytes, 16-byte aligned; calls that may overlap
+ * need one each, nothing in it needs clearing. */
+size_t q8mi_sample_scratch_bytes(uint32_t batch, uint32_t vocab);
+int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, uint32_t stride, const float *temperature,
+                const int32_t *top_k, const float *top_p, const float *min_p, const float *uniform,
+                q8mi_argmax_pair *out, void *scratch, void *stream);
+
 /* ---- argmax -------------------------------------------------------------- */
 /* replaces argmax_kernel, src/kernels_cuda.cu:1693-1734 (launched at :20759):
  * out2[0] = index (-1 if no element is above -inf), out2[1] = bits of the max.

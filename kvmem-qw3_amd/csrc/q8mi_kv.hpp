@@ -1,0 +1,56 @@
+// The paged key / value cache as the kernels see it: element types, row addresses, host checks.
+#pragma once
+
+#include <math.h>
+
+#include "q8mi_device.hpp"
+#include "q8mi_internal.hpp"
+
+namespace q8mi {
+
+constexpr uint32_t kMaxPageSize = 65536;
+
+__host__ __device__ inline uint32_t kv_element_bytes(int dtype) { return dtype == Q8MI_KV_E4M3 ? 1 : 2; }
+
+// Q8MI_OK when the descriptor is one the kernels serve.
+inline int check_kv_cache(const char *what, const q8mi_kv_cache *c) {
+    if (c == nullptr || c->k == nullptr || c->v == nullptr) return fail(Q8MI_REJECTED, "%s: null cache", what);
+    if (c->dtype != Q8MI_KV_BF16 && c->dtype != Q8MI_KV_F16 && c->dtype != Q8MI_KV_E4M3)
+        return fail(Q8MI_REJECTED, "%s: cache type %d", what, c->dtype);
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+        return fail(Q8MI_REJECTED, "%s: head_dim %u is not 64, 128 or 256", what, c->head_dim);
+    if (c->pages == 0 || c->pages > 0x7fffffffu || c->page_size == 0 || c->page_size > kMaxPageSize || c->kv_heads == 0)
+        return fail(Q8MI_REJECTED, "%s: cache of %u pages of %u tokens, %u heads", what, c->pages, c->page_size, c->kv_heads);
+    const uint64_t es = kv_element_bytes(c->dtype);
+    if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16 != 0 ||
+        (c->stride_page * es) % 16 != 0 || (c->stride_head * es) % 16 != 0 || (c->stride_token * es) % 16 != 0 ||
+        c->stride_token < c->head_dim)
+        return fail(Q8MI_REJECTED, "%s: cache rows must begin on 16-byte boundaries, stride_token >= head_dim", what);
+    if (c->dtype == Q8MI_KV_E4M3 &&
+        !(isfinite(c->k_scale) && isfinite(c->v_scale) && c->k_scale > 0.0f && c->v_scale > 0.0f))
+        return fail(Q8MI_REJECTED, "%s: e4m3 scales must be finite and above zero", what);
+    return Q8MI_OK;
+}
+
+// Four floats as four elements of a cache row (nearest even; e4m3: the quotient by the scale, clamped, NaN kept).
+__device__ __forceinline__ void store_kv4(void *row, uint32_t element, int dtype, float scale, const float (&v)[4]) {
+    if (dtype == Q8MI_KV_E4M3) {
+        float t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float q = v[i] / scale;
+            t[i] = q != q ? q : fminf(fmaxf(q, -448.0f), 448.0f);
+        }
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(t[0], t[1], 0, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], w, true);
+        *reinterpret_cast<int *>(static_cast<uint8_t *>(row) + element) = w;
+        return;
+    }
+    uint16_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = dtype == Q8MI_KV_BF16 ? float_to_bf16_bits(v[i]) : float_to_half_bits(v[i]);
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(row) + element) =
+        make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
+}
+
+}  // namespace q8mi

@@ -1,0 +1,243 @@
+// Per-head RMS norm of queries and keys, position rotation, and the append of keys and values to a paged cache: the
+// step between the Q/K/V projections and the attention, in one launch.
+//
+//   y = x / sqrt(mean(x^2) + eps) * w            over the head_dim elements of a head
+//   (a, b) -> (a cos t - b sin t, b cos t + a sin t),   t = position * freq
+//
+// A head is held by head_dim / 4 neighbouring lanes, four elements each: the sum of squares is a butterfly among them,
+// the rotation's partner element comes from another lane (or lies in the same one for neighbouring pairs).  The angle is
+// taken in revolutions in 64 bits and only its fraction, at most half a turn, goes to the 32-bit sine and cosine: an
+// fp32 product of position 200 000 and a frequency is off by up to 0.008 radians, the fraction by 2e-7.
+#include "q8mi_kv.hpp"
+#include "q8mi_quantize_core.hpp"
+
+namespace q8mi {
+namespace {
+
+constexpr uint32_t kAppendThreads = 256;
+constexpr uint32_t kAppendWaves = kAppendThreads / kWave;
+
+struct AppendParams {
+    const void *q, *k, *v;
+    void *q_out;
+    const float *q_weight, *k_weight;
+    const double *freqs;
+    const int32_t *positions;
+    const int64_t *slots;
+    q8mi_kv_cache cache;
+    uint32_t tokens, q_heads, kv_heads;
+    uint32_t stride_q_row, stride_q_head, stride_k_row, stride_v_row, stride_q_out_row;
+    uint32_t rotary_dim;
+    uint32_t heads_per_wave, waves_per_token;
+    int interleaved;
+    float eps;
+};
+
+template <bool BF16, bool VEC>
+__device__ __forceinline__ void load_act4(const void *base, uint64_t at, float (&v)[4]) {
+    if constexpr (BF16) {
+        const uint16_t *p = static_cast<const uint16_t *>(base) + at;
+        if (VEC) {
+            const uint2 t = *reinterpret_cast<const uint2 *>(p);
+            v[0] = bf16_bits_to_float(static_cast<uint16_t>(t.x & 0xffffu));
+            v[1] = bf16_bits_to_float(static_cast<uint16_t>(t.x >> 16));
+            v[2] = bf16_bits_to_float(static_cast<uint16_t>(t.y & 0xffffu));
+            v[3] = bf16_bits_to_float(static_cast<uint16_t>(t.y >> 16));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = bf16_bits_to_float(p[i]);
+        }
+    } else {
+        const Float4 t = load4<VEC>(static_cast<const float *>(base) + at);
+        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    }
+}
+
+template <bool BF16, bool VEC>
+__device__ __forceinline__ void store_act4(void *base, uint64_t at, const float (&v)[4]) {
+    if constexpr (BF16) {
+        uint16_t *p = static_cast<uint16_t *>(base) + at;
+        uint16_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = float_to_bf16_bits(v[i]);
+        if (VEC) {
+            *reinterpret_cast<uint2 *>(p) =
+                make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = h[i];
+        }
+    } else {
+        float *p = static_cast<float *>(base) + at;
+        if (VEC) {
+            *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = v[i];
+        }
+    }
+}
+
+// Sum over the LANES neighbouring lanes that hold a head.
+template <int LANES>
+__device__ __forceinline__ float head_sum(float v) {
+    v += lane_xor<1>(v);
+    v += lane_xor<2>(v);
+    v += lane_xor<4>(v);
+    v += lane_xor<8>(v);
+    if constexpr (LANES >= 32) v += lane_xor<16>(v);
+    if constexpr (LANES >= 64) v += lane_xor<32>(v);
+    return v;
+}
+
+// One wave: heads_per_wave heads of one token, 64 / (D / 4) of them at a time.  Heads are numbered queries, keys, values.
+template <bool BF16, uint32_t D, bool VEC>
+__global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendParams p) {
+    constexpr uint32_t kLanes = D / 4, kAtOnce = kWave / kLanes;
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t wave = blockIdx.x * kAppendWaves + threadIdx.x / kWave;
+    const uint32_t token = wave / p.waves_per_token;
+    if (token >= p.tokens) return;
+    const uint32_t first = (wave % p.waves_per_token) * p.heads_per_wave;
+    const uint32_t e0 = (lane % kLanes) * 4;
+    const uint32_t half = p.rotary_dim / 2;
+    const bool turns = e0 < p.rotary_dim;
+
+    float c[4] = {1.0f, 1.0f, 1.0f, 1.0f}, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (turns) {
+        const double position = p.positions[token] * 0.15915494309189533577;   // 1 / (2 pi): angles in revolutions
+        const uint32_t pair = p.interleaved ? e0 / 2 : (e0 < half ? e0 : e0 - half);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (p.interleaved && i >= 2) break;
+            const double turn = position * p.freqs[pair + i];
+            sincospif(2.0f * static_cast<float>(turn - rint(turn)), &s[i], &c[i]);
+        }
+    }
+    const int64_t slot = p.slots[token];
+    const bool held = slot >= 0 && static_cast<uint64_t>(slot) < static_cast<uint64_t>(p.cache.pages) * p.cache.page_size;
+    const uint64_t page = held ? static_cast<uint64_t>(slot) / p.cache.page_size : 0;
+    const uint64_t in_page = held ? static_cast<uint64_t>(slot) % p.cache.page_size : 0;
+    const uint64_t row0 = page * p.cache.stride_page + in_page * p.cache.stride_token;
+    const uint64_t element = kv_element_bytes(p.cache.dtype);
+
+    for (uint32_t h0 = first; h0 < first + p.heads_per_wave; h0 += kAtOnce) {
+        const uint32_t h = h0 + lane / kLanes;
+        const bool live = h < p.q_heads + 2 * p.kv_heads;
+        const bool is_q = h < p.q_heads, is_k = !is_q && h < p.q_heads + p.kv_heads;
+        const uint32_t hk = is_q ? 0 : is_k ? h - p.q_heads : h - p.q_heads - p.kv_heads;
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (live) {
+            if (is_q)
+                load_act4<BF16, VEC>(p.q, static_cast<uint64_t>(token) * p.stride_q_row + static_cast<uint64_t>(h) * p.stride_q_head + e0, x);
+            else if (is_k)
+                load_act4<BF16, VEC>(p.k, static_cast<uint64_t>(token) * p.stride_k_row + hk * D + e0, x);
+            else
+                load_act4<BF16, VEC>(p.v, static_cast<uint64_t>(token) * p.stride_v_row + hk * D + e0, x);
+        }
+        const float squares = head_sum<kLanes>((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]));
+        const float *w = is_q ? p.q_weight : is_k ? p.k_weight : nullptr;
+        float y[4] = {x[0], x[1], x[2], x[3]};
+        if (w != nullptr) {
+            const float scale = rms_scale(squares, D, p.eps);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) y[i] = (x[i] * scale) * w[e0 + i];
+        }
+        if (p.rotary_dim != 0) {   // uniform: the exchange needs every lane
+            float r[4];
+            if (p.interleaved) {
+                r[0] = y[0] * c[0] - y[1] * s[0];
+                r[1] = y[1] * c[0] + y[0] * s[0];
+                r[2] = y[2] * c[1] - y[3] * s[1];
+                r[3] = y[3] * c[1] + y[2] * s[1];
+            } else {
+                const bool low = e0 < half;
+                const uint32_t from = turns ? (low ? lane + half / 4 : lane - half / 4) : lane;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const float other = as_f32(__builtin_amdgcn_ds_bpermute(static_cast<int>(from * 4), as_i32(y[i])));
+                    r[i] = low ? y[i] * c[i] - other * s[i] : y[i] * c[i] + other * s[i];
+                }
+            }
+            if (turns && (is_q || is_k)) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) y[i] = r[i];
+            }
+        }
+        if (!live) continue;
+        if (is_q) {
+            store_act4<BF16, VEC>(p.q_out, static_cast<uint64_t>(token) * p.stride_q_out_row + h * D + e0, y);
+        } else if (held) {
+            uint8_t *pool = static_cast<uint8_t *>(is_k ? p.cache.k : p.cache.v);
+            store_kv4(pool + (row0 + hk * p.cache.stride_head) * element, e0, p.cache.dtype,
+                      is_k ? p.cache.k_scale : p.cache.v_scale, y);
+        }
+    }
+}
+
+template <bool BF16, uint32_t D>
+void launch_append(const AppendParams &p, bool vec, uint32_t grid, hipStream_t s) {
+    if (vec) append_kernel<BF16, D, true><<<grid, kAppendThreads, 0, s>>>(p);
+    else append_kernel<BF16, D, false><<<grid, kAppendThreads, 0, s>>>(p);
+}
+
+}  // namespace
+}  // namespace q8mi
+
+using namespace q8mi;
+
+extern "C" int q8mi_qk_norm_rope_append(const void *q, const void *k, const void *v, void *q_out, int is_bf16,
+                                        uint32_t tokens, uint32_t q_heads, uint32_t stride_q_row, uint32_t stride_q_head,
+                                        uint32_t stride_k_row, uint32_t stride_v_row, uint32_t stride_q_out_row,
+                                        const float *q_norm_weight, const float *k_norm_weight, float eps,
+                                        const double *freqs, uint32_t rotary_dim, int interleaved,
+                                        const int32_t *positions, const int64_t *slots, const q8mi_kv_cache *cache,
+                                        void *stream) {
+    const char *what = "qk_norm_rope_append";
+    if (const int rc = check_kv_cache(what, cache); rc != Q8MI_OK) return rc;
+    if (tokens == 0) return Q8MI_OK;
+    if (q == nullptr || k == nullptr || v == nullptr || q_out == nullptr || slots == nullptr)
+        return fail(Q8MI_REJECTED, "%s: null pointer", what);
+    if (rotary_dim % 8 != 0 || rotary_dim > cache->head_dim)
+        return fail(Q8MI_REJECTED, "%s: rotary_dim %u is not a multiple of 8 up to head_dim", what, rotary_dim);
+    if (rotary_dim != 0 && (freqs == nullptr || positions == nullptr))
+        return fail(Q8MI_REJECTED, "%s: rotation without frequencies or positions", what);
+    const uint64_t D = cache->head_dim;
+    if (q_heads == 0 || q_heads > 65536 || cache->kv_heads > 65536) return fail(Q8MI_REJECTED, "%s: %u query heads", what, q_heads);
+    if (stride_q_head < D || (tokens > 1 && (stride_q_row < (q_heads - 1) * static_cast<uint64_t>(stride_q_head) + D ||
+                                            stride_k_row < cache->kv_heads * D || stride_v_row < cache->kv_heads * D ||
+                                            stride_q_out_row < q_heads * D)))
+        return fail(Q8MI_REJECTED, "%s: rows overlap", what);
+    if (q_out == q && (stride_q_head != D || (tokens > 1 && stride_q_row != stride_q_out_row)))
+        return fail(Q8MI_REJECTED, "%s: in place needs dense heads and one row stride", what);
+
+    AppendParams p{};
+    p.q = q; p.k = k; p.v = v; p.q_out = q_out;
+    p.q_weight = q_norm_weight; p.k_weight = k_norm_weight;
+    p.freqs = freqs; p.positions = positions; p.slots = slots; p.cache = *cache;
+    p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = cache->kv_heads;
+    p.stride_q_row = stride_q_row; p.stride_q_head = stride_q_head; p.stride_k_row = stride_k_row;
+    p.stride_v_row = stride_v_row; p.stride_q_out_row = stride_q_out_row;
+    p.rotary_dim = rotary_dim; p.interleaved = interleaved; p.eps = eps;
+    const uint32_t at_once = kWave / (cache->head_dim / 4);
+    const uint32_t heads = q_heads + 2 * cache->kv_heads;
+    p.heads_per_wave = at_once;
+    p.waves_per_token = (heads + p.heads_per_wave - 1) / p.heads_per_wave;
+    const uint64_t grid = (static_cast<uint64_t>(tokens) * p.waves_per_token + kAppendWaves - 1) / kAppendWaves;
+    if (grid > 0x3fffffffull) return fail(Q8MI_REJECTED, "%s: too many heads for one launch", what);
+
+    const uintptr_t bases = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                            reinterpret_cast<uintptr_t>(q_out);
+    const uint32_t unit = is_bf16 ? 8 : 4;   // elements of 16 bytes
+    const bool vec = bases % 16 == 0 && (stride_q_row | stride_q_head | stride_k_row | stride_v_row | stride_q_out_row) % unit == 0;
+    hipStream_t s = as_stream(stream);
+    auto by_dim = [&](auto bf16) {
+        constexpr bool B = decltype(bf16)::value;
+        if (cache->head_dim == 64) launch_append<B, 64>(p, vec, static_cast<uint32_t>(grid), s);
+        else if (cache->head_dim == 128) launch_append<B, 128>(p, vec, static_cast<uint32_t>(grid), s);
+        else launch_append<B, 256>(p, vec, static_cast<uint32_t>(grid), s);
+    };
+    if (is_bf16) by_dim(std::true_type{});
+    else by_dim(std::false_type{});
+    return check_launch(what);
+}

@@ -15,11 +15,20 @@ QK = 32
 Q8_0_BYTES = 34
 Q8_1_BYTES = 36
 D4_BYTES = 144
+KV_BF16, KV_F16, KV_E4M3 = 0, 1, 2
 MAX_GEMV_BATCH = 8
 
 
 class ArgmaxPair(C.Structure):
     _fields_ = [("value", C.c_float), ("index", C.c_int32)]
+
+
+class KvCache(C.Structure):
+    """q8mi_kv_cache: pools of one layer's keys and values (strides in elements)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("pages", C.c_uint32),
+                ("page_size", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("stride_page", C.c_uint64), ("stride_head", C.c_uint64), ("stride_token", C.c_uint64),
+                ("k_scale", C.c_float), ("v_scale", C.c_float)]
 
 
 _u8p = C.c_void_p  # device pointers travel as plain addresses
@@ -73,6 +82,13 @@ SIGNATURES = {
     "q8mi_rms_norm": (_int, [_vp, _vp, _vp, _u32, _u32, _u32, _u32, C.c_float, _vp]),
     "q8mi_rms_norm_quantize_q8_1": (_int, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, C.c_float, _vp]),
     "q8mi_add_rms_norm": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, C.c_float, _vp]),
+    "q8mi_qk_norm_rope_append": (_int, [_vp] * 4 + [_int] + [_u32] * 7 + [_vp, _vp, C.c_float, _vp, _u32, _int, _vp, _vp,
+                                                                          C.POINTER(KvCache), _vp]),
+    "q8mi_paged_attention_scratch_bytes": (C.c_size_t, [_u32] * 6),
+    "q8mi_paged_attention": (_int, [_vp, _int, _u32, _u32, C.POINTER(KvCache), _vp, _u32, _vp, _vp, _u32, _u32, _u32,
+                                    _u32, C.c_float, _vp, _int, _u32, _vp, _vp]),
+    "q8mi_sample_scratch_bytes": (C.c_size_t, [_u32, _u32]),
+    "q8mi_sample": (_int, [_vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "q8mi_nqgemv": (_int, [_vp, _vp, _vp, C.c_float, _vp, _vp, _int, _u32, _u32, _u32, _vp]),
     "q8mi_nqgemv_silu_mul": (_int, [_vp, _vp, _vp, _vp, C.c_float, _vp, _vp, _u32, _u32, _u32, _vp]),
     "q8mi_nqgemv_fanout4": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, C.c_float, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32,

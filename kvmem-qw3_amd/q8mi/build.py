@@ -18,6 +18,9 @@ SOURCES = [
     "q8mi_get_rows.hip",
     "q8mi_rms_norm.hip",
     "q8mi_gemm.hip",
+    "q8mi_kv_append.hip",
+    "q8mi_attention.hip",
+    "q8mi_sample.hip",
 ]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
