@@ -2,93 +2,596 @@
 //
 //   out = sum_t p_t v_t,  p = softmax_t(scale * q . k_t),  t <= kv_len - rows + i
 //
-// One workgroup per query row and head.  Its four waves take every fourth token, a lane holds head_dim / 64 elements of
-// the query and of the output; each wave keeps a running maximum, sum and output, which meet in LDS at the end.
+// One pass over the cache with a running maximum and sum per query row.  A workgroup takes a chunk of a sequence's tokens
+// for one key head and all the query rows that read it (rows of the sequence x query heads of the group, in tiles of 16 a
+// wave); the chunks' (maximum, sum, output) meet in a second small launch, chunk by chunk in order, so results repeat.
+//
+// A step is a tile of 32 tokens, held in LDS exactly as in memory, each row's 16-byte pieces permuted by an exclusive or
+// with the token so that the reads below meet different banks.  Tiles travel global -> LDS without passing through
+// registers, one page lookup per 16 bytes and lane, so a page may end anywhere inside a tile.  Both products run on the
+// matrix cores with the tokens' side as the first operand:
+//   scores   S^T = K Q^T     a lane gets 8 tokens (2 x 4) of ONE query row, row lane % 16
+//   output   O^T += V^T P^T  V^T from the transposing LDS read; the order of the 32 tokens inside the product is the one
+//            the lane's 8 weights already have, so P needs no exchange between lanes, and a lane's outputs belong to the
+//            same row as its weights: rescaling by a new maximum is one factor per lane.
+// Precision: cache elements are exact operands (bf16, or fp16 for fp16 and e4m3).  The fp32 side, q and the weights, is
+// split into operands that add up to it: three bf16 terms (all 24 bits), or two fp16 terms (22 bits) after scaling by a
+// power of two that keeps the second term clear of fp16's subnormals.  Sums are fp32 throughout.
 #include "q8mi_kv.hpp"
 
 namespace q8mi {
 namespace {
 
-constexpr uint32_t kMaxRows = 16;     // new rows of a sequence
+constexpr uint32_t kMaxRows = 16;      // new rows of a sequence
 constexpr uint32_t kAttnThreads = 256;
+constexpr uint32_t kTile = 32;         // tokens of a step and wave
+constexpr uint32_t kMaxChunk = 2048;   // tokens of a workgroup: their page ids are held in LDS
+constexpr uint32_t kRowTile = 16;      // query rows of a wave
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
 struct AttnParams {
     const void *q;
     void *out;
+    float *part;       // [row][q_heads][splits][D]: a chunk's output, not yet divided by its sum
+    float2 *part_ml;   // [row][q_heads][splits]: its maximum (log2 units) and sum
     const int32_t *page_table, *kv_lens, *q_starts;
     q8mi_kv_cache cache;
     uint32_t q_rows, stride_q, stride_out, stride_page_table;
     uint32_t n_seqs, max_q_len, q_heads, group, max_kv_len;
-    float scale;
+    uint32_t chunk, splits, row_tiles;
+    float scale_log2;  // scale * log2(e) * k_scale
     int q_is_bf16, out_is_bf16;
 };
 
-__device__ __forceinline__ float load_kv(const void *pool, uint64_t at, int dtype) {
-    if (dtype == Q8MI_KV_E4M3) return __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t *>(pool)[at], 0);
-    const uint16_t h = static_cast<const uint16_t *>(pool)[at];
-    return dtype == Q8MI_KV_BF16 ? bf16_bits_to_float(h) : half_bits_to_float(h);
+// What a sequence's rows are and see.
+struct Rows {
+    int64_t start, count, kv_len;
+    uint32_t used;     // rows that are computed, 0 .. max_q_len
+    uint32_t tokens;   // tokens that some row may see, 0 .. max_kv_len
+};
+__device__ __forceinline__ Rows rows_of(const AttnParams &p, uint32_t seq) {
+    Rows r;
+    r.start = static_cast<int64_t>(seq) * p.max_q_len;
+    r.count = p.max_q_len;
+    if (p.q_starts != nullptr) {
+        r.start = p.q_starts[seq];
+        r.count = p.q_starts[seq + 1] - r.start;
+    }
+    r.kv_len = p.kv_lens[seq];
+    r.used = r.count < 0 ? 0u : r.count > p.max_q_len ? p.max_q_len : static_cast<uint32_t>(r.count);
+    r.tokens = r.kv_len < 0 ? 0u : r.kv_len > p.max_kv_len ? p.max_kv_len : static_cast<uint32_t>(r.kv_len);
+    return r;
 }
 
-template <uint32_t D>
-__global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParams p) {
-    constexpr uint32_t E = D / kWave;
-    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const uint32_t seq = blockIdx.x / p.max_q_len, i = blockIdx.x % p.max_q_len, head = blockIdx.y;
-    int64_t start = static_cast<int64_t>(seq) * p.max_q_len, rows = p.max_q_len;
-    if (p.q_starts != nullptr) {
-        start = p.q_starts[seq];
-        rows = p.q_starts[seq + 1] - start;
-    }
-    const int64_t row = start + i;
-    if (i >= rows || row < 0 || row >= p.q_rows) return;
-    const int64_t kv_len = p.kv_lens[seq];
-    int64_t seen = kv_len - rows + i + 1;
-    seen = seen > p.max_kv_len ? p.max_kv_len : seen;
-    const uint32_t kv_head = head / p.group;
+__device__ __forceinline__ void store_out(const AttnParams &p, uint64_t at, float v) {
+    if (p.out_is_bf16) static_cast<uint16_t *>(p.out)[at] = float_to_bf16_bits(v);
+    else static_cast<float *>(p.out)[at] = v;
+}
 
-    float q[E], o[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (uint32_t e = 0; e < E; ++e) {
-        const uint64_t at = static_cast<uint64_t>(row) * p.stride_q + head * D + e * kWave + lane;
-        q[e] = p.q_is_bf16 ? bf16_bits_to_float(static_cast<const uint16_t *>(p.q)[at]) : static_cast<const float *>(p.q)[at];
-        o[e] = 0.0f;
+// 16 bytes per lane, each lane from its own address, to LDS at lds_off + lane * 16.  Inline assembly, so that the
+// compiler does not make every later LDS read wait for it; the counts are waited for by hand.
+__device__ __forceinline__ void dma16_lanes(const void *lane_ptr, uint32_t lds_off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_off), "v"(lane_ptr)
+                 : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+using lds_ptr = __attribute__((address_space(3))) void *;
+__device__ __forceinline__ uint32_t lds_offset(const void *p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)p));
+}
+
+template <int KV>
+struct Operand;   // how eight elements become a matrix operand, and fp32 values a sum of operands
+template <>
+struct Operand<Q8MI_KV_BF16> {
+    static constexpr int kTerms = 3;
+    static constexpr float kWeightScale = 1.0f;
+    static __device__ __forceinline__ v4f mma(v8s a, v8s b, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
     }
-    const bool e4m3 = p.cache.dtype == Q8MI_KV_E4M3;
-    const float scale = p.scale * (e4m3 ? p.cache.k_scale : 1.0f);
-    for (int64_t t = wave; t < seen; t += kAttnThreads / kWave) {
-        const int32_t page = p.page_table[static_cast<uint64_t>(seq) * p.stride_page_table + t / p.cache.page_size];
-        if (page < 0 || static_cast<uint32_t>(page) >= p.cache.pages) continue;
-        const uint64_t at = page * p.cache.stride_page + kv_head * p.cache.stride_head + (t % p.cache.page_size) * p.cache.stride_token;
-        float dot = 0.0f;
+    // the upper 16 bits are a bf16: each term takes eight of the 24 bits, the last one is exact
+    static __device__ __forceinline__ void split(const float (&x)[8], v8s (&t)[kTerms]) {
 #pragma unroll
-        for (uint32_t e = 0; e < E; ++e) dot += q[e] * load_kv(p.cache.k, at + e * kWave + lane, p.cache.dtype);
-        const float score = wave_sum(dot) * scale;
-        const float top = fmaxf(m, score);
-        const float keep = m == top ? 1.0f : expf(m - top), w = expf(score - top);
-        l = l * keep + w;
+        for (int i = 0; i < 8; ++i) {
+            float r = x[i];
 #pragma unroll
-        for (uint32_t e = 0; e < E; ++e)
-            o[e] = o[e] * keep + w * load_kv(p.cache.v, at + e * kWave + lane, p.cache.dtype);
-        m = top;
-    }
-    __shared__ float om[4][D], mm[4], ll[4];
-#pragma unroll
-    for (uint32_t e = 0; e < E; ++e) om[wave][e * kWave + lane] = o[e];
-    if (lane == 0) { mm[wave] = m; ll[wave] = l; }
-    __syncthreads();
-    const float top = fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3]));
-    for (uint32_t d = threadIdx.x; d < D; d += kAttnThreads) {
-        float sum = 0.0f, total = 0.0f;
-        for (int w = 0; w < 4; ++w) {
-            const float f = ll[w] == 0.0f ? 0.0f : expf(mm[w] - top);
-            sum += f * om[w][d];
-            total += f * ll[w];
+            for (int k = 0; k < kTerms; ++k) {
+                const uint32_t hi = __builtin_bit_cast(uint32_t, r) & 0xffff0000u;
+                t[k][i] = static_cast<short>(hi >> 16);
+                r -= __builtin_bit_cast(float, hi);
+            }
         }
-        const float r = total == 0.0f ? 0.0f : sum / total * (e4m3 ? p.cache.v_scale : 1.0f);
-        const uint64_t at = static_cast<uint64_t>(row) * p.stride_out + head * D + d;
-        if (p.out_is_bf16) static_cast<uint16_t *>(p.out)[at] = float_to_bf16_bits(r);
-        else static_cast<float *>(p.out)[at] = r;
     }
+};
+template <>
+struct Operand<Q8MI_KV_F16> {
+    static constexpr int kTerms = 2;
+    static constexpr float kWeightScale = 16384.0f;   // weights are at most 1: the second term ends at 2^-38
+    static __device__ __forceinline__ v4f mma(v8s a, v8s b, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void split(const float (&x)[8], v8s (&t)[kTerms]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const _Float16 hi = static_cast<_Float16>(x[i]);
+            const _Float16 lo = static_cast<_Float16>(x[i] - static_cast<float>(hi));
+            t[0][i] = __builtin_bit_cast(short, hi);
+            t[1][i] = __builtin_bit_cast(short, lo);
+        }
+    }
+};
+template <>
+struct Operand<Q8MI_KV_E4M3> : Operand<Q8MI_KV_F16> {};
+
+__device__ __forceinline__ v8s e4m3_to_f16(v2i w) {   // exact: every e4m3 value is an fp16
+    union { v2h h[4]; v8s s; } u;
+    u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.x, 1.0f, false);
+    u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.x, 1.0f, true);
+    u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, 1.0f, false);
+    u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, 1.0f, true);
+    return u.s;
+}
+
+__device__ __forceinline__ float rows_max(float v) {   // over the four lanes that hold a query row
+    v = fmaxf(v, lane_xor<16>(v));
+    return fmaxf(v, lane_xor<32>(v));
+}
+__device__ __forceinline__ float rows_sum(float v) {
+    v += lane_xor<16>(v);
+    return v + lane_xor<32>(v);
+}
+
+// WR waves side by side on the query rows (16 each), 4 / WR of these groups on alternating tiles of tokens.
+template <uint32_t D, int KV, uint32_t WR>
+struct Layout {
+    static constexpr uint32_t kRowBytes = D * (KV == Q8MI_KV_E4M3 ? 1 : 2);
+    static constexpr uint32_t kLanesPerRow = kRowBytes / 16;
+    static constexpr uint32_t kRowsPerLoad = kWave / kLanesPerRow;    // tokens that one transfer instruction of a wave brings
+    static constexpr uint32_t kLoads = kTile / kRowsPerLoad;          // transfers of a tile
+    static constexpr uint32_t kLoadsPerWave = kLoads >= WR ? kLoads / WR : 1;
+    static constexpr uint32_t kSwizzle = (kLanesPerRow < 16 ? kLanesPerRow : 16) - 1;
+    static constexpr uint32_t kTileBytes = kTile * kRowBytes;
+    static constexpr uint32_t kGroups = 4 / WR;
+    static constexpr uint32_t kTiles = 0;                              // [group][K, V][tile]
+    static constexpr uint32_t kPages = kGroups * 2 * kTileBytes;       // page ids of the chunk
+    static constexpr uint32_t kMergeBytes = kGroups > 1 ? 4 * kRowTile * (D + 4) * 4 + 4 * kRowTile * 8 : 0;
+    static constexpr uint32_t kBytes = kPages + (kMaxChunk + 2) * 4 > kMergeBytes ? kPages + (kMaxChunk + 2) * 4 : kMergeBytes;
+};
+
+template <uint32_t D, int KV, uint32_t WR>
+__global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParams p) {
+    using L = Layout<D, KV, WR>;
+    using Op = Operand<KV>;
+    constexpr uint32_t kSteps = D / 32, kOuts = D / 16;
+    extern __shared__ __align__(16) uint8_t lds[];
+    int32_t *pages = reinterpret_cast<int32_t *>(lds + L::kPages);
+
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t wr = wave % WR, wg = wave / WR;
+    const uint32_t split = blockIdx.y;
+    const uint32_t row_tile = blockIdx.x % p.row_tiles;
+    const uint32_t kv_head = blockIdx.x / p.row_tiles % p.cache.kv_heads;
+    const uint32_t seq = blockIdx.x / p.row_tiles / p.cache.kv_heads;
+
+    const Rows rows = rows_of(p, seq);
+    const uint32_t used_splits = (rows.tokens + p.chunk - 1) / p.chunk;
+    if (split >= (used_splits ? used_splits : 1)) return;
+    const uint32_t n_rows = rows.used * p.group;
+    const uint32_t row0 = row_tile * (WR * kRowTile);
+    if (row0 >= n_rows) return;
+
+    const uint32_t t0 = split * p.chunk;                                       // the chunk: tokens t0 .. t1 - 1
+    const uint32_t t1 = t0 + p.chunk < rows.tokens ? t0 + p.chunk : rows.tokens;
+
+    // this lane's query row
+    const uint32_t g = lane / 16, row = row0 + wr * kRowTile + lane % 16;
+    const uint32_t token = row / p.group, head = kv_head * p.group + row % p.group;
+    const int64_t q_row = rows.start + token;
+    const bool live = row < n_rows && q_row >= 0 && q_row < p.q_rows;
+    const int64_t last64 = rows.kv_len - rows.count + token;                   // the last token it sees
+    const int32_t last = !live || last64 < 0 ? -1 : last64 >= p.max_kv_len ? static_cast<int32_t>(p.max_kv_len) - 1
+                                                                           : static_cast<int32_t>(last64);
+
+    // queries and page ids, requested together
+    float qv[kSteps][8];
+    if (p.q_is_bf16) {
+        const uint16_t *src = static_cast<const uint16_t *>(p.q) + (live ? static_cast<uint64_t>(q_row) * p.stride_q + head * D + g * 8 : 0);
+#pragma unroll
+        for (uint32_t j = 0; j < kSteps; ++j) {
+            const v4i w = live ? *reinterpret_cast<const v4i *>(src + j * 32) : v4i{0, 0, 0, 0};
+            const int ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                qv[j][2 * i] = as_f32(ws[i] << 16);
+                qv[j][2 * i + 1] = as_f32(ws[i] & static_cast<int>(0xffff0000u));
+            }
+        }
+    } else {
+        const float *src = static_cast<const float *>(p.q) + (live ? static_cast<uint64_t>(q_row) * p.stride_q + head * D + g * 8 : 0);
+#pragma unroll
+        for (uint32_t j = 0; j < kSteps; ++j) {
+            const v4f a = live ? *reinterpret_cast<const v4f *>(src + j * 32) : v4f{0, 0, 0, 0};
+            const v4f b = live ? *reinterpret_cast<const v4f *>(src + j * 32 + 4) : v4f{0, 0, 0, 0};
+            qv[j][0] = a.x; qv[j][1] = a.y; qv[j][2] = a.z; qv[j][3] = a.w;
+            qv[j][4] = b.x; qv[j][5] = b.y; qv[j][6] = b.z; qv[j][7] = b.w;
+        }
+    }
+    const uint32_t page0 = t0 / p.cache.page_size;
+    const uint32_t n_pages = t1 > t0 ? (t1 - 1) / p.cache.page_size - page0 + 1 : 0;
+    bool bad = false;
+    for (uint32_t i = threadIdx.x; i < n_pages; i += kAttnThreads) {
+        const int32_t id = p.page_table[static_cast<uint64_t>(seq) * p.stride_page_table + page0 + i];
+        const bool ok = id >= 0 && static_cast<uint32_t>(id) < p.cache.pages;
+        pages[i] = ok ? id : -1;
+        bad |= !ok;
+    }
+    const bool any_bad = __syncthreads_or(bad);
+
+    // fp16 operands: the row's largest |q| goes to 2^13 .. 2^14
+    float row_scale = 1.0f;
+    if constexpr (KV != Q8MI_KV_BF16) {
+        float top = 0.0f;
+#pragma unroll
+        for (uint32_t j = 0; j < kSteps; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(qv[j][i]));
+        top = rows_max(top);
+        int e = 0;
+        if (top > 0.0f && top < INFINITY) {
+            (void)frexpf(top, &e);
+            e = 14 - e;
+            e = e > 100 ? 100 : e;
+        }
+        row_scale = ldexpf(1.0f, e);
+    }
+    v8s qf[kSteps][Op::kTerms];
+#pragma unroll
+    for (uint32_t j = 0; j < kSteps; ++j) {
+        if constexpr (KV != Q8MI_KV_BF16) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) qv[j][i] *= row_scale;
+        }
+        Op::split(qv[j], qf[j]);
+    }
+    const float to_log2 = p.scale_log2 / row_scale;
+
+    // ---- the tiles' way into LDS ----
+    const uint32_t k_tile = L::kTiles + wg * 2 * L::kTileBytes, v_tile = k_tile + L::kTileBytes;
+    const uint32_t lds0 = lds_offset(lds);
+    const uint64_t element = kv_element_bytes(p.cache.dtype);
+    const uint8_t *k_pool = static_cast<const uint8_t *>(p.cache.k) + kv_head * p.cache.stride_head * element;
+    const uint8_t *v_pool = static_cast<const uint8_t *>(p.cache.v) + kv_head * p.cache.stride_head * element;
+    auto load_tile = [&](const uint8_t *pool, uint32_t tile, uint32_t first) {
+#pragma unroll
+        for (uint32_t u = 0; u < L::kLoadsPerWave; ++u) {
+            const uint32_t r = u * WR + wr;
+            if (L::kLoads < WR && r >= L::kLoads) break;   // uniform
+            const uint32_t slot = r * L::kRowsPerLoad + lane / L::kLanesPerRow;      // token of the tile
+            const uint32_t piece = (lane % L::kLanesPerRow) ^ (slot & L::kSwizzle);
+            const uint32_t t = first + slot;
+            uint64_t at = 0;                                                        // hidden: any row of the pool
+            if (t < t1) {
+                const uint32_t pg = t / p.cache.page_size;
+                const int32_t id = pages[pg - page0];
+                if (id >= 0) at = static_cast<uint32_t>(id) * p.cache.stride_page + (t - pg * p.cache.page_size) * p.cache.stride_token;
+            }
+            dma16_lanes(pool + at * element + piece * 16, lds0 + tile + r * 1024);
+        }
+    };
+    auto visible = [&](uint32_t t) { return t < t1 && pages[t / p.cache.page_size - page0] >= 0; };
+
+    // ---- the walk over the chunk ----
+    float m = -INFINITY, l = 0.0f;
+    v4f o[kOuts];
+#pragma unroll
+    for (uint32_t d = 0; d < kOuts; ++d) o[d] = v4f{0, 0, 0, 0};
+    const int64_t first_last = rows.kv_len - rows.count;   // what row 0 of the sequence sees last
+    const uint32_t n_steps = t1 > t0 ? (t1 - t0 + L::kGroups * kTile - 1) / (L::kGroups * kTile) : 0;
+    if (n_steps) {
+        load_tile(k_pool, k_tile, t0 + wg * kTile);
+        load_tile(v_pool, v_tile, t0 + wg * kTile);
+    }
+    for (uint32_t step = 0; step < n_steps; ++step) {
+        const uint32_t first = t0 + (step * L::kGroups + wg) * kTile;
+        const uint32_t next = first + L::kGroups * kTile;
+        const bool more = step + 1 < n_steps;
+
+        wait_loads<L::kLoadsPerWave>();   // the keys are here, the values may still travel
+        if constexpr (WR > 1) __syncthreads();
+        v4f s[2][Op::kTerms];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < Op::kTerms; ++k) s[h][k] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t j = 0; j < kSteps; ++j) {
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint32_t key = h * 16 + lane % 16;
+                v8s kf;
+                if constexpr (KV == Q8MI_KV_E4M3) {
+                    const uint32_t piece = (j * 2 + g / 2) ^ (key & L::kSwizzle);
+                    kf = e4m3_to_f16(*reinterpret_cast<const v2i *>(lds + k_tile + key * L::kRowBytes + piece * 16 + g % 2 * 8));
+                } else {
+                    const uint32_t piece = (j * 4 + g) ^ (key & L::kSwizzle);
+                    kf = *reinterpret_cast<const v8s *>(lds + k_tile + key * L::kRowBytes + piece * 16);
+                }
+#pragma unroll
+                for (int k = 0; k < Op::kTerms; ++k) s[h][k] = Op::mma(kf, qf[j][k], s[h][k]);
+            }
+        }
+        wait_lds_reads();
+        if constexpr (WR > 1) __syncthreads();
+        if (more) load_tile(k_pool, k_tile, next);
+
+        // a lane's eight tokens: first + h * 16 + g * 4 + i
+        const bool whole = !any_bad && first + kTile <= t1 && static_cast<int64_t>(first) + kTile - 1 <= first_last;   // uniform
+        float w[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float dot = s[h][Op::kTerms - 1][i];
+#pragma unroll
+                for (int k = Op::kTerms - 2; k >= 0; --k) dot += s[h][k][i];
+                w[h * 4 + i] = dot * to_log2;
+            }
+        uint32_t shown = 0xff;   // tokens of this lane that exist
+        if (!whole) {
+            shown = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const uint32_t t = first + i / 4 * 16 + g * 4 + i % 4;
+                const bool there = visible(t);
+                shown |= there ? 1u << i : 0u;
+                if (!there || static_cast<int32_t>(t) > last) w[i] = -INFINITY;
+            }
+        }
+        float top = fmaxf(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7])));
+        top = fmaxf(rows_max(top), m);
+        if (__builtin_amdgcn_ballot_w64(top != m) != 0) {   // uniform; NaN scores leave the maximum as it is
+            const float keep = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+            l *= keep;
+#pragma unroll
+            for (uint32_t d = 0; d < kOuts; ++d) o[d] *= keep;
+            m = top;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(w[i] - base);
+            l += w[i];
+            w[i] *= Op::kWeightScale;
+        }
+        v8s pf[Op::kTerms];
+        Op::split(w, pf);
+
+        if (more) wait_loads<L::kLoadsPerWave>();   // the values are here, the next keys may still travel
+        else wait_loads<0>();
+        if constexpr (WR > 1) __syncthreads();
+        // V^T operand of 16 outputs: the transposing read gives lane i of a group of 16 column i of the rows that the
+        // group's lanes point to, here its tokens g * 4 .. + 3 and 16 + g * 4 .. + 3
+        auto values = [&](uint32_t d) -> v8s {
+            if constexpr (KV == Q8MI_KV_E4M3) {
+                const uint32_t i = lane % 16, r = i / 2, key = (r < 4 ? 0 : 12) + g * 4 + r;
+                const uint32_t piece = d ^ (key & L::kSwizzle);
+                using tp = __attribute__((address_space(3))) v2i *;
+                const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((tp)(lds + v_tile + key * L::kRowBytes + piece * 16 + i % 2 * 8));
+                return e4m3_to_f16(x);
+            } else {
+                const uint32_t i = lane % 16, key = g * 4 + i / 4;
+                const uint32_t piece = (d * 2 + i % 4 / 2) ^ (key & L::kSwizzle);
+                using tp = __attribute__((address_space(3))) v4s *;
+                uint8_t *at = lds + v_tile + key * L::kRowBytes + piece * 16 + i % 2 * 8;
+                const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tp)at);
+                const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tp)(at + 16 * L::kRowBytes));
+                return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+        };
+        if (whole) {
+#pragma unroll
+            for (uint32_t d = 0; d < kOuts; ++d) {
+                const v8s vf = values(d);
+#pragma unroll
+                for (int k = Op::kTerms - 1; k >= 0; --k) o[d] = Op::mma(vf, pf[k], o[d]);
+            }
+        } else {
+            // What no row sees (rows behind the last token, tokens of a bad page) is cleared: a weight of 0 does not
+            // silence an infinity or NaN.  A new row's own token is seen by some rows only: where one of those holds
+            // such a value, every row of the sequence gets a pass of its own with just its tokens.
+            bool odd = false;
+            const int32_t some = first_last < -1 ? -1 : first_last > 0x7ffffffe ? 0x7ffffffe : static_cast<int32_t>(first_last);
+            auto masked = [&](v8s x, uint32_t keep) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = keep >> i & 1 ? x[i] : 0;
+                return x;
+            };
+            uint32_t partly = 0;   // tokens of this lane that only some rows see
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const int32_t t = static_cast<int32_t>(first + i / 4 * 16 + g * 4 + i % 4);
+                if ((shown >> i & 1) && t > some) partly |= 1u << i;
+            }
+            constexpr uint16_t kTop = KV == Q8MI_KV_BF16 ? 0x7f80 : 0x7c00;
+#pragma unroll
+            for (uint32_t d = 0; d < kOuts; ++d) {
+                const v8s vf = masked(values(d), partly);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) odd |= (vf[i] & kTop) == kTop;
+            }
+            const bool apart = __builtin_amdgcn_ballot_w64(odd) != 0;   // uniform
+            const uint32_t passes = apart ? rows.used : 1;
+            for (uint32_t pass = 0; pass < passes; ++pass) {
+                uint32_t keep = shown;
+                v8s pm[Op::kTerms];
+#pragma unroll
+                for (int k = 0; k < Op::kTerms; ++k) pm[k] = pf[k];
+                if (apart) {
+                    const int64_t limit = first_last + pass;
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        if (static_cast<int64_t>(first + i / 4 * 16 + g * 4 + i % 4) > limit) keep &= ~(1u << i);
+                    if (token != pass) {
+#pragma unroll
+                        for (int k = 0; k < Op::kTerms; ++k) pm[k] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
+                    }
+                }
+#pragma unroll
+                for (uint32_t d = 0; d < kOuts; ++d) {
+                    const v8s vf = masked(values(d), keep);
+                    v4f sum = apart ? v4f{0, 0, 0, 0} : o[d];
+#pragma unroll
+                    for (int k = Op::kTerms - 1; k >= 0; --k) sum = Op::mma(vf, pm[k], sum);
+                    if (!apart) o[d] = sum;
+                    else if (token == pass) o[d] += sum;
+                }
+            }
+        }
+        wait_lds_reads();
+        if constexpr (WR > 1) __syncthreads();
+        if (more) load_tile(v_pool, v_tile, next);
+    }
+    l = rows_sum(l);
+
+    // ---- the groups of a workgroup meet ----
+    if constexpr (L::kGroups > 1) {
+        // per wave [16 rows][D + 4] outputs, then [16 rows] maxima and sums; the pad spreads the rows over the banks
+        float *mo = reinterpret_cast<float *>(lds);
+        float2 *ml = reinterpret_cast<float2 *>(lds + 4 * kRowTile * (D + 4) * 4);
+        __syncthreads();
+        if (g == 0) ml[wave * kRowTile + lane % 16] = make_float2(m, l);
+        __syncthreads();
+        float all = -INFINITY;
+#pragma unroll
+        for (uint32_t k = 0; k < L::kGroups; ++k) all = fmaxf(all, ml[(k * WR + wr) * kRowTile + lane % 16].x);
+        float sum = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < L::kGroups; ++k) {
+            const float2 x = ml[(k * WR + wr) * kRowTile + lane % 16];
+            sum += x.x == all ? x.y : x.y * __builtin_amdgcn_exp2f(x.x - all);
+        }
+        const float f = m == all ? 1.0f : __builtin_amdgcn_exp2f(m - all);
+        m = all;
+        l = sum;
+#pragma unroll
+        for (uint32_t d = 0; d < kOuts; ++d) {
+            const v4f x = o[d] * f;
+            *reinterpret_cast<v4f *>(mo + (wave * kRowTile + lane % 16) * (D + 4) + d * 16 + g * 4) = x;
+        }
+        __syncthreads();
+        // every wave adds a share of the columns of its rows
+        constexpr uint32_t kShare = kOuts / L::kGroups;
+#pragma unroll
+        for (uint32_t u = 0; u < kShare; ++u) {
+            const uint32_t d = wg * kShare + u;
+            v4f x = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t k = 0; k < L::kGroups; ++k)
+                x += *reinterpret_cast<const v4f *>(mo + ((k * WR + wr) * kRowTile + lane % 16) * (D + 4) + d * 16 + g * 4);
+            o[u] = x;
+        }
+    }
+    constexpr uint32_t kOwn = kOuts / L::kGroups;
+    const uint32_t d0 = wg * kOwn;
+    if (!live) return;
+    if (used_splits <= 1) {
+        const float norm = l > 0.0f || l != l ? (KV == Q8MI_KV_E4M3 ? p.cache.v_scale : 1.0f) / Op::kWeightScale / l : 0.0f;
+        const uint64_t at = static_cast<uint64_t>(q_row) * p.stride_out + head * D + g * 4;
+#pragma unroll
+        for (uint32_t u = 0; u < kOwn; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) store_out(p, at + (d0 + u) * 16 + i, norm == 0.0f ? 0.0f : o[u][i] * norm);
+    } else {
+        const uint64_t at = (static_cast<uint64_t>(seq * p.max_q_len + token) * p.q_heads + head) * p.splits + split;
+#pragma unroll
+        for (uint32_t u = 0; u < kOwn; ++u) *reinterpret_cast<v4f *>(p.part + at * D + (d0 + u) * 16 + g * 4) = o[u];
+        if (g == 0 && wg == 0) p.part_ml[at] = make_float2(m, l);
+    }
+}
+
+// Joins the chunks of one query row and head, in their order.
+template <uint32_t D, int KV>
+__global__ __launch_bounds__(D) void attention_join_kernel(const AttnParams p) {
+    const uint32_t seq = blockIdx.x / p.max_q_len, token = blockIdx.x % p.max_q_len, head = blockIdx.y, d = threadIdx.x;
+    const Rows rows = rows_of(p, seq);
+    const uint32_t n = (rows.tokens + p.chunk - 1) / p.chunk;
+    const int64_t q_row = rows.start + token;
+    if (n <= 1 || token >= rows.used || q_row < 0 || q_row >= p.q_rows) return;
+    const uint64_t at = (static_cast<uint64_t>(blockIdx.x) * p.q_heads + head) * p.splits;
+    float top = -INFINITY;
+    for (uint32_t s = 0; s < n; ++s) top = fmaxf(top, p.part_ml[at + s].x);
+    float sum = 0.0f, out = 0.0f;
+    for (uint32_t s = 0; s < n; ++s) {
+        const float2 ml = p.part_ml[at + s];
+        const float f = ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
+        sum += f * ml.y;
+        out += f * p.part[(at + s) * D + d];
+    }
+    const float norm = (KV == Q8MI_KV_E4M3 ? p.cache.v_scale : 1.0f) / Operand<KV>::kWeightScale;
+    store_out(p, static_cast<uint64_t>(q_row) * p.stride_out + head * D + d, sum == 0.0f ? 0.0f : out / sum * norm);
+}
+
+// How a call is cut: tokens of a chunk, chunks of the longest sequence, row tiles and waves side by side on rows.
+struct Plan {
+    uint32_t chunk, splits, waves_on_rows, row_tiles;
+};
+Plan plan_of(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t max_kv_len) {
+    Plan r;
+    const uint32_t rows = max_q_len * (kv_heads ? q_heads / kv_heads : 0);
+    r.waves_on_rows = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    r.row_tiles = (rows + 16 * r.waves_on_rows - 1) / (16 * r.waves_on_rows);
+    const uint64_t items = static_cast<uint64_t>(n_seqs) * kv_heads * r.row_tiles;
+    r.chunk = kMaxChunk;
+    while (r.chunk > 128 && items * ((max_kv_len + r.chunk - 1) / r.chunk) < 512) r.chunk /= 2;
+    r.splits = max_kv_len ? (max_kv_len + r.chunk - 1) / r.chunk : 1;
+    return r;
+}
+
+template <uint32_t D, int KV, uint32_t WR>
+int launch_waves(const AttnParams &p, hipStream_t s) {
+    using L = Layout<D, KV, WR>;
+    if (L::kBytes > 64 * 1024) {
+        // more than the default grant: asked for once per instantiation and device
+        static thread_local int granted = -1;
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess) return check_launch("paged_attention");
+        if (dev != granted) {
+            if (hipFuncSetAttribute(reinterpret_cast<const void *>(attention_kernel<D, KV, WR>),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != hipSuccess)
+                return check_launch("paged_attention");
+            granted = dev;
+        }
+    }
+    attention_kernel<D, KV, WR><<<dim3(p.n_seqs * p.cache.kv_heads * p.row_tiles, p.splits), kAttnThreads, L::kBytes, s>>>(p);
+    if (p.splits > 1) attention_join_kernel<D, KV><<<dim3(p.n_seqs * p.max_q_len, p.q_heads), D, 0, s>>>(p);
+    return check_launch("paged_attention");
+}
+template <uint32_t D, int KV>
+int launch_dim(const AttnParams &p, uint32_t waves_on_rows, hipStream_t s) {
+    if (waves_on_rows == 1) return launch_waves<D, KV, 1>(p, s);
+    if (waves_on_rows == 2) return launch_waves<D, KV, 2>(p, s);
+    return launch_waves<D, KV, 4>(p, s);
+}
+template <int KV>
+int launch_type(const AttnParams &p, uint32_t waves_on_rows, hipStream_t s) {
+    if (p.cache.head_dim == 64) return launch_dim<64, KV>(p, waves_on_rows, s);
+    if (p.cache.head_dim == 128) return launch_dim<128, KV>(p, waves_on_rows, s);
+    return launch_dim<256, KV>(p, waves_on_rows, s);
+}
+
+uint64_t partial_slots(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t splits) {
+    return splits > 1 ? static_cast<uint64_t>(n_seqs) * max_q_len * q_heads * splits : 0;
 }
 
 }  // namespace
@@ -96,7 +599,11 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
 
 using namespace q8mi;
 
-extern "C" size_t q8mi_paged_attention_scratch_bytes(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) { return 16; }
+extern "C" size_t q8mi_paged_attention_scratch_bytes(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads,
+                                                     uint32_t head_dim, uint32_t max_kv_len) {
+    const Plan plan = plan_of(n_seqs, max_q_len, q_heads, kv_heads, max_kv_len);
+    return 16 + partial_slots(n_seqs, max_q_len, q_heads, plan.splits) * (head_dim + 2) * sizeof(float);
+}
 
 extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_rows, uint32_t stride_q_row,
                                     const q8mi_kv_cache *cache, const int32_t *page_table, uint32_t stride_page_table,
@@ -108,10 +615,10 @@ extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_row
     if (n_seqs == 0 || q_rows == 0) return Q8MI_OK;
     if (q == nullptr || out == nullptr || page_table == nullptr || kv_lens == nullptr || scratch == nullptr)
         return fail(Q8MI_REJECTED, "%s: null pointer", what);
-    if (q_heads == 0 || q_heads > 65536 || q_heads % cache->kv_heads != 0)
+    if (q_heads == 0 || q_heads > 65535 || q_heads % cache->kv_heads != 0)
         return fail(Q8MI_REJECTED, "%s: %u query heads over %u", what, q_heads, cache->kv_heads);
     if (max_q_len == 0 || max_q_len > kMaxRows) return fail(Q8MI_REJECTED, "%s: %u rows a sequence (1..%u)", what, max_q_len, kMaxRows);
-    if (max_kv_len > static_cast<uint64_t>(stride_page_table) * cache->page_size)
+    if (max_kv_len > 0x7fffffffu || max_kv_len > static_cast<uint64_t>(stride_page_table) * cache->page_size)
         return fail(Q8MI_REJECTED, "%s: max_kv_len %u is beyond a page table row of %u", what, max_kv_len, stride_page_table);
     if (!isfinite(scale)) return fail(Q8MI_REJECTED, "%s: scale is not finite", what);
     const uint64_t q_es = q_is_bf16 ? 2 : 4, o_es = out_is_bf16 ? 2 : 4, width = static_cast<uint64_t>(q_heads) * cache->head_dim;
@@ -119,17 +626,22 @@ extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_row
         stride_q_row * q_es % 16 != 0 || stride_out_row * o_es % 16 != 0)
         return fail(Q8MI_REJECTED, "%s: rows of q and out must begin on 16-byte boundaries", what);
     if (q_rows > 1 && (stride_q_row < width || stride_out_row < width)) return fail(Q8MI_REJECTED, "%s: rows overlap", what);
-    if (static_cast<uint64_t>(n_seqs) * max_q_len > 0x7fffffffull) return fail(Q8MI_REJECTED, "%s: too many sequences", what);
 
+    const Plan plan = plan_of(n_seqs, max_q_len, q_heads, cache->kv_heads, max_kv_len);
+    if (static_cast<uint64_t>(n_seqs) * cache->kv_heads * plan.row_tiles > 0x3fffffull || static_cast<uint64_t>(n_seqs) * max_q_len > 0x3fffffull ||
+        plan.splits > 65535)
+        return fail(Q8MI_REJECTED, "%s: %u sequences of %u tokens are too many for one launch", what, n_seqs, max_kv_len);
     AttnParams p{};
     p.q = q; p.out = out; p.page_table = page_table; p.kv_lens = kv_lens; p.q_starts = q_starts; p.cache = *cache;
+    p.part = static_cast<float *>(scratch);
+    p.part_ml = reinterpret_cast<float2 *>(p.part + partial_slots(n_seqs, max_q_len, q_heads, plan.splits) * cache->head_dim);
     p.q_rows = q_rows; p.stride_q = stride_q_row; p.stride_out = stride_out_row; p.stride_page_table = stride_page_table;
     p.n_seqs = n_seqs; p.max_q_len = max_q_len; p.q_heads = q_heads; p.group = q_heads / cache->kv_heads;
-    p.max_kv_len = max_kv_len; p.scale = scale; p.q_is_bf16 = q_is_bf16; p.out_is_bf16 = out_is_bf16;
-    const dim3 grid(n_seqs * max_q_len, q_heads);
+    p.max_kv_len = max_kv_len; p.chunk = plan.chunk; p.splits = plan.splits; p.row_tiles = plan.row_tiles;
+    p.scale_log2 = scale * 1.44269504088896340736f * (cache->dtype == Q8MI_KV_E4M3 ? cache->k_scale : 1.0f);
+    p.q_is_bf16 = q_is_bf16; p.out_is_bf16 = out_is_bf16;
     hipStream_t s = as_stream(stream);
-    if (cache->head_dim == 64) attention_kernel<64><<<grid, kAttnThreads, 0, s>>>(p);
-    else if (cache->head_dim == 128) attention_kernel<128><<<grid, kAttnThreads, 0, s>>>(p);
-    else attention_kernel<256><<<grid, kAttnThreads, 0, s>>>(p);
-    return check_launch(what);
+    if (cache->dtype == Q8MI_KV_BF16) return launch_type<Q8MI_KV_BF16>(p, plan.waves_on_rows, s);
+    if (cache->dtype == Q8MI_KV_F16) return launch_type<Q8MI_KV_F16>(p, plan.waves_on_rows, s);
+    return launch_type<Q8MI_KV_E4M3>(p, plan.waves_on_rows, s);
 }
