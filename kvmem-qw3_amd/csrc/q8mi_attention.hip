@@ -27,6 +27,7 @@ constexpr uint32_t kAttnThreads = 256;
 constexpr uint32_t kTile = 32;         // tokens of a step and wave
 constexpr uint32_t kMaxChunk = 2048;   // tokens of a workgroup: their page ids are held in LDS
 constexpr uint32_t kRowTile = 16;      // query rows of a wave
+constexpr uint32_t kJoinThreads = 512;
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -46,6 +47,8 @@ struct AttnParams {
     uint32_t q_rows, stride_q, stride_out, stride_page_table;
     uint32_t n_seqs, max_q_len, q_heads, group, max_kv_len;
     uint32_t chunk, splits, row_tiles;
+    uint32_t page_magic, page_shift;   // t / page_size = mulhi(t, page_magic) >> page_shift; magic 0: page_size 1
+    uint32_t unit_page, unit_token;    // cache strides in units of 16 bytes
     float scale_log2;  // scale * log2(e) * k_scale
     int q_is_bf16, out_is_bf16;
 };
@@ -68,6 +71,10 @@ __device__ __forceinline__ Rows rows_of(const AttnParams &p, uint32_t seq) {
     r.used = r.count < 0 ? 0u : r.count > p.max_q_len ? p.max_q_len : static_cast<uint32_t>(r.count);
     r.tokens = r.kv_len < 0 ? 0u : r.kv_len > p.max_kv_len ? p.max_kv_len : static_cast<uint32_t>(r.kv_len);
     return r;
+}
+
+__device__ __forceinline__ uint32_t page_of(const AttnParams &p, uint32_t t) {
+    return p.page_magic ? __umulhi(t, p.page_magic) >> p.page_shift : t;
 }
 
 __device__ __forceinline__ void store_out(const AttnParams &p, uint64_t at, float v) {
@@ -140,6 +147,15 @@ __device__ __forceinline__ v8s e4m3_to_f16(v2i w) {   // exact: every e4m3 value
     u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, 1.0f, false);
     u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, 1.0f, true);
     return u.s;
+}
+
+// Whether one of the elements in a word is an infinity or NaN.
+template <int KV>
+__device__ __forceinline__ bool not_finite(int w) {
+    if constexpr (KV == Q8MI_KV_E4M3)   // 0x7f / 0xff, the type's only ones: a byte whose lower seven bits carry into the eighth
+        return (((w & 0x7f7f7f7f) + 0x01010101) & static_cast<int>(0x80808080u)) != 0;
+    constexpr int kTop = KV == Q8MI_KV_BF16 ? 0x7f80 : 0x7c00;
+    return (w & kTop) == kTop || (w >> 16 & kTop) == kTop;
 }
 
 __device__ __forceinline__ float rows_max(float v) {   // over the four lanes that hold a query row
@@ -269,27 +285,32 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
     // ---- the tiles' way into LDS ----
     const uint32_t k_tile = L::kTiles + wg * 2 * L::kTileBytes, v_tile = k_tile + L::kTileBytes;
     const uint32_t lds0 = lds_offset(lds);
-    const uint64_t element = kv_element_bytes(p.cache.dtype);
-    const uint8_t *k_pool = static_cast<const uint8_t *>(p.cache.k) + kv_head * p.cache.stride_head * element;
-    const uint8_t *v_pool = static_cast<const uint8_t *>(p.cache.v) + kv_head * p.cache.stride_head * element;
-    auto load_tile = [&](const uint8_t *pool, uint32_t tile, uint32_t first) {
+    const uint64_t head_bytes = kv_head * p.cache.stride_head * kv_element_bytes(p.cache.dtype);
+    const uint8_t *k_pool = static_cast<const uint8_t *>(p.cache.k) + head_bytes;
+    const uint8_t *v_pool = static_cast<const uint8_t *>(p.cache.v) + head_bytes;
+    auto page_id = [&](uint32_t t) { return pages[page_of(p, t) - page0]; };   // t0 <= t < t1
+    auto visible = [&](uint32_t t) { return t < t1 && page_id(t) >= 0; };
+    // Where token first + lane % 32 lies, in units of 16 bytes; tokens that do not exist read the pool's first row.
+    auto locate = [&](uint32_t first) -> uint32_t {
+        const uint32_t t = first + lane % kTile;
+        if (t >= t1) return 0;
+        const uint32_t pg = page_of(p, t);
+        const int32_t id = pages[pg - page0];
+        return id < 0 ? 0 : static_cast<uint32_t>(id) * p.unit_page + (t - pg * p.cache.page_size) * p.unit_token;
+    };
+    const uint32_t piece0 = lane % L::kLanesPerRow ^ (lane / L::kLanesPerRow & L::kSwizzle);
+    auto load_tile = [&](const uint8_t *pool, uint32_t tile, uint32_t where) {
 #pragma unroll
         for (uint32_t u = 0; u < L::kLoadsPerWave; ++u) {
             const uint32_t r = u * WR + wr;
             if (L::kLoads < WR && r >= L::kLoads) break;   // uniform
-            const uint32_t slot = r * L::kRowsPerLoad + lane / L::kLanesPerRow;      // token of the tile
-            const uint32_t piece = (lane % L::kLanesPerRow) ^ (slot & L::kSwizzle);
-            const uint32_t t = first + slot;
-            uint64_t at = 0;                                                        // hidden: any row of the pool
-            if (t < t1) {
-                const uint32_t pg = t / p.cache.page_size;
-                const int32_t id = pages[pg - page0];
-                if (id >= 0) at = static_cast<uint32_t>(id) * p.cache.stride_page + (t - pg * p.cache.page_size) * p.cache.stride_token;
-            }
-            dma16_lanes(pool + at * element + piece * 16, lds0 + tile + r * 1024);
+            const uint32_t slot0 = r * L::kRowsPerLoad;
+            const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(
+                static_cast<int>((slot0 + lane / L::kLanesPerRow) * 4), static_cast<int>(where)));
+            const uint64_t off = static_cast<uint64_t>(at) + (piece0 ^ (slot0 & L::kSwizzle));
+            dma16_lanes(pool + off * 16, lds0 + tile + r * 1024);
         }
     };
-    auto visible = [&](uint32_t t) { return t < t1 && pages[t / p.cache.page_size - page0] >= 0; };
 
     // ---- the walk over the chunk ----
     float m = -INFINITY, l = 0.0f;
@@ -299,12 +320,13 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
     const int64_t first_last = rows.kv_len - rows.count;   // what row 0 of the sequence sees last
     const uint32_t n_steps = t1 > t0 ? (t1 - t0 + L::kGroups * kTile - 1) / (L::kGroups * kTile) : 0;
     if (n_steps) {
-        load_tile(k_pool, k_tile, t0 + wg * kTile);
-        load_tile(v_pool, v_tile, t0 + wg * kTile);
+        const uint32_t where = locate(t0 + wg * kTile);
+        load_tile(k_pool, k_tile, where);
+        load_tile(v_pool, v_tile, where);
     }
     for (uint32_t step = 0; step < n_steps; ++step) {
         const uint32_t first = t0 + (step * L::kGroups + wg) * kTile;
-        const uint32_t next = first + L::kGroups * kTile;
+        const uint32_t next = locate(first + L::kGroups * kTile);
         const bool more = step + 1 < n_steps;
 
         wait_loads<L::kLoadsPerWave>();   // the keys are here, the values may still travel
@@ -335,8 +357,10 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
         if constexpr (WR > 1) __syncthreads();
         if (more) load_tile(k_pool, k_tile, next);
 
-        // a lane's eight tokens: first + h * 16 + g * 4 + i
-        const bool whole = !any_bad && first + kTile <= t1 && static_cast<int64_t>(first) + kTile - 1 <= first_last;   // uniform
+        // a lane's eight tokens: first + h * 16 + g * 4 + i.  whole: every row sees the whole tile (with several waves on
+        // a tile: all tiles of the step, so that the barriers below are met by all)
+        const uint32_t behind = WR > 1 ? t0 + (step + 1) * L::kGroups * kTile : first + kTile;
+        const bool whole = !any_bad && behind <= t1 && static_cast<int64_t>(behind) - 1 <= first_last;   // uniform
         float w[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -347,15 +371,11 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
                 for (int k = Op::kTerms - 2; k >= 0; --k) dot += s[h][k][i];
                 w[h * 4 + i] = dot * to_log2;
             }
-        uint32_t shown = 0xff;   // tokens of this lane that exist
         if (!whole) {
-            shown = 0;
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
                 const uint32_t t = first + i / 4 * 16 + g * 4 + i % 4;
-                const bool there = visible(t);
-                shown |= there ? 1u << i : 0u;
-                if (!there || static_cast<int32_t>(t) > last) w[i] = -INFINITY;
+                if (!visible(t) || static_cast<int32_t>(t) > last) w[i] = -INFINITY;
             }
         }
         float top = fmaxf(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7])));
@@ -399,7 +419,27 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
                 return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
             }
         };
-        if (whole) {
+        bool apart = false;
+        if (!whole) {
+            // What no row sees (rows behind the last token, tokens of a bad page) is cleared: a weight of 0 does not
+            // silence an infinity or NaN.  A new row's own token is seen by some rows only: where one of those holds
+            // such a value, every row of the sequence gets a pass of its own, below.
+            const uint32_t slot = lane % kTile, t = first + slot;
+            v4i *mine = reinterpret_cast<v4i *>(lds + v_tile + slot * L::kRowBytes + lane / kTile * (L::kRowBytes / 2));
+            bool odd = false;
+            if (!visible(t)) {
+                for (uint32_t i = 0; i < L::kRowBytes / 32; ++i) mine[i] = v4i{0, 0, 0, 0};
+            } else if (static_cast<int64_t>(t) > first_last) {
+                for (uint32_t i = 0; i < L::kRowBytes / 32; ++i) {
+                    const v4i x = mine[i];
+                    odd |= not_finite<KV>(x.x) || not_finite<KV>(x.y) || not_finite<KV>(x.z) || not_finite<KV>(x.w);
+                }
+            }
+            if constexpr (WR > 1) apart = __syncthreads_or(odd);
+            else apart = __builtin_amdgcn_ballot_w64(odd) != 0;
+            wait_lds_reads();
+        }
+        if (!apart) {
 #pragma unroll
             for (uint32_t d = 0; d < kOuts; ++d) {
                 const v8s vf = values(d);
@@ -407,54 +447,22 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
                 for (int k = Op::kTerms - 1; k >= 0; --k) o[d] = Op::mma(vf, pf[k], o[d]);
             }
         } else {
-            // What no row sees (rows behind the last token, tokens of a bad page) is cleared: a weight of 0 does not
-            // silence an infinity or NaN.  A new row's own token is seen by some rows only: where one of those holds
-            // such a value, every row of the sequence gets a pass of its own with just its tokens.
-            bool odd = false;
-            const int32_t some = first_last < -1 ? -1 : first_last > 0x7ffffffe ? 0x7ffffffe : static_cast<int32_t>(first_last);
-            auto masked = [&](v8s x, uint32_t keep) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = keep >> i & 1 ? x[i] : 0;
-                return x;
-            };
-            uint32_t partly = 0;   // tokens of this lane that only some rows see
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const int32_t t = static_cast<int32_t>(first + i / 4 * 16 + g * 4 + i % 4);
-                if ((shown >> i & 1) && t > some) partly |= 1u << i;
-            }
-            constexpr uint16_t kTop = KV == Q8MI_KV_BF16 ? 0x7f80 : 0x7c00;
-#pragma unroll
-            for (uint32_t d = 0; d < kOuts; ++d) {
-                const v8s vf = masked(values(d), partly);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) odd |= (vf[i] & kTop) == kTop;
-            }
-            const bool apart = __builtin_amdgcn_ballot_w64(odd) != 0;   // uniform
-            const uint32_t passes = apart ? rows.used : 1;
-            for (uint32_t pass = 0; pass < passes; ++pass) {
-                uint32_t keep = shown;
-                v8s pm[Op::kTerms];
-#pragma unroll
-                for (int k = 0; k < Op::kTerms; ++k) pm[k] = pf[k];
-                if (apart) {
-                    const int64_t limit = first_last + pass;
-#pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i)
-                        if (static_cast<int64_t>(first + i / 4 * 16 + g * 4 + i % 4) > limit) keep &= ~(1u << i);
-                    if (token != pass) {
-#pragma unroll
-                        for (int k = 0; k < Op::kTerms; ++k) pm[k] = v8s{0, 0, 0, 0, 0, 0, 0, 0};
-                    }
+            for (uint32_t pass = rows.used; pass-- > 0;) {   // the last row sees most; what the next one no longer sees is cleared
+                const uint32_t slot = lane % kTile;
+                if constexpr (WR > 1) __syncthreads();
+                if (static_cast<int64_t>(first) + slot > first_last + pass) {
+                    v4i *mine = reinterpret_cast<v4i *>(lds + v_tile + slot * L::kRowBytes + lane / kTile * (L::kRowBytes / 2));
+                    for (uint32_t i = 0; i < L::kRowBytes / 32; ++i) mine[i] = v4i{0, 0, 0, 0};
                 }
+                if constexpr (WR > 1) __syncthreads();
+                wait_lds_reads();
 #pragma unroll
                 for (uint32_t d = 0; d < kOuts; ++d) {
-                    const v8s vf = masked(values(d), keep);
-                    v4f sum = apart ? v4f{0, 0, 0, 0} : o[d];
+                    const v8s vf = values(d);
+                    v4f sum = v4f{0, 0, 0, 0};
 #pragma unroll
-                    for (int k = Op::kTerms - 1; k >= 0; --k) sum = Op::mma(vf, pm[k], sum);
-                    if (!apart) o[d] = sum;
-                    else if (token == pass) o[d] += sum;
+                    for (int k = Op::kTerms - 1; k >= 0; --k) sum = Op::mma(vf, pf[k], sum);
+                    if (token == pass) o[d] += sum;
                 }
             }
         }
@@ -520,26 +528,50 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
     }
 }
 
-// Joins the chunks of one query row and head, in their order.
+// Joins the chunks of one query row and head, in an order that the sizes alone fix: kJoinGroups threads share a column,
+// chunk by chunk, and meet in LDS.
 template <uint32_t D, int KV>
-__global__ __launch_bounds__(D) void attention_join_kernel(const AttnParams p) {
-    const uint32_t seq = blockIdx.x / p.max_q_len, token = blockIdx.x % p.max_q_len, head = blockIdx.y, d = threadIdx.x;
+__global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const AttnParams p) {
+    constexpr uint32_t kGroups = kJoinThreads / (D / 4);
+    __shared__ float tops[kJoinThreads / kWave], sums[kGroups];
+    __shared__ v4f parts[kGroups][D / 4];
+    const uint32_t seq = blockIdx.x / p.max_q_len, token = blockIdx.x % p.max_q_len, head = blockIdx.y;
+    const uint32_t group = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4);
     const Rows rows = rows_of(p, seq);
     const uint32_t n = (rows.tokens + p.chunk - 1) / p.chunk;
     const int64_t q_row = rows.start + token;
     if (n <= 1 || token >= rows.used || q_row < 0 || q_row >= p.q_rows) return;
     const uint64_t at = (static_cast<uint64_t>(blockIdx.x) * p.q_heads + head) * p.splits;
     float top = -INFINITY;
-    for (uint32_t s = 0; s < n; ++s) top = fmaxf(top, p.part_ml[at + s].x);
-    float sum = 0.0f, out = 0.0f;
-    for (uint32_t s = 0; s < n; ++s) {
+    for (uint32_t s = threadIdx.x; s < n; s += kJoinThreads) top = fmaxf(top, p.part_ml[at + s].x);
+    top = fmaxf(top, lane_xor<1>(top)); top = fmaxf(top, lane_xor<2>(top)); top = fmaxf(top, lane_xor<4>(top));
+    top = fmaxf(top, lane_xor<8>(top)); top = fmaxf(top, lane_xor<16>(top)); top = fmaxf(top, lane_xor<32>(top));
+    if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kJoinThreads / kWave; ++i) top = fmaxf(top, tops[i]);
+    float sum = 0.0f;
+    v4f out = v4f{0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t s = group; s < n; s += kGroups) {
         const float2 ml = p.part_ml[at + s];
         const float f = ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
         sum += f * ml.y;
-        out += f * p.part[(at + s) * D + d];
+        out += f * *reinterpret_cast<const v4f *>(p.part + (at + s) * D + d * 4);
+    }
+    parts[group][d] = out;
+    if (d == 0) sums[group] = sum;
+    __syncthreads();
+    if (group != 0) return;
+#pragma unroll
+    for (uint32_t i = 1; i < kGroups; ++i) {
+        sum += sums[i];
+        out += parts[i][d];
     }
     const float norm = (KV == Q8MI_KV_E4M3 ? p.cache.v_scale : 1.0f) / Operand<KV>::kWeightScale;
-    store_out(p, static_cast<uint64_t>(q_row) * p.stride_out + head * D + d, sum == 0.0f ? 0.0f : out / sum * norm);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        store_out(p, static_cast<uint64_t>(q_row) * p.stride_out + head * D + d * 4 + i, sum == 0.0f ? 0.0f : out[i] / sum * norm);
 }
 
 // How a call is cut: tokens of a chunk, chunks of the longest sequence, row tiles and waves side by side on rows.
@@ -574,7 +606,7 @@ int launch_waves(const AttnParams &p, hipStream_t s) {
         }
     }
     attention_kernel<D, KV, WR><<<dim3(p.n_seqs * p.cache.kv_heads * p.row_tiles, p.splits), kAttnThreads, L::kBytes, s>>>(p);
-    if (p.splits > 1) attention_join_kernel<D, KV><<<dim3(p.n_seqs * p.max_q_len, p.q_heads), D, 0, s>>>(p);
+    if (p.splits > 1) attention_join_kernel<D, KV><<<dim3(p.n_seqs * p.max_q_len, p.q_heads), kJoinThreads, 0, s>>>(p);
     return check_launch("paged_attention");
 }
 template <uint32_t D, int KV>
@@ -631,7 +663,19 @@ extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_row
     if (static_cast<uint64_t>(n_seqs) * cache->kv_heads * plan.row_tiles > 0x3fffffull || static_cast<uint64_t>(n_seqs) * max_q_len > 0x3fffffull ||
         plan.splits > 65535)
         return fail(Q8MI_REJECTED, "%s: %u sequences of %u tokens are too many for one launch", what, n_seqs, max_kv_len);
+    const uint64_t es = kv_element_bytes(cache->dtype);
+    const uint64_t unit_page = cache->stride_page * es / 16, unit_token = cache->stride_token * es / 16;
+    if (unit_page > 0xffffffffull || unit_token > 0xffffffffull ||
+        (cache->pages - 1) * unit_page + (cache->page_size - 1) * unit_token > 0xffffffffull)
+        return fail(Q8MI_REJECTED, "%s: a pool of 64 GiB and more", what);
     AttnParams p{};
+    p.unit_page = static_cast<uint32_t>(unit_page); p.unit_token = static_cast<uint32_t>(unit_token);
+    if (cache->page_size > 1) {   // exact for every t below 2^31
+        uint32_t bits = 1;
+        while ((1u << bits) < cache->page_size) ++bits;
+        p.page_magic = static_cast<uint32_t>((1ull << (31 + bits)) / cache->page_size + 1);
+        p.page_shift = bits - 1;
+    }
     p.q = q; p.out = out; p.page_table = page_table; p.kv_lens = kv_lens; p.q_starts = q_starts; p.cache = *cache;
     p.part = static_cast<float *>(scratch);
     p.part_ml = reinterpret_cast<float2 *>(p.part + partial_slots(n_seqs, max_q_len, q_heads, plan.splits) * cache->head_dim);
