@@ -158,6 +158,18 @@ __device__ __forceinline__ bool not_finite(int w) {
     return (w & kTop) == kTop || (w >> 16 & kTop) == kTop;
 }
 
+// The word with such elements cleared.
+template <int KV>
+__device__ __forceinline__ int finite_part(int w) {
+    const uint32_t u = static_cast<uint32_t>(w);
+    if constexpr (KV == Q8MI_KV_E4M3) {
+        const uint32_t odd = ((u & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;   // bit 7 of every such byte
+        return static_cast<int>(u & ~(odd | (odd - (odd >> 7))));
+    }
+    constexpr uint32_t kTop = KV == Q8MI_KV_BF16 ? 0x7f80 : 0x7c00;
+    return static_cast<int>(((u & kTop) == kTop ? 0 : u & 0xffffu) | ((u >> 16 & kTop) == kTop ? 0 : u & 0xffff0000u));
+}
+
 __device__ __forceinline__ float rows_max(float v) {   // over the four lanes that hold a query row
     v = fmaxf(v, lane_xor<16>(v));
     return fmaxf(v, lane_xor<32>(v));
@@ -185,7 +197,7 @@ struct Layout {
 };
 
 template <uint32_t D, int KV, uint32_t WR>
-__global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParams p) {
+__global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 1024 ? 2 : 1)) void attention_kernel(const AttnParams p) {
     using L = Layout<D, KV, WR>;
     using Op = Operand<KV>;
     constexpr uint32_t kSteps = D / 32, kOuts = D / 16;
@@ -219,13 +231,13 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
     const int32_t last = !live || last64 < 0 ? -1 : last64 >= p.max_kv_len ? static_cast<int32_t>(p.max_kv_len) - 1
                                                                            : static_cast<int32_t>(last64);
 
-    // queries and page ids, requested together
+    // queries and page ids, requested together (lanes without a row read row 0: what they compute goes nowhere)
     float qv[kSteps][8];
     if (p.q_is_bf16) {
-        const uint16_t *src = static_cast<const uint16_t *>(p.q) + (live ? static_cast<uint64_t>(q_row) * p.stride_q + head * D + g * 8 : 0);
+        const uint16_t *src = static_cast<const uint16_t *>(p.q) + (live ? static_cast<uint64_t>(q_row) * p.stride_q : 0) + head * D + g * 8;
 #pragma unroll
         for (uint32_t j = 0; j < kSteps; ++j) {
-            const v4i w = live ? *reinterpret_cast<const v4i *>(src + j * 32) : v4i{0, 0, 0, 0};
+            const v4i w = *reinterpret_cast<const v4i *>(src + j * 32);
             const int ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -234,11 +246,11 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
             }
         }
     } else {
-        const float *src = static_cast<const float *>(p.q) + (live ? static_cast<uint64_t>(q_row) * p.stride_q + head * D + g * 8 : 0);
+        const float *src = static_cast<const float *>(p.q) + (live ? static_cast<uint64_t>(q_row) * p.stride_q : 0) + head * D + g * 8;
 #pragma unroll
         for (uint32_t j = 0; j < kSteps; ++j) {
-            const v4f a = live ? *reinterpret_cast<const v4f *>(src + j * 32) : v4f{0, 0, 0, 0};
-            const v4f b = live ? *reinterpret_cast<const v4f *>(src + j * 32 + 4) : v4f{0, 0, 0, 0};
+            const v4f a = *reinterpret_cast<const v4f *>(src + j * 32);
+            const v4f b = *reinterpret_cast<const v4f *>(src + j * 32 + 4);
             qv[j][0] = a.x; qv[j][1] = a.y; qv[j][2] = a.z; qv[j][3] = a.w;
             qv[j][4] = b.x; qv[j][5] = b.y; qv[j][6] = b.z; qv[j][7] = b.w;
         }
@@ -298,19 +310,33 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
         const int32_t id = pages[pg - page0];
         return id < 0 ? 0 : static_cast<uint32_t>(id) * p.unit_page + (t - pg * p.cache.page_size) * p.unit_token;
     };
-    const uint32_t piece0 = lane % L::kLanesPerRow ^ (lane / L::kLanesPerRow & L::kSwizzle);
+    uint32_t piece0 = lane % L::kLanesPerRow ^ (lane / L::kLanesPerRow & L::kSwizzle), source0 = lane / L::kLanesPerRow * 4;
     auto load_tile = [&](const uint8_t *pool, uint32_t tile, uint32_t where) {
+        asm volatile("" : "+v"(piece0), "+v"(source0));   // their sixteen variants are made anew, not held in registers
 #pragma unroll
         for (uint32_t u = 0; u < L::kLoadsPerWave; ++u) {
             const uint32_t r = u * WR + wr;
             if (L::kLoads < WR && r >= L::kLoads) break;   // uniform
             const uint32_t slot0 = r * L::kRowsPerLoad;
             const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(
-                static_cast<int>((slot0 + lane / L::kLanesPerRow) * 4), static_cast<int>(where)));
+                static_cast<int>(source0 + slot0 * 4), static_cast<int>(where)));
             const uint64_t off = static_cast<uint64_t>(at) + (piece0 ^ (slot0 & L::kSwizzle));
             dma16_lanes(pool + off * 16, lds0 + tile + r * 1024);
+            if (u % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // addresses of four transfers at a time, not of sixteen
         }
     };
+
+    // Where this lane reads its operands: piece c of a row lies at c ^ (token & kSwizzle), and c = (step or tile of
+    // outputs) * 4, 2 or 1 | (lane part), so that one exclusive or with the first part gives every address.
+    uint32_t k_at, v_at;
+    {
+        const uint32_t i = lane % 16;
+        const uint32_t k_piece = (KV == Q8MI_KV_E4M3 ? g / 2 : g) ^ (i & L::kSwizzle);
+        k_at = k_tile + i * L::kRowBytes + k_piece * 16 + (KV == Q8MI_KV_E4M3 ? g % 2 * 8 : 0);
+        const uint32_t v_token = KV == Q8MI_KV_E4M3 ? (i / 2 < 4 ? 0 : 12) + g * 4 + i / 2 : g * 4 + i / 4;
+        const uint32_t v_piece = (KV == Q8MI_KV_E4M3 ? 0 : i % 4 / 2) ^ (v_token & L::kSwizzle);
+        v_at = v_tile + v_token * L::kRowBytes + v_piece * 16 + i % 2 * 8;
+    }
 
     // ---- the walk over the chunk ----
     float m = -INFINITY, l = 0.0f;
@@ -331,27 +357,34 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
 
         wait_loads<L::kLoadsPerWave>();   // the keys are here, the values may still travel
         if constexpr (WR > 1) __syncthreads();
+        asm volatile("" : "+v"(k_at), "+v"(v_at));   // their variants are made anew each step: held, they cost 32 registers
         v4f s[2][Op::kTerms];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int k = 0; k < Op::kTerms; ++k) s[h][k] = v4f{0, 0, 0, 0};
+        // The operands of a step are read while the products of the step before run; the barriers keep the compiler from
+        // reading all of them ahead into registers that it does not have.
+        auto keys = [&](uint32_t j, uint32_t h) -> v8s {
+            if constexpr (KV == Q8MI_KV_E4M3)
+                return e4m3_to_f16(*reinterpret_cast<const v2i *>(lds + (k_at ^ j * 32) + h * 16 * L::kRowBytes));
+            else
+                return *reinterpret_cast<const v8s *>(lds + (k_at ^ j * 64) + h * 16 * L::kRowBytes);
+        };
+        v8s kf[2][2];
+        kf[0][0] = keys(0, 0);
+        kf[0][1] = keys(0, 1);
 #pragma unroll
         for (uint32_t j = 0; j < kSteps; ++j) {
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                const uint32_t key = h * 16 + lane % 16;
-                v8s kf;
-                if constexpr (KV == Q8MI_KV_E4M3) {
-                    const uint32_t piece = (j * 2 + g / 2) ^ (key & L::kSwizzle);
-                    kf = e4m3_to_f16(*reinterpret_cast<const v2i *>(lds + k_tile + key * L::kRowBytes + piece * 16 + g % 2 * 8));
-                } else {
-                    const uint32_t piece = (j * 4 + g) ^ (key & L::kSwizzle);
-                    kf = *reinterpret_cast<const v8s *>(lds + k_tile + key * L::kRowBytes + piece * 16);
-                }
-#pragma unroll
-                for (int k = 0; k < Op::kTerms; ++k) s[h][k] = Op::mma(kf, qf[j][k], s[h][k]);
+            if (j + 1 < kSteps) {
+                kf[(j + 1) % 2][0] = keys(j + 1, 0);
+                kf[(j + 1) % 2][1] = keys(j + 1, 1);
             }
+#pragma unroll
+            for (int k = 0; k < Op::kTerms; ++k)
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) s[h][k] = Op::mma(kf[j % 2][h], qf[j][k], s[h][k]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         wait_lds_reads();
         if constexpr (WR > 1) __syncthreads();
@@ -371,11 +404,13 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
                 for (int k = Op::kTerms - 2; k >= 0; --k) dot += s[h][k][i];
                 w[h * 4 + i] = dot * to_log2;
             }
+        uint32_t there = 0;   // not whole: bit i, token first + i exists
         if (!whole) {
+            there = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(visible(first + lane % kTile)));
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
-                const uint32_t t = first + i / 4 * 16 + g * 4 + i % 4;
-                if (!visible(t) || static_cast<int32_t>(t) > last) w[i] = -INFINITY;
+                const uint32_t slot = i / 4 * 16 + g * 4 + i % 4;
+                w[i] = (there >> slot & 1) && static_cast<int32_t>(first + slot) <= last ? w[i] : -INFINITY;
             }
         }
         float top = fmaxf(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7])));
@@ -404,67 +439,78 @@ __global__ __launch_bounds__(kAttnThreads) void attention_kernel(const AttnParam
         // group's lanes point to, here its tokens g * 4 .. + 3 and 16 + g * 4 .. + 3
         auto values = [&](uint32_t d) -> v8s {
             if constexpr (KV == Q8MI_KV_E4M3) {
-                const uint32_t i = lane % 16, r = i / 2, key = (r < 4 ? 0 : 12) + g * 4 + r;
-                const uint32_t piece = d ^ (key & L::kSwizzle);
                 using tp = __attribute__((address_space(3))) v2i *;
-                const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((tp)(lds + v_tile + key * L::kRowBytes + piece * 16 + i % 2 * 8));
-                return e4m3_to_f16(x);
+                return e4m3_to_f16(__builtin_amdgcn_ds_read_tr8_b64_v2i32((tp)(lds + (v_at ^ d * 16))));
             } else {
-                const uint32_t i = lane % 16, key = g * 4 + i / 4;
-                const uint32_t piece = (d * 2 + i % 4 / 2) ^ (key & L::kSwizzle);
                 using tp = __attribute__((address_space(3))) v4s *;
-                uint8_t *at = lds + v_tile + key * L::kRowBytes + piece * 16 + i % 2 * 8;
+                uint8_t *at = lds + (v_at ^ d * 32);
                 const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tp)at);
                 const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tp)(at + 16 * L::kRowBytes));
                 return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
             }
         };
-        bool apart = false;
         if (!whole) {
-            // What no row sees (rows behind the last token, tokens of a bad page) is cleared: a weight of 0 does not
-            // silence an infinity or NaN.  A new row's own token is seen by some rows only: where one of those holds
-            // such a value, every row of the sequence gets a pass of its own, below.
-            const uint32_t slot = lane % kTile, t = first + slot;
+            // A weight of 0 does not silence an infinity or NaN.  What no row sees (rows behind the last token, tokens of a
+            // bad page) is cleared; of a token that some rows see and others not, a new row's own, such elements are added
+            // here to the rows that see them, and cleared.
+            const uint32_t slot = lane % kTile;
             v4i *mine = reinterpret_cast<v4i *>(lds + v_tile + slot * L::kRowBytes + lane / kTile * (L::kRowBytes / 2));
+            const bool partly = static_cast<int64_t>(first) + slot > first_last;
             bool odd = false;
-            if (!visible(t)) {
+            if (!(there >> slot & 1)) {
                 for (uint32_t i = 0; i < L::kRowBytes / 32; ++i) mine[i] = v4i{0, 0, 0, 0};
-            } else if (static_cast<int64_t>(t) > first_last) {
+            } else if (partly) {
                 for (uint32_t i = 0; i < L::kRowBytes / 32; ++i) {
                     const v4i x = mine[i];
                     odd |= not_finite<KV>(x.x) || not_finite<KV>(x.y) || not_finite<KV>(x.z) || not_finite<KV>(x.w);
                 }
             }
-            if constexpr (WR > 1) apart = __syncthreads_or(odd);
-            else apart = __builtin_amdgcn_ballot_w64(odd) != 0;
-            wait_lds_reads();
-        }
-        if (!apart) {
+            uint64_t odd_lanes = __builtin_amdgcn_ballot_w64(odd);
+            uint32_t odd_slots = static_cast<uint32_t>(odd_lanes) | static_cast<uint32_t>(odd_lanes >> 32);
+            while (odd_slots != 0) {   // uniform
+                const uint32_t at = __builtin_ctz(odd_slots);
+                odd_slots &= odd_slots - 1;
+                float weight = 0.0f;   // of token first + at for this lane's row: register i of the lanes g = at / 4 % 4
 #pragma unroll
-            for (uint32_t d = 0; d < kOuts; ++d) {
-                const v8s vf = values(d);
-#pragma unroll
-                for (int k = Op::kTerms - 1; k >= 0; --k) o[d] = Op::mma(vf, pf[k], o[d]);
-            }
-        } else {
-            for (uint32_t pass = rows.used; pass-- > 0;) {   // the last row sees most; what the next one no longer sees is cleared
-                const uint32_t slot = lane % kTile;
-                if constexpr (WR > 1) __syncthreads();
-                if (static_cast<int64_t>(first) + slot > first_last + pass) {
-                    v4i *mine = reinterpret_cast<v4i *>(lds + v_tile + slot * L::kRowBytes + lane / kTile * (L::kRowBytes / 2));
-                    for (uint32_t i = 0; i < L::kRowBytes / 32; ++i) mine[i] = v4i{0, 0, 0, 0};
-                }
-                if constexpr (WR > 1) __syncthreads();
-                wait_lds_reads();
+                for (uint32_t i = 0; i < 8; ++i) weight = i == at / 16 * 4 + at % 4 ? w[i] : weight;
+                weight = as_f32(__builtin_amdgcn_ds_bpermute(static_cast<int>((at / 4 % 4 * 16 + lane % 16) * 4), as_i32(weight)));
+                const bool sees = static_cast<int64_t>(first) + at <= last;
 #pragma unroll
                 for (uint32_t d = 0; d < kOuts; ++d) {
-                    const v8s vf = values(d);
-                    v4f sum = v4f{0, 0, 0, 0};
 #pragma unroll
-                    for (int k = Op::kTerms - 1; k >= 0; --k) sum = Op::mma(vf, pf[k], sum);
-                    if (token == pass) o[d] += sum;
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const uint32_t e = d * 16 + g * 4 + i;   // element of the row
+                        const uint32_t byte = e * (KV == Q8MI_KV_E4M3 ? 1 : 2);
+                        const uint8_t *src = lds + v_tile + at * L::kRowBytes + (byte / 16 ^ (at & L::kSwizzle)) * 16 + byte % 16;
+                        const int raw = KV == Q8MI_KV_E4M3 ? *src : *reinterpret_cast<const uint16_t *>(src);
+                        // an infinity becomes one, NaN becomes NaN: fp32 with the sign and the fraction of the element
+                        const float v = KV == Q8MI_KV_BF16  ? as_f32(raw << 16)
+                                        : KV == Q8MI_KV_F16 ? half_bits_to_float(static_cast<uint16_t>(raw))
+                                                            : NAN;
+                        if (not_finite<KV>(raw) && sees) o[d][i] += weight * v;
+                    }
                 }
             }
+            if constexpr (WR > 1) __syncthreads();   // every wave has read what is cleared now
+            if (odd) {
+                for (uint32_t i = 0; i < L::kRowBytes / 32; ++i) {
+                    const v4i x = mine[i];
+                    mine[i] = v4i{finite_part<KV>(x.x), finite_part<KV>(x.y), finite_part<KV>(x.z), finite_part<KV>(x.w)};
+                }
+            }
+            if constexpr (WR > 1) __syncthreads();
+            wait_lds_reads();
+        }
+        constexpr uint32_t kAhead = D == 256 && KV == Q8MI_KV_BF16 ? 2 : 3;   // one fewer where registers are short
+        v8s vf[kAhead + 1];
+#pragma unroll
+        for (uint32_t d = 0; d < kAhead; ++d) vf[d] = values(d);
+#pragma unroll
+        for (uint32_t d = 0; d < kOuts; ++d) {
+            if (d + kAhead < kOuts) vf[(d + kAhead) % (kAhead + 1)] = values(d + kAhead);
+#pragma unroll
+            for (int k = Op::kTerms - 1; k >= 0; --k) o[d] = Op::mma(vf[d % (kAhead + 1)], pf[k], o[d]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         wait_lds_reads();
         if constexpr (WR > 1) __syncthreads();
