@@ -49,6 +49,7 @@ struct AttnParams {
     uint32_t chunk, splits, row_tiles;
     uint32_t page_magic, page_shift;   // t / page_size = mulhi(t, page_magic) >> page_shift; magic 0: page_size 1
     uint32_t unit_page, unit_token;    // cache strides in units of 16 bytes
+    int whole_loads;                   // the tokens of one transfer instruction never straddle pages
     float scale_log2;  // scale * log2(e) * k_scale
     int q_is_bf16, out_is_bf16;
 };
@@ -88,6 +89,17 @@ __device__ __forceinline__ void dma16_lanes(const void *lane_ptr, uint32_t lds_o
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_off), "v"(lane_ptr)
                  : "memory", "m0");
 }
+// The same from a scalar base plus a 32-bit offset per lane.
+__device__ __forceinline__ void dma16_base(const void *uniform_base, uint32_t lane_off, uint32_t lds_off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_off), "v"(lane_off), "s"(uniform_base)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ const uint8_t *uniform_ptr(const uint8_t *p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+    return reinterpret_cast<const uint8_t *>((static_cast<uint64_t>(hi) << 32) | lo);
+}
 template <int N>
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -101,6 +113,8 @@ template <int KV>
 struct Operand;   // how eight elements become a matrix operand, and fp32 values a sum of operands
 template <>
 struct Operand<Q8MI_KV_BF16> {
+    using Raw = v8s;
+    static __device__ __forceinline__ v8s operand(Raw x) { return x; }
     static constexpr int kTerms = 3;
     static constexpr float kWeightScale = 1.0f;
     static __device__ __forceinline__ v4f mma(v8s a, v8s b, v4f c) {
@@ -122,6 +136,8 @@ struct Operand<Q8MI_KV_BF16> {
 };
 template <>
 struct Operand<Q8MI_KV_F16> {
+    using Raw = v8s;
+    static __device__ __forceinline__ v8s operand(Raw x) { return x; }
     static constexpr int kTerms = 2;
     static constexpr float kWeightScale = 16384.0f;   // weights are at most 1: the second term ends at 2^-38
     static __device__ __forceinline__ v4f mma(v8s a, v8s b, v4f c) {
@@ -138,16 +154,17 @@ struct Operand<Q8MI_KV_F16> {
     }
 };
 template <>
-struct Operand<Q8MI_KV_E4M3> : Operand<Q8MI_KV_F16> {};
-
-__device__ __forceinline__ v8s e4m3_to_f16(v2i w) {   // exact: every e4m3 value is an fp16
-    union { v2h h[4]; v8s s; } u;
-    u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.x, 1.0f, false);
-    u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.x, 1.0f, true);
-    u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, 1.0f, false);
-    u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, 1.0f, true);
-    return u.s;
-}
+struct Operand<Q8MI_KV_E4M3> : Operand<Q8MI_KV_F16> {
+    using Raw = v2i;
+    static __device__ __forceinline__ v8s operand(Raw w) {   // exact: every e4m3 value is an fp16
+        union { v2h h[4]; v8s s; } u;
+        u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.x, 1.0f, false);
+        u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.x, 1.0f, true);
+        u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, 1.0f, false);
+        u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, 1.0f, true);
+        return u.s;
+    }
+};
 
 // Whether one of the elements in a word is an infinity or NaN.
 template <int KV>
@@ -201,6 +218,9 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     using L = Layout<D, KV, WR>;
     using Op = Operand<KV>;
     constexpr uint32_t kSteps = D / 32, kOuts = D / 16;
+    // steps that LDS reads run ahead of the products: fewer where registers are short
+    constexpr uint32_t kKeysAhead = D == 256 && KV == Q8MI_KV_BF16 && WR > 1 ? 1 : 2;
+    constexpr uint32_t kBlock = D == 256 && KV == Q8MI_KV_BF16 && WR > 1 ? 2 : 4;   // tiles of outputs worked on in turn
     extern __shared__ __align__(16) uint8_t lds[];
     int32_t *pages = reinterpret_cast<int32_t *>(lds + L::kPages);
 
@@ -209,8 +229,14 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     const uint32_t wr = wave % WR, wg = wave / WR;
     const uint32_t split = blockIdx.y;
     const uint32_t row_tile = blockIdx.x % p.row_tiles;
-    const uint32_t kv_head = blockIdx.x / p.row_tiles % p.cache.kv_heads;
-    const uint32_t seq = blockIdx.x / p.row_tiles / p.cache.kv_heads;
+    const uint32_t kv_head = __builtin_amdgcn_readfirstlane(blockIdx.x / p.row_tiles % p.cache.kv_heads);
+    const uint32_t seq = __builtin_amdgcn_readfirstlane(blockIdx.x / p.row_tiles / p.cache.kv_heads);
+
+    // a thread's first page id, asked for before the sequence's length is known: the table reaches max_kv_len
+    const uint32_t t0 = split * p.chunk;                                       // the chunk: tokens t0 .. t1 - 1
+    const uint32_t page0 = page_of(p, t0);
+    const int32_t *table = p.page_table + static_cast<uint64_t>(seq) * p.stride_page_table;
+    const int32_t id0 = static_cast<uint64_t>(page0 + threadIdx.x) * p.cache.page_size < p.max_kv_len ? table[page0 + threadIdx.x] : -1;
 
     const Rows rows = rows_of(p, seq);
     const uint32_t used_splits = (rows.tokens + p.chunk - 1) / p.chunk;
@@ -219,7 +245,6 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     const uint32_t row0 = row_tile * (WR * kRowTile);
     if (row0 >= n_rows) return;
 
-    const uint32_t t0 = split * p.chunk;                                       // the chunk: tokens t0 .. t1 - 1
     const uint32_t t1 = t0 + p.chunk < rows.tokens ? t0 + p.chunk : rows.tokens;
 
     // this lane's query row
@@ -231,68 +256,31 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     const int32_t last = !live || last64 < 0 ? -1 : last64 >= p.max_kv_len ? static_cast<int32_t>(p.max_kv_len) - 1
                                                                            : static_cast<int32_t>(last64);
 
-    // queries and page ids, requested together (lanes without a row read row 0: what they compute goes nowhere)
-    float qv[kSteps][8];
+    // the queries' bits (lanes without a row read row 0: what they compute goes nowhere)
+    v4i raw[kSteps][2] = {};
     if (p.q_is_bf16) {
         const uint16_t *src = static_cast<const uint16_t *>(p.q) + (live ? static_cast<uint64_t>(q_row) * p.stride_q : 0) + head * D + g * 8;
 #pragma unroll
-        for (uint32_t j = 0; j < kSteps; ++j) {
-            const v4i w = *reinterpret_cast<const v4i *>(src + j * 32);
-            const int ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                qv[j][2 * i] = as_f32(ws[i] << 16);
-                qv[j][2 * i + 1] = as_f32(ws[i] & static_cast<int>(0xffff0000u));
-            }
-        }
+        for (uint32_t j = 0; j < kSteps; ++j) raw[j][0] = *reinterpret_cast<const v4i *>(src + j * 32);
     } else {
         const float *src = static_cast<const float *>(p.q) + (live ? static_cast<uint64_t>(q_row) * p.stride_q : 0) + head * D + g * 8;
 #pragma unroll
         for (uint32_t j = 0; j < kSteps; ++j) {
-            const v4f a = *reinterpret_cast<const v4f *>(src + j * 32);
-            const v4f b = *reinterpret_cast<const v4f *>(src + j * 32 + 4);
-            qv[j][0] = a.x; qv[j][1] = a.y; qv[j][2] = a.z; qv[j][3] = a.w;
-            qv[j][4] = b.x; qv[j][5] = b.y; qv[j][6] = b.z; qv[j][7] = b.w;
+            raw[j][0] = *reinterpret_cast<const v4i *>(src + j * 32);
+            raw[j][1] = *reinterpret_cast<const v4i *>(src + j * 32 + 4);
         }
     }
-    const uint32_t page0 = t0 / p.cache.page_size;
-    const uint32_t n_pages = t1 > t0 ? (t1 - 1) / p.cache.page_size - page0 + 1 : 0;
+    const uint32_t n_pages = t1 > t0 ? page_of(p, t1 - 1) - page0 + 1 : 0;
     bool bad = false;
     for (uint32_t i = threadIdx.x; i < n_pages; i += kAttnThreads) {
-        const int32_t id = p.page_table[static_cast<uint64_t>(seq) * p.stride_page_table + page0 + i];
+        const int32_t id = i == threadIdx.x ? id0 : table[page0 + i];
         const bool ok = id >= 0 && static_cast<uint32_t>(id) < p.cache.pages;
         pages[i] = ok ? id : -1;
         bad |= !ok;
     }
+    // Everything requested so far is here before the first tile is asked for: a later wait for it would wait for the tile.
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
     const bool any_bad = __syncthreads_or(bad);
-
-    // fp16 operands: the row's largest |q| goes to 2^13 .. 2^14
-    float row_scale = 1.0f;
-    if constexpr (KV != Q8MI_KV_BF16) {
-        float top = 0.0f;
-#pragma unroll
-        for (uint32_t j = 0; j < kSteps; ++j)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(qv[j][i]));
-        top = rows_max(top);
-        int e = 0;
-        if (top > 0.0f && top < INFINITY) {
-            (void)frexpf(top, &e);
-            e = 14 - e;
-            e = e > 100 ? 100 : e;
-        }
-        row_scale = ldexpf(1.0f, e);
-    }
-    v8s qf[kSteps][Op::kTerms];
-#pragma unroll
-    for (uint32_t j = 0; j < kSteps; ++j) {
-        if constexpr (KV != Q8MI_KV_BF16) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) qv[j][i] *= row_scale;
-        }
-        Op::split(qv[j], qf[j]);
-    }
-    const float to_log2 = p.scale_log2 / row_scale;
 
     // ---- the tiles' way into LDS ----
     const uint32_t k_tile = L::kTiles + wg * 2 * L::kTileBytes, v_tile = k_tile + L::kTileBytes;
@@ -310,16 +298,29 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
         const int32_t id = pages[pg - page0];
         return id < 0 ? 0 : static_cast<uint32_t>(id) * p.unit_page + (t - pg * p.cache.page_size) * p.unit_token;
     };
-    uint32_t piece0 = lane % L::kLanesPerRow ^ (lane / L::kLanesPerRow & L::kSwizzle), source0 = lane / L::kLanesPerRow * 4;
+    uint32_t piece0 = lane % L::kLanesPerRow ^ (lane / L::kLanesPerRow & L::kSwizzle);
+    const uint32_t rows_off = lane / L::kLanesPerRow * p.unit_token * 16;   // used where p.whole_loads: below 4 GiB
     auto load_tile = [&](const uint8_t *pool, uint32_t tile, uint32_t where) {
-        asm volatile("" : "+v"(piece0), "+v"(source0));   // their sixteen variants are made anew, not held in registers
+        asm volatile("" : "+v"(piece0));   // its variants are made anew, not held in registers
+        if (p.whole_loads) {
+            // a transfer's tokens are neighbours in one page: a scalar base, and what the lanes add never changes
+#pragma unroll
+            for (uint32_t u = 0; u < L::kLoadsPerWave; ++u) {
+                const uint32_t r = u * WR + wr;
+                if (L::kLoads < WR && r >= L::kLoads) break;   // uniform
+                const uint32_t slot0 = r * L::kRowsPerLoad;
+                const uint64_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(where), static_cast<int>(slot0)));
+                dma16_base(uniform_ptr(pool + at * 16), rows_off + (piece0 ^ (slot0 & L::kSwizzle)) * 16, lds0 + tile + r * 1024);
+            }
+            return;
+        }
 #pragma unroll
         for (uint32_t u = 0; u < L::kLoadsPerWave; ++u) {
             const uint32_t r = u * WR + wr;
             if (L::kLoads < WR && r >= L::kLoads) break;   // uniform
             const uint32_t slot0 = r * L::kRowsPerLoad;
             const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(
-                static_cast<int>(source0 + slot0 * 4), static_cast<int>(where)));
+                static_cast<int>((lane / L::kLanesPerRow + slot0) * 4), static_cast<int>(where)));
             const uint64_t off = static_cast<uint64_t>(at) + (piece0 ^ (slot0 & L::kSwizzle));
             dma16_lanes(pool + off * 16, lds0 + tile + r * 1024);
             if (u % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // addresses of four transfers at a time, not of sixteen
@@ -350,6 +351,44 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
         load_tile(k_pool, k_tile, where);
         load_tile(v_pool, v_tile, where);
     }
+    __builtin_amdgcn_sched_barrier(0);
+
+    // the queries as operands, while the first tiles travel
+    float qv[kSteps][8];
+#pragma unroll
+    for (uint32_t j = 0; j < kSteps; ++j) {
+        const int ws[8] = {raw[j][0].x, raw[j][0].y, raw[j][0].z, raw[j][0].w, raw[j][1].x, raw[j][1].y, raw[j][1].z, raw[j][1].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            qv[j][i] = as_f32(!p.q_is_bf16 ? ws[i] : i % 2 ? ws[i / 2] & static_cast<int>(0xffff0000u) : ws[i / 2] << 16);
+    }
+    float row_scale = 1.0f;   // fp16 operands: the row's largest |q| goes to 2^13 .. 2^14
+    if constexpr (KV != Q8MI_KV_BF16) {
+        float top = 0.0f;
+#pragma unroll
+        for (uint32_t j = 0; j < kSteps; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(qv[j][i]));
+        top = rows_max(top);
+        int e = 0;
+        if (top > 0.0f && top < INFINITY) {
+            (void)frexpf(top, &e);
+            e = 14 - e;
+            e = e > 100 ? 100 : e;
+        }
+        row_scale = ldexpf(1.0f, e);
+    }
+    v8s qf[kSteps][Op::kTerms];
+#pragma unroll
+    for (uint32_t j = 0; j < kSteps; ++j) {
+        if constexpr (KV != Q8MI_KV_BF16) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) qv[j][i] *= row_scale;
+        }
+        Op::split(qv[j], qf[j]);
+    }
+    const float to_log2 = p.scale_log2 / row_scale;
+
     for (uint32_t step = 0; step < n_steps; ++step) {
         const uint32_t first = t0 + (step * L::kGroups + wg) * kTile;
         const uint32_t next = locate(first + L::kGroups * kTile);
@@ -365,25 +404,26 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
             for (int k = 0; k < Op::kTerms; ++k) s[h][k] = v4f{0, 0, 0, 0};
         // The operands of a step are read while the products of the step before run; the barriers keep the compiler from
         // reading all of them ahead into registers that it does not have.
-        auto keys = [&](uint32_t j, uint32_t h) -> v8s {
-            if constexpr (KV == Q8MI_KV_E4M3)
-                return e4m3_to_f16(*reinterpret_cast<const v2i *>(lds + (k_at ^ j * 32) + h * 16 * L::kRowBytes));
-            else
-                return *reinterpret_cast<const v8s *>(lds + (k_at ^ j * 64) + h * 16 * L::kRowBytes);
+        auto keys = [&](uint32_t j, uint32_t h) {
+            return *reinterpret_cast<const typename Op::Raw *>(lds + (k_at ^ j * (KV == Q8MI_KV_E4M3 ? 32 : 64)) + h * 16 * L::kRowBytes);
         };
-        v8s kf[2][2];
-        kf[0][0] = keys(0, 0);
-        kf[0][1] = keys(0, 1);
+        typename Op::Raw kf[kKeysAhead + 1][2];
+#pragma unroll
+        for (uint32_t j = 0; j < kKeysAhead; ++j) {
+            kf[j][0] = keys(j, 0);
+            kf[j][1] = keys(j, 1);
+        }
 #pragma unroll
         for (uint32_t j = 0; j < kSteps; ++j) {
-            if (j + 1 < kSteps) {
-                kf[(j + 1) % 2][0] = keys(j + 1, 0);
-                kf[(j + 1) % 2][1] = keys(j + 1, 1);
+            if (j + kKeysAhead < kSteps) {
+                kf[(j + kKeysAhead) % (kKeysAhead + 1)][0] = keys(j + kKeysAhead, 0);
+                kf[(j + kKeysAhead) % (kKeysAhead + 1)][1] = keys(j + kKeysAhead, 1);
             }
+            const v8s a[2] = {Op::operand(kf[j % (kKeysAhead + 1)][0]), Op::operand(kf[j % (kKeysAhead + 1)][1])};
 #pragma unroll
             for (int k = 0; k < Op::kTerms; ++k)
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) s[h][k] = Op::mma(kf[j % 2][h], qf[j][k], s[h][k]);
+                for (uint32_t h = 0; h < 2; ++h) s[h][k] = Op::mma(a[h], qf[j][k], s[h][k]);
             __builtin_amdgcn_sched_barrier(0);
         }
         wait_lds_reads();
@@ -414,8 +454,8 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
             }
         }
         float top = fmaxf(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7])));
-        top = fmaxf(rows_max(top), m);
-        if (__builtin_amdgcn_ballot_w64(top != m) != 0) {   // uniform; NaN scores leave the maximum as it is
+        if (__builtin_amdgcn_ballot_w64(top > m) != 0) {   // uniform, and rare after the first tiles; NaN changes no maximum
+            top = fmaxf(rows_max(top), m);
             const float keep = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
             l *= keep;
 #pragma unroll
@@ -437,10 +477,10 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
         if constexpr (WR > 1) __syncthreads();
         // V^T operand of 16 outputs: the transposing read gives lane i of a group of 16 column i of the rows that the
         // group's lanes point to, here its tokens g * 4 .. + 3 and 16 + g * 4 .. + 3
-        auto values = [&](uint32_t d) -> v8s {
+        auto values = [&](uint32_t d) -> typename Op::Raw {
             if constexpr (KV == Q8MI_KV_E4M3) {
                 using tp = __attribute__((address_space(3))) v2i *;
-                return e4m3_to_f16(__builtin_amdgcn_ds_read_tr8_b64_v2i32((tp)(lds + (v_at ^ d * 16))));
+                return __builtin_amdgcn_ds_read_tr8_b64_v2i32((tp)(lds + (v_at ^ d * 16)));
             } else {
                 using tp = __attribute__((address_space(3))) v4s *;
                 uint8_t *at = lds + (v_at ^ d * 32);
@@ -501,15 +541,23 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
             if constexpr (WR > 1) __syncthreads();
             wait_lds_reads();
         }
-        constexpr uint32_t kAhead = D == 256 && KV == Q8MI_KV_BF16 ? 2 : 3;   // one fewer where registers are short
-        v8s vf[kAhead + 1];
+        // kBlock accumulators in turn, so that a product does not wait for the one before it
+        typename Op::Raw vf[2][kBlock];
 #pragma unroll
-        for (uint32_t d = 0; d < kAhead; ++d) vf[d] = values(d);
+        for (uint32_t d = 0; d < kBlock; ++d) vf[0][d] = values(d);
 #pragma unroll
-        for (uint32_t d = 0; d < kOuts; ++d) {
-            if (d + kAhead < kOuts) vf[(d + kAhead) % (kAhead + 1)] = values(d + kAhead);
+        for (uint32_t b = 0; b < kOuts / kBlock; ++b) {
+            if ((b + 1) * kBlock < kOuts) {
 #pragma unroll
-            for (int k = Op::kTerms - 1; k >= 0; --k) o[d] = Op::mma(vf[d % (kAhead + 1)], pf[k], o[d]);
+                for (uint32_t d = 0; d < kBlock; ++d) vf[(b + 1) % 2][d] = values((b + 1) * kBlock + d);
+            }
+            v8s a[kBlock];
+#pragma unroll
+            for (uint32_t d = 0; d < kBlock; ++d) a[d] = Op::operand(vf[b % 2][d]);
+#pragma unroll
+            for (int k = Op::kTerms - 1; k >= 0; --k)
+#pragma unroll
+                for (uint32_t d = 0; d < kBlock; ++d) o[b * kBlock + d] = Op::mma(a[d], pf[k], o[b * kBlock + d]);
             __builtin_amdgcn_sched_barrier(0);
         }
         wait_lds_reads();
@@ -637,8 +685,9 @@ Plan plan_of(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_
 }
 
 template <uint32_t D, int KV, uint32_t WR>
-int launch_waves(const AttnParams &p, hipStream_t s) {
+int launch_waves(AttnParams &p, hipStream_t s) {
     using L = Layout<D, KV, WR>;
+    p.whole_loads = p.cache.page_size % L::kRowsPerLoad == 0 && static_cast<uint64_t>(L::kRowsPerLoad) * p.unit_token < 1u << 28;
     if (L::kBytes > 64 * 1024) {
         // more than the default grant: asked for once per instantiation and device
         static thread_local int granted = -1;
@@ -656,13 +705,13 @@ int launch_waves(const AttnParams &p, hipStream_t s) {
     return check_launch("paged_attention");
 }
 template <uint32_t D, int KV>
-int launch_dim(const AttnParams &p, uint32_t waves_on_rows, hipStream_t s) {
+int launch_dim(AttnParams &p, uint32_t waves_on_rows, hipStream_t s) {
     if (waves_on_rows == 1) return launch_waves<D, KV, 1>(p, s);
     if (waves_on_rows == 2) return launch_waves<D, KV, 2>(p, s);
     return launch_waves<D, KV, 4>(p, s);
 }
 template <int KV>
-int launch_type(const AttnParams &p, uint32_t waves_on_rows, hipStream_t s) {
+int launch_type(AttnParams &p, uint32_t waves_on_rows, hipStream_t s) {
     if (p.cache.head_dim == 64) return launch_dim<64, KV>(p, waves_on_rows, s);
     if (p.cache.head_dim == 128) return launch_dim<128, KV>(p, waves_on_rows, s);
     return launch_dim<256, KV>(p, waves_on_rows, s);
