@@ -210,7 +210,9 @@ struct Layout {
     static constexpr uint32_t kTiles = 0;                              // [group][K, V][tile]
     static constexpr uint32_t kPages = kGroups * 2 * kTileBytes;       // page ids of the chunk
     static constexpr uint32_t kMergeBytes = kGroups > 1 ? 4 * kRowTile * (D + 4) * 4 + 4 * kRowTile * 8 : 0;
-    static constexpr uint32_t kBytes = kPages + (kMaxChunk + 2) * 4 > kMergeBytes ? kPages + (kMaxChunk + 2) * 4 : kMergeBytes;
+    static constexpr uint32_t kScores = kPages + (kMaxChunk + 2) * 4;  // [wave][new row's token][row of the wave]
+    static constexpr uint32_t kEnd = kScores + 4 * kMaxRows * kRowTile * 4;
+    static constexpr uint32_t kBytes = kEnd > kMergeBytes ? kEnd : kMergeBytes;
 };
 
 template <uint32_t D, int KV, uint32_t WR>
@@ -223,6 +225,7 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     constexpr uint32_t kBlock = D == 256 && KV == Q8MI_KV_BF16 && WR > 1 ? 2 : 4;   // tiles of outputs worked on in turn
     extern __shared__ __align__(16) uint8_t lds[];
     int32_t *pages = reinterpret_cast<int32_t *>(lds + L::kPages);
+    float *kept_scores = reinterpret_cast<float *>(lds + L::kScores);
 
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -286,8 +289,8 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     const uint32_t k_tile = L::kTiles + wg * 2 * L::kTileBytes, v_tile = k_tile + L::kTileBytes;
     const uint32_t lds0 = lds_offset(lds);
     const uint64_t head_bytes = kv_head * p.cache.stride_head * kv_element_bytes(p.cache.dtype);
-    const uint8_t *k_pool = static_cast<const uint8_t *>(p.cache.k) + head_bytes;
-    const uint8_t *v_pool = static_cast<const uint8_t *>(p.cache.v) + head_bytes;
+    const uint8_t *k_pool = uniform_ptr(static_cast<const uint8_t *>(p.cache.k) + head_bytes);
+    const uint8_t *v_pool = uniform_ptr(static_cast<const uint8_t *>(p.cache.v) + head_bytes);
     auto page_id = [&](uint32_t t) { return pages[page_of(p, t) - page0]; };   // t0 <= t < t1
     auto visible = [&](uint32_t t) { return t < t1 && page_id(t) >= 0; };
     // Where token first + lane % 32 lies, in units of 16 bytes; tokens that do not exist read the pool's first row.
@@ -302,19 +305,20 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     const uint32_t rows_off = lane / L::kLanesPerRow * p.unit_token * 16;   // used where p.whole_loads: below 4 GiB
     auto load_tile = [&](const uint8_t *pool, uint32_t tile, uint32_t where) {
         asm volatile("" : "+v"(piece0));   // its variants are made anew, not held in registers
+        constexpr uint32_t kUnroll = L::kLoadsPerWave < 4 ? L::kLoadsPerWave : 4;   // of up to 16: code has to be fetched, too
         if (p.whole_loads) {
             // a transfer's tokens are neighbours in one page: a scalar base, and what the lanes add never changes
-#pragma unroll
+#pragma unroll kUnroll
             for (uint32_t u = 0; u < L::kLoadsPerWave; ++u) {
                 const uint32_t r = u * WR + wr;
                 if (L::kLoads < WR && r >= L::kLoads) break;   // uniform
                 const uint32_t slot0 = r * L::kRowsPerLoad;
                 const uint64_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(where), static_cast<int>(slot0)));
-                dma16_base(uniform_ptr(pool + at * 16), rows_off + (piece0 ^ (slot0 & L::kSwizzle)) * 16, lds0 + tile + r * 1024);
+                dma16_base(pool + at * 16, rows_off + (piece0 ^ (slot0 & L::kSwizzle)) * 16, lds0 + tile + r * 1024);
             }
             return;
         }
-#pragma unroll
+#pragma unroll kUnroll
         for (uint32_t u = 0; u < L::kLoadsPerWave; ++u) {
             const uint32_t r = u * WR + wr;
             if (L::kLoads < WR && r >= L::kLoads) break;   // uniform
@@ -323,7 +327,6 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
                 static_cast<int>((lane / L::kLanesPerRow + slot0) * 4), static_cast<int>(where)));
             const uint64_t off = static_cast<uint64_t>(at) + (piece0 ^ (slot0 & L::kSwizzle));
             dma16_lanes(pool + off * 16, lds0 + tile + r * 1024);
-            if (u % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // addresses of four transfers at a time, not of sixteen
         }
     };
 
@@ -345,6 +348,7 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
 #pragma unroll
     for (uint32_t d = 0; d < kOuts; ++d) o[d] = v4f{0, 0, 0, 0};
     const int64_t first_last = rows.kv_len - rows.count;   // what row 0 of the sequence sees last
+    uint32_t odd_tokens = 0;                               // bit i: token first_last + 1 + i holds values that are not finite
     const uint32_t n_steps = t1 > t0 ? (t1 - t0 + L::kGroups * kTile - 1) / (L::kGroups * kTile) : 0;
     if (n_steps) {
         const uint32_t where = locate(t0 + wg * kTile);
@@ -463,6 +467,9 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
             m = top;
         }
         const float base = m == -INFINITY ? 0.0f : m;
+        float scores[8];   // dead but for the rare tokens kept below
+#pragma unroll
+        for (int i = 0; i < 8; ++i) scores[i] = w[i];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             w[i] = __builtin_amdgcn_exp2f(w[i] - base);
@@ -491,8 +498,8 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
         };
         if (!whole) {
             // A weight of 0 does not silence an infinity or NaN.  What no row sees (rows behind the last token, tokens of a
-            // bad page) is cleared; of a token that some rows see and others not, a new row's own, such elements are added
-            // here to the rows that see them, and cleared.
+            // bad page) is cleared; of a token that some rows see and others not, a new row's own, such elements are cleared
+            // here and added behind the loop to the rows that see them.
             const uint32_t slot = lane % kTile;
             v4i *mine = reinterpret_cast<v4i *>(lds + v_tile + slot * L::kRowBytes + lane / kTile * (L::kRowBytes / 2));
             const bool partly = static_cast<int64_t>(first) + slot > first_last;
@@ -505,31 +512,17 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
                     odd |= not_finite<KV>(x.x) || not_finite<KV>(x.y) || not_finite<KV>(x.z) || not_finite<KV>(x.w);
                 }
             }
-            uint64_t odd_lanes = __builtin_amdgcn_ballot_w64(odd);
-            uint32_t odd_slots = static_cast<uint32_t>(odd_lanes) | static_cast<uint32_t>(odd_lanes >> 32);
-            while (odd_slots != 0) {   // uniform
-                const uint32_t at = __builtin_ctz(odd_slots);
-                odd_slots &= odd_slots - 1;
-                float weight = 0.0f;   // of token first + at for this lane's row: register i of the lanes g = at / 4 % 4
+            const uint64_t odd_lanes = __builtin_amdgcn_ballot_w64(odd);
+            for (uint32_t slots = static_cast<uint32_t>(odd_lanes) | static_cast<uint32_t>(odd_lanes >> 32); slots != 0; slots &= slots - 1) {
+                const uint32_t at = __builtin_ctz(slots);   // token first + at, new row number
+                const uint32_t number = static_cast<uint32_t>(static_cast<int64_t>(first) + at - first_last) - 1;
+                if (g == at / 4 % 4) {
+                    float score = -INFINITY;   // register i of these lanes
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) weight = i == at / 16 * 4 + at % 4 ? w[i] : weight;
-                weight = as_f32(__builtin_amdgcn_ds_bpermute(static_cast<int>((at / 4 % 4 * 16 + lane % 16) * 4), as_i32(weight)));
-                const bool sees = static_cast<int64_t>(first) + at <= last;
-#pragma unroll
-                for (uint32_t d = 0; d < kOuts; ++d) {
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const uint32_t e = d * 16 + g * 4 + i;   // element of the row
-                        const uint32_t byte = e * (KV == Q8MI_KV_E4M3 ? 1 : 2);
-                        const uint8_t *src = lds + v_tile + at * L::kRowBytes + (byte / 16 ^ (at & L::kSwizzle)) * 16 + byte % 16;
-                        const int raw = KV == Q8MI_KV_E4M3 ? *src : *reinterpret_cast<const uint16_t *>(src);
-                        // an infinity becomes one, NaN becomes NaN: fp32 with the sign and the fraction of the element
-                        const float v = KV == Q8MI_KV_BF16  ? as_f32(raw << 16)
-                                        : KV == Q8MI_KV_F16 ? half_bits_to_float(static_cast<uint16_t>(raw))
-                                                            : NAN;
-                        if (not_finite<KV>(raw) && sees) o[d][i] += weight * v;
-                    }
+                    for (uint32_t i = 0; i < 8; ++i) score = i == at / 16 * 4 + at % 4 ? scores[i] : score;
+                    kept_scores[(wave * kMaxRows + number) * kRowTile + lane % 16] = score;
                 }
+                odd_tokens |= 1u << number;
             }
             if constexpr (WR > 1) __syncthreads();   // every wave has read what is cleared now
             if (odd) {
@@ -565,6 +558,25 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
         if (more) load_tile(v_pool, v_tile, next);
     }
     l = rows_sum(l);
+    while (odd_tokens != 0) {   // uniform; see above
+        const uint32_t number = __builtin_ctz(odd_tokens);
+        odd_tokens &= odd_tokens - 1;
+        const uint32_t t = static_cast<uint32_t>(first_last + 1 + number);
+        const float weight = Op::kWeightScale * __builtin_amdgcn_exp2f(kept_scores[(wave * kMaxRows + number) * kRowTile + lane % 16] - m);
+        const bool sees = static_cast<int32_t>(t) <= last;
+        const uint32_t pg = page_of(p, t);
+        const uint64_t at = static_cast<uint64_t>(pages[pg - page0]) * p.unit_page + static_cast<uint64_t>(t - pg * p.cache.page_size) * p.unit_token;
+#pragma unroll
+        for (uint32_t d = 0; d < kOuts; ++d) {
+            const uint8_t *src = v_pool + at * 16 + (d * 16 + g * 4) * (KV == Q8MI_KV_E4M3 ? 1 : 2);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const int bits = KV == Q8MI_KV_E4M3 ? src[i] : reinterpret_cast<const uint16_t *>(src)[i];
+                const float v = KV == Q8MI_KV_BF16 ? as_f32(bits << 16) : KV == Q8MI_KV_F16 ? half_bits_to_float(static_cast<uint16_t>(bits)) : NAN;
+                o[d][i] = sees && not_finite<KV>(bits) ? o[d][i] + weight * v : o[d][i];
+            }
+        }
+    }
 
     // ---- the groups of a workgroup meet ----
     if constexpr (L::kGroups > 1) {
