@@ -207,8 +207,11 @@ struct Layout {
     static constexpr uint32_t kSwizzle = (kLanesPerRow < 16 ? kLanesPerRow : 16) - 1;
     static constexpr uint32_t kTileBytes = kTile * kRowBytes;
     static constexpr uint32_t kGroups = 4 / WR;
-    static constexpr uint32_t kTiles = 0;                              // [group][K, V][tile]
-    static constexpr uint32_t kPages = kGroups * 2 * kTileBytes;       // page ids of the chunk
+    // Waves that share a tile meet at barriers: a second stage hides what a load takes longer than a step.  Waves on tiles of
+    // their own are hidden by each other and by the second workgroup of the CU, which a second stage would not leave room for.
+    static constexpr uint32_t kStages = WR > 1 && kGroups * 4 * kTileBytes <= 64 * 1024 ? 2 : 1;
+    static constexpr uint32_t kTiles = 0;                              // [group][stage][K, V][tile]
+    static constexpr uint32_t kPages = kGroups * kStages * 2 * kTileBytes;   // page ids of the chunk
     static constexpr uint32_t kMergeBytes = kGroups > 1 ? 4 * kRowTile * (D + 4) * 4 + 4 * kRowTile * 8 : 0;
     static constexpr uint32_t kScores = kPages + (kMaxChunk + 2) * 4;  // [wave][new row's token][row of the wave]
     static constexpr uint32_t kEnd = kScores + 4 * kMaxRows * kRowTile * 4;
@@ -230,10 +233,12 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t wr = wave % WR, wg = wave / WR;
-    const uint32_t split = blockIdx.y;
-    const uint32_t row_tile = blockIdx.x % p.row_tiles;
-    const uint32_t kv_head = __builtin_amdgcn_readfirstlane(blockIdx.x / p.row_tiles % p.cache.kv_heads);
-    const uint32_t seq = __builtin_amdgcn_readfirstlane(blockIdx.x / p.row_tiles / p.cache.kv_heads);
+    // Neighbouring workgroups, which go to different XCDs, are chunks of one sequence, and begin at another chunk for the
+    // next: every XCD gets its share of a long sequence and of the chunks that only long ones have.
+    const uint32_t item = blockIdx.x / p.splits, split = (blockIdx.x + item) % p.splits;
+    const uint32_t row_tile = item % p.row_tiles;
+    const uint32_t kv_head = __builtin_amdgcn_readfirstlane(item / p.row_tiles % p.cache.kv_heads);
+    const uint32_t seq = __builtin_amdgcn_readfirstlane(item / p.row_tiles / p.cache.kv_heads);
 
     // a thread's first page id, asked for before the sequence's length is known: the table reaches max_kv_len
     const uint32_t t0 = split * p.chunk;                                       // the chunk: tokens t0 .. t1 - 1
@@ -286,7 +291,7 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     const bool any_bad = __syncthreads_or(bad);
 
     // ---- the tiles' way into LDS ----
-    const uint32_t k_tile = L::kTiles + wg * 2 * L::kTileBytes, v_tile = k_tile + L::kTileBytes;
+    uint32_t k_tile = L::kTiles + wg * L::kStages * 2 * L::kTileBytes, v_tile = k_tile + L::kTileBytes;   // of this step
     const uint32_t lds0 = lds_offset(lds);
     const uint64_t head_bytes = kv_head * p.cache.stride_head * kv_element_bytes(p.cache.dtype);
     const uint8_t *k_pool = uniform_ptr(static_cast<const uint8_t *>(p.cache.k) + head_bytes);
@@ -350,10 +355,12 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     const int64_t first_last = rows.kv_len - rows.count;   // what row 0 of the sequence sees last
     uint32_t odd_tokens = 0;                               // bit i: token first_last + 1 + i holds values that are not finite
     const uint32_t n_steps = t1 > t0 ? (t1 - t0 + L::kGroups * kTile - 1) / (L::kGroups * kTile) : 0;
-    if (n_steps) {
-        const uint32_t where = locate(t0 + wg * kTile);
-        load_tile(k_pool, k_tile, where);
-        load_tile(v_pool, v_tile, where);
+#pragma unroll
+    for (uint32_t st = 0; st < L::kStages; ++st) {
+        if (st >= n_steps) break;   // uniform
+        const uint32_t where = locate(t0 + (st * L::kGroups + wg) * kTile);
+        load_tile(k_pool, k_tile + st * 2 * L::kTileBytes, where);
+        load_tile(v_pool, v_tile + st * 2 * L::kTileBytes, where);
     }
     __builtin_amdgcn_sched_barrier(0);
 
@@ -395,10 +402,13 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
 
     for (uint32_t step = 0; step < n_steps; ++step) {
         const uint32_t first = t0 + (step * L::kGroups + wg) * kTile;
-        const uint32_t next = locate(first + L::kGroups * kTile);
-        const bool more = step + 1 < n_steps;
+        const uint32_t next = locate(first + L::kStages * L::kGroups * kTile);
+        const bool more = step + L::kStages < n_steps;         // this step's stage gets another tile
+        const bool behind_one = L::kStages > 1 && step + 1 < n_steps;
 
-        wait_loads<L::kLoadsPerWave>();   // the keys are here, the values may still travel
+        // the keys are here; this step's values, and the next step's tile, may still travel
+        if (behind_one) wait_loads<3 * L::kLoadsPerWave>();
+        else wait_loads<L::kLoadsPerWave>();
         if constexpr (WR > 1) __syncthreads();
         asm volatile("" : "+v"(k_at), "+v"(v_at));   // their variants are made anew each step: held, they cost 32 registers
         v4f s[2][Op::kTerms];
@@ -479,7 +489,9 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
         v8s pf[Op::kTerms];
         Op::split(w, pf);
 
-        if (more) wait_loads<L::kLoadsPerWave>();   // the values are here, the next keys may still travel
+        // the values are here; what was asked for after them may still travel
+        if (more) wait_loads<(2 * L::kStages - 1) * L::kLoadsPerWave>();
+        else if (behind_one) wait_loads<2 * L::kLoadsPerWave>();
         else wait_loads<0>();
         if constexpr (WR > 1) __syncthreads();
         // V^T operand of 16 outputs: the transposing read gives lane i of a group of 16 column i of the rows that the
@@ -556,6 +568,10 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
         wait_lds_reads();
         if constexpr (WR > 1) __syncthreads();
         if (more) load_tile(v_pool, v_tile, next);
+        if constexpr (L::kStages == 2) {
+            k_tile ^= 2 * L::kTileBytes; v_tile ^= 2 * L::kTileBytes;
+            k_at ^= 2 * L::kTileBytes; v_at ^= 2 * L::kTileBytes;
+        }
     }
     l = rows_sum(l);
     while (odd_tokens != 0) {   // uniform; see above
@@ -712,7 +728,7 @@ int launch_waves(AttnParams &p, hipStream_t s) {
             granted = dev;
         }
     }
-    attention_kernel<D, KV, WR><<<dim3(p.n_seqs * p.cache.kv_heads * p.row_tiles, p.splits), kAttnThreads, L::kBytes, s>>>(p);
+    attention_kernel<D, KV, WR><<<p.n_seqs * p.cache.kv_heads * p.row_tiles * p.splits, kAttnThreads, L::kBytes, s>>>(p);
     if (p.splits > 1) attention_join_kernel<D, KV><<<dim3(p.n_seqs * p.max_q_len, p.q_heads), kJoinThreads, 0, s>>>(p);
     return check_launch("paged_attention");
 }
@@ -767,8 +783,8 @@ extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_row
     if (q_rows > 1 && (stride_q_row < width || stride_out_row < width)) return fail(Q8MI_REJECTED, "%s: rows overlap", what);
 
     const Plan plan = plan_of(n_seqs, max_q_len, q_heads, cache->kv_heads, max_kv_len);
-    if (static_cast<uint64_t>(n_seqs) * cache->kv_heads * plan.row_tiles > 0x3fffffull || static_cast<uint64_t>(n_seqs) * max_q_len > 0x3fffffull ||
-        plan.splits > 65535)
+    if (static_cast<uint64_t>(n_seqs) * cache->kv_heads * plan.row_tiles * plan.splits > 0x3fffffull ||
+        static_cast<uint64_t>(n_seqs) * max_q_len > 0x3fffffull)
         return fail(Q8MI_REJECTED, "%s: %u sequences of %u tokens are too many for one launch", what, n_seqs, max_kv_len);
     const uint64_t es = kv_element_bytes(cache->dtype);
     const uint64_t unit_page = cache->stride_page * es / 16, unit_token = cache->stride_token * es / 16;
