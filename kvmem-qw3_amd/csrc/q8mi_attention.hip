@@ -27,7 +27,7 @@ constexpr uint32_t kAttnThreads = 256;
 constexpr uint32_t kTile = 32;         // tokens of a step and wave
 constexpr uint32_t kMaxChunk = 2048;   // tokens of a workgroup: their page ids are held in LDS
 constexpr uint32_t kRowTile = 16;      // query rows of a wave
-constexpr uint32_t kJoinThreads = 512;
+constexpr uint32_t kJoinThreads = 256;
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -40,13 +40,13 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 struct AttnParams {
     const void *q;
     void *out;
-    float *part;       // [row][q_heads][splits][D]: a chunk's output, not yet divided by its sum
-    float2 *part_ml;   // [row][q_heads][splits]: its maximum (log2 units) and sum
+    float *part;       // [workgroup][its first, its last piece][row of the tile][D]: outputs, not yet divided by their sum
+    float2 *part_ml;   // [workgroup][first, last][row of the tile]: maximum (log2 units) and sum
     const int32_t *page_table, *kv_lens, *q_starts;
     q8mi_kv_cache cache;
     uint32_t q_rows, stride_q, stride_out, stride_page_table;
     uint32_t n_seqs, max_q_len, q_heads, group, max_kv_len;
-    uint32_t chunk, splits, row_tiles;
+    uint32_t groups, unit, tile_rows;   // workgroups, tokens of a unit of work, query rows of a tile
     uint32_t page_magic, page_shift;   // t / page_size = mulhi(t, page_magic) >> page_shift; magic 0: page_size 1
     uint32_t unit_page, unit_token;    // cache strides in units of 16 bytes
     int whole_loads;                   // the tokens of one transfer instruction never straddle pages
@@ -72,6 +72,22 @@ __device__ __forceinline__ Rows rows_of(const AttnParams &p, uint32_t seq) {
     r.used = r.count < 0 ? 0u : r.count > p.max_q_len ? p.max_q_len : static_cast<uint32_t>(r.count);
     r.tokens = r.kv_len < 0 ? 0u : r.kv_len > p.max_kv_len ? p.max_kv_len : static_cast<uint32_t>(r.kv_len);
     return r;
+}
+
+// The work is counted in units: `unit` tokens of one key head and one tile of query rows, in the order sequence, head, row
+// tile, token.  Every workgroup takes an equal run of them, whatever the lengths of the sequences: the end of one item, whole
+// items, the beginning of one.  An item that several workgroups share is joined by a second kernel.
+__device__ __forceinline__ uint32_t units_of_item(const AttnParams &p, const Rows &r) {
+    return r.tokens ? (r.tokens + p.unit - 1) / p.unit : 1;   // an item without tokens still writes its zeros
+}
+__device__ __forceinline__ uint32_t units_of_seq(const AttnParams &p, const Rows &r) {
+    const uint32_t tiles = (r.used * p.group + p.tile_rows - 1) / p.tile_rows;
+    return tiles * p.cache.kv_heads * units_of_item(p, r);
+}
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    return v;
 }
 
 __device__ __forceinline__ uint32_t page_of(const AttnParams &p, uint32_t t) {
@@ -207,6 +223,7 @@ struct Layout {
     static constexpr uint32_t kSwizzle = (kLanesPerRow < 16 ? kLanesPerRow : 16) - 1;
     static constexpr uint32_t kTileBytes = kTile * kRowBytes;
     static constexpr uint32_t kGroups = 4 / WR;
+    static constexpr uint32_t kUnit = kGroups * kTile;                 // tokens of a step
     // Waves that share a tile meet at barriers: a second stage hides what a load takes longer than a step.  Waves on tiles of
     // their own are hidden by each other and by the second workgroup of the CU, which a second stage would not leave room for.
     static constexpr uint32_t kStages = WR > 1 && kGroups * 4 * kTileBytes <= 64 * 1024 ? 2 : 1;
@@ -216,10 +233,12 @@ struct Layout {
     static constexpr uint32_t kScores = kPages + (kMaxChunk + 2) * 4;  // [wave][new row's token][row of the wave]
     static constexpr uint32_t kEnd = kScores + 4 * kMaxRows * kRowTile * 4;
     static constexpr uint32_t kBytes = kEnd > kMergeBytes ? kEnd : kMergeBytes;
+    static constexpr uint32_t kByLds = 160 * 1024 / kBytes, kByRegisters = D == 64 ? 3 : 2;
+    static constexpr uint32_t kResident = kByLds < kByRegisters ? kByLds : kByRegisters;   // workgroups of a CU
 };
 
 template <uint32_t D, int KV, uint32_t WR>
-__global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 1024 ? 2 : 1)) void attention_kernel(const AttnParams p) {
+__global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void attention_kernel(const AttnParams p) {
     using L = Layout<D, KV, WR>;
     using Op = Operand<KV>;
     constexpr uint32_t kSteps = D / 32, kOuts = D / 16;
@@ -233,30 +252,64 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t wr = wave % WR, wg = wave / WR;
-    // Neighbouring workgroups, which go to different XCDs, are chunks of one sequence, and begin at another chunk for the
-    // next: every XCD gets its share of a long sequence and of the chunks that only long ones have.
-    const uint32_t item = blockIdx.x / p.splits, split = (blockIdx.x + item) % p.splits;
-    const uint32_t row_tile = item % p.row_tiles;
-    const uint32_t kv_head = __builtin_amdgcn_readfirstlane(item / p.row_tiles % p.cache.kv_heads);
-    const uint32_t seq = __builtin_amdgcn_readfirstlane(item / p.row_tiles / p.cache.kv_heads);
+    const uint32_t g = lane / 16;
 
-    // a thread's first page id, asked for before the sequence's length is known: the table reaches max_kv_len
-    const uint32_t t0 = split * p.chunk;                                       // the chunk: tokens t0 .. t1 - 1
-    const uint32_t page0 = page_of(p, t0);
-    const int32_t *table = p.page_table + static_cast<uint64_t>(seq) * p.stride_page_table;
-    const int32_t id0 = static_cast<uint64_t>(page0 + threadIdx.x) * p.cache.page_size < p.max_kv_len ? table[page0 + threadIdx.x] : -1;
+    // this workgroup's units: begin .. end - 1, the first of them in sequence seq, whose own begin at seq_begin
+    uint32_t total = 0;
+    for (uint32_t at = 0; at < p.n_seqs; at += kWave)
+        total += wave_sum_u32(at + lane < p.n_seqs ? units_of_seq(p, rows_of(p, at + lane)) : 0);
+    const uint32_t share = __builtin_amdgcn_readfirstlane((total + p.groups - 1) / p.groups);
+    uint32_t begin = blockIdx.x * share;
+    if (begin >= total) return;
+    const uint32_t end = __builtin_amdgcn_readfirstlane(begin + share < total ? begin + share : total);
+    uint32_t seq = 0, seq_begin = 0;
+    for (uint32_t at = 0; at < p.n_seqs; at += kWave) {
+        const uint32_t mine = at + lane < p.n_seqs ? units_of_seq(p, rows_of(p, at + lane)) : 0;
+        uint32_t upto = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t other = __shfl_up(upto, d);
+            upto += lane >= static_cast<uint32_t>(d) ? other : 0;
+        }
+        const uint64_t beyond = __builtin_amdgcn_ballot_w64(seq_begin + upto > begin);
+        if (beyond != 0) {
+            const int who = __builtin_ctzll(beyond);
+            seq = at + who;
+            seq_begin += __builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(mine, who);
+            break;
+        }
+        seq_begin += __builtin_amdgcn_readlane(upto, 63);
+    }
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    seq_begin = __builtin_amdgcn_readfirstlane(seq_begin);
 
+    for (uint32_t piece = 0; begin < end;) {
     const Rows rows = rows_of(p, seq);
-    const uint32_t used_splits = (rows.tokens + p.chunk - 1) / p.chunk;
-    if (split >= (used_splits ? used_splits : 1)) return;
-    const uint32_t n_rows = rows.used * p.group;
-    const uint32_t row0 = row_tile * (WR * kRowTile);
-    if (row0 >= n_rows) return;
+    const uint32_t item_units = units_of_item(p, rows), seq_units = units_of_seq(p, rows);
+    if (begin >= seq_begin + seq_units) {   // on to the next sequence
+        seq_begin += seq_units;
+        ++seq;
+        continue;
+    }
+    const uint32_t n_rows = rows.used * p.group, tiles = (n_rows + WR * kRowTile - 1) / (WR * kRowTile);
+    const uint32_t item = __builtin_amdgcn_readfirstlane((begin - seq_begin) / item_units);
+    const uint32_t unit0 = __builtin_amdgcn_readfirstlane((begin - seq_begin) % item_units);
+    const uint32_t units = item_units - unit0 < end - begin ? item_units - unit0 : end - begin;
+    const uint32_t kv_head = __builtin_amdgcn_readfirstlane(item / tiles);
+    const uint32_t row0 = (item - kv_head * tiles) * (WR * kRowTile);
+    const bool whole_item = units == item_units;
+    const uint32_t slot_of_piece = blockIdx.x * 2 + (piece ? 1 : 0);   // only a first or last piece is not whole
+    ++piece;
+    begin += units;
 
-    const uint32_t t1 = t0 + p.chunk < rows.tokens ? t0 + p.chunk : rows.tokens;
+    const int32_t *table = p.page_table + static_cast<uint64_t>(seq) * p.stride_page_table;
+    uint32_t t0 = unit0 * L::kUnit;                                           // tokens of this piece: t0 .. t_end - 1,
+    const uint32_t t_end = t0 + units * L::kUnit < rows.tokens ? t0 + units * L::kUnit : rows.tokens;
+    uint32_t t1 = t0 + kMaxChunk < t_end ? t0 + kMaxChunk : t_end;            // by chunks t0 .. t1 - 1 with their page ids in LDS
+    uint32_t page0 = page_of(p, t0);
 
     // this lane's query row
-    const uint32_t g = lane / 16, row = row0 + wr * kRowTile + lane % 16;
+    const uint32_t row = row0 + wr * kRowTile + lane % 16;
     const uint32_t token = row / p.group, head = kv_head * p.group + row % p.group;
     const int64_t q_row = rows.start + token;
     const bool live = row < n_rows && q_row >= 0 && q_row < p.q_rows;
@@ -278,17 +331,22 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
             raw[j][1] = *reinterpret_cast<const v4i *>(src + j * 32 + 4);
         }
     }
-    const uint32_t n_pages = t1 > t0 ? page_of(p, t1 - 1) - page0 + 1 : 0;
-    bool bad = false;
-    for (uint32_t i = threadIdx.x; i < n_pages; i += kAttnThreads) {
-        const int32_t id = i == threadIdx.x ? id0 : table[page0 + i];
-        const bool ok = id >= 0 && static_cast<uint32_t>(id) < p.cache.pages;
-        pages[i] = ok ? id : -1;
-        bad |= !ok;
-    }
-    // Everything requested so far is here before the first tile is asked for: a later wait for it would wait for the tile.
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
-    const bool any_bad = __syncthreads_or(bad);
+    bool any_bad = false;
+    auto load_pages = [&]() {
+        const uint32_t n_pages = t1 > t0 ? page_of(p, t1 - 1) - page0 + 1 : 0;
+        bool bad = false;
+        for (uint32_t i = threadIdx.x; i < n_pages; i += kAttnThreads) {
+            const int32_t id = table[page0 + i];
+            const bool ok = id >= 0 && static_cast<uint32_t>(id) < p.cache.pages;
+            pages[i] = ok ? id : -1;
+            bad |= !ok;
+        }
+        // Everything requested so far is here before the first tile is asked for: a later wait for it would wait for the tile.
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+        any_bad = __syncthreads_or(bad);
+    };
+    if (piece > 1) __syncthreads();   // the piece before has left LDS
+    load_pages();
 
     // ---- the tiles' way into LDS ----
     uint32_t k_tile = L::kTiles + wg * L::kStages * 2 * L::kTileBytes, v_tile = k_tile + L::kTileBytes;   // of this step
@@ -354,14 +412,17 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     for (uint32_t d = 0; d < kOuts; ++d) o[d] = v4f{0, 0, 0, 0};
     const int64_t first_last = rows.kv_len - rows.count;   // what row 0 of the sequence sees last
     uint32_t odd_tokens = 0;                               // bit i: token first_last + 1 + i holds values that are not finite
-    const uint32_t n_steps = t1 > t0 ? (t1 - t0 + L::kGroups * kTile - 1) / (L::kGroups * kTile) : 0;
+    uint32_t n_steps = (t1 - t0 + L::kUnit - 1) / L::kUnit;
+    auto load_first = [&]() {
 #pragma unroll
     for (uint32_t st = 0; st < L::kStages; ++st) {
         if (st >= n_steps) break;   // uniform
         const uint32_t where = locate(t0 + (st * L::kGroups + wg) * kTile);
-        load_tile(k_pool, k_tile + st * 2 * L::kTileBytes, where);
-        load_tile(v_pool, v_tile + st * 2 * L::kTileBytes, where);
+        load_tile(k_pool, k_tile ^ st * 2 * L::kTileBytes, where);
+        load_tile(v_pool, v_tile ^ st * 2 * L::kTileBytes, where);
     }
+    };
+    load_first();
     __builtin_amdgcn_sched_barrier(0);
 
     // the queries as operands, while the first tiles travel
@@ -400,7 +461,18 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     }
     const float to_log2 = p.scale_log2 / row_scale;
 
-    for (uint32_t step = 0; step < n_steps; ++step) {
+    for (uint32_t step = 0; n_steps != 0; ++step) {
+        if (step == n_steps) {   // the next chunk of the piece
+            if (t1 == t_end) break;
+            t0 = t1;
+            t1 = t0 + kMaxChunk < t_end ? t0 + kMaxChunk : t_end;
+            page0 = page_of(p, t0);
+            n_steps = (t1 - t0 + L::kUnit - 1) / L::kUnit;
+            step = 0;
+            __syncthreads();   // every wave has read the page ids it needed
+            load_pages();
+            load_first();
+        }
         const uint32_t first = t0 + (step * L::kGroups + wg) * kTile;
         const uint32_t next = locate(first + L::kStages * L::kGroups * kTile);
         const bool more = step + L::kStages < n_steps;         // this step's stage gets another tile
@@ -581,7 +653,7 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
         const float weight = Op::kWeightScale * __builtin_amdgcn_exp2f(kept_scores[(wave * kMaxRows + number) * kRowTile + lane % 16] - m);
         const bool sees = static_cast<int32_t>(t) <= last;
         const uint32_t pg = page_of(p, t);
-        const uint64_t at = static_cast<uint64_t>(pages[pg - page0]) * p.unit_page + static_cast<uint64_t>(t - pg * p.cache.page_size) * p.unit_token;
+        const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(table[pg])) * p.unit_page + static_cast<uint64_t>(t - pg * p.cache.page_size) * p.unit_token;
 #pragma unroll
         for (uint32_t d = 0; d < kOuts; ++d) {
             const uint8_t *src = v_pool + at * 16 + (d * 16 + g * 4) * (KV == Q8MI_KV_E4M3 ? 1 : 2);
@@ -634,38 +706,59 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kBytes <= 80 * 10
     }
     constexpr uint32_t kOwn = kOuts / L::kGroups;
     const uint32_t d0 = wg * kOwn;
-    if (!live) return;
-    if (used_splits <= 1) {
+    if (live && whole_item) {
         const float norm = l > 0.0f || l != l ? (KV == Q8MI_KV_E4M3 ? p.cache.v_scale : 1.0f) / Op::kWeightScale / l : 0.0f;
         const uint64_t at = static_cast<uint64_t>(q_row) * p.stride_out + head * D + g * 4;
 #pragma unroll
         for (uint32_t u = 0; u < kOwn; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) store_out(p, at + (d0 + u) * 16 + i, norm == 0.0f ? 0.0f : o[u][i] * norm);
-    } else {
-        const uint64_t at = (static_cast<uint64_t>(seq * p.max_q_len + token) * p.q_heads + head) * p.splits + split;
+    } else if (live) {
+        const uint64_t at = static_cast<uint64_t>(slot_of_piece) * (WR * kRowTile) + wr * kRowTile + lane % 16;
 #pragma unroll
         for (uint32_t u = 0; u < kOwn; ++u) *reinterpret_cast<v4f *>(p.part + at * D + (d0 + u) * 16 + g * 4) = o[u];
         if (g == 0 && wg == 0) p.part_ml[at] = make_float2(m, l);
     }
+    }
 }
 
-// Joins the chunks of one query row and head, in an order that the sizes alone fix: kJoinGroups threads share a column,
-// chunk by chunk, and meet in LDS.
+// Joins the pieces of one query row and head, in their order: kGroups threads share a column and meet in LDS.
 template <uint32_t D, int KV>
 __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const AttnParams p) {
     constexpr uint32_t kGroups = kJoinThreads / (D / 4);
     __shared__ float tops[kJoinThreads / kWave], sums[kGroups];
+    __shared__ uint32_t units[kJoinThreads / kWave][2];
     __shared__ v4f parts[kGroups][D / 4];
     const uint32_t seq = blockIdx.x / p.max_q_len, token = blockIdx.x % p.max_q_len, head = blockIdx.y;
     const uint32_t group = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4);
     const Rows rows = rows_of(p, seq);
-    const uint32_t n = (rows.tokens + p.chunk - 1) / p.chunk;
     const int64_t q_row = rows.start + token;
-    if (n <= 1 || token >= rows.used || q_row < 0 || q_row >= p.q_rows) return;
-    const uint64_t at = (static_cast<uint64_t>(blockIdx.x) * p.q_heads + head) * p.splits;
+    if (token >= rows.used || q_row < 0 || q_row >= p.q_rows) return;
+    uint32_t total = 0, before = 0;   // units of all sequences, and of those before this one
+    for (uint32_t s = threadIdx.x; s < p.n_seqs; s += kJoinThreads) {
+        const uint32_t u = units_of_seq(p, rows_of(p, s));
+        total += u;
+        before += s < seq ? u : 0;
+    }
+    total = wave_sum_u32(total);
+    before = wave_sum_u32(before);
+    if (threadIdx.x % kWave == 0) { units[threadIdx.x / kWave][0] = total; units[threadIdx.x / kWave][1] = before; }
+    __syncthreads();
+    total = before = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kJoinThreads / kWave; ++i) { total += units[i][0]; before += units[i][1]; }
+    const uint32_t share = (total + p.groups - 1) / p.groups;
+    const uint32_t row = token * p.group + head % p.group, tile = row / p.tile_rows;
+    const uint32_t tiles = (rows.used * p.group + p.tile_rows - 1) / p.tile_rows, item_units = units_of_item(p, rows);
+    const uint32_t begin = before + (head / p.group * tiles + tile) * item_units, end = begin + item_units;
+    const uint32_t w0 = begin / share, n = (end - 1) / share - w0 + 1;   // the workgroups that share the item
+    if (n == 1) return;
+    auto place = [&](uint32_t s) -> uint64_t {   // of the row in piece s
+        const uint64_t slot = static_cast<uint64_t>(w0 + s) * 2 + (s == 0 && begin > w0 * share ? 1 : 0);
+        return slot * p.tile_rows + row % p.tile_rows;
+    };
     float top = -INFINITY;
-    for (uint32_t s = threadIdx.x; s < n; s += kJoinThreads) top = fmaxf(top, p.part_ml[at + s].x);
+    for (uint32_t s = threadIdx.x; s < n; s += kJoinThreads) top = fmaxf(top, p.part_ml[place(s)].x);
     top = fmaxf(top, lane_xor<1>(top)); top = fmaxf(top, lane_xor<2>(top)); top = fmaxf(top, lane_xor<4>(top));
     top = fmaxf(top, lane_xor<8>(top)); top = fmaxf(top, lane_xor<16>(top)); top = fmaxf(top, lane_xor<32>(top));
     if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
@@ -676,10 +769,11 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Attn
     v4f out = v4f{0, 0, 0, 0};
 #pragma unroll 4
     for (uint32_t s = group; s < n; s += kGroups) {
-        const float2 ml = p.part_ml[at + s];
+        const uint64_t at = place(s);
+        const float2 ml = p.part_ml[at];
         const float f = ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
         sum += f * ml.y;
-        out += f * *reinterpret_cast<const v4f *>(p.part + (at + s) * D + d * 4);
+        out += f * *reinterpret_cast<const v4f *>(p.part + at * D + d * 4);
     }
     parts[group][d] = out;
     if (d == 0) sums[group] = sum;
@@ -696,19 +790,23 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Attn
         store_out(p, static_cast<uint64_t>(q_row) * p.stride_out + head * D + d * 4 + i, sum == 0.0f ? 0.0f : out[i] / sum * norm);
 }
 
-// How a call is cut: tokens of a chunk, chunks of the longest sequence, row tiles and waves side by side on rows.
+// How a call is cut: waves side by side on rows, and workgroups: as many as a chip of 256 CUs holds at once (one to three a CU,
+// by registers and LDS), so that equal runs of the work end together, or one a unit.  Sizes alone decide, for every device.
+constexpr uint32_t kChipCus = 256;
 struct Plan {
-    uint32_t chunk, splits, waves_on_rows, row_tiles;
+    uint32_t waves_on_rows, groups;
 };
-Plan plan_of(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t max_kv_len) {
+Plan plan_of(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_kv_len,
+             uint64_t *units = nullptr) {
     Plan r;
     const uint32_t rows = max_q_len * (kv_heads ? q_heads / kv_heads : 0);
     r.waves_on_rows = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    r.row_tiles = (rows + 16 * r.waves_on_rows - 1) / (16 * r.waves_on_rows);
-    const uint64_t items = static_cast<uint64_t>(n_seqs) * kv_heads * r.row_tiles;
-    r.chunk = kMaxChunk;
-    while (r.chunk > 128 && items * ((max_kv_len + r.chunk - 1) / r.chunk) < 512) r.chunk /= 2;
-    r.splits = max_kv_len ? (max_kv_len + r.chunk - 1) / r.chunk : 1;
+    const uint64_t tiles = (rows + kRowTile * r.waves_on_rows - 1) / (kRowTile * r.waves_on_rows);
+    const uint32_t unit = kTile * 4 / r.waves_on_rows;
+    const uint64_t most = n_seqs * static_cast<uint64_t>(kv_heads) * tiles * (max_kv_len ? (max_kv_len + unit - 1) / unit : 1);
+    const uint32_t resident = kChipCus * (head_dim == 64 ? 3 : 2);
+    r.groups = static_cast<uint32_t>(most < resident ? most : resident);
+    if (units) *units = most;
     return r;
 }
 
@@ -728,8 +826,12 @@ int launch_waves(AttnParams &p, hipStream_t s) {
             granted = dev;
         }
     }
-    attention_kernel<D, KV, WR><<<p.n_seqs * p.cache.kv_heads * p.row_tiles * p.splits, kAttnThreads, L::kBytes, s>>>(p);
-    if (p.splits > 1) attention_join_kernel<D, KV><<<dim3(p.n_seqs * p.max_q_len, p.q_heads), kJoinThreads, 0, s>>>(p);
+    p.unit = L::kUnit;
+    p.tile_rows = WR * kRowTile;
+    const uint32_t resident = kChipCus * L::kResident;
+    if (p.groups > resident) p.groups = resident;
+    attention_kernel<D, KV, WR><<<p.groups, kAttnThreads, L::kBytes, s>>>(p);
+    if (p.max_kv_len > L::kUnit) attention_join_kernel<D, KV><<<dim3(p.n_seqs * p.max_q_len, p.q_heads), kJoinThreads, 0, s>>>(p);
     return check_launch("paged_attention");
 }
 template <uint32_t D, int KV>
@@ -745,9 +847,7 @@ int launch_type(AttnParams &p, uint32_t waves_on_rows, hipStream_t s) {
     return launch_dim<256, KV>(p, waves_on_rows, s);
 }
 
-uint64_t partial_slots(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t splits) {
-    return splits > 1 ? static_cast<uint64_t>(n_seqs) * max_q_len * q_heads * splits : 0;
-}
+uint64_t partial_rows(const Plan &plan) { return 2ull * plan.groups * plan.waves_on_rows * kRowTile; }
 
 }  // namespace
 }  // namespace q8mi
@@ -756,8 +856,8 @@ using namespace q8mi;
 
 extern "C" size_t q8mi_paged_attention_scratch_bytes(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads,
                                                      uint32_t head_dim, uint32_t max_kv_len) {
-    const Plan plan = plan_of(n_seqs, max_q_len, q_heads, kv_heads, max_kv_len);
-    return 16 + partial_slots(n_seqs, max_q_len, q_heads, plan.splits) * (head_dim + 2) * sizeof(float);
+    const Plan plan = plan_of(n_seqs, max_q_len, q_heads, kv_heads, head_dim, max_kv_len);
+    return 16 + partial_rows(plan) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_rows, uint32_t stride_q_row,
@@ -782,9 +882,9 @@ extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_row
         return fail(Q8MI_REJECTED, "%s: rows of q and out must begin on 16-byte boundaries", what);
     if (q_rows > 1 && (stride_q_row < width || stride_out_row < width)) return fail(Q8MI_REJECTED, "%s: rows overlap", what);
 
-    const Plan plan = plan_of(n_seqs, max_q_len, q_heads, cache->kv_heads, max_kv_len);
-    if (static_cast<uint64_t>(n_seqs) * cache->kv_heads * plan.row_tiles * plan.splits > 0x3fffffull ||
-        static_cast<uint64_t>(n_seqs) * max_q_len > 0x3fffffull)
+    uint64_t units = 0;
+    const Plan plan = plan_of(n_seqs, max_q_len, q_heads, cache->kv_heads, cache->head_dim, max_kv_len, &units);
+    if (units > 0x3fffffffull || static_cast<uint64_t>(n_seqs) * max_q_len > 0x3fffffull)
         return fail(Q8MI_REJECTED, "%s: %u sequences of %u tokens are too many for one launch", what, n_seqs, max_kv_len);
     const uint64_t es = kv_element_bytes(cache->dtype);
     const uint64_t unit_page = cache->stride_page * es / 16, unit_token = cache->stride_token * es / 16;
@@ -801,10 +901,10 @@ extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_row
     }
     p.q = q; p.out = out; p.page_table = page_table; p.kv_lens = kv_lens; p.q_starts = q_starts; p.cache = *cache;
     p.part = static_cast<float *>(scratch);
-    p.part_ml = reinterpret_cast<float2 *>(p.part + partial_slots(n_seqs, max_q_len, q_heads, plan.splits) * cache->head_dim);
+    p.part_ml = reinterpret_cast<float2 *>(p.part + partial_rows(plan) * cache->head_dim);
     p.q_rows = q_rows; p.stride_q = stride_q_row; p.stride_out = stride_out_row; p.stride_page_table = stride_page_table;
     p.n_seqs = n_seqs; p.max_q_len = max_q_len; p.q_heads = q_heads; p.group = q_heads / cache->kv_heads;
-    p.max_kv_len = max_kv_len; p.chunk = plan.chunk; p.splits = plan.splits; p.row_tiles = plan.row_tiles;
+    p.max_kv_len = max_kv_len; p.groups = plan.groups;
     p.scale_log2 = scale * 1.44269504088896340736f * (cache->dtype == Q8MI_KV_E4M3 ? cache->k_scale : 1.0f);
     p.q_is_bf16 = q_is_bf16; p.out_is_bf16 = out_is_bf16;
     hipStream_t s = as_stream(stream);
