@@ -5,16 +5,16 @@
 // Weights are p = exp((logit - max) / temperature) rounded to multiples of 2^-42: sums are 64-bit integers, exact and
 // free of their order, so that neither the split of a row nor the arrival of atomics moves a border.
 //
-// No sort of the row.  Four launches, the first three over (chunks of 4096 logits) x rows:
-//   1  largest (logit, lowest index) of each chunk; clears the row's counters
-//   2  weights; where nothing is cut but by min-p, their sum per chunk, else a histogram of count and weight over 256
-//      steps of 1/8 in (max - logit) / temperature (what lies 31.9 and more below the maximum weighs nothing)
+// No sort of the row.  Four launches, the first three over (spans of chunks of 1024 logits) x rows:
+//   1  largest (logit, lowest index) of each span; clears the row's counters
+//   2  weights; where nothing is cut but by min-p, their sum per chunk, else a histogram of count and weight over 1024
+//      steps of 1/32 in (max - logit) / temperature (what lies 31.9 and more below the maximum weighs nothing)
 //   3  the histogram says in which steps the cuts fall: the few logits of those steps are collected, what lies above them
 //      is kept for certain and summed per chunk
-//   4  one workgroup a row sorts the collected logits, takes the cuts in them, finds the chunk that holds the drawn element
+//   4  one workgroup a row ranks the collected logits, takes the cuts in them, finds the chunk that holds the drawn element
 //      and walks it
-// A row with more than 4096 logits in the steps of its cuts (thousands of equal ones) is instead searched digit by digit
-// of the keys, by the fourth launch's workgroup alone.
+// A row with more than 4096 logits in the steps of its cuts (thousands of equal ones, a temperature that levels all) is
+// searched digit by digit of the keys instead, by the fourth launch's workgroup alone.
 #include "q8mi_device.hpp"
 #include "q8mi_internal.hpp"
 
@@ -22,12 +22,13 @@ namespace q8mi {
 namespace {
 
 constexpr uint32_t kMaxVocab = 1u << 20;
-constexpr uint32_t kChunk = 4096;                     // logits of a workgroup of launches 1 to 3
+constexpr uint32_t kChunk = 1024;                     // logits
 constexpr uint32_t kMaxChunks = kMaxVocab / kChunk;
-constexpr uint32_t kChunkThreads = 256;
+constexpr uint32_t kAhead = 4;                        // chunks that a workgroup of launches 1 to 3 loads at a time
+constexpr uint32_t kChunkThreads = kChunk / 4;
 constexpr uint32_t kRowThreads = 1024;                // launch 4
-constexpr uint32_t kBins = 256;
-constexpr double kBinsPerUnit = 8.0;
+constexpr uint32_t kBins = 1024;
+constexpr double kBinsPerUnit = 32.0;
 constexpr double kReach = 31.875;                     // exp(-31.875) * 2^42 rounds to 0
 constexpr uint32_t kMaxCandidates = 4096;
 constexpr double kOne = 4398046511104.0;              // 2^42: the weight of the largest logit; 2^20 of them sum below 2^63
@@ -39,13 +40,14 @@ struct SampleParams {
     const float *temperature, *top_p, *min_p, *uniform;
     const int32_t *top_k;
     q8mi_argmax_pair *out;
-    u64 *best;          // [row][chunk]: key << 32 | ~index of the chunk's rank 0
+    u64 *best;          // [row][span]: key << 32 | ~index of the span's rank 0
     u64 *chunk_mass;    // [row][chunk]: weight kept for certain
     u64 *bin_mass;      // [row][kBins]
     u64 *candidates;    // [row][kMaxCandidates]: key << 32 | ~index
     uint32_t *bin_count;     // [row][kBins]
     uint32_t *n_candidates;  // [row]
     uint32_t vocab, stride, chunks;
+    uint32_t span, spans;    // chunks of a workgroup of launches 1 to 3, such workgroups a row
     int vec;
 };
 
@@ -142,42 +144,62 @@ __device__ __forceinline__ void load4(const SampleParams &p, const float *x, uin
     for (uint32_t k = 0; k < 4; ++k) v[k] = i + k < p.vocab ? x[i + k] : -INFINITY;
 }
 
+// Calls f(v, i, chunk) for every four logits v (from element i) that this thread has of the workgroup's span, and
+// after(chunk) behind each chunk; kAhead chunks are loaded at a time.
+template <typename F, typename A>
+__device__ __forceinline__ void walk_span(const SampleParams &p, const float *x, F f, A after) {
+    const uint32_t first = blockIdx.x * p.span, end = first + p.span < p.chunks ? first + p.span : p.chunks;
+    for (uint32_t c = first; c < end; c += kAhead) {
+        float v[kAhead][4];
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) {
+            const uint32_t i = (c + u) * kChunk + threadIdx.x * 4;
+            if (c + u < end) load4(p, x, i, v[u]);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) {
+            if (c + u >= end) break;   // uniform
+            f(v[u], (c + u) * kChunk + threadIdx.x * 4);
+            after(c + u);
+        }
+    }
+}
+
 // ---- 1 ----------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kChunkThreads) void sample_best_kernel(const SampleParams p) {
     __shared__ u64 part[kChunkThreads / kWave];
-    const uint32_t t = threadIdx.x, chunk = blockIdx.x, row = blockIdx.y;
+    const uint32_t t = threadIdx.x, row = blockIdx.y;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
-    float v[4][4];
-#pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) load4(p, x, chunk * kChunk + u * 1024 + t * 4, v[u]);
-    if (chunk == 0) {
-        p.bin_mass[row * kBins + t] = 0;
-        p.bin_count[row * kBins + t] = 0;
-        if (t == 0) p.n_candidates[row] = 0;
-    }
     u64 best = 0;
-#pragma unroll
-    for (uint32_t u = 0; u < 4; ++u)
+    walk_span(p, x, [&](const float (&v)[4], uint32_t i) {
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
-            const u64 r = rank_of(key_of(v[u][k]), chunk * kChunk + u * 1024 + t * 4 + k);
+            const u64 r = rank_of(key_of(v[k]), i + k);
             best = r > best ? r : best;
         }
+    }, [](uint32_t) {});
+    if (blockIdx.x == 0) {
+        for (uint32_t b = t; b < kBins; b += kChunkThreads) {
+            p.bin_mass[static_cast<uint64_t>(row) * kBins + b] = 0;
+            p.bin_count[static_cast<uint64_t>(row) * kBins + b] = 0;
+        }
+        if (t == 0) p.n_candidates[row] = 0;
+    }
     best = wave_max_u64(best);
     if (t % kWave == 0) part[t / kWave] = best;
     __syncthreads();
     if (t == 0) {
 #pragma unroll
         for (uint32_t w = 1; w < kChunkThreads / kWave; ++w) best = part[w] > best ? part[w] : best;
-        p.best[row * p.chunks + chunk] = best;
+        p.best[static_cast<uint64_t>(row) * p.spans + blockIdx.x] = best;
     }
 }
 
 // The row's rank 0, by every wave for itself.
 __device__ __forceinline__ u64 row_best(const SampleParams &p, uint32_t row) {
     u64 best = 0;
-    for (uint32_t c = threadIdx.x % kWave; c < p.chunks; c += kWave) {
-        const u64 b = p.best[row * p.chunks + c];
+    for (uint32_t c = threadIdx.x % kWave; c < p.spans; c += kWave) {
+        const u64 b = p.best[static_cast<uint64_t>(row) * p.spans + c];
         best = b > best ? b : best;
     }
     return wave_max_u64(best);
@@ -187,188 +209,230 @@ __device__ __forceinline__ u64 row_best(const SampleParams &p, uint32_t row) {
 __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const SampleParams p) {
     __shared__ u64 mass[kBins];
     __shared__ uint32_t count[kBins];
-    __shared__ u64 part[kChunkThreads / kWave];
-    const uint32_t t = threadIdx.x, chunk = blockIdx.x, row = blockIdx.y;
+    __shared__ u64 part[kAhead][kChunkThreads / kWave];
+    const uint32_t t = threadIdx.x, row = blockIdx.y;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
-    float v[4][4];
-#pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) load4(p, x, chunk * kChunk + u * 1024 + t * 4, v[u]);
-    const uint32_t top = static_cast<uint32_t>(row_best(p, row) >> 32);
-    const Row r = row_of(p, row, top);
-    if (top == 0 || r.greedy) return;
-    const bool cuts = r.top_k != 0 || r.top_p < 1.0;
-    if (cuts) {
-        mass[t] = 0;
-        count[t] = 0;
+    const u64 best = row_best(p, row);
+    const Row r = row_of(p, row, static_cast<uint32_t>(best >> 32));
+    if (best >> 32 == 0 || r.greedy) return;
+    const bool by_count = r.top_k != 0, by_mass = r.top_p < 1.0;   // each needs its half of the histogram
+    if (by_count || by_mass) {
+        for (uint32_t b = t; b < kBins; b += kChunkThreads) { mass[b] = 0; count[b] = 0; }
         __syncthreads();
-    }
-    u64 sum = 0;
+        walk_span(p, x, [&](const float (&v)[4], uint32_t) {
 #pragma unroll
-    for (uint32_t u = 0; u < 4; ++u)
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-            const double depth = depth_of(key_of(v[u][k]), r);
-            if (!(depth < kReach)) continue;
-            if (cuts) {
+            for (uint32_t k = 0; k < 4; ++k) {
+                const double depth = depth_of(key_of(v[k]), r);
+                if (!(depth < kReach)) continue;
                 const uint32_t b = bin_at(depth);
-                atomicAdd(&mass[b], weight_at(depth, 0.0));
-                atomicAdd(&count[b], 1u);
-            } else {
-                sum += weight_at(depth, r.min_p);
+                if (by_count) atomicAdd(&count[b], 1u);
+                if (by_mass) atomicAdd(&mass[b], weight_at(depth, 0.0));
             }
-        }
-    if (cuts) {
+        }, [](uint32_t) {});
         __syncthreads();
-        if (count[t] != 0) {
-            atomicAdd(&p.bin_count[row * kBins + t], count[t]);
-            atomicAdd(&p.bin_mass[row * kBins + t], mass[t]);
+        for (uint32_t b = t; b < kBins; b += kChunkThreads) {
+            if (count[b] != 0) atomicAdd(&p.bin_count[static_cast<uint64_t>(row) * kBins + b], count[b]);
+            if (mass[b] != 0) atomicAdd(&p.bin_mass[static_cast<uint64_t>(row) * kBins + b], mass[b]);
         }
         return;
     }
-    sum = wave_sum_u64(sum);
-    if (t % kWave == 0) part[t / kWave] = sum;
-    __syncthreads();
-    if (t == 0) p.chunk_mass[row * p.chunks + chunk] = (part[0] + part[1]) + (part[2] + part[3]);
+    u64 sum = 0;
+    walk_span(p, x, [&](const float (&v)[4], uint32_t) {
+        sum = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) sum += weight_at(depth_of(key_of(v[k]), r), r.min_p);
+    }, [&](uint32_t chunk) {
+        sum = wave_sum_u64(sum);
+        u64 *mine = part[chunk % kAhead];   // another one is written before the next barrier
+        if (t % kWave == 0) mine[t / kWave] = sum;
+        __syncthreads();
+        if (t == 0) p.chunk_mass[static_cast<uint64_t>(row) * p.chunks + chunk] = (mine[0] + mine[1]) + (mine[2] + mine[3]);
+    });
 }
 
-// Where the cuts fall: steps below `sure` are kept, steps first .. last hold the last rank, step `k_bin` the top_k-th.
+// Where the cuts fall: steps below `sure` are kept, steps sure .. last hold the last rank, step `k_bin` the top_k-th
+// (kBins: nothing is cut there); the weight of the steps below `sure`, below k_bin, and of all; the count below k_bin.
 struct Cut {
-    uint32_t sure, last, k_bin;   // kBins: nothing is cut there
+    uint32_t sure, last, k_bin, k_count;
+    u64 sure_mass, k_mass, all_mass;
 };
-// Every thread of at least kBins calls it; `low`: kBins of LDS for counts and masses up to and with a step.
-__device__ __forceinline__ Cut find_cut(const SampleParams &p, uint32_t row, const Row &r, u64 *mass_upto, uint32_t *count_upto,
-                                        uint32_t *found) {
-    const uint32_t t = threadIdx.x, lane = t % kWave, wave = t / kWave;
-    u64 m = 0;
-    uint32_t c = 0;
-    if (t < kBins) {
-        m = p.bin_mass[row * kBins + t];
-        c = p.bin_count[row * kBins + t];
+struct CutSpace {   // LDS
+    u64 mass_upto[kBins];
+    u64 part[kRowThreads / kWave];
+    uint32_t found[3], k_count;
+};
+// Every thread of the workgroup calls it; the first kBins / 4 hold four steps each.
+template <uint32_t THREADS>
+__device__ __forceinline__ Cut find_cut(const SampleParams &p, uint32_t row, const Row &r, CutSpace &s) {
+    constexpr uint32_t kHolders = kBins / 4;
+    static_assert(THREADS >= kHolders, "four steps a thread");
+    const uint32_t t = threadIdx.x;
+    const bool holds = t < kHolders;
+    u64 m[4] = {}, c[4] = {}, all_mass, all_count;
+    if (holds) {
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const u64 om = __shfl_up(m, d);
-            const uint32_t oc = __shfl_up(c, d);
-            if (lane >= static_cast<uint32_t>(d)) { m += om; c += oc; }
+        for (uint32_t k = 0; k < 4; ++k) {
+            m[k] = p.bin_mass[static_cast<uint64_t>(row) * kBins + 4 * t + k];
+            c[k] = p.bin_count[static_cast<uint64_t>(row) * kBins + 4 * t + k];
         }
-        mass_upto[t] = m;
-        count_upto[t] = c;
     }
-    if (t == 0) { found[0] = found[1] = found[2] = kBins; }
+    if (t == 0) { s.found[0] = s.found[1] = s.found[2] = kBins; s.k_count = 0; }
+    u64 m_before = r.top_p < 1.0 ? sum_below<THREADS>((m[0] + m[1]) + (m[2] + m[3]), s.part, all_mass) : 0;
+    u64 c_before = r.top_k != 0 ? sum_below<THREADS>((c[0] + c[1]) + (c[2] + c[3]), s.part, all_count) : 0;
+    const u64 m_first = m_before;
     __syncthreads();
-    if (t < kBins) {
-        for (uint32_t w = 0; w < wave; ++w) { m += mass_upto[w * kWave + 63]; c += count_upto[w * kWave + 63]; }
+    if (holds) {
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            if (r.top_k != 0 && c_before < r.top_k && c_before + c[k] >= r.top_k) {   // one thread's one step
+                s.found[0] = 4 * t + k;
+                s.k_count = static_cast<uint32_t>(c_before);
+            }
+            c_before += c[k];
+            m_before += m[k];
+            s.mass_upto[4 * t + k] = m_before;
+        }
     }
-    __syncthreads();
-    if (t < kBins) { mass_upto[t] = m; count_upto[t] = c; }
-    __syncthreads();
-    const uint32_t c_before = t == 0 || t >= kBins ? 0 : count_upto[t - 1];
-    if (t < kBins && r.top_k != 0 && c_before < r.top_k && c >= r.top_k) found[0] = t;   // one thread
     __syncthreads();
     Cut cut;
-    cut.k_bin = found[0];
+    cut.k_bin = s.found[0];
+    cut.k_count = s.k_count;
     cut.sure = cut.last = cut.k_bin;
+    cut.sure_mass = cut.k_mass = cut.all_mass = 0;
     if (r.top_p < 1.0) {
-        // the mass that top_k keeps lies between these; so does the last rank that top_p keeps
-        const uint32_t kb = cut.k_bin < kBins ? cut.k_bin : kBins - 1;
-        const u64 hi = mass_upto[kb], lo = cut.k_bin < kBins ? (kb ? mass_upto[kb - 1] : 0) : hi;
+        // the weight that top_k keeps lies between these two; so does the last rank that top_p keeps
+        const u64 hi = s.mass_upto[cut.k_bin < kBins ? cut.k_bin : kBins - 1];
+        const u64 lo = cut.k_bin == kBins ? hi : cut.k_bin ? s.mass_upto[cut.k_bin - 1] : 0;
         const double limit_lo = r.top_p * static_cast<double>(lo), limit_hi = r.top_p * static_cast<double>(hi);
-        const u64 m_before = t == 0 || t >= kBins ? 0 : mass_upto[t - 1];
-        // the first step that reaches the limit: the mass before it falls short
-        if (t < kBins && m != m_before) {
-            if ((t == 0 || m_before == 0 || static_cast<double>(m_before) < limit_lo) && static_cast<double>(m) >= limit_lo) atomicMin(&found[1], t);
-            if ((t == 0 || m_before == 0 || static_cast<double>(m_before) < limit_hi) && static_cast<double>(m) >= limit_hi) atomicMin(&found[2], t);
+        if (holds) {
+            u64 b = m_first;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {   // the step that reaches a limit: one thread's
+                const u64 e = b + m[k];
+                const bool first = 4 * t + k == 0;   // rank 0 lies in step 0 and always stays
+                if ((first || static_cast<double>(b) < limit_lo) && static_cast<double>(e) >= limit_lo) s.found[1] = 4 * t + k;
+                if ((first || static_cast<double>(b) < limit_hi) && static_cast<double>(e) >= limit_hi) s.found[2] = 4 * t + k;
+                b = e;
+            }
         }
         __syncthreads();
-        cut.sure = found[1] < cut.k_bin ? found[1] : cut.k_bin;
-        cut.last = found[2] < cut.k_bin ? found[2] : cut.k_bin;
+        cut.sure = s.found[1] < cut.k_bin ? s.found[1] : cut.k_bin;
+        cut.last = s.found[2] < cut.k_bin ? s.found[2] : cut.k_bin;
+        cut.sure_mass = cut.sure ? s.mass_upto[cut.sure - 1] : 0;
+        cut.k_mass = lo;
+        cut.all_mass = s.mass_upto[kBins - 1];
     }
     return cut;
 }
 
 // ---- 3 ----------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const SampleParams p) {
-    __shared__ u64 mass_upto[kBins];
-    __shared__ uint32_t count_upto[kBins], found[3], n_here, base;
-    __shared__ u64 part[kChunkThreads / kWave];
-    const uint32_t t = threadIdx.x, chunk = blockIdx.x, row = blockIdx.y;
+    __shared__ CutSpace space;
+    __shared__ u64 part[kAhead][kChunkThreads / kWave];
+    const uint32_t t = threadIdx.x, row = blockIdx.y;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
-    float v[4][4];
-#pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) load4(p, x, chunk * kChunk + u * 1024 + t * 4, v[u]);
-    const uint32_t top = static_cast<uint32_t>(row_best(p, row) >> 32);
-    const Row r = row_of(p, row, top);
-    if (top == 0 || r.greedy || !(r.top_k != 0 || r.top_p < 1.0)) return;
-    if (t == 0) n_here = 0;
-    const Cut cut = find_cut(p, row, r, mass_upto, count_upto, found);
-    // the elements to collect, and their places among this chunk's
-    uint32_t mine = 0;   // bit per element
+    const u64 best = row_best(p, row);
+    const Row r = row_of(p, row, static_cast<uint32_t>(best >> 32));
+    if (best >> 32 == 0 || r.greedy || !(r.top_k != 0 || r.top_p < 1.0)) return;
+    const Cut cut = find_cut<kChunkThreads>(p, row, r, space);
+    u64 *list = p.candidates + static_cast<uint64_t>(row) * kMaxCandidates;
     u64 sum = 0;
-#pragma unroll
-    for (uint32_t u = 0; u < 4; ++u)
+    walk_span(p, x, [&](const float (&v)[4], uint32_t i) {
+        sum = 0;
+        uint32_t mine = 0;   // elements to collect
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
-            const double depth = depth_of(key_of(v[u][k]), r);
+            const double depth = depth_of(key_of(v[k]), r);
             if (!(depth < kReach)) continue;
             const uint32_t b = bin_at(depth);
             if (b < cut.sure) sum += weight_at(depth, r.min_p);
-            else if (b <= cut.last || b == cut.k_bin) mine |= 1u << (u * 4 + k);
+            else if (b <= cut.last || b == cut.k_bin) mine |= 1u << k;
         }
-    uint32_t at = mine ? atomicAdd(&n_here, static_cast<uint32_t>(__popc(mine))) : 0;
-    sum = wave_sum_u64(sum);
-    if (t % kWave == 0) part[t / kWave] = sum;
-    __syncthreads();
-    if (t == 0) {
-        p.chunk_mass[row * p.chunks + chunk] = (part[0] + part[1]) + (part[2] + part[3]);
-        base = n_here ? atomicAdd(&p.n_candidates[row], n_here) : 0;
-    }
-    __syncthreads();
-    at += base;
+        // places in the list: one atomic a wave
+        const uint32_t n = __popc(mine);
+        if (__builtin_amdgcn_ballot_w64(n != 0) != 0) {
+            uint32_t upto = n;
 #pragma unroll
-    for (uint32_t u = 0; u < 4; ++u)
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k)
-            if (mine >> (u * 4 + k) & 1) {
-                if (at < kMaxCandidates)
-                    p.candidates[static_cast<uint64_t>(row) * kMaxCandidates + at] = rank_of(key_of(v[u][k]), chunk * kChunk + u * 1024 + t * 4 + k);
-                ++at;
+            for (int d = 1; d < 64; d *= 2) {
+                const uint32_t o = __shfl_up(upto, d);
+                upto += t % kWave >= static_cast<uint32_t>(d) ? o : 0;
             }
+            uint32_t at = 0;
+            if (t % kWave == 63) at = atomicAdd(&p.n_candidates[row], upto);
+            at = __shfl(at, 63) + upto - n;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                if (mine >> k & 1) {
+                    if (at < kMaxCandidates) list[at] = rank_of(key_of(v[k]), i + k);
+                    ++at;
+                }
+        }
+    }, [&](uint32_t chunk) {
+        sum = wave_sum_u64(sum);
+        u64 *mine = part[chunk % kAhead];
+        if (t % kWave == 0) mine[t / kWave] = sum;
+        __syncthreads();
+        if (t == 0) p.chunk_mass[static_cast<uint64_t>(row) * p.chunks + chunk] = (mine[0] + mine[1]) + (mine[2] + mine[3]);
+    });
 }
 
 // ---- 4 ----------------------------------------------------------------------------------------------------------------
-// The last kept rank of a row by its keys' digits: eight bits a pass over the whole row, counts and weights of the 256
-// values in LDS, first for top_k, then for top_p among what that keeps.  The workgroup's scratch is the candidates' LDS.
-__device__ u64 cut_by_digits(const SampleParams &p, const float *x, const Row &r, u64 *lds) {
-    u64 *mass = lds, *part = lds + 256, *sh = lds + 256 + kRowThreads;
-    uint32_t *count = reinterpret_cast<uint32_t *>(sh + 8);
+struct DrawSpace {   // LDS
+    u64 cand[kMaxCandidates];
+    CutSpace cut;
+    u64 chunk_mass[kMaxChunks];
+    u64 last, target;
+    uint32_t at, bounds[2];
+};
+constexpr uint32_t kRankThreads = 512;   // up to as many candidates are ranked by counting, more are sorted
+
+// The last kept rank of a row by its keys' digits: eight bits a pass over the row, counts and weights of the 256 values in
+// LDS.  Only the steps that hold the cut count, what lies above them is known from the histogram.
+__device__ u64 cut_by_digits(const SampleParams &p, const float *x, const Row &r, const Cut &cut, DrawSpace &s) {
+    u64 *mass = s.cand, *sh = s.cand + 256, *ties_of = s.cand + 512;   // [kMaxChunks]
+    uint32_t *count = reinterpret_cast<uint32_t *>(s.cand + 512 + kMaxChunks);
     const uint32_t t = threadIdx.x;
-    uint32_t last_key = 1, last_ties = 0xffffffffu;   // elements above last_key, and the first last_ties of those equal to it
-    // The last rank that stays when ranks are taken in order: while fewer than `limit` (count or mass) came before it.
-    auto cut = [&](bool by_mass, u64 limit) {
+    auto walk = [&](auto f) {   // f(key, index) for every logit
+        for (uint32_t i = 4 * t; i < p.vocab; i += 4 * kRowThreads) {
+            float v[4];
+            load4(p, x, i, v);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                if (i + k < p.vocab) f(key_of(v[k]), i + k);
+        }
+    };
+    // The last rank that stays among the steps lo .. hi and not behind `after`, when fewer than `limit` (count or mass) of
+    // them may come before it.
+    auto find = [&](bool by_mass, uint32_t lo, uint32_t hi, u64 after, u64 limit) -> u64 {
         uint32_t prefix = 0;
         u64 before = 0;
         for (int shift = 24; shift >= 0; shift -= 8) {
             if (t < 256) { mass[t] = 0; count[t] = 0; }
             __syncthreads();
-            for (uint32_t i = t; i < p.vocab; i += kRowThreads) {
-                const uint32_t key = key_of(x[i]);
-                if (key < last_key || (shift != 24 && (key >> (shift + 8)) != prefix)) continue;
+            walk([&](uint32_t key, uint32_t i) {
+                if (shift != 24 && (key >> (shift + 8)) != prefix) return;
+                if (rank_of(key, i) < after) return;
                 const double depth = depth_of(key, r);
-                if (!(depth < kReach)) continue;
+                if (!(depth < kReach)) return;
+                const uint32_t b = bin_at(depth);
+                if (b < lo || b > hi) return;
                 atomicAdd(&count[(key >> shift) & 255], 1u);
                 if (by_mass) atomicAdd(&mass[(key >> shift) & 255], weight_at(depth, 0.0));
-            }
+            });
             __syncthreads();
             if (t == 0) {
-                int digit = -1;
-                u64 upto = 0;
+                int digit = 0;
+                u64 upto = before;
+                bool any = false;
                 for (int d = 255; d >= 0; --d) {
                     if (count[d] == 0) continue;
-                    if (digit >= 0) before = upto;
+                    if (any) before = upto;
+                    any = true;
                     digit = d;
                     upto = before + (by_mass ? mass[d] : count[d]);
                     if (upto >= limit) break;
                 }
-                sh[0] = static_cast<u64>(prefix << 8 | static_cast<uint32_t>(digit));
+                sh[0] = prefix << 8 | static_cast<uint32_t>(digit);
                 sh[1] = before;
                 sh[2] = count[digit];
             }
@@ -377,56 +441,53 @@ __device__ u64 cut_by_digits(const SampleParams &p, const float *x, const Row &r
             before = sh[1];
             __syncthreads();
         }
-        uint32_t ties = static_cast<uint32_t>(sh[2]);
+        u64 ties = sh[2];   // of the key `prefix`: as many stay as begin below the limit
         const u64 left = limit > before ? limit - before : 1;
         const u64 each = by_mass ? weight_at(depth_of(prefix, r), 0.0) : 1;
-        if (each != 0) {
-            const u64 need = (left + each - 1) / each;
-            if (need < ties) ties = static_cast<uint32_t>(need);
-        }
-        if (prefix != last_key || ties < last_ties) last_ties = ties;
-        last_key = prefix;
+        if (each != 0 && (left + each - 1) / each < ties) ties = (left + each - 1) / each;
+        // the index of the last of them: ties per chunk, then that chunk
+        for (uint32_t c = t; c < kMaxChunks; c += kRowThreads) ties_of[c] = 0;
         __syncthreads();
+        walk([&](uint32_t key, uint32_t i) {
+            if (key == prefix && rank_of(key, i) >= after) atomicAdd(&ties_of[i / kChunk], 1ull);
+        });
+        __syncthreads();
+        u64 all;
+        const u64 mine = ties_of[t], below = sum_below<kRowThreads>(mine, s.cut.part, all);
+        if (below < ties && ties <= below + mine) { sh[3] = t; sh[4] = ties - below; }
+        __syncthreads();
+        const uint32_t i = static_cast<uint32_t>(sh[3]) * kChunk + t;
+        const uint32_t key = i < p.vocab ? key_of(x[i]) : 0;
+        const u64 is = key == prefix && rank_of(key, i) >= after;
+        const u64 under = sum_below<kRowThreads>(is, s.cut.part, all);
+        if (is && under + 1 == sh[4]) sh[5] = rank_of(key, i);
+        __syncthreads();
+        const u64 last = sh[5];
+        __syncthreads();
+        return last;
     };
-    const uint32_t per = (p.vocab + kRowThreads - 1) / kRowThreads;
-    const uint32_t lo = t * per < p.vocab ? t * per : p.vocab, hi = lo + per < p.vocab ? lo + per : p.vocab;
-    auto ties_below = [&]() {   // elements equal to last_key before this thread's range
-        u64 mine = 0, all;
-        for (uint32_t i = lo; i < hi; ++i) mine += key_of(x[i]) == last_key;
-        return static_cast<uint32_t>(sum_below<kRowThreads>(mine, part, all));
-    };
-    if (r.top_k != 0) cut(false, r.top_k);
+    u64 last = 0;
+    if (cut.k_bin < kBins) last = find(false, cut.k_bin, cut.k_bin, 0, r.top_k - cut.k_count);
     if (r.top_p < 1.0) {
-        uint32_t seen = ties_below();
-        u64 sum = 0, all;
-        for (uint32_t i = lo; i < hi; ++i) {
-            const uint32_t key = key_of(x[i]);
-            if (key < last_key || (key == last_key && seen++ >= last_ties)) continue;
-            sum += weight_at(depth_of(key, r), 0.0);
+        u64 kept = cut.all_mass;   // the weight that top_k keeps
+        if (cut.k_bin < kBins) {
+            u64 sum = 0;
+            walk([&](uint32_t key, uint32_t i) {
+                const double depth = depth_of(key, r);
+                if (depth < kReach && bin_at(depth) == cut.k_bin && rank_of(key, i) >= last) sum += weight_at(depth, 0.0);
+            });
+            (void)sum_below<kRowThreads>(sum, s.cut.part, kept);
+            kept += cut.k_mass;
         }
-        (void)sum_below<kRowThreads>(sum, part, all);
-        const double limit = ceil(r.top_p * static_cast<double>(all));
-        cut(true, limit > 1.0 ? static_cast<u64>(limit) : 1ull);   // rank 0 always stays
+        const double limit_f = ceil(r.top_p * static_cast<double>(kept));
+        const u64 limit = limit_f > 1.0 ? static_cast<u64>(limit_f) : 1ull;   // rank 0 always stays
+        last = find(true, cut.sure, cut.last, last, limit - cut.sure_mass);
     }
-    // the index of the last tie that stays
-    uint32_t seen = ties_below();
-    __syncthreads();
-    if (t == 0) sh[3] = 0xffffffffu;
-    __syncthreads();
-    for (uint32_t i = lo; i < hi; ++i)
-        if (key_of(x[i]) == last_key && ++seen == last_ties) sh[3] = i;
-    __syncthreads();
-    return rank_of(last_key, static_cast<uint32_t>(sh[3]));
+    return last;
 }
 
 __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SampleParams p) {
-    __shared__ u64 cand[kMaxCandidates];
-    __shared__ u64 mass_upto[kBins];
-    __shared__ uint32_t count_upto[kBins], found[3];
-    __shared__ u64 part[kRowThreads / kWave];
-    __shared__ u64 chunk_mass[kMaxChunks];
-    __shared__ u64 shared_last, shared_target;
-    __shared__ uint32_t shared_at, bounds[2];
+    __shared__ DrawSpace s;
     const uint32_t t = threadIdx.x, row = blockIdx.x;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
     const u64 best = row_best(p, row);
@@ -441,153 +502,143 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
         if (t == 0) p.out[row] = q8mi_argmax_pair{x[i], static_cast<int32_t>(i)};
         return;
     }
+    const bool cuts = r.top_k != 0 || r.top_p < 1.0;
+    const uint32_t n = cuts ? p.n_candidates[row] : 0;
+    u64 mine = t < p.chunks && n <= kMaxCandidates ? p.chunk_mass[static_cast<uint64_t>(row) * p.chunks + t] : 0;
+    s.chunk_mass[t] = mine;
     u64 last = 0;   // rank of the last kept element: everything from it up is kept
-    for (uint32_t c = t; c < p.chunks; c += kRowThreads) chunk_mass[c] = 0;
-    bool from_chunks = true;   // launches 2 and 3 have left the chunks' sums
-    if (r.top_k != 0 || r.top_p < 1.0) {
-        const uint32_t n = p.n_candidates[row];
+    if (cuts) {
+        const Cut cut = find_cut<kRowThreads>(p, row, r, s.cut);
         if (n > kMaxCandidates) {
-            last = cut_by_digits(p, x, r, cand);
-            from_chunks = false;
-        } else {
-            const Cut cut = find_cut(p, row, r, mass_upto, count_upto, found);
-            uint32_t size = 2;
-            while (size < n) size *= 2;
-            for (uint32_t i = t; i < size; i += kRowThreads) cand[i] = i < n ? p.candidates[static_cast<uint64_t>(row) * kMaxCandidates + i] : 0;
-            __syncthreads();
-            for (uint32_t k = 2; k <= size; k *= 2)           // bitonic, descending
-                for (uint32_t j = k / 2; j > 0; j /= 2) {
-                    for (uint32_t i = t; i < size; i += kRowThreads) {
-                        const uint32_t o = i ^ j;
-                        if (o > i) {
-                            const u64 a = cand[i], b = cand[o];
-                            if ((a < b) == ((i & k) == 0)) { cand[i] = b; cand[o] = a; }
-                        }
-                    }
-                    __syncthreads();
+            last = cut_by_digits(p, x, r, cut, s);
+            for (uint32_t i = 4 * t; i < p.vocab; i += 4 * kRowThreads) {
+                float v[4];
+                load4(p, x, i, v);
+                u64 sum = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const uint32_t key = key_of(v[k]);
+                    if (rank_of(key, i + k) >= last) sum += weight_at(depth_of(key, r), r.min_p);
                 }
-            // this thread's candidates, neighbours in rank: 4 * t ..
-            u64 w[4], sum = 0, all;
-            uint32_t bin[4];
+                if (sum) atomicAdd(&s.chunk_mass[i / kChunk], sum);
+            }
+            __syncthreads();
+        } else {
+            const u64 *list = p.candidates + static_cast<uint64_t>(row) * kMaxCandidates;
+            u64 w[4], sum = 0, all;   // this thread's candidates, neighbours in rank, from `c0` on
+            uint32_t bin[4], c0, held;
+            if (n <= kRankThreads) {
+                u64 my = 0;
+                if (t < n) { my = list[t]; s.cand[kMaxCandidates / 2 + t] = my; }
+                __syncthreads();
+                if (t < n) {
+                    uint32_t above = 0;
+                    for (uint32_t i = 0; i < n; ++i) above += s.cand[kMaxCandidates / 2 + i] > my;
+                    s.cand[above] = my;   // ranks differ
+                }
+                __syncthreads();
+                c0 = t; held = t < n ? 1 : 0;
+            } else {
+                uint32_t size = 2;
+                while (size < n) size *= 2;
+                for (uint32_t i = t; i < size; i += kRowThreads) s.cand[i] = i < n ? list[i] : 0;
+                __syncthreads();
+                for (uint32_t k = 2; k <= size; k *= 2)           // bitonic, descending
+                    for (uint32_t j = k / 2; j > 0; j /= 2) {
+                        for (uint32_t i = t; i < size; i += kRowThreads) {
+                            const uint32_t o = i ^ j;
+                            if (o > i) {
+                                const u64 a = s.cand[i], b = s.cand[o];
+                                if ((a < b) == ((i & k) == 0)) { s.cand[i] = b; s.cand[o] = a; }
+                            }
+                        }
+                        __syncthreads();
+                    }
+                c0 = 4 * t; held = c0 < n ? (n - c0 < 4 ? n - c0 : 4) : 0;
+            }
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t c = 4 * t + i;
-                const double depth = c < n ? depth_of(static_cast<uint32_t>(cand[c] >> 32), r) : INFINITY;
+                const double depth = i < held ? depth_of(static_cast<uint32_t>(s.cand[c0 + i] >> 32), r) : INFINITY;
                 w[i] = weight_at(depth, 0.0);
-                bin[i] = c < n ? bin_at(depth) : kBins;
+                bin[i] = i < held ? bin_at(depth) : kBins;
                 sum += w[i];
             }
-            // k: candidates of the steps up to cut.last begin at 0; those of a separate k_bin behind them
-            if (t == 0) { bounds[0] = bounds[1] = n; shared_last = 0; }
-            const u64 before_me = sum_below<kRowThreads>(sum, part, all);
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-                if (4 * t + i < n && bin[i] == cut.k_bin) atomicMin(&bounds[0], 4 * t + i);   // the first candidate of the k step
-            __syncthreads();
-            uint32_t kept = n;          // candidates in rank order that stay
-            u64 mass_k = mass_upto[kBins - 1];
+            uint32_t kept = n;   // candidates that stay: a prefix of their ranks
+            u64 mass_k = cut.all_mass;
             if (cut.k_bin < kBins) {
-                const uint32_t first = bounds[0], count0 = cut.k_bin ? count_upto[cut.k_bin - 1] : 0;
-                kept = first + (r.top_k - count0);
-                // the k step's kept weight: sum over [first, kept)
-                u64 in_step = 0;
+                if (t == 0) s.bounds[0] = n;
+                __syncthreads();
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i)
-                    if (4 * t + i >= first && 4 * t + i < kept) in_step += w[i];
-                u64 step_all;
-                (void)sum_below<kRowThreads>(in_step, part, step_all);
-                mass_k = (cut.k_bin ? mass_upto[cut.k_bin - 1] : 0) + step_all;
+                    if (i < held && bin[i] == cut.k_bin) atomicMin(&s.bounds[0], c0 + i);   // the first candidate of that step
+                __syncthreads();
+                const uint32_t first = s.bounds[0];
+                kept = first + (r.top_k - cut.k_count);
+                if (r.top_p < 1.0) {
+                    u64 in_step = 0, step_all;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i)
+                        if (i < held && c0 + i >= first && c0 + i < kept) in_step += w[i];
+                    (void)sum_below<kRowThreads>(in_step, s.cut.part, step_all);
+                    mass_k = cut.k_mass + step_all;
+                }
             }
             if (r.top_p < 1.0) {
                 const double limit_f = ceil(r.top_p * static_cast<double>(mass_k));
                 const u64 limit = limit_f > 1.0 ? static_cast<u64>(limit_f) : 1ull;   // rank 0 always stays
-                const u64 sure = cut.sure ? mass_upto[cut.sure - 1] : 0;
-                // candidates of the steps first .. last follow one another in rank from the mass `sure` on
-                u64 run = sure + before_me;
+                if (t == 0) s.bounds[1] = 0;
+                u64 run = cut.sure_mass + sum_below<kRowThreads>(sum, s.cut.part, all);
                 uint32_t stay = 0;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
-                    if (4 * t + i < n && bin[i] <= cut.last && run < limit) stay = 4 * t + i + 1;
+                    if (i < held && bin[i] <= cut.last && run < limit) stay = c0 + i + 1;
                     run += w[i];
                 }
-                if (t == 0) bounds[1] = 0;
+                if (stay) atomicMax(&s.bounds[1], stay);
                 __syncthreads();
-                if (stay) atomicMax(&bounds[1], stay);
-                __syncthreads();
-                kept = bounds[1] < kept ? bounds[1] : kept;
+                kept = s.bounds[1] < kept ? s.bounds[1] : kept;
             }
-            if (kept > 0 && t == 0) shared_last = cand[kept - 1];
-            __syncthreads();
-            last = shared_last;
-            if (kept == 0) last = 0;   // everything above the candidates: handled by the sums below
-            for (uint32_t c = t; c < p.chunks; c += kRowThreads) chunk_mass[c] = p.chunk_mass[row * p.chunks + c];
-            __syncthreads();
+            last = s.cand[kept - 1];   // each cut keeps a candidate: the step before which it falls short holds it
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t c = 4 * t + i;
-                if (c < kept && w[i] != 0) {
-                    const uint32_t index = 0xffffffffu - static_cast<uint32_t>(cand[c]);
-                    const u64 kept_w = weight_at(depth_of(static_cast<uint32_t>(cand[c] >> 32), r), r.min_p);
-                    atomicAdd(&chunk_mass[index / kChunk], kept_w);
+            for (uint32_t i = 0; i < 4; ++i)
+                if (i < held && c0 + i < kept) {
+                    const uint32_t index = 0xffffffffu - static_cast<uint32_t>(s.cand[c0 + i]);
+                    const u64 kept_w = r.min_p > 0.0 ? weight_at(depth_of(static_cast<uint32_t>(s.cand[c0 + i] >> 32), r), r.min_p) : w[i];
+                    if (kept_w) atomicAdd(&s.chunk_mass[index / kChunk], kept_w);
                 }
-            }
             __syncthreads();
         }
-    } else {
-        for (uint32_t c = t; c < p.chunks; c += kRowThreads) chunk_mass[c] = p.chunk_mass[row * p.chunks + c];
-        __syncthreads();
-    }
-    auto kept_weight = [&](float v, uint32_t i) -> u64 {
-        const uint32_t key = key_of(v);
-        return rank_of(key, i) >= last ? weight_at(depth_of(key, r), r.min_p) : 0;
-    };
-    if (!from_chunks) {
-        __syncthreads();
-        for (uint32_t c = 0; c < p.chunks; ++c) {
-            float v[4];
-            load4(p, x, c * kChunk + 4 * t, v);
-            u64 sum = 0, all;
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) sum += kept_weight(v[k], c * kChunk + 4 * t + k);
-            (void)sum_below<kRowThreads>(sum, part, all);
-            if (t == 0) chunk_mass[c] = all;
-        }
-        __syncthreads();
+        mine = s.chunk_mass[t];
     }
 
     // the chunk, then the element, at which the sum exceeds uniform * all
     u64 all;
-    const u64 mine = t < p.chunks ? chunk_mass[t] : 0;
-    const u64 before = sum_below<kRowThreads>(mine, part, all);
+    const u64 before = sum_below<kRowThreads>(mine, s.cut.part, all);
     float u = p.uniform[row];
     u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
     u64 target = static_cast<u64>(static_cast<double>(u) * static_cast<double>(all));
     if (target >= all) target = all - 1;
-    if (before <= target && target < before + mine) { shared_at = t; shared_target = target - before; }
+    if (before <= target && target < before + mine) { s.at = t; s.target = target - before; }
     __syncthreads();
-    const uint32_t chunk = shared_at;
-    target = shared_target;
-    float v[4];
-    u64 w[4], sum = 0;
-    load4(p, x, chunk * kChunk + 4 * t, v);
-#pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) {
-        w[k] = kept_weight(v[k], chunk * kChunk + 4 * t + k);
-        sum += w[k];
+    const uint32_t i = s.at * kChunk + t;
+    target = s.target;
+    u64 w = 0;
+    float v = 0.0f;
+    if (i < p.vocab) {
+        v = x[i];
+        const uint32_t key = key_of(v);
+        if (rank_of(key, i) >= last) w = weight_at(depth_of(key, r), r.min_p);
     }
-    u64 run = sum_below<kRowThreads>(sum, part, all);
-    if (run <= target && target < run + sum) {
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-            if (run <= target && target < run + w[k]) p.out[row] = q8mi_argmax_pair{v[k], static_cast<int32_t>(chunk * kChunk + 4 * t + k)};
-            run += w[k];
-        }
-    }
+    const u64 run = sum_below<kRowThreads>(w, s.cut.part, all);
+    if (run <= target && target < run + w) p.out[row] = q8mi_argmax_pair{v, static_cast<int32_t>(i)};
 }
 
 uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
-// u64 words of a row: best and chunk_mass, bin_mass, candidates, bin_count; n_candidates behind all rows
+// u64 words of a row: best (at most one a chunk) and chunk_mass, bin_mass, candidates, bin_count; n_candidates behind all rows
 uint64_t row_words(uint32_t vocab) { return 2ull * chunks_of(vocab) + kBins + kMaxCandidates + kBins / 2; }
+// Chunks of a workgroup: one while that leaves CUs idle, up to kMostSpan where rows are many (the histogram of a workgroup
+// is then cleared and added to the row's once for several chunks).
+constexpr uint32_t kMostSpan = 16, kGridWanted = 1024;
 
 }  // namespace
 }  // namespace q8mi
@@ -611,6 +662,9 @@ extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, 
     p.logits = logits; p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
     p.uniform = uniform; p.out = out; p.vocab = vocab; p.stride = stride;
     p.chunks = chunks_of(vocab);
+    const uint64_t crowd = static_cast<uint64_t>(batch) * p.chunks / kGridWanted;
+    p.span = crowd < 1 ? 1 : crowd > kMostSpan ? kMostSpan : static_cast<uint32_t>(crowd);
+    p.spans = (p.chunks + p.span - 1) / p.span;
     p.vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (batch == 1 || stride % 4 == 0);
     u64 *words = static_cast<u64 *>(scratch);
     auto take = [&](uint64_t n) { u64 *at = words; words += n; return at; };
@@ -621,7 +675,7 @@ extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, 
     p.bin_count = reinterpret_cast<uint32_t *>(take(static_cast<uint64_t>(batch) * kBins / 2));
     p.n_candidates = reinterpret_cast<uint32_t *>(words);
     hipStream_t s = as_stream(stream);
-    const dim3 grid(p.chunks, batch);
+    const dim3 grid(p.spans, batch);
     sample_best_kernel<<<grid, kChunkThreads, 0, s>>>(p);
     sample_weigh_kernel<<<grid, kChunkThreads, 0, s>>>(p);
     if (top_k != nullptr || top_p != nullptr) sample_collect_kernel<<<grid, kChunkThreads, 0, s>>>(p);
