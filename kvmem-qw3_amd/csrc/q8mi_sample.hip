@@ -35,6 +35,13 @@ constexpr double kOne = 4398046511104.0;              // 2^42: the weight of the
 
 typedef unsigned long long u64;
 
+// Where the cuts fall: steps below `sure` are kept, steps sure .. last hold the last rank, step `k_bin` the top_k-th
+// (kBins: nothing is cut there); the weight of the steps below `sure`, below k_bin, and of all; the count below k_bin.
+struct Cut {
+    uint32_t sure, last, k_bin, k_count;
+    u64 sure_mass, k_mass, all_mass;
+};
+
 struct SampleParams {
     const float *logits;
     const float *temperature, *top_p, *min_p, *uniform;
@@ -44,6 +51,8 @@ struct SampleParams {
     u64 *chunk_mass;    // [row][chunk]: weight kept for certain
     u64 *bin_mass;      // [row][kBins]
     u64 *candidates;    // [row][kMaxCandidates]: key << 32 | ~index
+    u64 *top;           // [row]: rank 0 of the row (launch 2)
+    Cut *cut;           // [row] (launch 3)
     uint32_t *bin_count;     // [row][kBins]
     uint32_t *n_candidates;  // [row]
     uint32_t vocab, stride, chunks;
@@ -67,7 +76,7 @@ __device__ __forceinline__ u64 rank_of(uint32_t key, uint32_t index) {   // larg
 struct Row {
     float max;
     double per_unit;   // 1 / temperature
-    double min_p;      // 0: off
+    double deepest;    // what min_p keeps lies no deeper: p >= min_p <=> depth <= -log(min_p)
     uint32_t top_k;    // 0: off
     double top_p;      // 1: off
     bool greedy;
@@ -79,7 +88,7 @@ __device__ __forceinline__ Row row_of(const SampleParams &p, uint32_t row, uint3
     r.greedy = !(t > 0.0f);
     r.per_unit = r.greedy ? 1.0 : 1.0 / static_cast<double>(t);
     const float min_p = p.min_p ? p.min_p[row] : 0.0f;
-    r.min_p = min_p > 0.0f ? (min_p < 1.0f ? min_p : 1.0) : 0.0;
+    r.deepest = min_p > 0.0f ? (min_p < 1.0f ? -log(static_cast<double>(min_p)) : 0.0) : INFINITY;
     const int32_t k = p.top_k ? p.top_k[row] : 0;
     r.top_k = k > 0 && static_cast<uint32_t>(k) < p.vocab ? k : 0;
     const float top_p = p.top_p ? p.top_p[row] : 1.0f;
@@ -92,11 +101,32 @@ __device__ __forceinline__ double depth_of(uint32_t key, const Row &r) {
     const float v = logit_of(key);
     return v == r.max ? 0.0 : (static_cast<double>(r.max) - static_cast<double>(v)) * r.per_unit;
 }
-__device__ __forceinline__ u64 weight_at(double depth, double min_p) {
+// exp(-depth) * 2^42 rounded to an integer: 2^(42 - depth * log2(e)) = 2^n * 2^f, 0 <= f < 1, with 2^f from its series in
+// f * ln(2) - ln(2) / 2 around the middle (terms up to the 12th power: below 1e-16), whose bits are the integer but for a
+// shift.  Off by 1e-14 of itself and the last rounding; depth 0 gives 2^42.
+__device__ __forceinline__ u64 weight_at(double depth) {
     if (!(depth < kReach)) return 0;
-    const double s = exp(-depth);
-    return s >= min_p ? static_cast<u64>(rint(s * kOne)) : 0;
+    if (depth == 0.0) return static_cast<u64>(kOne);
+    const double y = fma(depth, -1.44269504088896340736, 42.0), n = floor(y);
+    const double z = fma(y - n, 0.693147180559945309417, -0.346573590279972654709);
+    double e = 1.0 / 479001600.0;
+    e = fma(e, z, 1.0 / 39916800.0);
+    e = fma(e, z, 1.0 / 3628800.0);
+    e = fma(e, z, 1.0 / 362880.0);
+    e = fma(e, z, 1.0 / 40320.0);
+    e = fma(e, z, 1.0 / 5040.0);
+    e = fma(e, z, 1.0 / 720.0);
+    e = fma(e, z, 1.0 / 120.0);
+    e = fma(e, z, 1.0 / 24.0);
+    e = fma(e, z, 1.0 / 6.0);
+    e = fma(e, z, 0.5);
+    e = fma(e, z, 1.0);
+    e = fma(e, z, 1.0) * 1.41421356237309504880;   // 2^f; rounding may take it to 2, whose bits still follow on
+    const u64 bits = __builtin_bit_cast(u64, e) - (1022ull << 52);           // (exponent + 1) << 52 | fraction: as an integer 2^52 * 2^f
+    const int shift = 52 - static_cast<int>(n);                                                  // 10 .. 56
+    return (bits + (1ull << (shift - 1))) >> shift;
 }
+__device__ __forceinline__ u64 kept_weight_at(double depth, const Row &r) { return depth <= r.deepest ? weight_at(depth) : 0; }
 __device__ __forceinline__ uint32_t bin_at(double depth) { return static_cast<uint32_t>(depth * kBinsPerUnit); }
 
 __device__ __forceinline__ u64 xor_u64(u64 v, int d) { return __shfl_xor(v, d); }
@@ -213,12 +243,19 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
     const u64 best = row_best(p, row);
+    if (blockIdx.x == 0 && t == 0) p.top[row] = best;
     const Row r = row_of(p, row, static_cast<uint32_t>(best >> 32));
     if (best >> 32 == 0 || r.greedy) return;
     const bool by_count = r.top_k != 0, by_mass = r.top_p < 1.0;   // each needs its half of the histogram
     if (by_count || by_mass) {
         for (uint32_t b = t; b < kBins; b += kChunkThreads) { mass[b] = 0; count[b] = 0; }
         __syncthreads();
+        // The row's steps are added up by atomics, so few are sent.  Where this span alone has top_k above a step, the cut
+        // lies above it, too.  Without top_k: all of a row of `vocab` logits below depth d weigh at most vocab * exp(-d), and
+        // the cut does not lie where this is no more than the 1 - top_p of the whole that may be dropped; the whole is at
+        // least 1.  From there on only the sum counts, in the last step, which no logit reaches.
+        const double far = by_count ? kReach : fmin(kReach, log(static_cast<double>(p.vocab) / (1.0 - r.top_p)) + 0.1);
+        u64 rest = 0;
         walk_span(p, x, [&](const float (&v)[4], uint32_t) {
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
@@ -226,13 +263,26 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
                 if (!(depth < kReach)) continue;
                 const uint32_t b = bin_at(depth);
                 if (by_count) atomicAdd(&count[b], 1u);
-                if (by_mass) atomicAdd(&mass[b], weight_at(depth, 0.0));
+                if (!by_mass) continue;
+                const u64 w = weight_at(depth);
+                if (depth < far) atomicAdd(&mass[b], w);
+                else rest += w;
             }
         }, [](uint32_t) {});
+        rest = wave_sum_u64(rest);
+        if (t % kWave == 0 && rest != 0) atomicAdd(&mass[kBins - 1], rest);
         __syncthreads();
-        for (uint32_t b = t; b < kBins; b += kChunkThreads) {
-            if (count[b] != 0) atomicAdd(&p.bin_count[static_cast<uint64_t>(row) * kBins + b], count[b]);
+        uint32_t mine[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) mine[k] = count[4 * t + k];
+        u64 all, before = by_count ? sum_below<kChunkThreads>((mine[0] + mine[1]) + (mine[2] + mine[3]), part[0], all) : 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            const uint32_t b = 4 * t + k;
+            if (by_count && before >= r.top_k) break;
+            if (mine[k] != 0) atomicAdd(&p.bin_count[static_cast<uint64_t>(row) * kBins + b], mine[k]);
             if (mass[b] != 0) atomicAdd(&p.bin_mass[static_cast<uint64_t>(row) * kBins + b], mass[b]);
+            before += mine[k];
         }
         return;
     }
@@ -240,7 +290,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
     walk_span(p, x, [&](const float (&v)[4], uint32_t) {
         sum = 0;
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) sum += weight_at(depth_of(key_of(v[k]), r), r.min_p);
+        for (uint32_t k = 0; k < 4; ++k) sum += kept_weight_at(depth_of(key_of(v[k]), r), r);
     }, [&](uint32_t chunk) {
         sum = wave_sum_u64(sum);
         u64 *mine = part[chunk % kAhead];   // another one is written before the next barrier
@@ -250,12 +300,6 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
     });
 }
 
-// Where the cuts fall: steps below `sure` are kept, steps sure .. last hold the last rank, step `k_bin` the top_k-th
-// (kBins: nothing is cut there); the weight of the steps below `sure`, below k_bin, and of all; the count below k_bin.
-struct Cut {
-    uint32_t sure, last, k_bin, k_count;
-    u64 sure_mass, k_mass, all_mass;
-};
 struct CutSpace {   // LDS
     u64 mass_upto[kBins];
     u64 part[kRowThreads / kWave];
@@ -331,10 +375,15 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
     __shared__ u64 part[kAhead][kChunkThreads / kWave];
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
-    const u64 best = row_best(p, row);
+    const u64 best = p.top[row];
     const Row r = row_of(p, row, static_cast<uint32_t>(best >> 32));
     if (best >> 32 == 0 || r.greedy || !(r.top_k != 0 || r.top_p < 1.0)) return;
     const Cut cut = find_cut<kChunkThreads>(p, row, r, space);
+    if (blockIdx.x == 0 && t == 0) p.cut[row] = cut;
+    // logits well below the last step of interest need no 64-bit depth
+    const uint32_t deep = cut.k_bin < kBins ? cut.k_bin : cut.last;
+    const double reach = (deep + 1) / kBinsPerUnit / r.per_unit;
+    const float least = isfinite(r.max) && reach < 1e30 ? static_cast<float>(r.max - reach) - (fabsf(r.max) + static_cast<float>(reach)) * 1e-6f : -INFINITY;
     u64 *list = p.candidates + static_cast<uint64_t>(row) * kMaxCandidates;
     u64 sum = 0;
     walk_span(p, x, [&](const float (&v)[4], uint32_t i) {
@@ -342,10 +391,11 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
         uint32_t mine = 0;   // elements to collect
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
+            if (!(v[k] >= least)) continue;
             const double depth = depth_of(key_of(v[k]), r);
             if (!(depth < kReach)) continue;
             const uint32_t b = bin_at(depth);
-            if (b < cut.sure) sum += weight_at(depth, r.min_p);
+            if (b < cut.sure) sum += kept_weight_at(depth, r);
             else if (b <= cut.last || b == cut.k_bin) mine |= 1u << k;
         }
         // places in the list: one atomic a wave
@@ -379,7 +429,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
 // ---- 4 ----------------------------------------------------------------------------------------------------------------
 struct DrawSpace {   // LDS
     u64 cand[kMaxCandidates];
-    CutSpace cut;
+    u64 part[kRowThreads / kWave];
     u64 chunk_mass[kMaxChunks];
     u64 last, target;
     uint32_t at, bounds[2];
@@ -417,7 +467,7 @@ __device__ u64 cut_by_digits(const SampleParams &p, const float *x, const Row &r
                 const uint32_t b = bin_at(depth);
                 if (b < lo || b > hi) return;
                 atomicAdd(&count[(key >> shift) & 255], 1u);
-                if (by_mass) atomicAdd(&mass[(key >> shift) & 255], weight_at(depth, 0.0));
+                if (by_mass) atomicAdd(&mass[(key >> shift) & 255], weight_at(depth));
             });
             __syncthreads();
             if (t == 0) {
@@ -443,7 +493,7 @@ __device__ u64 cut_by_digits(const SampleParams &p, const float *x, const Row &r
         }
         u64 ties = sh[2];   // of the key `prefix`: as many stay as begin below the limit
         const u64 left = limit > before ? limit - before : 1;
-        const u64 each = by_mass ? weight_at(depth_of(prefix, r), 0.0) : 1;
+        const u64 each = by_mass ? weight_at(depth_of(prefix, r)) : 1;
         if (each != 0 && (left + each - 1) / each < ties) ties = (left + each - 1) / each;
         // the index of the last of them: ties per chunk, then that chunk
         for (uint32_t c = t; c < kMaxChunks; c += kRowThreads) ties_of[c] = 0;
@@ -453,13 +503,13 @@ __device__ u64 cut_by_digits(const SampleParams &p, const float *x, const Row &r
         });
         __syncthreads();
         u64 all;
-        const u64 mine = ties_of[t], below = sum_below<kRowThreads>(mine, s.cut.part, all);
+        const u64 mine = ties_of[t], below = sum_below<kRowThreads>(mine, s.part, all);
         if (below < ties && ties <= below + mine) { sh[3] = t; sh[4] = ties - below; }
         __syncthreads();
         const uint32_t i = static_cast<uint32_t>(sh[3]) * kChunk + t;
         const uint32_t key = i < p.vocab ? key_of(x[i]) : 0;
         const u64 is = key == prefix && rank_of(key, i) >= after;
-        const u64 under = sum_below<kRowThreads>(is, s.cut.part, all);
+        const u64 under = sum_below<kRowThreads>(is, s.part, all);
         if (is && under + 1 == sh[4]) sh[5] = rank_of(key, i);
         __syncthreads();
         const u64 last = sh[5];
@@ -474,9 +524,9 @@ __device__ u64 cut_by_digits(const SampleParams &p, const float *x, const Row &r
             u64 sum = 0;
             walk([&](uint32_t key, uint32_t i) {
                 const double depth = depth_of(key, r);
-                if (depth < kReach && bin_at(depth) == cut.k_bin && rank_of(key, i) >= last) sum += weight_at(depth, 0.0);
+                if (depth < kReach && bin_at(depth) == cut.k_bin && rank_of(key, i) >= last) sum += weight_at(depth);
             });
-            (void)sum_below<kRowThreads>(sum, s.cut.part, kept);
+            (void)sum_below<kRowThreads>(sum, s.part, kept);
             kept += cut.k_mass;
         }
         const double limit_f = ceil(r.top_p * static_cast<double>(kept));
@@ -490,7 +540,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
     __shared__ DrawSpace s;
     const uint32_t t = threadIdx.x, row = blockIdx.x;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
-    const u64 best = row_best(p, row);
+    const u64 best = p.top[row];
     const uint32_t top = static_cast<uint32_t>(best >> 32);
     if (top == 0) {
         if (t == 0) p.out[row] = q8mi_argmax_pair{-INFINITY, -1};
@@ -508,7 +558,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
     s.chunk_mass[t] = mine;
     u64 last = 0;   // rank of the last kept element: everything from it up is kept
     if (cuts) {
-        const Cut cut = find_cut<kRowThreads>(p, row, r, s.cut);
+        const Cut cut = p.cut[row];
         if (n > kMaxCandidates) {
             last = cut_by_digits(p, x, r, cut, s);
             for (uint32_t i = 4 * t; i < p.vocab; i += 4 * kRowThreads) {
@@ -518,7 +568,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k) {
                     const uint32_t key = key_of(v[k]);
-                    if (rank_of(key, i + k) >= last) sum += weight_at(depth_of(key, r), r.min_p);
+                    if (rank_of(key, i + k) >= last) sum += kept_weight_at(depth_of(key, r), r);
                 }
                 if (sum) atomicAdd(&s.chunk_mass[i / kChunk], sum);
             }
@@ -559,7 +609,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 const double depth = i < held ? depth_of(static_cast<uint32_t>(s.cand[c0 + i] >> 32), r) : INFINITY;
-                w[i] = weight_at(depth, 0.0);
+                w[i] = weight_at(depth);
                 bin[i] = i < held ? bin_at(depth) : kBins;
                 sum += w[i];
             }
@@ -579,7 +629,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
 #pragma unroll
                     for (uint32_t i = 0; i < 4; ++i)
                         if (i < held && c0 + i >= first && c0 + i < kept) in_step += w[i];
-                    (void)sum_below<kRowThreads>(in_step, s.cut.part, step_all);
+                    (void)sum_below<kRowThreads>(in_step, s.part, step_all);
                     mass_k = cut.k_mass + step_all;
                 }
             }
@@ -587,7 +637,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
                 const double limit_f = ceil(r.top_p * static_cast<double>(mass_k));
                 const u64 limit = limit_f > 1.0 ? static_cast<u64>(limit_f) : 1ull;   // rank 0 always stays
                 if (t == 0) s.bounds[1] = 0;
-                u64 run = cut.sure_mass + sum_below<kRowThreads>(sum, s.cut.part, all);
+                u64 run = cut.sure_mass + sum_below<kRowThreads>(sum, s.part, all);
                 uint32_t stay = 0;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
@@ -603,7 +653,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
             for (uint32_t i = 0; i < 4; ++i)
                 if (i < held && c0 + i < kept) {
                     const uint32_t index = 0xffffffffu - static_cast<uint32_t>(s.cand[c0 + i]);
-                    const u64 kept_w = r.min_p > 0.0 ? weight_at(depth_of(static_cast<uint32_t>(s.cand[c0 + i] >> 32), r), r.min_p) : w[i];
+                    const u64 kept_w = depth_of(static_cast<uint32_t>(s.cand[c0 + i] >> 32), r) <= r.deepest ? w[i] : 0;
                     if (kept_w) atomicAdd(&s.chunk_mass[index / kChunk], kept_w);
                 }
             __syncthreads();
@@ -613,7 +663,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
 
     // the chunk, then the element, at which the sum exceeds uniform * all
     u64 all;
-    const u64 before = sum_below<kRowThreads>(mine, s.cut.part, all);
+    const u64 before = sum_below<kRowThreads>(mine, s.part, all);
     float u = p.uniform[row];
     u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
     u64 target = static_cast<u64>(static_cast<double>(u) * static_cast<double>(all));
@@ -627,15 +677,15 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
     if (i < p.vocab) {
         v = x[i];
         const uint32_t key = key_of(v);
-        if (rank_of(key, i) >= last) w = weight_at(depth_of(key, r), r.min_p);
+        if (rank_of(key, i) >= last) w = kept_weight_at(depth_of(key, r), r);
     }
-    const u64 run = sum_below<kRowThreads>(w, s.cut.part, all);
+    const u64 run = sum_below<kRowThreads>(w, s.part, all);
     if (run <= target && target < run + w) p.out[row] = q8mi_argmax_pair{v, static_cast<int32_t>(i)};
 }
 
 uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
-// u64 words of a row: best (at most one a chunk) and chunk_mass, bin_mass, candidates, bin_count; n_candidates behind all rows
-uint64_t row_words(uint32_t vocab) { return 2ull * chunks_of(vocab) + kBins + kMaxCandidates + kBins / 2; }
+// u64 words of a row: best (at most one a chunk) and chunk_mass, bin_mass, candidates, bin_count, top, cut; n_candidates behind all rows
+uint64_t row_words(uint32_t vocab) { return 2ull * chunks_of(vocab) + kBins + kMaxCandidates + kBins / 2 + 1 + sizeof(Cut) / 8; }
 // Chunks of a workgroup: one while that leaves CUs idle, up to kMostSpan where rows are many (the histogram of a workgroup
 // is then cleared and added to the row's once for several chunks).
 constexpr uint32_t kMostSpan = 16, kGridWanted = 1024;
@@ -673,6 +723,8 @@ extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, 
     p.bin_mass = take(static_cast<uint64_t>(batch) * kBins);
     p.candidates = take(static_cast<uint64_t>(batch) * kMaxCandidates);
     p.bin_count = reinterpret_cast<uint32_t *>(take(static_cast<uint64_t>(batch) * kBins / 2));
+    p.top = take(batch);
+    p.cut = reinterpret_cast<Cut *>(take(static_cast<uint64_t>(batch) * sizeof(Cut) / 8));
     p.n_candidates = reinterpret_cast<uint32_t *>(words);
     hipStream_t s = as_stream(stream);
     const dim3 grid(p.spans, batch);
