@@ -6,15 +6,17 @@
 // free of their order, so that neither the split of a row nor the arrival of atomics moves a border.
 //
 // No sort of the row.  Four launches, the first three over (spans of chunks of 1024 logits) x rows:
-//   1  largest (logit, lowest index) of each span; clears the row's counters
-//   2  weights; where nothing is cut but by min-p, their sum per chunk, else a histogram of count and weight over 1024
-//      steps of 1/32 in (max - logit) / temperature (what lies 31.9 and more below the maximum weighs nothing)
+//   1  largest logit of each chunk; clears the row's counters
+//   2  where top_k is no more than the chunks: the top_k-th largest of their maxima is no larger than the top_k-th logit, so
+//      the few logits from it up are collected.  Otherwise the weights: where nothing is cut but by min-p, their sum per
+//      chunk, else a histogram of count and weight over 1024 steps of 1/32 in (max - logit) / temperature (what lies 31.9
+//      and more below the maximum weighs nothing)
 //   3  the histogram says in which steps the cuts fall: the few logits of those steps are collected, what lies above them
 //      is kept for certain and summed per chunk
 //   4  one workgroup a row ranks the collected logits, takes the cuts in them, finds the chunk that holds the drawn element
 //      and walks it
-// A row with more than 4096 logits in the steps of its cuts (thousands of equal ones, a temperature that levels all) is
-// searched digit by digit of the keys instead, by the fourth launch's workgroup alone.
+// A row with more than 4096 logits to collect (thousands of equal ones, a temperature that levels all) is searched by the
+// fourth launch's workgroup alone, digit by digit of the ranks.
 #include "q8mi_device.hpp"
 #include "q8mi_internal.hpp"
 
@@ -24,9 +26,10 @@ namespace {
 constexpr uint32_t kMaxVocab = 1u << 20;
 constexpr uint32_t kChunk = 1024;                     // logits
 constexpr uint32_t kMaxChunks = kMaxVocab / kChunk;
+constexpr uint32_t kMostSpan = 16;                    // chunks of a workgroup of launches 1 to 3
 constexpr uint32_t kAhead = 4;                        // chunks that a workgroup of launches 1 to 3 loads at a time
 constexpr uint32_t kChunkThreads = kChunk / 4;
-constexpr uint32_t kRowThreads = 1024;                // launch 4
+constexpr uint32_t kRowThreads = 256;                 // launch 4
 constexpr uint32_t kBins = 1024;
 constexpr double kBinsPerUnit = 32.0;
 constexpr double kReach = 31.875;                     // exp(-31.875) * 2^42 rounds to 0
@@ -35,10 +38,11 @@ constexpr double kOne = 4398046511104.0;              // 2^42: the weight of the
 
 typedef unsigned long long u64;
 
-// Where the cuts fall: steps below `sure` are kept, steps sure .. last hold the last rank, step `k_bin` the top_k-th
-// (kBins: nothing is cut there); the weight of the steps below `sure`, below k_bin, and of all; the count below k_bin.
+// Where the cuts fall: steps below `sure` are kept, steps sure .. last hold the last rank, steps k_first .. k_last the
+// top_k-th (kBins: top_k cuts nothing); the weight of the steps below `sure`, below k_first, and of all; the count below
+// k_first.
 struct Cut {
-    uint32_t sure, last, k_bin, k_count;
+    uint32_t sure, last, k_first, k_last, k_count, unused;
     u64 sure_mass, k_mass, all_mass;
 };
 
@@ -47,12 +51,13 @@ struct SampleParams {
     const float *temperature, *top_p, *min_p, *uniform;
     const int32_t *top_k;
     q8mi_argmax_pair *out;
-    u64 *best;          // [row][span]: key << 32 | ~index of the span's rank 0
     u64 *chunk_mass;    // [row][chunk]: weight kept for certain
     u64 *bin_mass;      // [row][kBins]
     u64 *candidates;    // [row][kMaxCandidates]: key << 32 | ~index
-    u64 *top;           // [row]: rank 0 of the row (launch 2)
-    Cut *cut;           // [row] (launch 3)
+    Cut *cut;           // [row] (launch 2 or 3)
+    uint32_t *best;     // [row][chunk]: largest key
+    uint32_t *top;      // [row]: largest key (launch 2)
+    uint32_t *listed;   // [row]: launch 2 has collected everything from rank 0 to the cuts
     uint32_t *bin_count;     // [row][kBins]
     uint32_t *n_candidates;  // [row]
     uint32_t vocab, stride, chunks;
@@ -130,11 +135,6 @@ __device__ __forceinline__ u64 kept_weight_at(double depth, const Row &r) { retu
 __device__ __forceinline__ uint32_t bin_at(double depth) { return static_cast<uint32_t>(depth * kBinsPerUnit); }
 
 __device__ __forceinline__ u64 xor_u64(u64 v, int d) { return __shfl_xor(v, d); }
-__device__ __forceinline__ u64 wave_max_u64(u64 v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) { const u64 o = xor_u64(v, d); v = o > v ? o : v; }
-    return v;
-}
 __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) v += xor_u64(v, d);
@@ -195,57 +195,127 @@ __device__ __forceinline__ void walk_span(const SampleParams &p, const float *x,
     }
 }
 
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    auto larger = [](uint32_t a, int b) { return a > static_cast<uint32_t>(b) ? a : static_cast<uint32_t>(b); };
+    v = larger(v, dpp_i32<kDppXor1>(static_cast<int>(v)));
+    v = larger(v, dpp_i32<kDppXor2>(static_cast<int>(v)));
+    v = larger(v, dpp_i32<kDppRowHalfMirror>(static_cast<int>(v)));
+    v = larger(v, dpp_i32<kDppRowMirror>(static_cast<int>(v)));
+    const uint32_t a = larger(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
+    return larger(larger(a, __builtin_amdgcn_readlane(v, 32)), __builtin_amdgcn_readlane(v, 48));
+}
+
 // ---- 1 ----------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kChunkThreads) void sample_best_kernel(const SampleParams p) {
-    __shared__ u64 part[kChunkThreads / kWave];
-    const uint32_t t = threadIdx.x, row = blockIdx.y;
+    __shared__ uint32_t best[kMostSpan][kChunkThreads / kWave];
+    const uint32_t t = threadIdx.x, row = blockIdx.y, first = blockIdx.x * p.span;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
-    u64 best = 0;
     walk_span(p, x, [&](const float (&v)[4], uint32_t i) {
+        uint32_t key = 0;
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-            const u64 r = rank_of(key_of(v[k]), i + k);
-            best = r > best ? r : best;
-        }
+        for (uint32_t k = 0; k < 4; ++k) key = key_of(v[k]) > key ? key_of(v[k]) : key;
+        key = wave_max_u32(key);
+        if (t % kWave == 0) best[i / kChunk - first][t / kWave] = key;
     }, [](uint32_t) {});
     if (blockIdx.x == 0) {
         for (uint32_t b = t; b < kBins; b += kChunkThreads) {
             p.bin_mass[static_cast<uint64_t>(row) * kBins + b] = 0;
             p.bin_count[static_cast<uint64_t>(row) * kBins + b] = 0;
         }
-        if (t == 0) p.n_candidates[row] = 0;
+        if (t == 0) p.n_candidates[row] = p.listed[row] = 0;
     }
-    best = wave_max_u64(best);
-    if (t % kWave == 0) part[t / kWave] = best;
     __syncthreads();
-    if (t == 0) {
+    if (t < p.span && first + t < p.chunks) {
+        uint32_t key = 0;
 #pragma unroll
-        for (uint32_t w = 1; w < kChunkThreads / kWave; ++w) best = part[w] > best ? part[w] : best;
-        p.best[static_cast<uint64_t>(row) * p.spans + blockIdx.x] = best;
+        for (uint32_t w = 0; w < kChunkThreads / kWave; ++w) key = best[t][w] > key ? best[t][w] : key;
+        p.best[static_cast<uint64_t>(row) * p.chunks + first + t] = key;
     }
 }
 
-// The row's rank 0, by every wave for itself.
-__device__ __forceinline__ u64 row_best(const SampleParams &p, uint32_t row) {
-    u64 best = 0;
-    for (uint32_t c = threadIdx.x % kWave; c < p.spans; c += kWave) {
-        const u64 b = p.best[static_cast<uint64_t>(row) * p.spans + c];
-        best = b > best ? b : best;
+// Places in the row's list for the elements (bits of `mine`) of the four logits v from element i on: one atomic a wave.
+__device__ __forceinline__ void collect(const SampleParams &p, uint32_t row, const float (&v)[4], uint32_t i, uint32_t mine) {
+    const uint32_t n = __popc(mine), lane = threadIdx.x % kWave;
+    if (__builtin_amdgcn_ballot_w64(n != 0) == 0) return;
+    uint32_t upto = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t o = __shfl_up(upto, d);
+        upto += lane >= static_cast<uint32_t>(d) ? o : 0;
     }
-    return wave_max_u64(best);
+    uint32_t at = 0;
+    if (lane == 63) at = atomicAdd(&p.n_candidates[row], upto);
+    at = __shfl(at, 63) + upto - n;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+        if (mine >> k & 1) {
+            if (at < kMaxCandidates) p.candidates[static_cast<uint64_t>(row) * kMaxCandidates + at] = rank_of(key_of(v[k]), i + k);
+            ++at;
+        }
 }
 
 // ---- 2 ----------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const SampleParams p) {
     __shared__ u64 mass[kBins];
-    __shared__ uint32_t count[kBins];
+    __shared__ __align__(16) uint32_t count[kBins];
     __shared__ u64 part[kAhead][kChunkThreads / kWave];
+    __shared__ uint32_t threshold;
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
-    const u64 best = row_best(p, row);
-    if (blockIdx.x == 0 && t == 0) p.top[row] = best;
-    const Row r = row_of(p, row, static_cast<uint32_t>(best >> 32));
-    if (best >> 32 == 0 || r.greedy) return;
+    // the chunks' maxima: the row's, and the top_k-th of them
+    uint32_t *keys = count, top = 0, own[kMaxChunks / kChunkThreads];
+#pragma unroll
+    for (uint32_t u = 0; u < kMaxChunks / kChunkThreads; ++u) {
+        const uint32_t c = u * kChunkThreads + t;
+        own[u] = c < p.chunks ? p.best[static_cast<uint64_t>(row) * p.chunks + c] : 0;
+        keys[c] = own[u];
+        top = own[u] > top ? own[u] : top;
+    }
+    top = wave_max_u32(top);
+    uint32_t *tops = reinterpret_cast<uint32_t *>(part[0]);
+    if (t % kWave == 0) tops[t / kWave] = top;
+    if (t == 0) threshold = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kChunkThreads / kWave; ++w) top = tops[w] > top ? tops[w] : top;
+    if (blockIdx.x == 0 && t == 0) p.top[row] = top;
+    const Row r = row_of(p, row, top);
+    if (top == 0 || r.greedy) return;
+    if (r.top_k != 0 && r.top_k <= p.chunks) {
+        uint32_t above[kMaxChunks / kChunkThreads] = {};
+#pragma unroll 4
+        for (uint32_t c = 0; c < p.chunks; c += 4) {   // zeros behind the last chunk are above nothing
+            const uint4 q = *reinterpret_cast<const uint4 *>(keys + c);
+#pragma unroll
+            for (uint32_t u = 0; u < kMaxChunks / kChunkThreads; ++u) {
+                const uint32_t me = u * kChunkThreads + t;
+                if (u != 0 && u * kChunkThreads >= p.chunks) break;   // uniform
+                above[u] += (q.x > own[u] || (q.x == own[u] && c < me)) + (q.y > own[u] || (q.y == own[u] && c + 1 < me)) +
+                            (q.z > own[u] || (q.z == own[u] && c + 2 < me)) + (q.w > own[u] || (q.w == own[u] && c + 3 < me));
+            }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kMaxChunks / kChunkThreads; ++u)
+            if (u * kChunkThreads + t < p.chunks && above[u] + 1 == r.top_k) threshold = own[u];   // one thread's one chunk
+        __syncthreads();
+        const uint32_t least = threshold;
+        if (least != 0) {
+            if (blockIdx.x == 0 && t == 0) {
+                Cut cut{};
+                cut.last = cut.k_last = kBins - 1;
+                p.cut[row] = cut;
+                p.listed[row] = 1;
+            }
+            walk_span(p, x, [&](const float (&v)[4], uint32_t i) {
+                uint32_t mine = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) mine |= key_of(v[k]) >= least ? 1u << k : 0;
+                collect(p, row, v, i, mine);
+            }, [](uint32_t) {});
+            return;
+        }
+    }
+    __syncthreads();   // every thread has read the keys that the histogram overwrites
     const bool by_count = r.top_k != 0, by_mass = r.top_p < 1.0;   // each needs its half of the histogram
     if (by_count || by_mass) {
         for (uint32_t b = t; b < kBins; b += kChunkThreads) { mass[b] = 0; count[b] = 0; }
@@ -338,15 +408,13 @@ __device__ __forceinline__ Cut find_cut(const SampleParams &p, uint32_t row, con
         }
     }
     __syncthreads();
-    Cut cut;
-    cut.k_bin = s.found[0];
+    Cut cut{};
+    cut.k_first = cut.k_last = cut.sure = cut.last = s.found[0];
     cut.k_count = s.k_count;
-    cut.sure = cut.last = cut.k_bin;
-    cut.sure_mass = cut.k_mass = cut.all_mass = 0;
     if (r.top_p < 1.0) {
         // the weight that top_k keeps lies between these two; so does the last rank that top_p keeps
-        const u64 hi = s.mass_upto[cut.k_bin < kBins ? cut.k_bin : kBins - 1];
-        const u64 lo = cut.k_bin == kBins ? hi : cut.k_bin ? s.mass_upto[cut.k_bin - 1] : 0;
+        const u64 hi = s.mass_upto[cut.k_first < kBins ? cut.k_first : kBins - 1];
+        const u64 lo = cut.k_first == kBins ? hi : cut.k_first ? s.mass_upto[cut.k_first - 1] : 0;
         const double limit_lo = r.top_p * static_cast<double>(lo), limit_hi = r.top_p * static_cast<double>(hi);
         if (holds) {
             u64 b = m_first;
@@ -360,8 +428,8 @@ __device__ __forceinline__ Cut find_cut(const SampleParams &p, uint32_t row, con
             }
         }
         __syncthreads();
-        cut.sure = s.found[1] < cut.k_bin ? s.found[1] : cut.k_bin;
-        cut.last = s.found[2] < cut.k_bin ? s.found[2] : cut.k_bin;
+        cut.sure = s.found[1] < cut.k_first ? s.found[1] : cut.k_first;
+        cut.last = s.found[2] < cut.k_first ? s.found[2] : cut.k_first;
         cut.sure_mass = cut.sure ? s.mass_upto[cut.sure - 1] : 0;
         cut.k_mass = lo;
         cut.all_mass = s.mass_upto[kBins - 1];
@@ -375,16 +443,16 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
     __shared__ u64 part[kAhead][kChunkThreads / kWave];
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
-    const u64 best = p.top[row];
-    const Row r = row_of(p, row, static_cast<uint32_t>(best >> 32));
-    if (best >> 32 == 0 || r.greedy || !(r.top_k != 0 || r.top_p < 1.0)) return;
+    const uint32_t top = p.top[row];
+    const Row r = row_of(p, row, top);
+    if (top == 0 || r.greedy || !(r.top_k != 0 || r.top_p < 1.0)) return;
+    if (p.listed[row]) return;
     const Cut cut = find_cut<kChunkThreads>(p, row, r, space);
     if (blockIdx.x == 0 && t == 0) p.cut[row] = cut;
     // logits well below the last step of interest need no 64-bit depth
-    const uint32_t deep = cut.k_bin < kBins ? cut.k_bin : cut.last;
+    const uint32_t deep = cut.k_first < kBins ? cut.k_first : cut.last;
     const double reach = (deep + 1) / kBinsPerUnit / r.per_unit;
     const float least = isfinite(r.max) && reach < 1e30 ? static_cast<float>(r.max - reach) - (fabsf(r.max) + static_cast<float>(reach)) * 1e-6f : -INFINITY;
-    u64 *list = p.candidates + static_cast<uint64_t>(row) * kMaxCandidates;
     u64 sum = 0;
     walk_span(p, x, [&](const float (&v)[4], uint32_t i) {
         sum = 0;
@@ -396,27 +464,9 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
             if (!(depth < kReach)) continue;
             const uint32_t b = bin_at(depth);
             if (b < cut.sure) sum += kept_weight_at(depth, r);
-            else if (b <= cut.last || b == cut.k_bin) mine |= 1u << k;
+            else if (b <= cut.last || b == cut.k_first) mine |= 1u << k;
         }
-        // places in the list: one atomic a wave
-        const uint32_t n = __popc(mine);
-        if (__builtin_amdgcn_ballot_w64(n != 0) != 0) {
-            uint32_t upto = n;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const uint32_t o = __shfl_up(upto, d);
-                upto += t % kWave >= static_cast<uint32_t>(d) ? o : 0;
-            }
-            uint32_t at = 0;
-            if (t % kWave == 63) at = atomicAdd(&p.n_candidates[row], upto);
-            at = __shfl(at, 63) + upto - n;
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k)
-                if (mine >> k & 1) {
-                    if (at < kMaxCandidates) list[at] = rank_of(key_of(v[k]), i + k);
-                    ++at;
-                }
-        }
+        collect(p, row, v, i, mine);
     }, [&](uint32_t chunk) {
         sum = wave_sum_u64(sum);
         u64 *mine = part[chunk % kAhead];
@@ -431,264 +481,242 @@ struct DrawSpace {   // LDS
     u64 cand[kMaxCandidates];
     u64 part[kRowThreads / kWave];
     u64 chunk_mass[kMaxChunks];
-    u64 last, target;
+    u64 mass[256], result[2];
+    uint32_t count[256];
+    u64 target;
     uint32_t at, bounds[2];
 };
-constexpr uint32_t kRankThreads = 512;   // up to as many candidates are ranked by counting, more are sorted
 
-// The last kept rank of a row by its keys' digits: eight bits a pass over the row, counts and weights of the 256 values in
-// LDS.  Only the steps that hold the cut count, what lies above them is known from the histogram.
-__device__ u64 cut_by_digits(const SampleParams &p, const float *x, const Row &r, const Cut &cut, DrawSpace &s) {
-    u64 *mass = s.cand, *sh = s.cand + 256, *ties_of = s.cand + 512;   // [kMaxChunks]
-    uint32_t *count = reinterpret_cast<uint32_t *>(s.cand + 512 + kMaxChunks);
+// The last rank that stays among those from `after` up in the steps lo .. hi, when fewer than `limit` (count or weight) of
+// them may come before it: eight bits of the 64-bit ranks a pass, counts and weights of the 256 values in LDS.
+// walk(f) calls f(rank) for every element in question, whose bits from `width` on are alike.
+template <typename W>
+__device__ u64 find_by_digits(W walk, const Row &r, bool by_mass, uint32_t lo, uint32_t hi, u64 after, u64 limit, uint32_t width,
+                              u64 prefix, DrawSpace &s) {
     const uint32_t t = threadIdx.x;
-    auto walk = [&](auto f) {   // f(key, index) for every logit
-        for (uint32_t i = 4 * t; i < p.vocab; i += 4 * kRowThreads) {
-            float v[4];
-            load4(p, x, i, v);
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k)
-                if (i + k < p.vocab) f(key_of(v[k]), i + k);
-        }
-    };
-    // The last rank that stays among the steps lo .. hi and not behind `after`, when fewer than `limit` (count or mass) of
-    // them may come before it.
-    auto find = [&](bool by_mass, uint32_t lo, uint32_t hi, u64 after, u64 limit) -> u64 {
-        uint32_t prefix = 0;
-        u64 before = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (t < 256) { mass[t] = 0; count[t] = 0; }
-            __syncthreads();
-            walk([&](uint32_t key, uint32_t i) {
-                if (shift != 24 && (key >> (shift + 8)) != prefix) return;
-                if (rank_of(key, i) < after) return;
-                const double depth = depth_of(key, r);
-                if (!(depth < kReach)) return;
-                const uint32_t b = bin_at(depth);
-                if (b < lo || b > hi) return;
-                atomicAdd(&count[(key >> shift) & 255], 1u);
-                if (by_mass) atomicAdd(&mass[(key >> shift) & 255], weight_at(depth));
-            });
-            __syncthreads();
-            if (t == 0) {
-                int digit = 0;
-                u64 upto = before;
-                bool any = false;
-                for (int d = 255; d >= 0; --d) {
-                    if (count[d] == 0) continue;
-                    if (any) before = upto;
-                    any = true;
-                    digit = d;
-                    upto = before + (by_mass ? mass[d] : count[d]);
-                    if (upto >= limit) break;
-                }
-                sh[0] = prefix << 8 | static_cast<uint32_t>(digit);
-                sh[1] = before;
-                sh[2] = count[digit];
-            }
-            __syncthreads();
-            prefix = static_cast<uint32_t>(sh[0]);
-            before = sh[1];
-            __syncthreads();
-        }
-        u64 ties = sh[2];   // of the key `prefix`: as many stay as begin below the limit
-        const u64 left = limit > before ? limit - before : 1;
-        const u64 each = by_mass ? weight_at(depth_of(prefix, r)) : 1;
-        if (each != 0 && (left + each - 1) / each < ties) ties = (left + each - 1) / each;
-        // the index of the last of them: ties per chunk, then that chunk
-        for (uint32_t c = t; c < kMaxChunks; c += kRowThreads) ties_of[c] = 0;
+    u64 before = 0;
+    for (uint32_t shift = width; shift != 0;) {   // prefix: the bits from `shift` on
+        const uint32_t bits = shift < 8 ? shift : 8, next = shift - bits;
+        s.mass[t] = 0;
+        s.count[t] = 0;
+        if (t == 0) { s.at = 0; s.result[0] = ~0ull; }
         __syncthreads();
-        walk([&](uint32_t key, uint32_t i) {
-            if (key == prefix && rank_of(key, i) >= after) atomicAdd(&ties_of[i / kChunk], 1ull);
+        walk([&](u64 rank) {
+            if (rank < after || (shift < 64 && rank >> shift != prefix)) return;
+            const double depth = depth_of(static_cast<uint32_t>(rank >> 32), r);
+            const uint32_t b = depth < kReach ? bin_at(depth) : kBins - 1;
+            if (b < lo || b > hi) return;
+            const uint32_t digit = static_cast<uint32_t>(rank >> next) & ((1u << bits) - 1);
+            atomicAdd(&s.count[digit], 1u);
+            if (by_mass) atomicAdd(&s.mass[digit], weight_at(depth));
         });
         __syncthreads();
+        const uint32_t mine = 255 - t;   // larger digits come first
+        const uint32_t n = s.count[mine];
+        const u64 v = by_mass ? s.mass[mine] : n;
         u64 all;
-        const u64 mine = ties_of[t], below = sum_below<kRowThreads>(mine, s.part, all);
-        if (below < ties && ties <= below + mine) { sh[3] = t; sh[4] = ties - below; }
+        const u64 upto = before + sum_below<kRowThreads>(v, s.part, all);
+        if (n != 0) atomicMax(&s.at, t);   // where the limit is beyond all: the last value that occurs
+        if (upto < limit && upto + v >= limit) { s.result[0] = mine; s.result[1] = upto; }
         __syncthreads();
-        const uint32_t i = static_cast<uint32_t>(sh[3]) * kChunk + t;
-        const uint32_t key = i < p.vocab ? key_of(x[i]) : 0;
-        const u64 is = key == prefix && rank_of(key, i) >= after;
-        const u64 under = sum_below<kRowThreads>(is, s.part, all);
-        if (is && under + 1 == sh[4]) sh[5] = rank_of(key, i);
+        if (s.result[0] == ~0ull && t == s.at) { s.result[0] = mine; s.result[1] = upto; }
         __syncthreads();
-        const u64 last = sh[5];
+        prefix = (shift < 64 ? prefix << bits : 0) | s.result[0];
+        before = s.result[1];
+        shift = next;
         __syncthreads();
-        return last;
-    };
-    u64 last = 0;
-    if (cut.k_bin < kBins) last = find(false, cut.k_bin, cut.k_bin, 0, r.top_k - cut.k_count);
-    if (r.top_p < 1.0) {
-        u64 kept = cut.all_mass;   // the weight that top_k keeps
-        if (cut.k_bin < kBins) {
-            u64 sum = 0;
-            walk([&](uint32_t key, uint32_t i) {
-                const double depth = depth_of(key, r);
-                if (depth < kReach && bin_at(depth) == cut.k_bin && rank_of(key, i) >= last) sum += weight_at(depth);
-            });
-            (void)sum_below<kRowThreads>(sum, s.part, kept);
-            kept += cut.k_mass;
-        }
-        const double limit_f = ceil(r.top_p * static_cast<double>(kept));
-        const u64 limit = limit_f > 1.0 ? static_cast<u64>(limit_f) : 1ull;   // rank 0 always stays
-        last = find(true, cut.sure, cut.last, last, limit - cut.sure_mass);
     }
-    return last;
+    return prefix;
 }
 
 __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SampleParams p) {
     __shared__ DrawSpace s;
     const uint32_t t = threadIdx.x, row = blockIdx.x;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
-    const u64 best = p.top[row];
-    const uint32_t top = static_cast<uint32_t>(best >> 32);
+    const uint32_t top = p.top[row];
     if (top == 0) {
         if (t == 0) p.out[row] = q8mi_argmax_pair{-INFINITY, -1};
         return;
     }
     const Row r = row_of(p, row, top);
-    if (r.greedy) {
-        const uint32_t i = 0xffffffffu - static_cast<uint32_t>(best);
-        if (t == 0) p.out[row] = q8mi_argmax_pair{x[i], static_cast<int32_t>(i)};
+    if (r.greedy) {   // the first chunk with that key, its first such element
+        if (t == 0) s.at = kMaxChunks;
+        __syncthreads();
+        for (uint32_t c = t; c < p.chunks; c += kRowThreads)
+            if (p.best[static_cast<uint64_t>(row) * p.chunks + c] == top) atomicMin(&s.at, c);
+        if (t == 0) s.bounds[0] = 0xffffffffu;
+        __syncthreads();
+        const uint32_t i = s.at * kChunk + 4 * t;
+        float v[4];
+        load4(p, x, i, v);
+        uint32_t k = 0;
+        while (k < 4 && key_of(v[k]) != top) ++k;
+        if (k < 4) atomicMin(&s.bounds[0], i + k);
+        __syncthreads();
+        if (k < 4 && s.bounds[0] == i + k) p.out[row] = q8mi_argmax_pair{x[i + k], static_cast<int32_t>(i + k)};
         return;
     }
     const bool cuts = r.top_k != 0 || r.top_p < 1.0;
     const uint32_t n = cuts ? p.n_candidates[row] : 0;
-    u64 mine = t < p.chunks && n <= kMaxCandidates ? p.chunk_mass[static_cast<uint64_t>(row) * p.chunks + t] : 0;
-    s.chunk_mass[t] = mine;
+    const bool listed = cuts && p.listed[row] != 0;
+    const bool summed = !listed && n <= kMaxCandidates;   // the earlier launches have left the chunks' sums
+#pragma unroll
+    for (uint32_t c = t; c < kMaxChunks; c += kRowThreads)
+        s.chunk_mass[c] = summed && c < p.chunks ? p.chunk_mass[static_cast<uint64_t>(row) * p.chunks + c] : 0;
     u64 last = 0;   // rank of the last kept element: everything from it up is kept
-    if (cuts) {
+    if (cuts && n > kRowThreads) {
+        // many candidates, or more than the list holds: then all logits of the row are
+        const bool whole = n > kMaxCandidates;
+        const u64 *list = p.candidates + static_cast<uint64_t>(row) * kMaxCandidates;
         const Cut cut = p.cut[row];
-        if (n > kMaxCandidates) {
-            last = cut_by_digits(p, x, r, cut, s);
-            for (uint32_t i = 4 * t; i < p.vocab; i += 4 * kRowThreads) {
-                float v[4];
-                load4(p, x, i, v);
-                u64 sum = 0;
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) {
-                    const uint32_t key = key_of(v[k]);
-                    if (rank_of(key, i + k) >= last) sum += kept_weight_at(depth_of(key, r), r);
-                }
-                if (sum) atomicAdd(&s.chunk_mass[i / kChunk], sum);
+        auto walk = [&](auto f) {
+            if (!whole) {
+                for (uint32_t c = t; c < n; c += kRowThreads) f(s.cand[c]);
+                return;
             }
-            __syncthreads();
-        } else {
-            const u64 *list = p.candidates + static_cast<uint64_t>(row) * kMaxCandidates;
-            u64 w[4], sum = 0, all;   // this thread's candidates, neighbours in rank, from `c0` on
-            uint32_t bin[4], c0, held;
-            if (n <= kRankThreads) {
-                u64 my = 0;
-                if (t < n) { my = list[t]; s.cand[kMaxCandidates / 2 + t] = my; }
-                __syncthreads();
-                if (t < n) {
-                    uint32_t above = 0;
-                    for (uint32_t i = 0; i < n; ++i) above += s.cand[kMaxCandidates / 2 + i] > my;
-                    s.cand[above] = my;   // ranks differ
-                }
-                __syncthreads();
-                c0 = t; held = t < n ? 1 : 0;
-            } else {
-                uint32_t size = 2;
-                while (size < n) size *= 2;
-                for (uint32_t i = t; i < size; i += kRowThreads) s.cand[i] = i < n ? list[i] : 0;
-                __syncthreads();
-                for (uint32_t k = 2; k <= size; k *= 2)           // bitonic, descending
-                    for (uint32_t j = k / 2; j > 0; j /= 2) {
-                        for (uint32_t i = t; i < size; i += kRowThreads) {
-                            const uint32_t o = i ^ j;
-                            if (o > i) {
-                                const u64 a = s.cand[i], b = s.cand[o];
-                                if ((a < b) == ((i & k) == 0)) { s.cand[i] = b; s.cand[o] = a; }
-                            }
-                        }
-                        __syncthreads();
+            for (uint32_t i0 = 4 * t; i0 < p.vocab; i0 += 16 * kRowThreads) {
+                float v[4][4];
+#pragma unroll
+                for (uint32_t u = 0; u < 4; ++u)
+                    if (i0 + u * 4 * kRowThreads < p.vocab) load4(p, x, i0 + u * 4 * kRowThreads, v[u]);
+#pragma unroll
+                for (uint32_t u = 0; u < 4; ++u)
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        const uint32_t i = i0 + u * 4 * kRowThreads + k;
+                        if (i < p.vocab && key_of(v[u][k]) != 0) f(rank_of(key_of(v[u][k]), i));
                     }
-                c0 = 4 * t; held = c0 < n ? (n - c0 < 4 ? n - c0 : 4) : 0;
             }
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const double depth = i < held ? depth_of(static_cast<uint32_t>(s.cand[c0 + i] >> 32), r) : INFINITY;
-                w[i] = weight_at(depth);
-                bin[i] = i < held ? bin_at(depth) : kBins;
-                sum += w[i];
+        };
+        uint32_t width = 64;   // bits in which the ranks differ
+        u64 prefix = 0;
+        if (!whole) {
+            if (t == 0) { s.result[0] = 0; s.result[1] = ~0ull; }
+            __syncthreads();
+            u64 any = 0, every = ~0ull;
+            for (uint32_t c = t; c < n; c += kRowThreads) {
+                const u64 rank = list[c];
+                s.cand[c] = rank;
+                any |= rank;
+                every &= rank;
             }
-            uint32_t kept = n;   // candidates that stay: a prefix of their ranks
-            u64 mass_k = cut.all_mass;
-            if (cut.k_bin < kBins) {
-                if (t == 0) s.bounds[0] = n;
-                __syncthreads();
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i)
-                    if (i < held && bin[i] == cut.k_bin) atomicMin(&s.bounds[0], c0 + i);   // the first candidate of that step
-                __syncthreads();
-                const uint32_t first = s.bounds[0];
-                kept = first + (r.top_k - cut.k_count);
-                if (r.top_p < 1.0) {
-                    u64 in_step = 0, step_all;
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i)
-                        if (i < held && c0 + i >= first && c0 + i < kept) in_step += w[i];
-                    (void)sum_below<kRowThreads>(in_step, s.part, step_all);
-                    mass_k = cut.k_mass + step_all;
-                }
-            }
-            if (r.top_p < 1.0) {
-                const double limit_f = ceil(r.top_p * static_cast<double>(mass_k));
-                const u64 limit = limit_f > 1.0 ? static_cast<u64>(limit_f) : 1ull;   // rank 0 always stays
-                if (t == 0) s.bounds[1] = 0;
-                u64 run = cut.sure_mass + sum_below<kRowThreads>(sum, s.part, all);
-                uint32_t stay = 0;
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    if (i < held && bin[i] <= cut.last && run < limit) stay = c0 + i + 1;
-                    run += w[i];
-                }
-                if (stay) atomicMax(&s.bounds[1], stay);
-                __syncthreads();
-                kept = s.bounds[1] < kept ? s.bounds[1] : kept;
-            }
-            last = s.cand[kept - 1];   // each cut keeps a candidate: the step before which it falls short holds it
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-                if (i < held && c0 + i < kept) {
-                    const uint32_t index = 0xffffffffu - static_cast<uint32_t>(s.cand[c0 + i]);
-                    const u64 kept_w = depth_of(static_cast<uint32_t>(s.cand[c0 + i] >> 32), r) <= r.deepest ? w[i] : 0;
-                    if (kept_w) atomicAdd(&s.chunk_mass[index / kChunk], kept_w);
-                }
+            atomicOr(&s.result[0], any);
+            atomicAnd(&s.result[1], every);
+            __syncthreads();
+            width = 64 - __clzll(s.result[0] ^ s.result[1]);   // candidates are more than one, and differ
+            prefix = width < 64 ? s.result[0] >> width : 0;
             __syncthreads();
         }
-        mine = s.chunk_mass[t];
+        if (cut.k_first < kBins)
+            last = find_by_digits(walk, r, false, cut.k_first, cut.k_last, 0, r.top_k - cut.k_count, width, prefix, s);
+        if (r.top_p < 1.0) {
+            u64 kept = cut.all_mass;   // the weight that top_k keeps
+            if (cut.k_first < kBins) {
+                u64 sum = 0;
+                walk([&](u64 rank) {
+                    const double depth = depth_of(static_cast<uint32_t>(rank >> 32), r);
+                    if (rank >= last && depth < kReach && bin_at(depth) >= cut.k_first) sum += weight_at(depth);
+                });
+                (void)sum_below<kRowThreads>(sum, s.part, kept);
+                kept += cut.k_mass;
+            }
+            const double limit_f = ceil(r.top_p * static_cast<double>(kept));
+            const u64 limit = limit_f > 1.0 ? static_cast<u64>(limit_f) : 1ull;   // rank 0 always stays
+            last = find_by_digits(walk, r, true, cut.sure, cut.last, last, limit - cut.sure_mass, width, prefix, s);
+        }
+        walk([&](u64 rank) {
+            if (rank < last) return;
+            const u64 w = kept_weight_at(depth_of(static_cast<uint32_t>(rank >> 32), r), r);
+            if (w) atomicAdd(&s.chunk_mass[(0xffffffffu - static_cast<uint32_t>(rank)) / kChunk], w);
+        });
+    } else if (cuts) {
+        // a candidate a thread, ranked by counting
+        const Cut cut = p.cut[row];
+        u64 own = t < n ? p.candidates[static_cast<uint64_t>(row) * kMaxCandidates + t] : 0;
+        s.cand[kRowThreads + t] = own;
+        __syncthreads();
+        uint32_t above = 0;
+#pragma unroll 8
+        for (uint32_t i = 0; i < n; ++i) above += s.cand[kRowThreads + i] > own;
+        if (t < n) s.cand[above] = own;   // ranks differ
+        __syncthreads();
+        own = t < n ? s.cand[t] : 0;
+        const double depth = depth_of(static_cast<uint32_t>(own >> 32), r);
+        const uint32_t step = depth < kReach ? bin_at(depth) : kBins - 1;
+        const u64 w = t < n ? weight_at(depth) : 0;
+        uint32_t kept = n;   // candidates that stay: a prefix of their ranks
+        u64 mass_k = cut.all_mass, all;
+        if (cut.k_first < kBins) {
+            uint32_t first = 0;   // the first candidate of top_k's step
+            if (!listed) {
+                if (t == 0) s.bounds[0] = n;
+                __syncthreads();
+                if (t < n && step == cut.k_first) atomicMin(&s.bounds[0], t);
+                __syncthreads();
+                first = s.bounds[0];
+            }
+            kept = first + (r.top_k - cut.k_count);
+            if (r.top_p < 1.0) {
+                (void)sum_below<kRowThreads>(t >= first && t < kept ? w : 0, s.part, mass_k);
+                mass_k += cut.k_mass;
+            }
+        }
+        if (r.top_p < 1.0) {
+            const double limit_f = ceil(r.top_p * static_cast<double>(mass_k));
+            const u64 limit = limit_f > 1.0 ? static_cast<u64>(limit_f) : 1ull;   // rank 0 always stays
+            if (t == 0) s.bounds[1] = 0;
+            const u64 run = cut.sure_mass + sum_below<kRowThreads>(w, s.part, all);
+            if (t < n && step <= cut.last && run < limit) atomicMax(&s.bounds[1], t + 1);
+            __syncthreads();
+            kept = s.bounds[1] < kept ? s.bounds[1] : kept;
+        }
+        last = s.cand[kept - 1];   // each cut keeps a candidate: the step before which it falls short holds it
+        if (t < kept && w != 0 && depth <= r.deepest) atomicAdd(&s.chunk_mass[(0xffffffffu - static_cast<uint32_t>(own)) / kChunk], w);
     }
+    __syncthreads();
 
     // the chunk, then the element, at which the sum exceeds uniform * all
-    u64 all;
-    const u64 before = sum_below<kRowThreads>(mine, s.part, all);
+    u64 of[4], sum = 0, all;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) sum += of[k] = s.chunk_mass[4 * t + k];
+    u64 before = sum_below<kRowThreads>(sum, s.part, all);
     float u = p.uniform[row];
     u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
     u64 target = static_cast<u64>(static_cast<double>(u) * static_cast<double>(all));
     if (target >= all) target = all - 1;
-    if (before <= target && target < before + mine) { s.at = t; s.target = target - before; }
-    __syncthreads();
-    const uint32_t i = s.at * kChunk + t;
-    target = s.target;
-    u64 w = 0;
-    float v = 0.0f;
-    if (i < p.vocab) {
-        v = x[i];
-        const uint32_t key = key_of(v);
-        if (rank_of(key, i) >= last) w = kept_weight_at(depth_of(key, r), r);
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+        if (before <= target && target < before + of[k]) { s.at = 4 * t + k; s.target = target - before; }
+        before += of[k];
     }
-    const u64 run = sum_below<kRowThreads>(w, s.part, all);
-    if (run <= target && target < run + w) p.out[row] = q8mi_argmax_pair{v, static_cast<int32_t>(i)};
+    __syncthreads();
+    const uint32_t i = s.at * kChunk + 4 * t;
+    target = s.target;
+    float v[4];
+    load4(p, x, i, v);
+    sum = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+        const uint32_t key = key_of(v[k]);
+        sum += of[k] = rank_of(key, i + k) >= last ? kept_weight_at(depth_of(key, r), r) : 0;
+    }
+    u64 run = sum_below<kRowThreads>(sum, s.part, all);
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+        if (run <= target && target < run + of[k]) p.out[row] = q8mi_argmax_pair{v[k], static_cast<int32_t>(i + k)};
+        run += of[k];
+    }
 }
 
-uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
-// u64 words of a row: best (at most one a chunk) and chunk_mass, bin_mass, candidates, bin_count, top, cut; n_candidates behind all rows
-uint64_t row_words(uint32_t vocab) { return 2ull * chunks_of(vocab) + kBins + kMaxCandidates + kBins / 2 + 1 + sizeof(Cut) / 8; }
 // Chunks of a workgroup: one while that leaves CUs idle, up to kMostSpan where rows are many (the histogram of a workgroup
 // is then cleared and added to the row's once for several chunks).
-constexpr uint32_t kMostSpan = 16, kGridWanted = 1024;
+constexpr uint32_t kGridWanted = 1024;
+
+uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
+// Bytes of a row: chunk_mass, bin_mass, candidates, cut, bin_count, best, top, listed, n_candidates.
+uint64_t row_bytes(uint32_t vocab) {
+    return 8ull * (chunks_of(vocab) + kBins + kMaxCandidates) + sizeof(Cut) + 4ull * (kBins + chunks_of(vocab) + 3);
+}
 
 }  // namespace
 }  // namespace q8mi
@@ -696,7 +724,7 @@ constexpr uint32_t kMostSpan = 16, kGridWanted = 1024;
 using namespace q8mi;
 
 extern "C" size_t q8mi_sample_scratch_bytes(uint32_t batch, uint32_t vocab) {
-    return 16 + batch * (row_words(vocab) * 8 + 4);
+    return 16 + batch * row_bytes(vocab);
 }
 
 extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, uint32_t stride, const float *temperature,
@@ -716,16 +744,17 @@ extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, 
     p.span = crowd < 1 ? 1 : crowd > kMostSpan ? kMostSpan : static_cast<uint32_t>(crowd);
     p.spans = (p.chunks + p.span - 1) / p.span;
     p.vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (batch == 1 || stride % 4 == 0);
-    u64 *words = static_cast<u64 *>(scratch);
-    auto take = [&](uint64_t n) { u64 *at = words; words += n; return at; };
-    p.best = take(static_cast<uint64_t>(batch) * p.chunks);
-    p.chunk_mass = take(static_cast<uint64_t>(batch) * p.chunks);
-    p.bin_mass = take(static_cast<uint64_t>(batch) * kBins);
-    p.candidates = take(static_cast<uint64_t>(batch) * kMaxCandidates);
-    p.bin_count = reinterpret_cast<uint32_t *>(take(static_cast<uint64_t>(batch) * kBins / 2));
-    p.top = take(batch);
-    p.cut = reinterpret_cast<Cut *>(take(static_cast<uint64_t>(batch) * sizeof(Cut) / 8));
-    p.n_candidates = reinterpret_cast<uint32_t *>(words);
+    uint8_t *at = static_cast<uint8_t *>(scratch);
+    auto take = [&](uint64_t bytes) { uint8_t *a = at; at += batch * bytes; return a; };
+    p.chunk_mass = reinterpret_cast<u64 *>(take(8ull * p.chunks));
+    p.bin_mass = reinterpret_cast<u64 *>(take(8ull * kBins));
+    p.candidates = reinterpret_cast<u64 *>(take(8ull * kMaxCandidates));
+    p.cut = reinterpret_cast<Cut *>(take(sizeof(Cut)));
+    p.bin_count = reinterpret_cast<uint32_t *>(take(4ull * kBins));
+    p.best = reinterpret_cast<uint32_t *>(take(4ull * p.chunks));
+    p.top = reinterpret_cast<uint32_t *>(take(4));
+    p.listed = reinterpret_cast<uint32_t *>(take(4));
+    p.n_candidates = reinterpret_cast<uint32_t *>(take(4));
     hipStream_t s = as_stream(stream);
     const dim3 grid(p.spans, batch);
     sample_best_kernel<<<grid, kChunkThreads, 0, s>>>(p);
