@@ -33,7 +33,8 @@ constexpr uint32_t kRowThreads = 256;                 // launch 4
 constexpr uint32_t kBins = 1024;
 constexpr double kBinsPerUnit = 32.0;
 constexpr double kReach = 31.875;                     // exp(-31.875) * 2^42 rounds to 0
-constexpr uint32_t kMaxCandidates = 4096;
+constexpr uint32_t kMaxCandidates = 4096;             // of a row
+constexpr uint32_t kChunkCandidates = 64;             // of a chunk
 constexpr double kOne = 4398046511104.0;              // 2^42: the weight of the largest logit; 2^20 of them sum below 2^63
 
 typedef unsigned long long u64;
@@ -53,13 +54,13 @@ struct SampleParams {
     q8mi_argmax_pair *out;
     u64 *chunk_mass;    // [row][chunk]: weight kept for certain
     u64 *bin_mass;      // [row][kBins]
-    u64 *candidates;    // [row][kMaxCandidates]: key << 32 | ~index
+    u64 *candidates;    // [row][chunk][kChunkCandidates]: key << 32 | ~index, in any order
     Cut *cut;           // [row] (launch 2 or 3)
     uint32_t *best;     // [row][chunk]: largest key
     uint32_t *top;      // [row]: largest key (launch 2)
     uint32_t *listed;   // [row]: launch 2 has collected everything from rank 0 to the cuts
     uint32_t *bin_count;     // [row][kBins]
-    uint32_t *n_candidates;  // [row]
+    uint32_t *n_candidates;  // [row][chunk]: may be beyond kChunkCandidates
     uint32_t vocab, stride, chunks;
     uint32_t span, spans;    // chunks of a workgroup of launches 1 to 3, such workgroups a row
     int vec;
@@ -174,26 +175,40 @@ __device__ __forceinline__ void load4(const SampleParams &p, const float *x, uin
     for (uint32_t k = 0; k < 4; ++k) v[k] = i + k < p.vocab ? x[i + k] : -INFINITY;
 }
 
-// Calls f(v, i, chunk) for every four logits v (from element i) that this thread has of the workgroup's span, and
-// after(chunk) behind each chunk; kAhead chunks are loaded at a time.
-template <typename F, typename A>
-__device__ __forceinline__ void walk_span(const SampleParams &p, const float *x, F f, A after) {
-    const uint32_t first = blockIdx.x * p.span, end = first + p.span < p.chunks ? first + p.span : p.chunks;
-    for (uint32_t c = first; c < end; c += kAhead) {
-        float v[kAhead][4];
+// A workgroup's span of chunks, kAhead chunks in registers: asked for when the object is made, and the next ones before
+// those in hand are looked at.
+struct Span {
+    const SampleParams &p;
+    const float *x;
+    uint32_t first, end;
+    float v[kAhead][4];
+
+    __device__ __forceinline__ Span(const SampleParams &params, const float *row) : p(params), x(row) {
+        first = blockIdx.x * p.span;
+        end = first + p.span < p.chunks ? first + p.span : p.chunks;
+        load(first, v);
+    }
+    __device__ __forceinline__ void load(uint32_t c, float (&to)[kAhead][4]) const {
 #pragma unroll
-        for (uint32_t u = 0; u < kAhead; ++u) {
-            const uint32_t i = (c + u) * kChunk + threadIdx.x * 4;
-            if (c + u < end) load4(p, x, i, v[u]);
-        }
+        for (uint32_t u = 0; u < kAhead; ++u)
+            if (c + u < end) load4(p, x, (c + u) * kChunk + threadIdx.x * 4, to[u]);
+    }
+    // f(v, i, c) for every four logits v, from element i, that this thread has of the span's chunk c (counted from 0)
+    template <typename F>
+    __device__ __forceinline__ void walk(F f) {
+        for (uint32_t c = first; c < end; c += kAhead) {
+            float next[kAhead][4];
+            load(c + kAhead, next);
 #pragma unroll
-        for (uint32_t u = 0; u < kAhead; ++u) {
-            if (c + u >= end) break;   // uniform
-            f(v[u], (c + u) * kChunk + threadIdx.x * 4);
-            after(c + u);
+            for (uint32_t u = 0; u < kAhead; ++u)
+                if (c + u < end) f(v[u], (c + u) * kChunk + threadIdx.x * 4, c + u - first);   // uniform
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u)
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) v[u][k] = next[u][k];
         }
     }
-}
+};
 
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     auto larger = [](uint32_t a, int b) { return a > static_cast<uint32_t>(b) ? a : static_cast<uint32_t>(b); };
@@ -208,48 +223,46 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 // ---- 1 ----------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kChunkThreads) void sample_best_kernel(const SampleParams p) {
     __shared__ uint32_t best[kMostSpan][kChunkThreads / kWave];
-    const uint32_t t = threadIdx.x, row = blockIdx.y, first = blockIdx.x * p.span;
-    const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
-    walk_span(p, x, [&](const float (&v)[4], uint32_t i) {
-        uint32_t key = 0;
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) key = key_of(v[k]) > key ? key_of(v[k]) : key;
-        key = wave_max_u32(key);
-        if (t % kWave == 0) best[i / kChunk - first][t / kWave] = key;
-    }, [](uint32_t) {});
+    const uint32_t t = threadIdx.x, row = blockIdx.y;
+    Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
     if (blockIdx.x == 0) {
         for (uint32_t b = t; b < kBins; b += kChunkThreads) {
             p.bin_mass[static_cast<uint64_t>(row) * kBins + b] = 0;
             p.bin_count[static_cast<uint64_t>(row) * kBins + b] = 0;
         }
-        if (t == 0) p.n_candidates[row] = p.listed[row] = 0;
+        if (t == 0) p.listed[row] = 0;
     }
+    span.walk([&](const float (&v)[4], uint32_t, uint32_t c) {
+        uint32_t key = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) key = key_of(v[k]) > key ? key_of(v[k]) : key;
+        key = wave_max_u32(key);
+        if (t % kWave == 0) best[c][t / kWave] = key;
+    });
     __syncthreads();
-    if (t < p.span && first + t < p.chunks) {
+    if (span.first + t < span.end) {
         uint32_t key = 0;
 #pragma unroll
         for (uint32_t w = 0; w < kChunkThreads / kWave; ++w) key = best[t][w] > key ? best[t][w] : key;
-        p.best[static_cast<uint64_t>(row) * p.chunks + first + t] = key;
+        p.best[static_cast<uint64_t>(row) * p.chunks + span.first + t] = key;
     }
 }
 
-// Places in the row's list for the elements (bits of `mine`) of the four logits v from element i on: one atomic a wave.
-__device__ __forceinline__ void collect(const SampleParams &p, uint32_t row, const float (&v)[4], uint32_t i, uint32_t mine) {
-    const uint32_t n = __popc(mine), lane = threadIdx.x % kWave;
-    if (__builtin_amdgcn_ballot_w64(n != 0) == 0) return;
-    uint32_t upto = n;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint32_t o = __shfl_up(upto, d);
-        upto += lane >= static_cast<uint32_t>(d) ? o : 0;
-    }
-    uint32_t at = 0;
-    if (lane == 63) at = atomicAdd(&p.n_candidates[row], upto);
-    at = __shfl(at, 63) + upto - n;
+// Sums and candidates of a span's chunks on their way out of a workgroup.
+struct ChunkSpace {   // LDS
+    u64 mass[kMostSpan][kChunkThreads / kWave];
+    uint32_t n[kMostSpan];
+};
+// The elements (bits of `mine`) of the four logits v from element i on go to their chunk's list, c-th of the span.
+__device__ __forceinline__ void collect(const SampleParams &p, uint32_t row, ChunkSpace &s, const float (&v)[4], uint32_t i, uint32_t c,
+                                        uint32_t mine) {
+    if (mine == 0) return;
+    uint32_t at = atomicAdd(&s.n[c], static_cast<uint32_t>(__popc(mine)));
+    u64 *list = p.candidates + (static_cast<uint64_t>(row) * p.chunks + i / kChunk) * kChunkCandidates;
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k)
         if (mine >> k & 1) {
-            if (at < kMaxCandidates) p.candidates[static_cast<uint64_t>(row) * kMaxCandidates + at] = rank_of(key_of(v[k]), i + k);
+            if (at < kChunkCandidates) list[at] = rank_of(key_of(v[k]), i + k);
             ++at;
         }
 }
@@ -258,10 +271,12 @@ __device__ __forceinline__ void collect(const SampleParams &p, uint32_t row, con
 __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const SampleParams p) {
     __shared__ u64 mass[kBins];
     __shared__ __align__(16) uint32_t count[kBins];
-    __shared__ u64 part[kAhead][kChunkThreads / kWave];
+    __shared__ u64 part[kChunkThreads / kWave];
+    __shared__ ChunkSpace out;
     __shared__ uint32_t threshold;
     const uint32_t t = threadIdx.x, row = blockIdx.y;
-    const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
+    Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
+    if (t < kMostSpan) out.n[t] = 0;
     // the chunks' maxima: the row's, and the top_k-th of them
     uint32_t *keys = count, top = 0, own[kMaxChunks / kChunkThreads];
 #pragma unroll
@@ -272,7 +287,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
         top = own[u] > top ? own[u] : top;
     }
     top = wave_max_u32(top);
-    uint32_t *tops = reinterpret_cast<uint32_t *>(part[0]);
+    uint32_t *tops = reinterpret_cast<uint32_t *>(part);
     if (t % kWave == 0) tops[t / kWave] = top;
     if (t == 0) threshold = 0;
     __syncthreads();
@@ -306,12 +321,14 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
                 p.cut[row] = cut;
                 p.listed[row] = 1;
             }
-            walk_span(p, x, [&](const float (&v)[4], uint32_t i) {
+            span.walk([&](const float (&v)[4], uint32_t i, uint32_t c) {
                 uint32_t mine = 0;
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k) mine |= key_of(v[k]) >= least ? 1u << k : 0;
-                collect(p, row, v, i, mine);
-            }, [](uint32_t) {});
+                collect(p, row, out, v, i, c, mine);
+            });
+            __syncthreads();
+            if (span.first + t < span.end) p.n_candidates[static_cast<uint64_t>(row) * p.chunks + span.first + t] = out.n[t];
             return;
         }
     }
@@ -326,7 +343,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
         // least 1.  From there on only the sum counts, in the last step, which no logit reaches.
         const double far = by_count ? kReach : fmin(kReach, log(static_cast<double>(p.vocab) / (1.0 - r.top_p)) + 0.1);
         u64 rest = 0;
-        walk_span(p, x, [&](const float (&v)[4], uint32_t) {
+        span.walk([&](const float (&v)[4], uint32_t, uint32_t) {
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
                 const double depth = depth_of(key_of(v[k]), r);
@@ -338,14 +355,14 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
                 if (depth < far) atomicAdd(&mass[b], w);
                 else rest += w;
             }
-        }, [](uint32_t) {});
+        });
         rest = wave_sum_u64(rest);
         if (t % kWave == 0 && rest != 0) atomicAdd(&mass[kBins - 1], rest);
         __syncthreads();
         uint32_t mine[4];
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) mine[k] = count[4 * t + k];
-        u64 all, before = by_count ? sum_below<kChunkThreads>((mine[0] + mine[1]) + (mine[2] + mine[3]), part[0], all) : 0;
+        u64 all, before = by_count ? sum_below<kChunkThreads>((mine[0] + mine[1]) + (mine[2] + mine[3]), part, all) : 0;
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
             const uint32_t b = 4 * t + k;
@@ -356,18 +373,16 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
         }
         return;
     }
-    u64 sum = 0;
-    walk_span(p, x, [&](const float (&v)[4], uint32_t) {
-        sum = 0;
+    span.walk([&](const float (&v)[4], uint32_t, uint32_t c) {
+        u64 sum = 0;
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) sum += kept_weight_at(depth_of(key_of(v[k]), r), r);
-    }, [&](uint32_t chunk) {
         sum = wave_sum_u64(sum);
-        u64 *mine = part[chunk % kAhead];   // another one is written before the next barrier
-        if (t % kWave == 0) mine[t / kWave] = sum;
-        __syncthreads();
-        if (t == 0) p.chunk_mass[static_cast<uint64_t>(row) * p.chunks + chunk] = (mine[0] + mine[1]) + (mine[2] + mine[3]);
+        if (t % kWave == 0) out.mass[c][t / kWave] = sum;
     });
+    __syncthreads();
+    if (span.first + t < span.end)
+        p.chunk_mass[static_cast<uint64_t>(row) * p.chunks + span.first + t] = (out.mass[t][0] + out.mass[t][1]) + (out.mass[t][2] + out.mass[t][3]);
 }
 
 struct CutSpace {   // LDS
@@ -440,9 +455,10 @@ __device__ __forceinline__ Cut find_cut(const SampleParams &p, uint32_t row, con
 // ---- 3 ----------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const SampleParams p) {
     __shared__ CutSpace space;
-    __shared__ u64 part[kAhead][kChunkThreads / kWave];
+    __shared__ ChunkSpace out;
     const uint32_t t = threadIdx.x, row = blockIdx.y;
-    const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
+    Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
+    if (t < kMostSpan) out.n[t] = 0;   // find_cut's barriers follow
     const uint32_t top = p.top[row];
     const Row r = row_of(p, row, top);
     if (top == 0 || r.greedy || !(r.top_k != 0 || r.top_p < 1.0)) return;
@@ -453,9 +469,8 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
     const uint32_t deep = cut.k_first < kBins ? cut.k_first : cut.last;
     const double reach = (deep + 1) / kBinsPerUnit / r.per_unit;
     const float least = isfinite(r.max) && reach < 1e30 ? static_cast<float>(r.max - reach) - (fabsf(r.max) + static_cast<float>(reach)) * 1e-6f : -INFINITY;
-    u64 sum = 0;
-    walk_span(p, x, [&](const float (&v)[4], uint32_t i) {
-        sum = 0;
+    span.walk([&](const float (&v)[4], uint32_t i, uint32_t c) {
+        u64 sum = 0;
         uint32_t mine = 0;   // elements to collect
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
@@ -466,14 +481,16 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
             if (b < cut.sure) sum += kept_weight_at(depth, r);
             else if (b <= cut.last || b == cut.k_first) mine |= 1u << k;
         }
-        collect(p, row, v, i, mine);
-    }, [&](uint32_t chunk) {
-        sum = wave_sum_u64(sum);
-        u64 *mine = part[chunk % kAhead];
-        if (t % kWave == 0) mine[t / kWave] = sum;
-        __syncthreads();
-        if (t == 0) p.chunk_mass[static_cast<uint64_t>(row) * p.chunks + chunk] = (mine[0] + mine[1]) + (mine[2] + mine[3]);
+        collect(p, row, out, v, i, c, mine);
+        if (__builtin_amdgcn_ballot_w64(sum != 0) != 0) sum = wave_sum_u64(sum);   // uniform
+        if (t % kWave == 0) out.mass[c][t / kWave] = sum;
     });
+    __syncthreads();
+    if (span.first + t < span.end) {
+        const uint64_t at = static_cast<uint64_t>(row) * p.chunks + span.first + t;
+        p.chunk_mass[at] = (out.mass[t][0] + out.mass[t][1]) + (out.mass[t][2] + out.mass[t][3]);
+        p.n_candidates[at] = out.n[t];
+    }
 }
 
 // ---- 4 ----------------------------------------------------------------------------------------------------------------
@@ -521,10 +538,23 @@ __device__ u64 find_by_digits(W walk, const Row &r, bool by_mass, uint32_t lo, u
         __syncthreads();
         if (s.result[0] == ~0ull && t == s.at) { s.result[0] = mine; s.result[1] = upto; }
         __syncthreads();
+        const bool alone = s.count[s.result[0]] == 1;
         prefix = (shift < 64 ? prefix << bits : 0) | s.result[0];
         before = s.result[1];
         shift = next;
         __syncthreads();
+        if (alone && shift != 0) {   // its other bits at once
+            walk([&](u64 rank) {
+                if (rank < after || rank >> shift != prefix) return;
+                const double depth = depth_of(static_cast<uint32_t>(rank >> 32), r);
+                const uint32_t b = depth < kReach ? bin_at(depth) : kBins - 1;
+                if (b >= lo && b <= hi) s.result[0] = rank;
+            });
+            __syncthreads();
+            prefix = s.result[0];
+            __syncthreads();
+            break;
+        }
     }
     return prefix;
 }
@@ -557,17 +587,39 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
         return;
     }
     const bool cuts = r.top_k != 0 || r.top_p < 1.0;
-    const uint32_t n = cuts ? p.n_candidates[row] : 0;
     const bool listed = cuts && p.listed[row] != 0;
-    const bool summed = !listed && n <= kMaxCandidates;   // the earlier launches have left the chunks' sums
+    // the candidates of the chunks, one list after the other; `whole`: more than their places hold
+    uint32_t n = 0;
+    bool whole = false;
+    if (cuts) {
+        uint32_t of[4];
+        u64 sum = 0, all;
+        bool full = false;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            of[k] = 4 * t + k < p.chunks ? p.n_candidates[static_cast<uint64_t>(row) * p.chunks + 4 * t + k] : 0;
+            full |= of[k] > kChunkCandidates;
+            sum += of[k];
+        }
+        uint32_t at = static_cast<uint32_t>(sum_below<kRowThreads>(sum, s.part, all));
+        n = static_cast<uint32_t>(all);
+        whole = __syncthreads_or(full) || n > kMaxCandidates;
+        if (!whole) {
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                const u64 *list = p.candidates + (static_cast<uint64_t>(row) * p.chunks + 4 * t + k) * kChunkCandidates;
+                for (uint32_t i = 0; i < of[k]; ++i) s.cand[at++] = list[i];
+            }
+        }
+        __syncthreads();
+    }
+    const bool summed = !listed && !whole;   // the earlier launches have left the chunks' sums
 #pragma unroll
     for (uint32_t c = t; c < kMaxChunks; c += kRowThreads)
         s.chunk_mass[c] = summed && c < p.chunks ? p.chunk_mass[static_cast<uint64_t>(row) * p.chunks + c] : 0;
     u64 last = 0;   // rank of the last kept element: everything from it up is kept
-    if (cuts && n > kRowThreads) {
-        // many candidates, or more than the list holds: then all logits of the row are
-        const bool whole = n > kMaxCandidates;
-        const u64 *list = p.candidates + static_cast<uint64_t>(row) * kMaxCandidates;
+    if (cuts && (whole || n > kRowThreads)) {
+        // many candidates, or more than the lists hold: then all logits of the row are
         const Cut cut = p.cut[row];
         auto walk = [&](auto f) {
             if (!whole) {
@@ -595,8 +647,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
             __syncthreads();
             u64 any = 0, every = ~0ull;
             for (uint32_t c = t; c < n; c += kRowThreads) {
-                const u64 rank = list[c];
-                s.cand[c] = rank;
+                const u64 rank = s.cand[c];
                 any |= rank;
                 every &= rank;
             }
@@ -632,7 +683,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
     } else if (cuts) {
         // a candidate a thread, ranked by counting
         const Cut cut = p.cut[row];
-        u64 own = t < n ? p.candidates[static_cast<uint64_t>(row) * kMaxCandidates + t] : 0;
+        u64 own = t < n ? s.cand[t] : 0;
         s.cand[kRowThreads + t] = own;
         __syncthreads();
         uint32_t above = 0;
@@ -713,9 +764,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
 constexpr uint32_t kGridWanted = 1024;
 
 uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
-// Bytes of a row: chunk_mass, bin_mass, candidates, cut, bin_count, best, top, listed, n_candidates.
+// Bytes of a row: chunk_mass, bin_mass, candidates, cut, bin_count, best, n_candidates, top, listed.
 uint64_t row_bytes(uint32_t vocab) {
-    return 8ull * (chunks_of(vocab) + kBins + kMaxCandidates) + sizeof(Cut) + 4ull * (kBins + chunks_of(vocab) + 3);
+    const uint64_t chunks = chunks_of(vocab);
+    return 8 * (chunks + kBins + chunks * kChunkCandidates) + sizeof(Cut) + 4 * (kBins + 2 * chunks + 2);
 }
 
 }  // namespace
@@ -748,13 +800,13 @@ extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, 
     auto take = [&](uint64_t bytes) { uint8_t *a = at; at += batch * bytes; return a; };
     p.chunk_mass = reinterpret_cast<u64 *>(take(8ull * p.chunks));
     p.bin_mass = reinterpret_cast<u64 *>(take(8ull * kBins));
-    p.candidates = reinterpret_cast<u64 *>(take(8ull * kMaxCandidates));
+    p.candidates = reinterpret_cast<u64 *>(take(8ull * p.chunks * kChunkCandidates));
     p.cut = reinterpret_cast<Cut *>(take(sizeof(Cut)));
     p.bin_count = reinterpret_cast<uint32_t *>(take(4ull * kBins));
     p.best = reinterpret_cast<uint32_t *>(take(4ull * p.chunks));
+    p.n_candidates = reinterpret_cast<uint32_t *>(take(4ull * p.chunks));
     p.top = reinterpret_cast<uint32_t *>(take(4));
     p.listed = reinterpret_cast<uint32_t *>(take(4));
-    p.n_candidates = reinterpret_cast<uint32_t *>(take(4));
     hipStream_t s = as_stream(stream);
     const dim3 grid(p.spans, batch);
     sample_best_kernel<<<grid, kChunkThreads, 0, s>>>(p);
