@@ -267,53 +267,46 @@ __device__ __forceinline__ void collect(const SampleParams &p, uint32_t row, Chu
         }
 }
 
+// The largest key, in its upper 24 bits, that k of the chunks' maxima reach (0: none).  Every wave for itself.
+template <uint32_t N>
+__device__ __forceinline__ uint32_t reached_by(const uint32_t *best, uint32_t chunks, uint32_t k) {
+    uint32_t keys[N], least = 0;
+#pragma unroll
+    for (uint32_t u = 0; u < N; ++u) {
+        const uint32_t c = u * kWave + threadIdx.x % kWave;
+        keys[u] = c < chunks ? best[c] : 0;
+    }
+#pragma unroll 1
+    for (uint32_t bit = 1u << 31; bit >= 1u << 8; bit >>= 1) {
+        uint32_t reach = 0;
+#pragma unroll
+        for (uint32_t u = 0; u < N; ++u) reach += __popcll(__builtin_amdgcn_ballot_w64(keys[u] >= (least | bit)));
+        if (reach >= k) least |= bit;
+    }
+    return least;
+}
+
 // ---- 2 ----------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const SampleParams p) {
     __shared__ u64 mass[kBins];
-    __shared__ __align__(16) uint32_t count[kBins];
+    __shared__ uint32_t count[kBins];
     __shared__ u64 part[kChunkThreads / kWave];
     __shared__ ChunkSpace out;
-    __shared__ uint32_t threshold;
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
     if (t < kMostSpan) out.n[t] = 0;
-    // the chunks' maxima: the row's, and the top_k-th of them
-    uint32_t *keys = count, top = 0, own[kMaxChunks / kChunkThreads];
-#pragma unroll
-    for (uint32_t u = 0; u < kMaxChunks / kChunkThreads; ++u) {
-        const uint32_t c = u * kChunkThreads + t;
-        own[u] = c < p.chunks ? p.best[static_cast<uint64_t>(row) * p.chunks + c] : 0;
-        keys[c] = own[u];
-        top = own[u] > top ? own[u] : top;
-    }
+    // the row's largest key
+    const uint32_t *best = p.best + static_cast<uint64_t>(row) * p.chunks;
+    uint32_t top = 0;
+    for (uint32_t c = t % kWave; c < p.chunks; c += kWave) top = best[c] > top ? best[c] : top;
     top = wave_max_u32(top);
-    uint32_t *tops = reinterpret_cast<uint32_t *>(part);
-    if (t % kWave == 0) tops[t / kWave] = top;
-    if (t == 0) threshold = 0;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t w = 0; w < kChunkThreads / kWave; ++w) top = tops[w] > top ? tops[w] : top;
     if (blockIdx.x == 0 && t == 0) p.top[row] = top;
     const Row r = row_of(p, row, top);
     if (top == 0 || r.greedy) return;
     if (r.top_k != 0 && r.top_k <= p.chunks) {
-        uint32_t above[kMaxChunks / kChunkThreads] = {};
-#pragma unroll 4
-        for (uint32_t c = 0; c < p.chunks; c += 4) {   // zeros behind the last chunk are above nothing
-            const uint4 q = *reinterpret_cast<const uint4 *>(keys + c);
-#pragma unroll
-            for (uint32_t u = 0; u < kMaxChunks / kChunkThreads; ++u) {
-                const uint32_t me = u * kChunkThreads + t;
-                if (u != 0 && u * kChunkThreads >= p.chunks) break;   // uniform
-                above[u] += (q.x > own[u] || (q.x == own[u] && c < me)) + (q.y > own[u] || (q.y == own[u] && c + 1 < me)) +
-                            (q.z > own[u] || (q.z == own[u] && c + 2 < me)) + (q.w > own[u] || (q.w == own[u] && c + 3 < me));
-            }
-        }
-#pragma unroll
-        for (uint32_t u = 0; u < kMaxChunks / kChunkThreads; ++u)
-            if (u * kChunkThreads + t < p.chunks && above[u] + 1 == r.top_k) threshold = own[u];   // one thread's one chunk
-        __syncthreads();
-        const uint32_t least = threshold;
+        const uint32_t least = p.chunks <= 4 * kWave ? reached_by<4>(best, p.chunks, r.top_k)
+                                                     : reached_by<kMaxChunks / kWave>(best, p.chunks, r.top_k);
+        __syncthreads();   // the lists' counts are cleared
         if (least != 0) {
             if (blockIdx.x == 0 && t == 0) {
                 Cut cut{};
@@ -332,7 +325,6 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
             return;
         }
     }
-    __syncthreads();   // every thread has read the keys that the histogram overwrites
     const bool by_count = r.top_k != 0, by_mass = r.top_p < 1.0;   // each needs its half of the histogram
     if (by_count || by_mass) {
         for (uint32_t b = t; b < kBins; b += kChunkThreads) { mass[b] = 0; count[b] = 0; }
