@@ -16,6 +16,9 @@ namespace {
 
 constexpr uint32_t kAppendThreads = 256;
 constexpr uint32_t kAppendWaves = kAppendThreads / kWave;
+// Few tokens: a wave per head (or two, or four, that fit its lanes), so that one token occupies several CUs.  From kManyWaves
+// waves on, several a wave: the angles of a token are worked out once for all of them.
+constexpr uint32_t kManyHeads = 4, kManyWaves = 4096;
 
 struct AppendParams {
     const void *q, *k, *v;
@@ -28,8 +31,10 @@ struct AppendParams {
     uint32_t tokens, q_heads, kv_heads;
     uint32_t stride_q_row, stride_q_head, stride_k_row, stride_v_row, stride_q_out_row;
     uint32_t rotary_dim;
-    uint32_t heads_per_wave, waves_per_token;
+    uint32_t waves_per_token;
     int interleaved;
+    int small;            // slots are below 2^32: a 32-bit division finds the page
+    uint64_t slots_end;   // pages * page_size
     float eps;
 };
 
@@ -90,58 +95,71 @@ __device__ __forceinline__ float head_sum(float v) {
     return v;
 }
 
-// One wave: heads_per_wave heads of one token, 64 / (D / 4) of them at a time.  Heads are numbered queries, keys, values.
-template <bool BF16, uint32_t D, bool VEC>
+// One wave: kBatch x kAtOnce neighbouring heads of one token, kAtOnce = 64 / (D / 4) of them side by side on its lanes, all
+// asked for before the first is looked at.  Heads are numbered queries, keys, values.
+template <bool BF16, uint32_t D, bool VEC, uint32_t kBatch>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendParams p) {
     constexpr uint32_t kLanes = D / 4, kAtOnce = kWave / kLanes;
     const uint32_t lane = threadIdx.x % kWave;
-    const uint32_t wave = blockIdx.x * kAppendWaves + threadIdx.x / kWave;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kAppendWaves + threadIdx.x / kWave);
     const uint32_t token = wave / p.waves_per_token;
     if (token >= p.tokens) return;
-    const uint32_t first = (wave % p.waves_per_token) * p.heads_per_wave;
+    const uint32_t first = (wave - token * p.waves_per_token) * kBatch * kAtOnce + lane / kLanes;
     const uint32_t e0 = (lane % kLanes) * 4;
     const uint32_t half = p.rotary_dim / 2;
     const bool turns = e0 < p.rotary_dim;
+    const uint32_t heads = p.q_heads + 2 * p.kv_heads;
+
+    float x[kBatch][4];
+#pragma unroll
+    for (uint32_t u = 0; u < kBatch; ++u) {
+        const uint32_t h = first + u * kAtOnce;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[u][i] = 0.0f;
+        if (h < p.q_heads)
+            load_act4<BF16, VEC>(p.q, static_cast<uint64_t>(token) * p.stride_q_row + static_cast<uint64_t>(h) * p.stride_q_head + e0, x[u]);
+        else if (h < p.q_heads + p.kv_heads)
+            load_act4<BF16, VEC>(p.k, static_cast<uint64_t>(token) * p.stride_k_row + (h - p.q_heads) * D + e0, x[u]);
+        else if (h < heads)
+            load_act4<BF16, VEC>(p.v, static_cast<uint64_t>(token) * p.stride_v_row + (h - p.q_heads - p.kv_heads) * D + e0, x[u]);
+    }
+    float qw[4], kw[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        qw[i] = p.q_weight != nullptr ? p.q_weight[e0 + i] : 1.0f;
+        kw[i] = p.k_weight != nullptr ? p.k_weight[e0 + i] : 1.0f;
+    }
+    const int64_t slot = p.slots[token];
 
     float c[4] = {1.0f, 1.0f, 1.0f, 1.0f}, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (turns) {
         const double position = p.positions[token] * 0.15915494309189533577;   // 1 / (2 pi): angles in revolutions
         const uint32_t pair = p.interleaved ? e0 / 2 : (e0 < half ? e0 : e0 - half);
+        const uint32_t pairs = p.interleaved ? 2 : 4;
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-            if (p.interleaved && i >= 2) break;
+            if (i >= pairs) break;   // uniform
             const double turn = position * p.freqs[pair + i];
             sincospif(2.0f * static_cast<float>(turn - rint(turn)), &s[i], &c[i]);
         }
     }
-    const int64_t slot = p.slots[token];
-    const bool held = slot >= 0 && static_cast<uint64_t>(slot) < static_cast<uint64_t>(p.cache.pages) * p.cache.page_size;
-    const uint64_t page = held ? static_cast<uint64_t>(slot) / p.cache.page_size : 0;
-    const uint64_t in_page = held ? static_cast<uint64_t>(slot) % p.cache.page_size : 0;
-    const uint64_t row0 = page * p.cache.stride_page + in_page * p.cache.stride_token;
+    const bool held = slot >= 0 && static_cast<uint64_t>(slot) < p.slots_end;
+    const uint32_t slot32 = static_cast<uint32_t>(slot);
+    const uint64_t page = p.small ? slot32 / p.cache.page_size : static_cast<uint64_t>(slot) / p.cache.page_size;
+    const uint64_t row0 = page * p.cache.stride_page + (static_cast<uint64_t>(slot) - page * p.cache.page_size) * p.cache.stride_token;
     const uint64_t element = kv_element_bytes(p.cache.dtype);
 
-    for (uint32_t h0 = first; h0 < first + p.heads_per_wave; h0 += kAtOnce) {
-        const uint32_t h = h0 + lane / kLanes;
-        const bool live = h < p.q_heads + 2 * p.kv_heads;
+#pragma unroll
+    for (uint32_t u = 0; u < kBatch; ++u) {
+        const uint32_t h = first + u * kAtOnce;
         const bool is_q = h < p.q_heads, is_k = !is_q && h < p.q_heads + p.kv_heads;
         const uint32_t hk = is_q ? 0 : is_k ? h - p.q_heads : h - p.q_heads - p.kv_heads;
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (live) {
-            if (is_q)
-                load_act4<BF16, VEC>(p.q, static_cast<uint64_t>(token) * p.stride_q_row + static_cast<uint64_t>(h) * p.stride_q_head + e0, x);
-            else if (is_k)
-                load_act4<BF16, VEC>(p.k, static_cast<uint64_t>(token) * p.stride_k_row + hk * D + e0, x);
-            else
-                load_act4<BF16, VEC>(p.v, static_cast<uint64_t>(token) * p.stride_v_row + hk * D + e0, x);
-        }
-        const float squares = head_sum<kLanes>((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]));
-        const float *w = is_q ? p.q_weight : is_k ? p.k_weight : nullptr;
-        float y[4] = {x[0], x[1], x[2], x[3]};
-        if (w != nullptr) {
+        float y[4] = {x[u][0], x[u][1], x[u][2], x[u][3]};
+        const float squares = head_sum<kLanes>((y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]));
+        if (is_q ? p.q_weight != nullptr : is_k && p.k_weight != nullptr) {
             const float scale = rms_scale(squares, D, p.eps);
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) y[i] = (x[i] * scale) * w[e0 + i];
+            for (uint32_t i = 0; i < 4; ++i) y[i] = (y[i] * scale) * (is_q ? qw[i] : kw[i]);
         }
         if (p.rotary_dim != 0) {   // uniform: the exchange needs every lane
             float r[4];
@@ -164,10 +182,9 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendPara
                 for (uint32_t i = 0; i < 4; ++i) y[i] = r[i];
             }
         }
-        if (!live) continue;
         if (is_q) {
             store_act4<BF16, VEC>(p.q_out, static_cast<uint64_t>(token) * p.stride_q_out_row + h * D + e0, y);
-        } else if (held) {
+        } else if (held && h < heads) {
             uint8_t *pool = static_cast<uint8_t *>(is_k ? p.cache.k : p.cache.v);
             store_kv4(pool + (row0 + hk * p.cache.stride_head) * element, e0, p.cache.dtype,
                       is_k ? p.cache.k_scale : p.cache.v_scale, y);
@@ -176,9 +193,11 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendPara
 }
 
 template <bool BF16, uint32_t D>
-void launch_append(const AppendParams &p, bool vec, uint32_t grid, hipStream_t s) {
-    if (vec) append_kernel<BF16, D, true><<<grid, kAppendThreads, 0, s>>>(p);
-    else append_kernel<BF16, D, false><<<grid, kAppendThreads, 0, s>>>(p);
+void launch_append(const AppendParams &p, uint32_t batch, bool vec, uint32_t grid, hipStream_t s) {
+    if (batch == 1 && vec) append_kernel<BF16, D, true, 1><<<grid, kAppendThreads, 0, s>>>(p);
+    else if (batch == 1) append_kernel<BF16, D, false, 1><<<grid, kAppendThreads, 0, s>>>(p);
+    else if (vec) append_kernel<BF16, D, true, kManyHeads><<<grid, kAppendThreads, 0, s>>>(p);
+    else append_kernel<BF16, D, false, kManyHeads><<<grid, kAppendThreads, 0, s>>>(p);
 }
 
 }  // namespace
@@ -221,8 +240,11 @@ extern "C" int q8mi_qk_norm_rope_append(const void *q, const void *k, const void
     p.rotary_dim = rotary_dim; p.interleaved = interleaved; p.eps = eps;
     const uint32_t at_once = kWave / (cache->head_dim / 4);
     const uint32_t heads = q_heads + 2 * cache->kv_heads;
-    p.heads_per_wave = at_once;
-    p.waves_per_token = (heads + p.heads_per_wave - 1) / p.heads_per_wave;
+    const uint32_t groups = (heads + at_once - 1) / at_once;
+    const uint32_t batch = static_cast<uint64_t>(tokens) * groups >= kManyWaves ? kManyHeads : 1;
+    p.waves_per_token = (groups + batch - 1) / batch;
+    p.slots_end = static_cast<uint64_t>(cache->pages) * cache->page_size;
+    p.small = p.slots_end <= 0xffffffffull;
     const uint64_t grid = (static_cast<uint64_t>(tokens) * p.waves_per_token + kAppendWaves - 1) / kAppendWaves;
     if (grid > 0x3fffffffull) return fail(Q8MI_REJECTED, "%s: too many heads for one launch", what);
 
@@ -233,9 +255,9 @@ extern "C" int q8mi_qk_norm_rope_append(const void *q, const void *k, const void
     hipStream_t s = as_stream(stream);
     auto by_dim = [&](auto bf16) {
         constexpr bool B = decltype(bf16)::value;
-        if (cache->head_dim == 64) launch_append<B, 64>(p, vec, static_cast<uint32_t>(grid), s);
-        else if (cache->head_dim == 128) launch_append<B, 128>(p, vec, static_cast<uint32_t>(grid), s);
-        else launch_append<B, 256>(p, vec, static_cast<uint32_t>(grid), s);
+        if (cache->head_dim == 64) launch_append<B, 64>(p, batch, vec, static_cast<uint32_t>(grid), s);
+        else if (cache->head_dim == 128) launch_append<B, 128>(p, batch, vec, static_cast<uint32_t>(grid), s);
+        else launch_append<B, 256>(p, batch, vec, static_cast<uint32_t>(grid), s);
     };
     if (is_bf16) by_dim(std::true_type{});
     else by_dim(std::false_type{});

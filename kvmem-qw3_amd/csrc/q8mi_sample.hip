@@ -753,7 +753,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
 
 // Chunks of a workgroup: one while that leaves CUs idle, up to kMostSpan where rows are many (the histogram of a workgroup
 // is then cleared and added to the row's once for several chunks).
-constexpr uint32_t kGridWanted = 1024;
+constexpr uint32_t kGridWanted = 512;
 
 uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
 // Bytes of a row: chunk_mass, bin_mass, candidates, cut, bin_count, best, n_candidates, top, listed.
