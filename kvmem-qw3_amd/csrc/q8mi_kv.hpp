@@ -32,6 +32,15 @@ inline int check_kv_cache(const char *what, const q8mi_kv_cache *c) {
     return Q8MI_OK;
 }
 
+// Two floats as bf16, nearest even (v_cvt_pk_bf16_f32), the first in the lower half.
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    v2bf r;
+    r.x = static_cast<__bf16>(a);
+    r.y = static_cast<__bf16>(b);
+    return __builtin_bit_cast(uint32_t, r);
+}
+
 // Four floats as four elements of a cache row (nearest even; e4m3: the quotient by the scale, clamped, NaN kept).
 __device__ __forceinline__ void store_kv4(void *row, uint32_t element, int dtype, float scale, const float (&v)[4]) {
     if (dtype == Q8MI_KV_E4M3) {
@@ -46,11 +55,16 @@ __device__ __forceinline__ void store_kv4(void *row, uint32_t element, int dtype
         *reinterpret_cast<int *>(static_cast<uint8_t *>(row) + element) = w;
         return;
     }
-    uint16_t h[4];
+    uint2 w;
+    if (dtype == Q8MI_KV_BF16) {
+        w = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    } else {
+        uint32_t h[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = dtype == Q8MI_KV_BF16 ? float_to_bf16_bits(v[i]) : float_to_half_bits(v[i]);
-    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(row) + element) =
-        make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
+        for (int i = 0; i < 4; ++i) h[i] = float_to_half_bits(v[i]);
+        w = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    }
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(row) + element) = w;
 }
 
 }  // namespace q8mi

@@ -17,7 +17,7 @@ namespace {
 constexpr uint32_t kAppendThreads = 256;
 constexpr uint32_t kAppendWaves = kAppendThreads / kWave;
 // Few tokens: a wave per head (or two, or four, that fit its lanes), so that one token occupies several CUs.  From kManyWaves
-// waves on, several a wave: the angles of a token are worked out once for all of them.
+// heads on, a workgroup per token, several heads a wave: the angles of a token are worked out once for all of them.
 constexpr uint32_t kManyHeads = 4, kManyWaves = 4096;
 
 struct AppendParams {
@@ -62,15 +62,12 @@ template <bool BF16, bool VEC>
 __device__ __forceinline__ void store_act4(void *base, uint64_t at, const float (&v)[4]) {
     if constexpr (BF16) {
         uint16_t *p = static_cast<uint16_t *>(base) + at;
-        uint16_t h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = float_to_bf16_bits(v[i]);
+        const uint2 h = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
         if (VEC) {
-            *reinterpret_cast<uint2 *>(p) =
-                make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
+            *reinterpret_cast<uint2 *>(p) = h;
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = h[i];
+            p[0] = static_cast<uint16_t>(h.x); p[1] = static_cast<uint16_t>(h.x >> 16);
+            p[2] = static_cast<uint16_t>(h.y); p[3] = static_cast<uint16_t>(h.y >> 16);
         }
     } else {
         float *p = static_cast<float *>(base) + at;
@@ -95,34 +92,51 @@ __device__ __forceinline__ float head_sum(float v) {
     return v;
 }
 
-// One wave: kBatch x kAtOnce neighbouring heads of one token, kAtOnce = 64 / (D / 4) of them side by side on its lanes, all
-// asked for before the first is looked at.  Heads are numbered queries, keys, values.
+// Sine and cosine of a token's pair.
+__device__ __forceinline__ float2 angle_of(const AppendParams &p, double position_turns, uint32_t pair) {
+    const double turn = position_turns * p.freqs[pair];
+    float2 r;
+    sincospif(2.0f * static_cast<float>(turn - rint(turn)), &r.x, &r.y);
+    return r;
+}
+
+// A wave takes kBatch x kAtOnce neighbouring heads of one token at a time, kAtOnce = 64 / (D / 4) of them side by side on its
+// lanes, all asked for before the first is looked at.  Heads are numbered queries, keys, values.
+//   kBatch = 1: every wave has heads of its own and works its angles out itself
+//   kBatch > 1: a workgroup has a token, whose angles it works out once, in LDS
 template <bool BF16, uint32_t D, bool VEC, uint32_t kBatch>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendParams p) {
     constexpr uint32_t kLanes = D / 4, kAtOnce = kWave / kLanes;
+    constexpr bool kTokenPerGroup = kBatch > 1;
+    __shared__ float2 angles[kTokenPerGroup ? D / 2 : 1];
     const uint32_t lane = threadIdx.x % kWave;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kAppendWaves + threadIdx.x / kWave);
-    const uint32_t token = wave / p.waves_per_token;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane((kTokenPerGroup ? 0 : blockIdx.x * kAppendWaves) + threadIdx.x / kWave);
+    const uint32_t token = kTokenPerGroup ? blockIdx.x : wave / p.waves_per_token;
     if (token >= p.tokens) return;
-    const uint32_t first = (wave - token * p.waves_per_token) * kBatch * kAtOnce + lane / kLanes;
+    const uint32_t heads = p.q_heads + 2 * p.kv_heads;
     const uint32_t e0 = (lane % kLanes) * 4;
     const uint32_t half = p.rotary_dim / 2;
     const bool turns = e0 < p.rotary_dim;
-    const uint32_t heads = p.q_heads + 2 * p.kv_heads;
+    const uint32_t first_pair = !turns ? 0 : p.interleaved ? e0 / 2 : e0 < half ? e0 : e0 - half;
+    const uint32_t pairs = !turns ? 0 : p.interleaved ? 2 : 4;
 
     float x[kBatch][4];
+    auto load = [&](uint32_t first) {   // heads from `first` on
 #pragma unroll
-    for (uint32_t u = 0; u < kBatch; ++u) {
-        const uint32_t h = first + u * kAtOnce;
+        for (uint32_t u = 0; u < kBatch; ++u) {
+            const uint32_t h = first + u * kAtOnce + lane / kLanes;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[u][i] = 0.0f;
-        if (h < p.q_heads)
-            load_act4<BF16, VEC>(p.q, static_cast<uint64_t>(token) * p.stride_q_row + static_cast<uint64_t>(h) * p.stride_q_head + e0, x[u]);
-        else if (h < p.q_heads + p.kv_heads)
-            load_act4<BF16, VEC>(p.k, static_cast<uint64_t>(token) * p.stride_k_row + (h - p.q_heads) * D + e0, x[u]);
-        else if (h < heads)
-            load_act4<BF16, VEC>(p.v, static_cast<uint64_t>(token) * p.stride_v_row + (h - p.q_heads - p.kv_heads) * D + e0, x[u]);
-    }
+            for (int i = 0; i < 4; ++i) x[u][i] = 0.0f;
+            if (h < p.q_heads)
+                load_act4<BF16, VEC>(p.q, static_cast<uint64_t>(token) * p.stride_q_row + static_cast<uint64_t>(h) * p.stride_q_head + e0, x[u]);
+            else if (h < p.q_heads + p.kv_heads)
+                load_act4<BF16, VEC>(p.k, static_cast<uint64_t>(token) * p.stride_k_row + (h - p.q_heads) * D + e0, x[u]);
+            else if (h < heads)
+                load_act4<BF16, VEC>(p.v, static_cast<uint64_t>(token) * p.stride_v_row + (h - p.q_heads - p.kv_heads) * D + e0, x[u]);
+        }
+    };
+    uint32_t first = (kTokenPerGroup ? wave : wave - token * p.waves_per_token) * kBatch * kAtOnce;
+    load(first);
     float qw[4], kw[4];
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
@@ -132,16 +146,19 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendPara
     const int64_t slot = p.slots[token];
 
     float c[4] = {1.0f, 1.0f, 1.0f, 1.0f}, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (turns) {
+    if (p.rotary_dim != 0) {   // uniform
         const double position = p.positions[token] * 0.15915494309189533577;   // 1 / (2 pi): angles in revolutions
-        const uint32_t pair = p.interleaved ? e0 / 2 : (e0 < half ? e0 : e0 - half);
-        const uint32_t pairs = p.interleaved ? 2 : 4;
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            if (i >= pairs) break;   // uniform
-            const double turn = position * p.freqs[pair + i];
-            sincospif(2.0f * static_cast<float>(turn - rint(turn)), &s[i], &c[i]);
+        if constexpr (kTokenPerGroup) {
+            if (threadIdx.x < half) angles[threadIdx.x] = angle_of(p, position, threadIdx.x);
+            __syncthreads();
         }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            if (i < pairs) {
+                const float2 a = kTokenPerGroup ? angles[first_pair + i] : angle_of(p, position, first_pair + i);
+                s[i] = a.x;
+                c[i] = a.y;
+            }
     }
     const bool held = slot >= 0 && static_cast<uint64_t>(slot) < p.slots_end;
     const uint32_t slot32 = static_cast<uint32_t>(slot);
@@ -149,15 +166,17 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendPara
     const uint64_t row0 = page * p.cache.stride_page + (static_cast<uint64_t>(slot) - page * p.cache.page_size) * p.cache.stride_token;
     const uint64_t element = kv_element_bytes(p.cache.dtype);
 
+    for (;;) {
 #pragma unroll
     for (uint32_t u = 0; u < kBatch; ++u) {
-        const uint32_t h = first + u * kAtOnce;
+        const uint32_t h = first + u * kAtOnce + lane / kLanes;
         const bool is_q = h < p.q_heads, is_k = !is_q && h < p.q_heads + p.kv_heads;
         const uint32_t hk = is_q ? 0 : is_k ? h - p.q_heads : h - p.q_heads - p.kv_heads;
         float y[4] = {x[u][0], x[u][1], x[u][2], x[u][3]};
         const float squares = head_sum<kLanes>((y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]));
         if (is_q ? p.q_weight != nullptr : is_k && p.k_weight != nullptr) {
-            const float scale = rms_scale(squares, D, p.eps);
+            // the hardware's reciprocal root is good to one step of fp32; every lane of a head has the same sum
+            const float scale = __builtin_amdgcn_rsqf(squares * (1.0f / D) + p.eps);
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) y[i] = (y[i] * scale) * (is_q ? qw[i] : kw[i]);
         }
@@ -189,6 +208,11 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendPara
             store_kv4(pool + (row0 + hk * p.cache.stride_head) * element, e0, p.cache.dtype,
                       is_k ? p.cache.k_scale : p.cache.v_scale, y);
         }
+    }
+        if constexpr (!kTokenPerGroup) break;
+        first += kAppendWaves * kBatch * kAtOnce;
+        if (first >= heads) break;
+        load(first);
     }
 }
 
@@ -242,10 +266,10 @@ extern "C" int q8mi_qk_norm_rope_append(const void *q, const void *k, const void
     const uint32_t heads = q_heads + 2 * cache->kv_heads;
     const uint32_t groups = (heads + at_once - 1) / at_once;
     const uint32_t batch = static_cast<uint64_t>(tokens) * groups >= kManyWaves ? kManyHeads : 1;
-    p.waves_per_token = (groups + batch - 1) / batch;
+    p.waves_per_token = groups;
     p.slots_end = static_cast<uint64_t>(cache->pages) * cache->page_size;
     p.small = p.slots_end <= 0xffffffffull;
-    const uint64_t grid = (static_cast<uint64_t>(tokens) * p.waves_per_token + kAppendWaves - 1) / kAppendWaves;
+    const uint64_t grid = batch > 1 ? tokens : (static_cast<uint64_t>(tokens) * groups + kAppendWaves - 1) / kAppendWaves;
     if (grid > 0x3fffffffull) return fail(Q8MI_REJECTED, "%s: too many heads for one launch", what);
 
     const uintptr_t bases = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
