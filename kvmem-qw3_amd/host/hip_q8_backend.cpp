@@ -67,6 +67,25 @@ struct HipWeight final : DeviceWeight {
     }
 };
 
+struct HipKvCache final : DeviceKvCache {
+    void *k = nullptr, *v = nullptr;
+    ~HipKvCache() override {
+        if (k) (void)hipFree(k);
+        if (v) (void)hipFree(v);
+    }
+    q8mi_kv_cache descriptor() const {
+        q8mi_kv_cache c{};
+        c.k = k; c.v = v;
+        c.dtype = dtype == DeviceTensorDType::FP8_E4M3 ? Q8MI_KV_E4M3 : dtype == DeviceTensorDType::F16 ? Q8MI_KV_F16 : Q8MI_KV_BF16;
+        c.pages = pages; c.page_size = page_size; c.kv_heads = kv_heads; c.head_dim = head_dim;
+        c.stride_token = head_dim;
+        c.stride_head = static_cast<uint64_t>(page_size) * head_dim;
+        c.stride_page = kv_heads * c.stride_head;
+        c.k_scale = k_scale; c.v_scale = v_scale;
+        return c;
+    }
+};
+
 struct HipArgmaxBuffer final : DeviceArgmaxBuffer {
     q8mi_argmax_pair *ptr = nullptr;
     ~HipArgmaxBuffer() override {
@@ -109,9 +128,11 @@ HipQ8Backend::HipQ8Backend() : owner_(std::make_shared<Owner>()) {
 HipQ8Backend::~HipQ8Backend() {
     owner_->backend = nullptr;   // tensors and weights that outlive the backend have nobody to tell
     if (stream_) (void)hipStreamSynchronize(stream_);
-    for (Scratch *s : {&q8_1_, &d4_, &argmax_partial_, &argmax_result_, &lm_head_, &lm_rows_, &out_f32_, &row_ids_}) {
+    for (Scratch *s : {&q8_1_, &d4_, &argmax_partial_, &argmax_result_, &lm_head_, &lm_rows_, &out_f32_, &row_ids_, &attention_,
+                       &sample_}) {
         if (s->ptr) (void)hipFree(s->ptr);
     }
+    for (void *p : retired_) (void)hipFree(p);
     if (argmax_dev_) (void)hipFree(argmax_dev_);
     if (lm_host_) (void)hipHostFree(lm_host_);
     if (argmax_host_) (void)hipHostFree(argmax_host_);
@@ -146,6 +167,11 @@ DeviceStatus HipQ8Backend::end_capture() {
     if (graph_exec_) { (void)hipGraphExecDestroy(graph_exec_); graph_exec_ = nullptr; }
     if (graph_) { (void)hipGraphDestroy(graph_); graph_ = nullptr; }
     if (auto st = hip_status(hipStreamEndCapture(stream_, &graph_), "hip end capture"); !st.ok) return st;
+    if (!retired_.empty()) {   // named by the graph just destroyed
+        (void)hipStreamSynchronize(stream_);
+        for (void *p : retired_) (void)hipFree(p);
+        retired_.clear();
+    }
     if (!flushed.ok) return flushed;
     return hip_status(hipGraphInstantiate(&graph_exec_, graph_, nullptr, nullptr, 0), "hip graph instantiate");
 }
@@ -166,6 +192,51 @@ std::unique_ptr<DeviceTensor> HipQ8Backend::tensor_f32(uint64_t count, const cha
 std::unique_ptr<DeviceTensor> HipQ8Backend::tensor_bf16(uint64_t count, const char *) {
     forget_quantized();
     return make_tensor(count, 2, DeviceTensorDType::BF16, owner_);
+}
+
+std::unique_ptr<DeviceTensor> HipQ8Backend::tensor_i32(uint64_t count, const char *) {
+    forget_quantized();
+    return make_tensor(count, 4, DeviceTensorDType::I32, owner_);
+}
+
+std::unique_ptr<DeviceTensor> HipQ8Backend::tensor_i64(uint64_t count, const char *) {
+    forget_quantized();
+    return make_tensor(count, 8, DeviceTensorDType::I32, owner_);
+}
+
+std::unique_ptr<DeviceWeight> HipQ8Backend::rope_frequencies(const double *radians, uint64_t count, const char *) {
+    auto w = std::make_unique<HipWeight>();
+    w->owner = owner_;
+    w->rows = 1;
+    w->cols = count;
+    w->format = DeviceWeightFormat::F32;   // the nearest name: `bytes` tells 64-bit elements apart
+    w->bytes = count * 8;
+    if (hipMalloc(reinterpret_cast<void **>(&w->ptr), w->bytes ? w->bytes : 1) != hipSuccess ||
+        hipMemcpy(w->ptr, radians, w->bytes, hipMemcpyHostToDevice) != hipSuccess) {
+        (void)hipGetLastError();
+        return nullptr;
+    }
+    return w;
+}
+
+std::unique_ptr<DeviceKvCache> HipQ8Backend::kv_cache(DeviceTensorDType dtype, uint32_t pages, uint32_t page_size,
+                                                      uint32_t kv_heads, uint32_t head_dim, float k_scale, float v_scale,
+                                                      const char *) {
+    if (capturing_) return nullptr;
+    const bool fp8 = dtype == DeviceTensorDType::FP8_E4M3;
+    if (!fp8 && dtype != DeviceTensorDType::F16 && dtype != DeviceTensorDType::BF16) return nullptr;
+    if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || pages == 0 || page_size == 0 || kv_heads == 0) return nullptr;
+    auto c = std::make_unique<HipKvCache>();
+    c->dtype = dtype;
+    c->pages = pages; c->page_size = page_size; c->kv_heads = kv_heads; c->head_dim = head_dim;
+    c->k_scale = k_scale; c->v_scale = v_scale;
+    const uint64_t bytes = static_cast<uint64_t>(pages) * page_size * kv_heads * head_dim * (fp8 ? 1 : 2);
+    for (void **pool : {&c->k, &c->v})
+        if (hipMalloc(pool, bytes) != hipSuccess || hipMemsetAsync(*pool, 0, bytes, stream_) != hipSuccess) {
+            (void)hipGetLastError();
+            return nullptr;
+        }
+    return c;
 }
 
 std::unique_ptr<DeviceWeight> HipQ8Backend::weight_f32(const float *data, uint64_t count, const char *) {
@@ -248,7 +319,8 @@ DeviceStatus HipQ8Backend::ensure(Scratch &s, size_t need, const char *what) {
     if (&s == &q8_1_) forget_quantized();
     if (s.ptr) {
         (void)hipStreamSynchronize(stream_);
-        (void)hipFree(s.ptr);
+        if (graph_exec_) retired_.push_back(s.ptr);   // a replay may still use it
+        else (void)hipFree(s.ptr);
         s.ptr = nullptr;
         s.capacity = 0;
     }
@@ -1034,6 +1106,102 @@ DeviceStatus HipQ8Backend::lm_head_verify(const DeviceWeight &w_out, const Devic
     accepted = static_cast<uint32_t>(host_acc[0]);
     next_token = host_acc[1];
     return {};
+}
+
+// ---- between the projections and behind the LM head --------------------------------------------
+namespace {
+
+// Whether `rows` rows of `width` elements, `stride` apart, fit a tensor.
+bool fits(const DeviceTensor &t, uint64_t rows, uint64_t stride, uint64_t width) {
+    return rows == 0 || (rows - 1) * stride + width <= t.count;
+}
+bool is_i32(const DeviceTensor &t) { return t.dtype == DeviceTensorDType::I32 && t.elem_size == 4; }
+bool is_act(const DeviceTensor &t) { return t.dtype == DeviceTensorDType::F32 || t.dtype == DeviceTensorDType::BF16; }
+
+}  // namespace
+
+DeviceStatus HipQ8Backend::qk_norm_rope_append(DeviceTensor &q_out, const DeviceTensor &q, const DeviceTensor &k,
+                                               const DeviceTensor &v, const DeviceWeight *q_norm, const DeviceWeight *k_norm,
+                                               float eps, const DeviceWeight *freqs, uint32_t rotary_dim, bool interleaved,
+                                               const DeviceTensor &positions, const DeviceTensor &slots, uint32_t tokens,
+                                               uint32_t q_heads, uint32_t stride_q_row, uint32_t stride_q_head,
+                                               uint32_t stride_k_row, uint32_t stride_v_row, uint32_t stride_q_out_row,
+                                               DeviceKvCache &cache) {
+    if (tokens == 0) return {};
+    const auto &c = static_cast<const HipKvCache &>(cache);
+    const uint64_t dim = c.head_dim, kv_width = c.kv_heads * dim;
+    if (!is_act(q) || k.dtype != q.dtype || v.dtype != q.dtype || q_out.dtype != q.dtype)
+        return {false, "qk_norm_rope_append: q, k, v and q_out must be fp32, or bf16, together"};
+    if (q_heads == 0 || !fits(q, tokens, stride_q_row, (q_heads - 1ull) * stride_q_head + dim) ||
+        !fits(k, tokens, stride_k_row, kv_width) || !fits(v, tokens, stride_v_row, kv_width) ||
+        !fits(q_out, tokens, stride_q_out_row, q_heads * dim))
+        return {false, "qk_norm_rope_append: rows outside their tensors"};
+    for (const DeviceWeight *w : {q_norm, k_norm})
+        if (w && (w->format != DeviceWeightFormat::F32 || w->cols < dim || W(*w).bytes != w->cols * 4))
+            return {false, "qk_norm_rope_append: a norm weight needs head_dim fp32 elements"};
+    if (rotary_dim != 0 && (!freqs || W(*freqs).bytes < rotary_dim / 2 * 8ull || W(*freqs).bytes != freqs->cols * 8))
+        return {false, "qk_norm_rope_append: too few frequencies"};
+    if (!is_i32(positions) || positions.count < tokens || slots.elem_size != 8 || slots.count < tokens)
+        return {false, "qk_norm_rope_append: positions (32 bits) and slots (64 bits) of every token"};
+    if (auto st = flush_norm(); !st.ok) return st;
+    wrote(T(q_out).ptr);
+    const q8mi_kv_cache d = c.descriptor();
+    const int rc = q8mi_qk_norm_rope_append(
+        T(q).ptr, T(k).ptr, T(v).ptr, T(q_out).ptr, q.dtype == DeviceTensorDType::BF16, tokens, q_heads, stride_q_row, stride_q_head,
+        stride_k_row, stride_v_row, stride_q_out_row, q_norm ? reinterpret_cast<const float *>(W(*q_norm).ptr) : nullptr,
+        k_norm ? reinterpret_cast<const float *>(W(*k_norm).ptr) : nullptr, eps,
+        freqs ? reinterpret_cast<const double *>(W(*freqs).ptr) : nullptr, rotary_dim, interleaved,
+        static_cast<const int32_t *>(T(positions).ptr), static_cast<const int64_t *>(T(slots).ptr), &d, stream_);
+    if (rc != Q8MI_OK) return failed("qk_norm_rope_append");
+    return launch_status("hip qk_norm_rope_append");
+}
+
+DeviceStatus HipQ8Backend::paged_attention(DeviceTensor &out, const DeviceTensor &q, const DeviceKvCache &cache,
+                                           const DeviceTensor &page_table, uint32_t stride_page_table,
+                                           const DeviceTensor &kv_lens, const DeviceTensor *q_starts, uint32_t n_seqs,
+                                           uint32_t q_rows, uint32_t max_q_len, uint32_t q_heads, uint32_t max_kv_len,
+                                           float scale, uint32_t stride_q_row, uint32_t stride_out_row) {
+    if (n_seqs == 0 || q_rows == 0) return {};
+    const auto &c = static_cast<const HipKvCache &>(cache);
+    if (!is_act(q) || !is_act(out)) return {false, "paged_attention: q and out must be fp32 or bf16"};
+    const uint64_t width = static_cast<uint64_t>(q_heads) * c.head_dim;
+    if (!fits(q, q_rows, stride_q_row, width) || !fits(out, q_rows, stride_out_row, width))
+        return {false, "paged_attention: rows outside their tensors"};
+    if (!is_i32(page_table) || !fits(page_table, n_seqs, stride_page_table, stride_page_table) || !is_i32(kv_lens) ||
+        kv_lens.count < n_seqs || (q_starts && (!is_i32(*q_starts) || q_starts->count < n_seqs + 1ull)))
+        return {false, "paged_attention: page table, lengths or starts too small"};
+    if (auto st = flush_norm(); !st.ok) return st;
+    const size_t need = q8mi_paged_attention_scratch_bytes(n_seqs, max_q_len, q_heads, c.kv_heads, c.head_dim, max_kv_len);
+    if (auto st = ensure(attention_, need, "paged attention scratch alloc"); !st.ok) return st;
+    wrote(T(out).ptr);
+    const q8mi_kv_cache d = c.descriptor();
+    const int rc = q8mi_paged_attention(
+        T(q).ptr, q.dtype == DeviceTensorDType::BF16, q_rows, stride_q_row, &d, static_cast<const int32_t *>(T(page_table).ptr),
+        stride_page_table, static_cast<const int32_t *>(T(kv_lens).ptr),
+        q_starts ? static_cast<const int32_t *>(T(*q_starts).ptr) : nullptr, n_seqs, max_q_len, q_heads, max_kv_len, scale,
+        T(out).ptr, out.dtype == DeviceTensorDType::BF16, stride_out_row, attention_.ptr, stream_);
+    if (rc != Q8MI_OK) return failed("paged_attention");
+    return launch_status("hip paged_attention");
+}
+
+DeviceStatus HipQ8Backend::sample_rows(const DeviceTensor &logits, uint32_t batch, uint32_t vocab, uint32_t row_stride,
+                                       const DeviceTensor *temperature, const DeviceTensor *top_k, const DeviceTensor *top_p,
+                                       const DeviceTensor *min_p, const DeviceTensor &uniform, DeviceArgmaxBuffer &out) {
+    if (batch == 0) return {};
+    auto &dst = static_cast<HipArgmaxBuffer &>(out);
+    if (logits.dtype != DeviceTensorDType::F32 || !fits(logits, batch, row_stride, vocab))
+        return {false, "sample_rows: logits must be fp32 rows inside their tensor"};
+    if (dst.count < batch) return {false, "sample_rows: output smaller than the batch"};
+    for (const DeviceTensor *t : {temperature, top_p, min_p, &uniform})
+        if (t && (t->dtype != DeviceTensorDType::F32 || t->count < batch)) return {false, "sample_rows: parameters need one fp32 element a row"};
+    if (top_k && (!is_i32(*top_k) || top_k->count < batch)) return {false, "sample_rows: top_k needs one 32-bit element a row"};
+    if (auto st = flush_norm(); !st.ok) return st;
+    if (auto st = ensure(sample_, q8mi_sample_scratch_bytes(batch, vocab), "sample scratch alloc"); !st.ok) return st;
+    auto f32 = [](const DeviceTensor *t) { return t ? static_cast<const float *>(T(*t).ptr) : nullptr; };
+    if (q8mi_sample(T(logits).f32(), batch, vocab, row_stride, f32(temperature), top_k ? static_cast<const int32_t *>(T(*top_k).ptr) : nullptr,
+                    f32(top_p), f32(min_p), f32(&uniform), dst.ptr, sample_.ptr, stream_) != Q8MI_OK)
+        return failed("sample");
+    return launch_status("hip sample_rows");
 }
 
 }  // namespace qw3

@@ -64,6 +64,16 @@ struct DeviceArgmaxBuffer {
     uint64_t count = 0;
 };
 
+// One layer's paged key / value cache.  This and the operators on it below are this library's own interface (the reference's
+// attention virtuals are not restated): what they compute is documented with q8mi_qk_norm_rope_append and
+// q8mi_paged_attention in include/q8mi.h.
+struct DeviceKvCache {
+    virtual ~DeviceKvCache() = default;
+    DeviceTensorDType dtype = DeviceTensorDType::BF16;   // BF16, F16 or FP8_E4M3
+    uint32_t pages = 0, page_size = 0, kv_heads = 0, head_dim = 0;
+    float k_scale = 1.0f, v_scale = 1.0f;                // FP8_E4M3 only
+};
+
 class HipQ8Backend {
 public:
     HipQ8Backend();
@@ -103,6 +113,15 @@ public:
     // tensors / weights
     std::unique_ptr<DeviceTensor> tensor_f32(uint64_t count, const char *label);
     std::unique_ptr<DeviceTensor> tensor_bf16(uint64_t count, const char *label);
+    // whole numbers for the cache operators: positions, page tables, lengths (elem_size 4) and slots (elem_size 8; the
+    // reference's dtypes have no name for it)
+    std::unique_ptr<DeviceTensor> tensor_i32(uint64_t count, const char *label);
+    std::unique_ptr<DeviceTensor> tensor_i64(uint64_t count, const char *label);
+    // rotation frequencies in radians per position, one per pair: rows = 1, cols = count, 64-bit
+    std::unique_ptr<DeviceWeight> rope_frequencies(const double *radians, uint64_t count, const char *label);
+    // a cache of pages x page_size tokens, zeroed; null when its type or head_dim is not served or memory is short
+    std::unique_ptr<DeviceKvCache> kv_cache(DeviceTensorDType dtype, uint32_t pages, uint32_t page_size, uint32_t kv_heads,
+                                            uint32_t head_dim, float k_scale, float v_scale, const char *label);
     // fp32 vector (norm weights): rows = 1, cols = count (src/kernels_cuda.cu: weight_f32)
     std::unique_ptr<DeviceWeight> weight_f32(const float *data, uint64_t count, const char *label);
     // `data`: interleaved GGUF Q8_0 blocks (34 B); stored split-plane on the device
@@ -185,6 +204,30 @@ public:
     DeviceStatus copy_argmax_buffer_to_host(const DeviceArgmaxBuffer &src, DeviceArgmax *host, uint32_t count);
     DeviceStatus argmax_batch(const DeviceTensor &x, uint32_t batch, uint32_t row_stride,
                               std::vector<DeviceArgmax> &out);
+
+    // Between the Q/K/V projections and the attention: norm of every query and key head (a null weight: none), rotation of
+    // their first rotary_dim elements, keys and values to slots[token] = page * page_size + row of the cache (below zero:
+    // skipped).  q_out may be q when stride_q_head == head_dim and the row strides agree.  fp32, or bf16 throughout.
+    DeviceStatus qk_norm_rope_append(DeviceTensor &q_out, const DeviceTensor &q, const DeviceTensor &k, const DeviceTensor &v,
+                                     const DeviceWeight *q_norm, const DeviceWeight *k_norm, float eps,
+                                     const DeviceWeight *freqs, uint32_t rotary_dim, bool interleaved,
+                                     const DeviceTensor &positions, const DeviceTensor &slots, uint32_t tokens,
+                                     uint32_t q_heads, uint32_t stride_q_row, uint32_t stride_q_head, uint32_t stride_k_row,
+                                     uint32_t stride_v_row, uint32_t stride_q_out_row, DeviceKvCache &cache);
+    // Attention of each sequence's 1..16 newest rows over its cached tokens.  page_table: n_seqs rows of
+    // stride_page_table ids; q_starts (n_seqs + 1) null: max_q_len rows a sequence.  The lengths, starts and ids are read on
+    // the device, so that a captured call follows them; max_q_len and max_kv_len are their bounds.
+    DeviceStatus paged_attention(DeviceTensor &out, const DeviceTensor &q, const DeviceKvCache &cache,
+                                 const DeviceTensor &page_table, uint32_t stride_page_table, const DeviceTensor &kv_lens,
+                                 const DeviceTensor *q_starts, uint32_t n_seqs, uint32_t q_rows, uint32_t max_q_len,
+                                 uint32_t q_heads, uint32_t max_kv_len, float scale, uint32_t stride_q_row,
+                                 uint32_t stride_out_row);
+    // One token per row of fp32 logits into out[0 .. batch - 1] (q8mi_sample in include/q8mi.h), where
+    // q8_0_get_row_from_argmax reads them.  Parameter tensors: one element a row; temperature, top_k (I32), top_p and min_p
+    // may be null.
+    DeviceStatus sample_rows(const DeviceTensor &logits, uint32_t batch, uint32_t vocab, uint32_t row_stride,
+                             const DeviceTensor *temperature, const DeviceTensor *top_k, const DeviceTensor *top_p,
+                             const DeviceTensor *min_p, const DeviceTensor &uniform, DeviceArgmaxBuffer &out);
 
     // embedding lookup: dequantized rows of a Q8_0 matrix
     // (include/qw3/device_backend.hpp:276-299, src/kernels_cuda.cu:10613-10755).
@@ -315,7 +358,8 @@ private:
     bool norm_shortcuts_ = true;
     std::shared_ptr<Owner> owner_;
     QuantizedRows quantized_;
-    Scratch q8_1_, d4_, argmax_partial_, argmax_result_, lm_head_, lm_rows_, out_f32_, row_ids_;
+    Scratch q8_1_, d4_, argmax_partial_, argmax_result_, lm_head_, lm_rows_, out_f32_, row_ids_, attention_, sample_;
+    std::vector<void *> retired_;   // outgrown scratch that the captured graph still names
     int32_t *argmax_dev_ = nullptr;    // {token, logit bits}
     int32_t *argmax_host_ = nullptr;   // pinned mirror
     uint8_t *lm_host_ = nullptr;       // pinned mirror of lm_head_verify's row pairs and {accepted, next}
