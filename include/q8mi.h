@@ -327,16 +327,19 @@ int q8mi_qk_norm_rope_append(const void *q, const void *k, const void *v, void *
  * n sees the tokens up to kv_lens[s] - n + i:
  *   out = sum_t p_t v_t,  p = softmax_t(scale * q . k_t)
  * for every query head h with the keys and values of head h / (q_heads / kv_heads).  What a row does not see
- * has no influence on it, whatever it holds; a row that sees nothing is zero; rows of q outside every
- * sequence leave out as it was.
+ * has no influence on it, whatever it holds (an infinity or NaN that it sees does, also where its weight is 0);
+ * a row that sees nothing is zero; rows of q outside every sequence leave out as it was.
  * q and out: rows stride_q_row / stride_out_row elements apart, heads dense; fp32, or bf16 per *_is_bf16.
  * kv_lens, q_starts and page_table are device memory and may change between replays of a captured call;
  * the host gives their bounds: n_seqs, q_rows (rows of q and out), max_q_len (1..16) and max_kv_len (at most
  * stride_page_table * page_size).  Tokens from max_kv_len on are not read, rows of a sequence from
- * max_q_len on and rows from q_rows on not computed, and a page id outside the pool hides its tokens.
+ * max_q_len on and rows from q_rows on not computed, and a page id outside the pool hides its tokens.  A row
+ * of q must not belong to two sequences, and out must not overlap q.  The first call of a head_dim, cache type
+ * and number of rows asks the runtime for its LDS: make it outside a graph capture.
  * scratch: q8mi_paged_attention_scratch_bytes() device bytes, 16-byte aligned; calls that may overlap need
- * one each.  Nothing in it needs clearing.  Q8MI_REJECTED: q_heads not a multiple of kv_heads, the bounds
- * above, q or out or their strides in bytes not multiples of 16, a scale that is not finite. */
+ * one each.  Nothing in it needs clearing.  Results repeat bit by bit.  Q8MI_REJECTED: q_heads not a multiple of
+ * kv_heads or above 65535, the bounds above, q, out or their strides in bytes not multiples of 16, a scale that
+ * is not finite, a pool of 64 GiB and more, 2^22 rows and more. */
 size_t q8mi_paged_attention_scratch_bytes(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads,
                                           uint32_t head_dim, uint32_t max_kv_len);
 int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_rows, uint32_t stride_q_row,
@@ -351,18 +354,18 @@ int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_rows, uint32_t
  * index first, and p_i = exp((logit_i - max) / temperature):
  *   top_k   keeps the first top_k ranks (<= 0: all);
  *   top_p   keeps of those a rank when the p of the ranks before it sum to less than top_p times the p of all
- *           that top_k kept (>= 1: all; the first rank always stays);
- *   min_p   keeps of those the ranks with p_i >= min_p (<= 0: all, above 1 counts as 1);
+ *           that top_k kept (>= 1 or NaN: all; the first rank always stays);
+ *   min_p   keeps of those the ranks with p_i >= min_p (<= 0 or NaN: all, above 1 counts as 1);
  *   token   the lowest index at which the sum of the kept p, in the order of the indices, exceeds uniform
  *           times their whole sum.
- * A temperature that is not above zero takes rank 0 (the row's argmax).  The five parameter arrays are device
+ * A temperature that is not above zero, or NaN, takes rank 0 (the row's argmax).  The five parameter arrays are device
  * memory, one element a row; temperature (1), top_k, top_p and min_p (off) may be NULL.  Each p is rounded to
  * a multiple of 2^-42 and all sums are integers, so that their order never changes a token; a logit more than
  * about 30 temperatures below the maximum counts as 0 and is never drawn.  NaN and -inf logits are never
  * drawn either; +inf logits share the whole mass.  uniform is clamped to [0, 1), NaN counts as 0.
  *   out[j] = {the token's logit, the token}: what q8mi_get_row_from_argmax reads; {-inf, -1} when every
  *            logit of the row is NaN or -inf.
- * vocab: 1 .. 2^20.  scratch: q8mi_sample_scratch_bytes() device bytes, 16-byte aligned; calls that may overlap
+ * vocab: 1 .. 2^20, batch up to 65535.  scratch: q8mi_sample_scratch_bytes() device bytes, 16-byte aligned; calls that may overlap
  * need one each, nothing in it needs clearing. */
 size_t q8mi_sample_scratch_bytes(uint32_t batch, uint32_t vocab);
 int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, uint32_t stride, const float *temperature,

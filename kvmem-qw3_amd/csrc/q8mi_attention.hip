@@ -59,7 +59,7 @@ struct AttnParams {
 struct Rows {
     int64_t start, count, kv_len;
     uint32_t used;     // rows that are computed, 0 .. max_q_len
-    uint32_t tokens;   // tokens that some row may see, 0 .. max_kv_len
+    uint32_t tokens;   // tokens that some row sees, 0 .. max_kv_len
 };
 __device__ __forceinline__ Rows rows_of(const AttnParams &p, uint32_t seq) {
     Rows r;
@@ -71,7 +71,8 @@ __device__ __forceinline__ Rows rows_of(const AttnParams &p, uint32_t seq) {
     }
     r.kv_len = p.kv_lens[seq];
     r.used = r.count < 0 ? 0u : r.count > p.max_q_len ? p.max_q_len : static_cast<uint32_t>(r.count);
-    r.tokens = r.kv_len < 0 ? 0u : r.kv_len > p.max_kv_len ? p.max_kv_len : static_cast<uint32_t>(r.kv_len);
+    const int64_t seen = r.kv_len - (r.count > r.used ? r.count - r.used : 0);   // by the last computed row
+    r.tokens = seen < 0 ? 0u : seen > p.max_kv_len ? p.max_kv_len : static_cast<uint32_t>(seen);
     return r;
 }
 

@@ -270,7 +270,7 @@ extern "C" int q8mi_qk_norm_rope_append(const void *q, const void *k, const void
     p.slots_end = static_cast<uint64_t>(cache->pages) * cache->page_size;
     p.small = p.slots_end <= 0xffffffffull;
     const uint64_t grid = batch > 1 ? tokens : (static_cast<uint64_t>(tokens) * groups + kAppendWaves - 1) / kAppendWaves;
-    if (grid > 0x3fffffffull) return fail(Q8MI_REJECTED, "%s: too many heads for one launch", what);
+    if (grid > 0xffffffull) return fail(Q8MI_REJECTED, "%s: %u tokens are too many for one launch", what, tokens);
 
     const uintptr_t bases = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
                             reinterpret_cast<uintptr_t>(q_out);

@@ -43,7 +43,7 @@ typedef unsigned long long u64;
 // top_k-th (kBins: top_k cuts nothing); the weight of the steps below `sure`, below k_first, and of all; the count below
 // k_first.
 struct Cut {
-    uint32_t sure, last, k_first, k_last, k_count, unused;
+    uint32_t sure, last, k_first, k_last, k_count;
     u64 sure_mass, k_mass, all_mass;
 };
 
@@ -330,10 +330,11 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
         for (uint32_t b = t; b < kBins; b += kChunkThreads) { mass[b] = 0; count[b] = 0; }
         __syncthreads();
         // The row's steps are added up by atomics, so few are sent.  Where this span alone has top_k above a step, the cut
-        // lies above it, too.  Without top_k: all of a row of `vocab` logits below depth d weigh at most vocab * exp(-d), and
-        // the cut does not lie where this is no more than the 1 - top_p of the whole that may be dropped; the whole is at
-        // least 1.  From there on only the sum counts, in the last step, which no logit reaches.
-        const double far = by_count ? kReach : fmin(kReach, log(static_cast<double>(p.vocab) / (1.0 - r.top_p)) + 0.1);
+        // lies above it, too.  Without top_k: the largest weighs 1, so 1 - top_p may always be dropped, and `vocab` logits below
+        // a depth whose weight is (1 - top_p) / vocab, less the half step that rounding may add to it, cannot hold the cut.
+        // From there on only the sum counts, in the last step, which no logit reaches.
+        const double spare = (1.0 - r.top_p) / p.vocab - 0.5 / kOne;
+        const double far = by_count || !(spare > 0.0) ? kReach : fmin(kReach, 0.1 - log(spare));
         u64 rest = 0;
         span.walk([&](const float (&v)[4], uint32_t, uint32_t) {
 #pragma unroll

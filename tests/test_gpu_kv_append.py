@@ -149,3 +149,38 @@ def test_stream_and_graph(gpu):
         assert np.array_equal(out.download(np.uint32, n), want[:n])
         for name in "kv":
             assert np.array_equal(pools.download()[name], pool[name])
+
+
+@pytest.mark.parametrize("case", [dict(gated=True), dict(pad=8), dict(pad=3), dict(order="thd"), dict(in_place=True), dict(norms=False),
+                                  dict(misalign=1), dict(misalign=2, act="bf16"), dict(page=7, gated=True, pad=4), dict(rot=0),
+                                  dict(rot=128, interleaved=True), dict(kind="e4m3", act="bf16", scale=(1 / 16, 1 / 32))], ids=str)
+@pytest.mark.parametrize("dim,heads,kv_heads", [(128, 21, 3), (64, 40, 5), (256, 6, 1)])
+def test_many_tokens(gpu, dim, heads, kv_heads, case):
+    """A workgroup a token: the strides, forms and paddings once more, head counts that do not fill the waves."""
+    case = {"rot": 32, **case}
+    if case["rot"] > dim:
+        case["rot"] = dim
+    tokens = 1400
+    slots = np.random.default_rng(9).permutation(tokens).astype(np.int64)
+    slots[::13] = -1
+    run(tokens, heads, kv_heads, dim, slots=slots, seed=dim, **case)
+
+
+def test_two_calls_at_once(gpu):
+    """Two streams on caches of their own: nothing is shared."""
+    a, b = hip.Stream(), hip.Stream()
+    first = run(40, 24, 4, 256, 64, seed=30, stream=a.handle)
+    second = run(1500, 8, 2, 128, 128, "f16", "bf16", seed=31, stream=b.handle)
+    want = [(o.download(np.uint8).copy(), p.download()) for _, _, o, p in (first, second)]
+    for _, _, o, p in (first, second):
+        o.fill(0)
+        p.upload()
+    hip.synchronize()
+    ok(q8mi.lib().q8mi_qk_norm_rope_append(*first[0]), "append")
+    ok(q8mi.lib().q8mi_qk_norm_rope_append(*second[0]), "append")
+    a.synchronize()
+    b.synchronize()
+    for (_, _, o, p), (out, pool), n in zip((first, second), want, (40 * 24 * 256 * 4, 1500 * 8 * 128 * 2)):
+        assert np.array_equal(o.download(np.uint8)[:n], out[:n])
+        for name in "kv":
+            assert np.array_equal(p.download()[name], pool[name])

@@ -261,3 +261,133 @@ def test_results_repeat(gpu):
         c.launch()
     hip.synchronize()
     assert np.array_equal(a, c.dout.download(np.uint32))
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads,kind", [(64, 4, 2, "e4m3"), (64, 16, 4, "f16"), (128, 4, 4, "e4m3"), (256, 6, 2, "bf16"),
+                                                     (256, 12, 2, "e4m3")])
+@pytest.mark.parametrize("page", [1, 4, 5, 16, 24, 64])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_page_sizes_of_every_type(gpu, page, dim, heads, kv_heads, kind, rows):
+    """Pages that a transfer of several tokens fits into, and pages it does not."""
+    run([203, 64, 9], [rows, 1, rows], heads, kv_heads, dim, kind, page=page, seed=page + rows)
+
+
+@pytest.mark.parametrize("n", [63, 64, 65, 200])
+def test_many_sequences(gpu, n):
+    """More sequences than a wave has lanes: the search for a workgroup's place goes through them 64 at a time."""
+    rng = np.random.default_rng(n)
+    run(rng.integers(0, 90, n).tolist(), rng.integers(0, 4, n).tolist(), 4, 2, 128, "f16", seed=n, max_q=3)
+    run([0] * (n - 1) + [500], [1] * n, 4, 2, 128, "f16", seed=n)
+
+
+@pytest.mark.parametrize("page,dim,kind,rows", [(1, 64, "f16", 1), (1, 256, "bf16", 2), (7, 128, "e4m3", 16), (2048, 128, "bf16", 3)])
+def test_runs_beyond_one_chunk(gpu, page, dim, kind, rows):
+    """So many sequences (of one text: they share its pages) that one workgroup walks more than 2048 tokens of an item: its page
+    ids are loaded in turns."""
+    c = Case([5000], [rows], 4, 2, dim, kind, page=page, seed=rows, q_scale=1.0, spare_rows=0)
+    n, lens = 600, [5000, 4999, 2049, 4097, 4096, 2048, 3001]
+    kv = np.asarray([lens[s % 7] for s in range(n)], np.int32)
+    dt, dl = hip.to_device(np.tile(c.table, (n, 1))), hip.to_device(kv)
+    dq, out = hip.to_device(np.tile(c.q, (n, 1))), hip.DeviceBuffer(4 * n * rows * c.width).fill(0xff)
+    L = q8mi.lib()
+    scratch = hip.DeviceBuffer(L.q8mi_paged_attention_scratch_bytes(n, rows, 4, 2, dim, 5000)).fill(0xff)
+    ok(L.q8mi_paged_attention(dq.ptr, 0, n * rows, c.width, c.pools.ref, dt.ptr, c.wide, dl.ptr, None, n, rows, 4, 5000, c.scale,
+                              out.ptr, 0, c.width, scratch.ptr, NULL), "paged_attention")
+    hip.synchronize()
+    got = out.download(np.uint32).reshape(n, rows, c.width)
+    for s in range(7):                      # the sequences of one length agree (a different cut: other roundings) with the first
+        c.lens, first = [lens[s]], got[s].view(np.float32)
+        c.dout.upload(first)
+        c.check()
+        rest = got[s::7].view(np.float32)
+        assert np.abs(rest - first).max() < 1e-4 and np.isfinite(rest).all()
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads,rows", [(128, 6, 1, 4), (256, 12, 1, 2), (64, 40, 1, 2), (256, 20, 1, 16)])
+def test_bad_pages_with_rows_side_by_side(gpu, dim, heads, kv_heads, rows):
+    c = Case([300, 70], [rows, rows], heads, kv_heads, dim, "f16", page=16, seed=40 + rows)
+    bad = {(0, 1): -1, (0, 9): c.pools.pages, (1, 0): 2 ** 31 - 1}
+    for (s, p), v in bad.items():
+        c.table[s, p] = v
+    c.dt.upload(c.table)
+    c.launch()
+    hip.synchronize()
+    c.check(hidden=lambda s, t: (s, t // 16) in bad)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "e4m3"])
+@pytest.mark.parametrize("dim,heads,kv_heads,rows", [(128, 2, 2, 8), (128, 6, 2, 8), (256, 6, 1, 16), (64, 40, 1, 5)])
+def test_later_tokens_of_several_rows(gpu, dim, heads, kv_heads, rows, kind):
+    """Every other new token holds NaN in some elements of key and value: each row is not finite exactly where a token it sees makes
+    it so."""
+    n = 90
+    c = Case([n], [rows], heads, kv_heads, dim, kind, page=32, seed=50 + rows)
+    nan = {"bf16": 0x7fc0, "f16": 0x7e00, "e4m3": 0x7f}[kind]
+    for t in range(n - rows + 2, n, 2):        # value elements: those columns of rows from t's own on
+        at = c.pools.at(c.table[0, t // 32], t % 32)
+        c.pools.host["v"][at[:, t % 5::7]] = nan
+        c.v[0][t, :, t % 5::7] = np.nan
+    c.pools.host["k"][c.pools.at(c.table[0, (n - 1) // 32], (n - 1) % 32)[:, 3]] = nan
+    c.k[0][n - 1, :, 3] = np.nan               # the last key: all of the last row
+    c.pools.upload()
+    c.launch()
+    hip.synchronize()
+    got = c.dout.download(np.float32).reshape(c.q_rows, c.so)
+    for r in range(rows):
+        q = R.act_value(c.q[r, :c.width], c.act).reshape(c.heads, c.dim)
+        want, mag, _ = R.attention(q, c.k[0], c.v[0], c.scale, n - rows + r + 1)
+        g = got[r, :c.width].reshape(c.heads, c.dim)
+        assert np.array_equal(np.isfinite(g), np.isfinite(want)), r
+        fine = np.isfinite(want)
+        assert not fine.any() or np.abs(g - want)[fine].max() < 1e-4, r
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_rows_beyond_the_bound_hold_nothing_back(gpu, kind):
+    """A sequence with more rows than max_q_len: the tokens of the rows that are not computed are seen by nobody, whatever they
+    hold."""
+    c = Case([200, 33], [60, 20], 4, 2, 128, kind, max_q=3, seed=60)
+    for s, n in enumerate([200, 33]):
+        for t in range(n - c.rows[s] + 3, n):
+            for name in "kv":
+                c.pools.host[name][c.pools.at(c.table[s, t // 16], t % 16)] = 0x7f if kind == "e4m3" else 0x7fc0
+    c.pools.upload()
+    c.launch()
+    hip.synchronize()
+    c.check()
+
+
+@pytest.mark.parametrize("page", [16, 3])
+def test_a_context_behind_4_gib(gpu, page):
+    """Pages whose bytes lie beyond 32-bit offsets of the pools, through both ways of addressing."""
+    c = Case([70], [1], 4, 2, 128, "f16", page=page, seed=70)
+    pages, stride = 40, (1 << 26) + 512 * page       # elements: 128 MiB a page and a little
+    values = stride // 16 * 8                        # they lie half a page stride behind the keys
+    big = hip.DeviceBuffer(2 * stride * pages)
+    for i in range((70 + page - 1) // page):
+        for name, off in (("k", 0), ("v", values)):
+            src = c.pools.host[name].reshape(c.pools.pages, c.pools.sp)[c.table[0, i]]
+            big.upload(src, 2 * ((pages - 1 - i) * stride + off))
+        c.table[0, i] = pages - 1 - i
+    c.dt.upload(c.table)
+    d = c.pools.desc
+    d.k, d.v, d.pages, d.stride_page = big.ptr, big.at(2 * values), pages, stride
+    c.launch()
+    hip.synchronize()
+    c.check()
+    big.free()
+
+
+def test_two_calls_at_once(gpu):
+    """Two streams, a scratch each."""
+    a, b = hip.Stream(), hip.Stream()
+    c = Case([3000, 1], [1, 1], 12, 2, 256, seed=80)
+    d = Case([700] * 20, [4] * 20, 16, 4, 128, "f16", seed=81)
+    hip.synchronize()
+    for _ in range(4):
+        c.launch(a.handle)
+        d.launch(b.handle)
+    a.synchronize()
+    b.synchronize()
+    c.check()
+    d.check()

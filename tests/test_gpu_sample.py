@@ -171,3 +171,61 @@ def test_token_feeds_the_embedding_lookup(gpu):
         ok(q8mi.lib().q8mi_get_row(dw.ptr, token, vocab, cols, want.ptr, 0, NULL), "row")
         hip.synchronize()
         assert np.array_equal(out.download(np.uint32), want.download(np.uint32))
+
+
+@pytest.mark.parametrize("depth", [29.45, 29.6, 29.9])
+def test_a_tail_of_the_least_weights(gpu, depth):
+    """2^20 logits whose weight rounds to one unit (or none) against 1 - top_p of a few units each: rounding moves the cut into
+    the tail."""
+    z = np.full((3, 1 << 20), -depth)
+    z[:, 12345] = 0.0
+    run(z, top_p=[1 - 3 * 2.0 ** -24, 1 - 2.0 ** -24, 1 - 2.0 ** -20], u=1 - 2.0 ** -24)
+
+
+@pytest.mark.parametrize("spread", [0.0, 1e-3])
+def test_more_candidates_than_a_list_holds(gpu, spread):
+    """All that top_k wants in a few chunks, whose lists overflow; and equal logits all over the row."""
+    rng = np.random.default_rng(21)
+    z = rng.standard_normal((4, 100000))
+    z[:2, 3000:4500] = 30 + spread * rng.standard_normal((2, 1500))
+    z[2:] = spread * rng.standard_normal((2, 100000))
+    run(z, top_k=[60, 90, 97, 5], top_p=[0.9, 1.0, 0.5, 1.0], u=[0.3, 0.9, 0.99, 0.5])
+
+
+def test_the_largest_vocabulary_by_count(gpu):
+    """top_k up to the number of chunks (1024), and just above it."""
+    run(logits(3, 1 << 20, 22), temperature=1.5, top_k=[1000, 1024, 1025], top_p=[0.9, 1.0, 0.99], seed=23)
+
+
+@pytest.mark.parametrize("pad,shift", [(1, 0), (3, 1), (4, 0), (0, 3)])
+def test_rows_on_any_boundary(gpu, pad, shift):
+    """Strides and addresses that keep rows off 16-byte boundaries."""
+    z = logits(5, 5003, 24)
+    c = Case(z, temperature=0.9, top_k=30, top_p=0.9, pad=pad, seed=25)
+    wide = np.full(5 * c.stride + shift, 99.0, np.float32)
+    wide[shift:].reshape(5, c.stride)[:, :5003] = z
+    big = hip.to_device(wide)
+    x, t, k, p, m, u = (d.ptr if d is not None else None for d in c.dev)
+    ok(q8mi.lib().q8mi_sample(big.ptr + 4 * shift, 5, 5003, c.stride, t, k, p, m, u, c.out.ptr, c.scratch.ptr, NULL), "sample")
+    hip.synchronize()
+    c.check()
+
+
+def test_two_calls_at_once(gpu):
+    """Two streams, a scratch each."""
+    a, b = hip.Stream(), hip.Stream()
+    c = Case(logits(16, 60000, 26), temperature=0.9, top_p=0.95, seed=27)
+    d = Case(logits(8, 151936, 28), temperature=1.1, top_k=64, seed=29)
+    hip.synchronize()
+    for _ in range(4):
+        c.launch(a.handle)
+        d.launch(b.handle)
+    a.synchronize()
+    b.synchronize()
+    c.check()
+    d.check()
+
+
+def test_many_rows(gpu):
+    """A row each for many sequences, several chunks to a workgroup."""
+    run(logits(300, 9001, 30), temperature=0.8, top_k=[5, 0, 700] * 100, top_p=[0.9, 0.95, 0.8] * 100, seed=31)

@@ -58,7 +58,8 @@ def test_null_cache():
 
 @pytest.mark.parametrize("bad", [dict(q=0), dict(k=0), dict(v=0), dict(q_out=0), dict(slots=0), dict(freqs=0), dict(positions=0),
                                  dict(rot=60), dict(rot=136), dict(q_heads=0), dict(sqh=120), dict(sqr=508), dict(skr=255),
-                                 dict(svr=100), dict(sor=511), dict(q_out=P, sqh=256, sqr=1024), dict(q_out=P, sqr=1024)], ids=str)
+                                 dict(svr=100), dict(sor=511), dict(q_out=P, sqh=256, sqr=1024), dict(q_out=P, sqr=1024), dict(tokens=1 << 24),
+                                 dict(q_heads=65537, sqr=1 << 31)], ids=str)
 def test_append(bad):
     assert append(**bad) == q8mi.REJECTED
     assert q8mi.last_error()
@@ -67,14 +68,14 @@ def test_append(bad):
 @pytest.mark.parametrize("bad", [dict(q=0), dict(out=0), dict(table=0), dict(lens=0), dict(scratch=0), dict(heads=0), dict(heads=5),
                                  dict(new=0), dict(new=17), dict(max_kv=65), dict(scale=NAN), dict(scale=INF), dict(q=P + 4),
                                  dict(out=P + 8), dict(scratch=P + 4), dict(sq=514), dict(so=510), dict(sq=256), dict(so=508),
-                                 dict(q_is_bf16=1, sq=516)], ids=str)
+                                 dict(q_is_bf16=1, sq=516), dict(n=1 << 22), dict(heads=65538, sq=1 << 24, so=1 << 24)], ids=str)
 def test_attention(bad):
     assert attend(**bad) == q8mi.REJECTED
     assert q8mi.last_error()
 
 
 @pytest.mark.parametrize("bad", [dict(x=0), dict(u=0), dict(out=0), dict(scratch=0), dict(vocab=0), dict(vocab=(1 << 20) + 1),
-                                 dict(stride=99)], ids=str)
+                                 dict(stride=99), dict(scratch=P + 8), dict(batch=65536)], ids=str)
 def test_sample(bad):
     assert sample(**bad) == q8mi.REJECTED
     assert q8mi.last_error()
