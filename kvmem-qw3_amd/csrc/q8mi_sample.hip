@@ -26,7 +26,8 @@ namespace {
 constexpr uint32_t kMaxVocab = 1u << 20;
 constexpr uint32_t kChunk = 1024;                     // logits
 constexpr uint32_t kMaxChunks = kMaxVocab / kChunk;
-constexpr uint32_t kMostSpan = 16;                    // chunks of a workgroup of launches 1 to 3
+constexpr uint32_t kMostSpan = 8;                     // chunks of a workgroup of launches 2 and 3
+constexpr uint32_t kMostSpanOfBest = 2;               // and of launch 1, which has nothing to hold for a row
 constexpr uint32_t kAhead = 4;                        // chunks that a workgroup of launches 1 to 3 loads at a time
 constexpr uint32_t kChunkThreads = kChunk / 4;
 constexpr uint32_t kRowThreads = 256;                 // launch 4
@@ -36,8 +37,11 @@ constexpr double kReach = 31.875;                     // exp(-31.875) * 2^42 rou
 constexpr uint32_t kMaxCandidates = 4096;             // of a row
 constexpr uint32_t kChunkCandidates = 64;             // of a chunk
 constexpr double kOne = 4398046511104.0;              // 2^42: the weight of the largest logit; 2^20 of them sum below 2^63
+constexpr double kBottom = 64.0;                      // the depth of everything that is deeper, or never drawn
+constexpr uint32_t kRoots = 32;                       // 2^(i / 32): 256 bytes, so that no two of them share a bank of LDS
 
 typedef unsigned long long u64;
+typedef float v4f __attribute__((ext_vector_type(4)));
 
 // Where the cuts fall: steps below `sure` are kept, steps sure .. last hold the last rank, steps k_first .. k_last the
 // top_k-th (kBins: top_k cuts nothing); the weight of the steps below `sure`, below k_first, and of all; the count below
@@ -62,7 +66,7 @@ struct SampleParams {
     uint32_t *bin_count;     // [row][kBins]
     uint32_t *n_candidates;  // [row][chunk]: may be beyond kChunkCandidates
     uint32_t vocab, stride, chunks;
-    uint32_t span, spans;    // chunks of a workgroup of launches 1 to 3, such workgroups a row
+    uint32_t span;           // chunks of a workgroup (launches 1 to 3)
     int vec;
 };
 
@@ -80,8 +84,8 @@ __device__ __forceinline__ u64 rank_of(uint32_t key, uint32_t index) {   // larg
 }
 
 struct Row {
-    float max;
-    double per_unit;   // 1 / temperature
+    double max;
+    double per_unit;   // 1 / temperature, above zero
     double deepest;    // what min_p keeps lies no deeper: p >= min_p <=> depth <= -log(min_p)
     uint32_t top_k;    // 0: off
     double top_p;      // 1: off
@@ -92,54 +96,68 @@ __device__ __forceinline__ Row row_of(const SampleParams &p, uint32_t row, uint3
     r.max = logit_of(top_key);
     const float t = p.temperature ? p.temperature[row] : 1.0f;
     r.greedy = !(t > 0.0f);
-    r.per_unit = r.greedy ? 1.0 : 1.0 / static_cast<double>(t);
+    // an infinite temperature: depths below 1e-250, which no other one gives, where p is 1 and -inf still lies at the bottom
+    r.per_unit = r.greedy ? 1.0 : fmax(1.0 / static_cast<double>(t), 1e-300);
     const float min_p = p.min_p ? p.min_p[row] : 0.0f;
-    r.deepest = min_p > 0.0f ? (min_p < 1.0f ? -log(static_cast<double>(min_p)) : 0.0) : INFINITY;
+    r.deepest = min_p > 0.0f ? (min_p < 1.0f ? -log(static_cast<double>(min_p)) : 1e-250) : INFINITY;
     const int32_t k = p.top_k ? p.top_k[row] : 0;
     r.top_k = k > 0 && static_cast<uint32_t>(k) < p.vocab ? k : 0;
     const float top_p = p.top_p ? p.top_p[row] : 1.0f;
     r.top_p = top_p < 1.0f ? top_p : 1.0;
     return r;
 }
-// How far below the maximum, in temperatures; not below kReach (or NaN): weighs nothing.
-__device__ __forceinline__ double depth_of(uint32_t key, const Row &r) {
-    if (key == 0) return INFINITY;
-    const float v = logit_of(key);
-    return v == r.max ? 0.0 : (static_cast<double>(r.max) - static_cast<double>(v)) * r.per_unit;
+// How far below the maximum, in temperatures, 0 .. kBottom.  NaN and -inf lie at the bottom; below +inf, it itself is the only
+// number that does not (inf - inf is no number, whose larger with 0 is 0).
+__device__ __forceinline__ double depth_at(float v, const Row &r) {
+    return fmin(fmax((r.max - static_cast<double>(fmaxf(v, -INFINITY))) * r.per_unit, 0.0), kBottom);
 }
-// exp(-depth) * 2^42 rounded to an integer: 2^(42 - depth * log2(e)) = 2^n * 2^f, 0 <= f < 1, with 2^f from its series in
-// f * ln(2) - ln(2) / 2 around the middle (terms up to the 12th power: below 1e-16), whose bits are the integer but for a
-// shift.  Off by 1e-14 of itself and the last rounding; depth 0 gives 2^42.
-__device__ __forceinline__ u64 weight_at(double depth) {
-    if (!(depth < kReach)) return 0;
-    if (depth == 0.0) return static_cast<u64>(kOne);
-    const double y = fma(depth, -1.44269504088896340736, 42.0), n = floor(y);
-    const double z = fma(y - n, 0.693147180559945309417, -0.346573590279972654709);
-    double e = 1.0 / 479001600.0;
-    e = fma(e, z, 1.0 / 39916800.0);
-    e = fma(e, z, 1.0 / 3628800.0);
-    e = fma(e, z, 1.0 / 362880.0);
-    e = fma(e, z, 1.0 / 40320.0);
-    e = fma(e, z, 1.0 / 5040.0);
-    e = fma(e, z, 1.0 / 720.0);
-    e = fma(e, z, 1.0 / 120.0);
-    e = fma(e, z, 1.0 / 24.0);
-    e = fma(e, z, 1.0 / 6.0);
-    e = fma(e, z, 0.5);
-    e = fma(e, z, 1.0);
-    e = fma(e, z, 1.0) * 1.41421356237309504880;   // 2^f; rounding may take it to 2, whose bits still follow on
-    const u64 bits = __builtin_bit_cast(u64, e) - (1022ull << 52);           // (exponent + 1) << 52 | fraction: as an integer 2^52 * 2^f
-    const int shift = 52 - static_cast<int>(n);                                                  // 10 .. 56
-    return (bits + (1ull << (shift - 1))) >> shift;
+__device__ __forceinline__ double depth_of(uint32_t key, const Row &r) { return depth_at(key ? logit_of(key) : -INFINITY, r); }
+
+// The table of weight_at, worked out anew from the series of the exponential (0 gives 1 exactly): 16 dependent steps, where
+// fetching it from memory cost each launch 2 us.  A barrier follows before the first weight.
+__device__ __forceinline__ void make_roots(double *roots) {
+    if (threadIdx.x >= kRoots) return;
+    const double x = threadIdx.x * (0.693147180559945309417 / kRoots);
+    double e = 1.0;
+#pragma unroll
+    for (int k = 16; k > 0; --k) e = fma(x * (1.0 / k), e, 1.0);
+    roots[threadIdx.x] = e;
 }
-__device__ __forceinline__ u64 kept_weight_at(double depth, const Row &r) { return depth <= r.deepest ? weight_at(depth) : 0; }
+
+// exp(-depth) * 2^42 rounded to an integer: 2^(y / 32), y = 32 * (42 - depth * log2(e)) = 32 n + i + f with -1/2 <= f <= 1/2,
+// is 2^n from the exponent, 2^(i / 32) from the table and 2^(f / 32) from its series (terms up to the 5th power: 2e-15).
+// Adding 1.5 * 2^52 leaves 32 n + i in the sum's low bits, adding 2^52 the rounded integer.  Off by 1e-14 of itself and the
+// last rounding; depth 0 gives 2^42.  About 25 instructions, a third of the series alone (9.7 M weights: 41 -> XX us).
+__device__ __forceinline__ u64 weight_at(double depth, const double *roots) {
+    constexpr double kHead = 6755399441055744.0, kLn = 0.693147180559945309417 / kRoots;
+    const double y = fma(depth, -1.44269504088896340736 * kRoots, 42.0 * kRoots), head = y + kHead, f = y - (head - kHead);
+    const int k = static_cast<int>(__builtin_bit_cast(u64, head));
+    double e = kLn * kLn * kLn * kLn * kLn / 120.0;
+    e = fma(e, f, kLn * kLn * kLn * kLn / 24.0);
+    e = fma(e, f, kLn * kLn * kLn / 6.0);
+    e = fma(e, f, kLn * kLn / 2.0);
+    e = fma(e, f, kLn);
+    e = fma(e, f, 1.0) * roots[k & (kRoots - 1)];
+    const u64 scaled = __builtin_bit_cast(u64, e) + (static_cast<u64>(static_cast<uint32_t>(k >> 5) << 20) << 32);
+    return __builtin_bit_cast(u64, __builtin_bit_cast(double, scaled) + 4503599627370496.0) - 0x4330000000000000ull;
+}
+__device__ __forceinline__ u64 kept_weight_at(double depth, const Row &r, const double *roots) {
+    return depth <= r.deepest ? weight_at(depth, roots) : 0;
+}
 __device__ __forceinline__ uint32_t bin_at(double depth) { return static_cast<uint32_t>(depth * kBinsPerUnit); }
 
-__device__ __forceinline__ u64 xor_u64(u64 v, int d) { return __shfl_xor(v, d); }
 __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
+    auto add = [](u64 a, int lo, int hi) { return a + (static_cast<u64>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo)); };
+    auto low = [](u64 a) { return static_cast<int>(a); };
+    auto high = [](u64 a) { return static_cast<int>(a >> 32); };
+    v = add(v, dpp_i32<kDppXor1>(low(v)), dpp_i32<kDppXor1>(high(v)));
+    v = add(v, dpp_i32<kDppXor2>(low(v)), dpp_i32<kDppXor2>(high(v)));
+    v = add(v, dpp_i32<kDppRowHalfMirror>(low(v)), dpp_i32<kDppRowHalfMirror>(high(v)));
+    v = add(v, dpp_i32<kDppRowMirror>(low(v)), dpp_i32<kDppRowMirror>(high(v)));
+    u64 all = 0;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += xor_u64(v, d);
-    return v;
+    for (int row = 0; row < 64; row += 16) all = add(all, __builtin_amdgcn_readlane(low(v), row), __builtin_amdgcn_readlane(high(v), row));
+    return all;
 }
 // Sum of v over the threads below this one, and of all (`part`: one u64 a wave of LDS).
 template <uint32_t THREADS>
@@ -165,15 +183,22 @@ __device__ __forceinline__ u64 sum_below(u64 v, u64 *part, u64 &all) {
 }
 
 // Four logits from element i (a multiple of 4) of a row; those past its end are -inf.
-__device__ __forceinline__ void load4(const SampleParams &p, const float *x, uint32_t i, float (&v)[4]) {
-    if (p.vec && i + 4 <= p.vocab) {
-        const float4 t = *reinterpret_cast<const float4 *>(x + i);
-        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-        return;
-    }
-#pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) v[k] = i + k < p.vocab ? x[i + k] : -INFINITY;
+__device__ __forceinline__ v4f load4(const SampleParams &p, const float *x, uint32_t i) {
+    if (p.vec && i + 4 <= p.vocab) return *reinterpret_cast<const v4f *>(x + i);
+    auto one = [&](uint32_t k) {
+        const float v = x[k < p.vocab ? k : p.vocab - 1];
+        return k < p.vocab ? v : -INFINITY;
+    };
+    return v4f{one(i), one(i + 1), one(i + 2), one(i + 3)};
 }
+// Register u of four by selection: what works on them is written once in a loop and not four times in a row.  Code is
+// fetched, too: the four launches fit the 64 KiB instruction cache together, so that a call finds what the last one left
+// (108 KB unrolled: XX us more a call).
+__device__ __forceinline__ v4f pick(const v4f (&v)[4], uint32_t u) {
+    const v4f a = v[0], b = v[1], c = v[2], d = v[3];   // selected as values, so that they stay in registers
+    return u == 0 ? a : u == 1 ? b : u == 2 ? c : d;
+}
+__device__ __forceinline__ void unpack(v4f t, float (&v)[4]) { v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w; }
 
 // A workgroup's span of chunks, kAhead chunks in registers: asked for when the object is made, and the next ones before
 // those in hand are looked at.
@@ -181,34 +206,46 @@ struct Span {
     const SampleParams &p;
     const float *x;
     uint32_t first, end;
-    float v[kAhead][4];
+    v4f v[kAhead];
 
     __device__ __forceinline__ Span(const SampleParams &params, const float *row) : p(params), x(row) {
         first = blockIdx.x * p.span;
         end = first + p.span < p.chunks ? first + p.span : p.chunks;
-        load(first, v);
-    }
-    __device__ __forceinline__ void load(uint32_t c, float (&to)[kAhead][4]) const {
 #pragma unroll
-        for (uint32_t u = 0; u < kAhead; ++u)
-            if (c + u < end) load4(p, x, (c + u) * kChunk + threadIdx.x * 4, to[u]);
-    }
-    // f(v, i, c) for every four logits v, from element i, that this thread has of the span's chunk c (counted from 0)
-    template <typename F>
-    __device__ __forceinline__ void walk(F f) {
-        for (uint32_t c = first; c < end; c += kAhead) {
-            float next[kAhead][4];
-            load(c + kAhead, next);
-#pragma unroll
-            for (uint32_t u = 0; u < kAhead; ++u)
-                if (c + u < end) f(v[u], (c + u) * kChunk + threadIdx.x * 4, c + u - first);   // uniform
-#pragma unroll
-            for (uint32_t u = 0; u < kAhead; ++u)
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) v[u][k] = next[u][k];
+        for (uint32_t u = 0; u < kAhead; ++u) {
+            v[u] = v4f{0, 0, 0, 0};
+            if (first + u < end) v[u] = load4(p, x, (first + u) * kChunk + threadIdx.x * 4);
         }
     }
+    // f(v, i, c) for every four logits v, from element i, that this thread has of the span's chunk c (counted from 0), of
+    // the chunks that want(c): only the first kAhead of the others are read
+    template <typename F, typename W>
+    __device__ __forceinline__ void walk(F f, W want) {
+#pragma unroll 1
+        for (uint32_t c = first; c < end; c += kAhead) {
+            v4f next[kAhead] = {};
+            if (c + kAhead < end) {
+#pragma unroll
+                for (uint32_t u = 0; u < kAhead; ++u) {
+                    const uint32_t n = c + kAhead + u;
+                    if (n < end && want(n - first)) next[u] = load4(p, x, n * kChunk + threadIdx.x * 4);   // uniform
+                }
+            }
+#pragma unroll 1
+            for (uint32_t u = 0; u < kAhead && c + u < end; ++u) {
+                if (!want(c + u - first)) continue;   // uniform
+                float four[4];
+                unpack(pick(v, u), four);
+                f(four, (c + u) * kChunk + threadIdx.x * 4, c + u - first);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u) v[u] = next[u];
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void walk(F f) { walk(f, [](uint32_t) { return true; }); }
 };
+static_assert(kAhead == 4, "pick() takes one of four");
 
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     auto larger = [](uint32_t a, int b) { return a > static_cast<uint32_t>(b) ? a : static_cast<uint32_t>(b); };
@@ -222,7 +259,7 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 
 // ---- 1 ----------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kChunkThreads) void sample_best_kernel(const SampleParams p) {
-    __shared__ uint32_t best[kMostSpan][kChunkThreads / kWave];
+    __shared__ uint32_t best[kMostSpanOfBest][kChunkThreads / kWave];
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
     if (blockIdx.x == 0) {
@@ -251,8 +288,19 @@ __global__ __launch_bounds__(kChunkThreads) void sample_best_kernel(const Sample
 // Sums and candidates of a span's chunks on their way out of a workgroup.
 struct ChunkSpace {   // LDS
     u64 mass[kMostSpan][kChunkThreads / kWave];
-    uint32_t n[kMostSpan];
+    double roots[kRoots];
+    uint32_t n[kMostSpan], best[kMostSpan];
 };
+// Clears it, makes the table and fetches the chunks' maxima; a barrier follows.
+__device__ __forceinline__ void open_space(ChunkSpace &s, const Span &span, const uint32_t *best) {
+    const uint32_t t = threadIdx.x;
+    make_roots(s.roots);
+    if (t >= kMostSpan) return;
+    s.n[t] = 0;
+    s.best[t] = span.first + t < span.end ? best[span.first + t] : 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kChunkThreads / kWave; ++w) s.mass[t][w] = 0;
+}
 // The elements (bits of `mine`) of the four logits v from element i on go to their chunk's list, c-th of the span.
 __device__ __forceinline__ void collect(const SampleParams &p, uint32_t row, ChunkSpace &s, const float (&v)[4], uint32_t i, uint32_t c,
                                         uint32_t mine) {
@@ -294,9 +342,9 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
     __shared__ ChunkSpace out;
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
-    if (t < kMostSpan) out.n[t] = 0;
-    // the row's largest key
     const uint32_t *best = p.best + static_cast<uint64_t>(row) * p.chunks;
+    open_space(out, span, best);
+    // the row's largest key
     uint32_t top = 0;
     for (uint32_t c = t % kWave; c < p.chunks; c += kWave) top = best[c] > top ? best[c] : top;
     top = wave_max_u32(top);
@@ -306,7 +354,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
     if (r.top_k != 0 && r.top_k <= p.chunks) {
         const uint32_t least = p.chunks <= 4 * kWave ? reached_by<4>(best, p.chunks, r.top_k)
                                                      : reached_by<kMaxChunks / kWave>(best, p.chunks, r.top_k);
-        __syncthreads();   // the lists' counts are cleared
+        __syncthreads();
         if (least != 0) {
             if (blockIdx.x == 0 && t == 0) {
                 Cut cut{};
@@ -319,7 +367,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k) mine |= key_of(v[k]) >= least ? 1u << k : 0;
                 collect(p, row, out, v, i, c, mine);
-            });
+            }, [&](uint32_t c) { return out.best[c] >= least; });
             __syncthreads();
             if (span.first + t < span.end) p.n_candidates[static_cast<uint64_t>(row) * p.chunks + span.first + t] = out.n[t];
             return;
@@ -339,12 +387,12 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
         span.walk([&](const float (&v)[4], uint32_t, uint32_t) {
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
-                const double depth = depth_of(key_of(v[k]), r);
+                const double depth = depth_at(v[k], r);
                 if (!(depth < kReach)) continue;
                 const uint32_t b = bin_at(depth);
                 if (by_count) atomicAdd(&count[b], 1u);
                 if (!by_mass) continue;
-                const u64 w = weight_at(depth);
+                const u64 w = weight_at(depth, out.roots);
                 if (depth < far) atomicAdd(&mass[b], w);
                 else rest += w;
             }
@@ -366,10 +414,11 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
         }
         return;
     }
+    __syncthreads();
     span.walk([&](const float (&v)[4], uint32_t, uint32_t c) {
         u64 sum = 0;
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) sum += kept_weight_at(depth_of(key_of(v[k]), r), r);
+        for (uint32_t k = 0; k < 4; ++k) sum += kept_weight_at(depth_at(v[k], r), r, out.roots);
         sum = wave_sum_u64(sum);
         if (t % kWave == 0) out.mass[c][t / kWave] = sum;
     });
@@ -451,7 +500,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
     __shared__ ChunkSpace out;
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
-    if (t < kMostSpan) out.n[t] = 0;   // find_cut's barriers follow
+    open_space(out, span, p.best + static_cast<uint64_t>(row) * p.chunks);   // find_cut's barriers follow
     const uint32_t top = p.top[row];
     const Row r = row_of(p, row, top);
     if (top == 0 || r.greedy || !(r.top_k != 0 || r.top_p < 1.0)) return;
@@ -461,23 +510,23 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
     // logits well below the last step of interest need no 64-bit depth
     const uint32_t deep = cut.k_first < kBins ? cut.k_first : cut.last;
     const double reach = (deep + 1) / kBinsPerUnit / r.per_unit;
-    const float least = isfinite(r.max) && reach < 1e30 ? static_cast<float>(r.max - reach) - (fabsf(r.max) + static_cast<float>(reach)) * 1e-6f : -INFINITY;
+    const float least = r.max < INFINITY && reach < 1e30 ? static_cast<float>(r.max - reach - (fabs(r.max) + reach) * 1e-6) : -INFINITY;
     span.walk([&](const float (&v)[4], uint32_t i, uint32_t c) {
         u64 sum = 0;
         uint32_t mine = 0;   // elements to collect
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
             if (!(v[k] >= least)) continue;
-            const double depth = depth_of(key_of(v[k]), r);
+            const double depth = depth_at(v[k], r);
             if (!(depth < kReach)) continue;
             const uint32_t b = bin_at(depth);
-            if (b < cut.sure) sum += kept_weight_at(depth, r);
+            if (b < cut.sure) sum += kept_weight_at(depth, r, out.roots);
             else if (b <= cut.last || b == cut.k_first) mine |= 1u << k;
         }
         collect(p, row, out, v, i, c, mine);
         if (__builtin_amdgcn_ballot_w64(sum != 0) != 0) sum = wave_sum_u64(sum);   // uniform
         if (t % kWave == 0) out.mass[c][t / kWave] = sum;
-    });
+    }, [&](uint32_t c) { return out.best[c] != 0 && logit_of(out.best[c]) >= least; });
     __syncthreads();
     if (span.first + t < span.end) {
         const uint64_t at = static_cast<uint64_t>(row) * p.chunks + span.first + t;
@@ -495,68 +544,31 @@ struct DrawSpace {   // LDS
     uint32_t count[256];
     u64 target;
     uint32_t at, bounds[2];
+    double roots[kRoots];
 };
-
-// The last rank that stays among those from `after` up in the steps lo .. hi, when fewer than `limit` (count or weight) of
-// them may come before it: eight bits of the 64-bit ranks a pass, counts and weights of the 256 values in LDS.
-// walk(f) calls f(rank) for every element in question, whose bits from `width` on are alike.
-template <typename W>
-__device__ u64 find_by_digits(W walk, const Row &r, bool by_mass, uint32_t lo, uint32_t hi, u64 after, u64 limit, uint32_t width,
-                              u64 prefix, DrawSpace &s) {
-    const uint32_t t = threadIdx.x;
-    u64 before = 0;
-    for (uint32_t shift = width; shift != 0;) {   // prefix: the bits from `shift` on
-        const uint32_t bits = shift < 8 ? shift : 8, next = shift - bits;
-        s.mass[t] = 0;
-        s.count[t] = 0;
-        if (t == 0) { s.at = 0; s.result[0] = ~0ull; }
-        __syncthreads();
-        walk([&](u64 rank) {
-            if (rank < after || (shift < 64 && rank >> shift != prefix)) return;
-            const double depth = depth_of(static_cast<uint32_t>(rank >> 32), r);
-            const uint32_t b = depth < kReach ? bin_at(depth) : kBins - 1;
-            if (b < lo || b > hi) return;
-            const uint32_t digit = static_cast<uint32_t>(rank >> next) & ((1u << bits) - 1);
-            atomicAdd(&s.count[digit], 1u);
-            if (by_mass) atomicAdd(&s.mass[digit], weight_at(depth));
-        });
-        __syncthreads();
-        const uint32_t mine = 255 - t;   // larger digits come first
-        const uint32_t n = s.count[mine];
-        const u64 v = by_mass ? s.mass[mine] : n;
-        u64 all;
-        const u64 upto = before + sum_below<kRowThreads>(v, s.part, all);
-        if (n != 0) atomicMax(&s.at, t);   // where the limit is beyond all: the last value that occurs
-        if (upto < limit && upto + v >= limit) { s.result[0] = mine; s.result[1] = upto; }
-        __syncthreads();
-        if (s.result[0] == ~0ull && t == s.at) { s.result[0] = mine; s.result[1] = upto; }
-        __syncthreads();
-        const bool alone = s.count[s.result[0]] == 1;
-        prefix = (shift < 64 ? prefix << bits : 0) | s.result[0];
-        before = s.result[1];
-        shift = next;
-        __syncthreads();
-        if (alone && shift != 0) {   // its other bits at once
-            walk([&](u64 rank) {
-                if (rank < after || rank >> shift != prefix) return;
-                const double depth = depth_of(static_cast<uint32_t>(rank >> 32), r);
-                const uint32_t b = depth < kReach ? bin_at(depth) : kBins - 1;
-                if (b >= lo && b <= hi) s.result[0] = rank;
-            });
-            __syncthreads();
-            prefix = s.result[0];
-            __syncthreads();
-            break;
-        }
-    }
-    return prefix;
-}
 
 __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SampleParams p) {
     __shared__ DrawSpace s;
     const uint32_t t = threadIdx.x, row = blockIdx.x;
     const float *x = p.logits + static_cast<uint64_t>(row) * p.stride;
+    // Everything the earlier launches left, asked for at once: the counts and the first two candidates of this thread's four
+    // chunks (most have no more), and the chunks' sums.  What a row's settings did not write is not looked at.
     const uint32_t top = p.top[row];
+    const bool may_cut = p.top_k != nullptr || p.top_p != nullptr;
+    uint32_t of[4] = {};
+    u64 two[4][2] = {}, left[4] = {};
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+        const uint64_t c = static_cast<uint64_t>(row) * p.chunks + 4 * t + k;
+        if (4 * t + k >= p.chunks) continue;
+        left[k] = p.chunk_mass[c];
+        if (!may_cut) continue;   // uniform
+        of[k] = p.n_candidates[c];
+        two[k][0] = p.candidates[c * kChunkCandidates];
+        two[k][1] = p.candidates[c * kChunkCandidates + 1];
+    }
+    const Cut cut = p.cut[row];
+    float u = p.uniform[row];
     if (top == 0) {
         if (t == 0) p.out[row] = q8mi_argmax_pair{-INFINITY, -1};
         return;
@@ -571,7 +583,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
         __syncthreads();
         const uint32_t i = s.at * kChunk + 4 * t;
         float v[4];
-        load4(p, x, i, v);
+        unpack(load4(p, x, i), v);
         uint32_t k = 0;
         while (k < 4 && key_of(v[k]) != top) ++k;
         if (k < 4) atomicMin(&s.bounds[0], i + k);
@@ -579,18 +591,17 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
         if (k < 4 && s.bounds[0] == i + k) p.out[row] = q8mi_argmax_pair{x[i + k], static_cast<int32_t>(i + k)};
         return;
     }
+    make_roots(s.roots);   // sum_below's barriers follow
     const bool cuts = r.top_k != 0 || r.top_p < 1.0;
     const bool listed = cuts && p.listed[row] != 0;
     // the candidates of the chunks, one list after the other; `whole`: more than their places hold
     uint32_t n = 0;
     bool whole = false;
     if (cuts) {
-        uint32_t of[4];
         u64 sum = 0, all;
         bool full = false;
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
-            of[k] = 4 * t + k < p.chunks ? p.n_candidates[static_cast<uint64_t>(row) * p.chunks + 4 * t + k] : 0;
             full |= of[k] > kChunkCandidates;
             sum += of[k];
         }
@@ -601,40 +612,22 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
                 const u64 *list = p.candidates + (static_cast<uint64_t>(row) * p.chunks + 4 * t + k) * kChunkCandidates;
-                for (uint32_t i = 0; i < of[k]; ++i) s.cand[at++] = list[i];
+                for (uint32_t i = 0; i < of[k]; ++i) s.cand[at++] = i == 0 ? two[k][0] : i == 1 ? two[k][1] : list[i];
             }
         }
         __syncthreads();
     }
     const bool summed = !listed && !whole;   // the earlier launches have left the chunks' sums
 #pragma unroll
-    for (uint32_t c = t; c < kMaxChunks; c += kRowThreads)
-        s.chunk_mass[c] = summed && c < p.chunks ? p.chunk_mass[static_cast<uint64_t>(row) * p.chunks + c] : 0;
+    for (uint32_t k = 0; k < 4; ++k) s.chunk_mass[4 * t + k] = summed ? left[k] : 0;
     u64 last = 0;   // rank of the last kept element: everything from it up is kept
     if (cuts && (whole || n > kRowThreads)) {
-        // many candidates, or more than the lists hold: then all logits of the row are
-        const Cut cut = p.cut[row];
-        auto walk = [&](auto f) {
-            if (!whole) {
-                for (uint32_t c = t; c < n; c += kRowThreads) f(s.cand[c]);
-                return;
-            }
-            for (uint32_t i0 = 4 * t; i0 < p.vocab; i0 += 16 * kRowThreads) {
-                float v[4][4];
-#pragma unroll
-                for (uint32_t u = 0; u < 4; ++u)
-                    if (i0 + u * 4 * kRowThreads < p.vocab) load4(p, x, i0 + u * 4 * kRowThreads, v[u]);
-#pragma unroll
-                for (uint32_t u = 0; u < 4; ++u)
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) {
-                        const uint32_t i = i0 + u * 4 * kRowThreads + k;
-                        if (i < p.vocab && key_of(v[u][k]) != 0) f(rank_of(key_of(v[u][k]), i));
-                    }
-            }
-        };
+        // Many candidates, or more than the lists hold: then all logits of the row are.  The last rank that a cut keeps, of
+        // the steps lo .. hi and from `after` up, is the one before which fewer than `limit` (by count or weight) come: eight
+        // bits of the 64-bit ranks a walk, with counts and weights of the 256 values in LDS.  One loop around one walk, since
+        // the code of a walk is long.
         uint32_t width = 64;   // bits in which the ranks differ
-        u64 prefix = 0;
+        u64 prefix = 0;        // the others
         if (!whole) {
             if (t == 0) { s.result[0] = 0; s.result[1] = ~0ull; }
             __syncthreads();
@@ -651,31 +644,108 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
             prefix = width < 64 ? s.result[0] >> width : 0;
             __syncthreads();
         }
-        if (cut.k_first < kBins)
-            last = find_by_digits(walk, r, false, cut.k_first, cut.k_last, 0, r.top_k - cut.k_count, width, prefix, s);
-        if (r.top_p < 1.0) {
-            u64 kept = cut.all_mass;   // the weight that top_k keeps
-            if (cut.k_first < kBins) {
-                u64 sum = 0;
-                walk([&](u64 rank) {
-                    const double depth = depth_of(static_cast<uint32_t>(rank >> 32), r);
-                    if (rank >= last && depth < kReach && bin_at(depth) >= cut.k_first) sum += weight_at(depth);
-                });
-                (void)sum_below<kRowThreads>(sum, s.part, kept);
-                kept += cut.k_mass;
-            }
+        enum { kByCount, kSum, kByMass, kKeep };
+        uint32_t stage = cut.k_first < kBins ? kByCount : r.top_p < 1.0 ? kByMass : kKeep;
+        bool alone = false;        // one rank has the digits found so far: the rest of it at once
+        uint32_t shift = width;    // found: the bits from `shift` on
+        u64 found = prefix, before = 0, after = 0, sum = 0;
+        u64 limit = r.top_k - cut.k_count;
+        auto mass_limit = [&](u64 kept) {   // of a cut by weight, when top_k keeps `kept`
             const double limit_f = ceil(r.top_p * static_cast<double>(kept));
-            const u64 limit = limit_f > 1.0 ? static_cast<u64>(limit_f) : 1ull;   // rank 0 always stays
-            last = find_by_digits(walk, r, true, cut.sure, cut.last, last, limit - cut.sure_mass, width, prefix, s);
+            return (limit_f > 1.0 ? static_cast<u64>(limit_f) : 1ull) - cut.sure_mass;   // rank 0 always stays
+        };
+        if (stage == kByMass) limit = mass_limit(cut.all_mass);
+        for (;;) {   // everything that steers it is uniform
+            const bool digits = stage == kByCount || stage == kByMass;
+            const uint32_t lo = stage == kByCount ? cut.k_first : cut.sure, hi = stage == kByCount ? cut.k_last : cut.last;
+            const uint32_t bits = shift < 8 ? shift : 8, next = shift - bits;
+            if (digits && !alone) {
+                s.mass[t] = 0;
+                s.count[t] = 0;
+                if (t == 0) { s.at = 0; s.result[0] = ~0ull; }
+                __syncthreads();
+            }
+            auto visit = [&](u64 rank) {
+                const double depth = depth_of(static_cast<uint32_t>(rank >> 32), r);
+                const uint32_t b = depth < kReach ? bin_at(depth) : kBins - 1;
+                if (digits) {
+                    if (rank < after || (shift < 64 && rank >> shift != found) || b < lo || b > hi) return;
+                    if (alone) {
+                        s.result[0] = rank;
+                        return;
+                    }
+                    const uint32_t digit = static_cast<uint32_t>(rank >> next) & ((1u << bits) - 1);
+                    atomicAdd(&s.count[digit], 1u);
+                    if (stage == kByMass) atomicAdd(&s.mass[digit], weight_at(depth, s.roots));
+                } else if (rank >= last) {
+                    const u64 w = weight_at(depth, s.roots);
+                    if (stage == kSum) sum += b >= cut.k_first ? w : 0;
+                    else if (w != 0 && depth <= r.deepest) atomicAdd(&s.chunk_mass[(0xffffffffu - static_cast<uint32_t>(rank)) / kChunk], w);
+                }
+            };
+            if (!whole) {
+#pragma unroll 1
+                for (uint32_t c = t; c < n; c += kRowThreads) visit(s.cand[c]);
+            } else {
+#pragma unroll 1
+                for (uint32_t i0 = 4 * t; i0 < p.vocab; i0 += 16 * kRowThreads) {
+                    v4f v[4];
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u) {
+                        const uint32_t i = i0 + u * 4 * kRowThreads;
+                        v[u] = load4(p, x, i);
+                    }
+#pragma unroll 1
+                    for (uint32_t u = 0; u < 4; ++u) {
+                        float four[4];
+                        unpack(pick(v, u), four);
+                        const uint32_t i = i0 + u * 4 * kRowThreads;
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k)
+                            if (key_of(four[k]) != 0) visit(rank_of(key_of(four[k]), i + k));
+                    }
+                }
+            }
+            __syncthreads();
+            if (digits) {
+                if (!alone) {
+                    const uint32_t mine = 255 - t;   // larger digits come first
+                    const uint32_t of = s.count[mine];
+                    const u64 v = stage == kByMass ? s.mass[mine] : of;
+                    u64 all;
+                    const u64 upto = before + sum_below<kRowThreads>(v, s.part, all);
+                    if (of != 0) atomicMax(&s.at, t);   // where the limit is beyond all: the last value that occurs
+                    if (upto < limit && upto + v >= limit) { s.result[0] = mine; s.result[1] = upto; }
+                    __syncthreads();
+                    if (s.result[0] == ~0ull && t == s.at) { s.result[0] = mine; s.result[1] = upto; }
+                    __syncthreads();
+                    alone = s.count[s.result[0]] == 1 && next != 0;
+                    found = (shift < 64 ? found << bits : 0) | s.result[0];
+                    before = s.result[1];
+                    shift = next;
+                    __syncthreads();
+                    if (shift != 0) continue;
+                } else {
+                    found = s.result[0];
+                    __syncthreads();
+                }
+                last = after = found;
+                stage = stage == kByCount && r.top_p < 1.0 ? kSum : kKeep;
+            } else if (stage == kSum) {
+                u64 kept;
+                (void)sum_below<kRowThreads>(sum, s.part, kept);
+                limit = mass_limit(kept + cut.k_mass);
+                stage = kByMass;
+                alone = false;
+                shift = width;
+                found = prefix;
+                before = 0;
+            } else {
+                break;
+            }
         }
-        walk([&](u64 rank) {
-            if (rank < last) return;
-            const u64 w = kept_weight_at(depth_of(static_cast<uint32_t>(rank >> 32), r), r);
-            if (w) atomicAdd(&s.chunk_mass[(0xffffffffu - static_cast<uint32_t>(rank)) / kChunk], w);
-        });
     } else if (cuts) {
         // a candidate a thread, ranked by counting
-        const Cut cut = p.cut[row];
         u64 own = t < n ? s.cand[t] : 0;
         s.cand[kRowThreads + t] = own;
         __syncthreads();
@@ -687,7 +757,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
         own = t < n ? s.cand[t] : 0;
         const double depth = depth_of(static_cast<uint32_t>(own >> 32), r);
         const uint32_t step = depth < kReach ? bin_at(depth) : kBins - 1;
-        const u64 w = t < n ? weight_at(depth) : 0;
+        const u64 w = t < n ? weight_at(depth, s.roots) : 0;
         uint32_t kept = n;   // candidates that stay: a prefix of their ranks
         u64 mass_k = cut.all_mass, all;
         if (cut.k_first < kBins) {
@@ -720,35 +790,34 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
     __syncthreads();
 
     // the chunk, then the element, at which the sum exceeds uniform * all
-    u64 of[4], sum = 0, all;
+    u64 share[4], sum = 0, all;
 #pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) sum += of[k] = s.chunk_mass[4 * t + k];
+    for (uint32_t k = 0; k < 4; ++k) sum += share[k] = s.chunk_mass[4 * t + k];
     u64 before = sum_below<kRowThreads>(sum, s.part, all);
-    float u = p.uniform[row];
     u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
     u64 target = static_cast<u64>(static_cast<double>(u) * static_cast<double>(all));
     if (target >= all) target = all - 1;
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
-        if (before <= target && target < before + of[k]) { s.at = 4 * t + k; s.target = target - before; }
-        before += of[k];
+        if (before <= target && target < before + share[k]) { s.at = 4 * t + k; s.target = target - before; }
+        before += share[k];
     }
     __syncthreads();
     const uint32_t i = s.at * kChunk + 4 * t;
     target = s.target;
     float v[4];
-    load4(p, x, i, v);
+    unpack(load4(p, x, i), v);
     sum = 0;
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
         const uint32_t key = key_of(v[k]);
-        sum += of[k] = rank_of(key, i + k) >= last ? kept_weight_at(depth_of(key, r), r) : 0;
+        sum += share[k] = rank_of(key, i + k) >= last ? kept_weight_at(depth_of(key, r), r, s.roots) : 0;
     }
     u64 run = sum_below<kRowThreads>(sum, s.part, all);
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
-        if (run <= target && target < run + of[k]) p.out[row] = q8mi_argmax_pair{v[k], static_cast<int32_t>(i + k)};
-        run += of[k];
+        if (run <= target && target < run + share[k]) p.out[row] = q8mi_argmax_pair{v[k], static_cast<int32_t>(i + k)};
+        run += share[k];
     }
 }
 
@@ -786,8 +855,7 @@ extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, 
     p.uniform = uniform; p.out = out; p.vocab = vocab; p.stride = stride;
     p.chunks = chunks_of(vocab);
     const uint64_t crowd = static_cast<uint64_t>(batch) * p.chunks / kGridWanted;
-    p.span = crowd < 1 ? 1 : crowd > kMostSpan ? kMostSpan : static_cast<uint32_t>(crowd);
-    p.spans = (p.chunks + p.span - 1) / p.span;
+    auto span_of = [&](uint32_t most) { return crowd < 1 ? 1u : crowd > most ? most : static_cast<uint32_t>(crowd); };
     p.vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (batch == 1 || stride % 4 == 0);
     uint8_t *at = static_cast<uint8_t *>(scratch);
     auto take = [&](uint64_t bytes) { uint8_t *a = at; at += batch * bytes; return a; };
@@ -801,8 +869,10 @@ extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, 
     p.top = reinterpret_cast<uint32_t *>(take(4));
     p.listed = reinterpret_cast<uint32_t *>(take(4));
     hipStream_t s = as_stream(stream);
-    const dim3 grid(p.spans, batch);
-    sample_best_kernel<<<grid, kChunkThreads, 0, s>>>(p);
+    p.span = span_of(kMostSpanOfBest);
+    sample_best_kernel<<<dim3((p.chunks + p.span - 1) / p.span, batch), kChunkThreads, 0, s>>>(p);
+    p.span = span_of(kMostSpan);
+    const dim3 grid((p.chunks + p.span - 1) / p.span, batch);
     sample_weigh_kernel<<<grid, kChunkThreads, 0, s>>>(p);
     if (top_k != nullptr || top_p != nullptr) sample_collect_kernel<<<grid, kChunkThreads, 0, s>>>(p);
     sample_draw_kernel<<<batch, kRowThreads, 0, s>>>(p);
