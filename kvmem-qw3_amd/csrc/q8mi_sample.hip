@@ -6,7 +6,7 @@
 // free of their order, so that neither the split of a row nor the arrival of atomics moves a border.
 //
 // No sort of the row.  Four launches, the first three over (spans of chunks of 1024 logits) x rows:
-//   1  largest logit of each chunk; clears the row's counters
+//   1  largest logit of each quarter of a chunk; clears the row's counters
 //   2  where top_k is no more than the chunks: the top_k-th largest of their maxima is no larger than the top_k-th logit, so
 //      the few logits from it up are collected.  Otherwise the weights: where nothing is cut but by min-p, their sum per
 //      chunk, else a histogram of count and weight over 1024 steps of 1/32 in (max - logit) / temperature (what lies 31.9
@@ -26,8 +26,11 @@ namespace {
 constexpr uint32_t kMaxVocab = 1u << 20;
 constexpr uint32_t kChunk = 1024;                     // logits
 constexpr uint32_t kMaxChunks = kMaxVocab / kChunk;
-constexpr uint32_t kMostSpan = 8;                     // chunks of a workgroup of launches 2 and 3
-constexpr uint32_t kMostSpanOfBest = 2;               // and of launch 1, which has nothing to hold for a row
+// Chunks of a workgroup: one while that leaves CUs idle, up to these where rows are many.  In launches 2 and 3 a span clears a
+// histogram and sends it off, or adds one up, once for all its chunks, while long spans leave the chip unevenly loaded by rows
+// of unlike settings (64 rows of 248320, spans of 4, 8, 16: 83, 71, 75 us); launch 1 holds nothing (spans of 2, 8: 2 us apart).
+constexpr uint32_t kMostSpan = 8, kMostSpanOfBest = 2;
+constexpr uint32_t kGridWanted = 512;                 // spans above one begin at twice this many workgroups
 constexpr uint32_t kAhead = 4;                        // chunks that a workgroup of launches 1 to 3 loads at a time
 constexpr uint32_t kChunkThreads = kChunk / 4;
 constexpr uint32_t kRowThreads = 256;                 // launch 4
@@ -57,16 +60,17 @@ struct SampleParams {
     const int32_t *top_k;
     q8mi_argmax_pair *out;
     u64 *chunk_mass;    // [row][chunk]: weight kept for certain
-    u64 *bin_mass;      // [row][kBins]
+    u64 *bin_mass;      // [row][copy][kBins]
     u64 *candidates;    // [row][chunk][kChunkCandidates]: key << 32 | ~index, in any order
     Cut *cut;           // [row] (launch 2 or 3)
-    uint32_t *best;     // [row][chunk]: largest key
+    uint32_t *best;     // [row][chunk][quarter]: largest key
     uint32_t *top;      // [row]: largest key (launch 2)
     uint32_t *listed;   // [row]: launch 2 has collected everything from rank 0 to the cuts
-    uint32_t *bin_count;     // [row][kBins]
+    uint32_t *bin_count;     // [row][copy][kBins]
     uint32_t *n_candidates;  // [row][chunk]: may be beyond kChunkCandidates
     uint32_t vocab, stride, chunks;
     uint32_t span;           // chunks of a workgroup (launches 1 to 3)
+    uint32_t copies;         // of a row's histogram
     int vec;
 };
 
@@ -127,7 +131,8 @@ __device__ __forceinline__ void make_roots(double *roots) {
 // exp(-depth) * 2^42 rounded to an integer: 2^(y / 32), y = 32 * (42 - depth * log2(e)) = 32 n + i + f with -1/2 <= f <= 1/2,
 // is 2^n from the exponent, 2^(i / 32) from the table and 2^(f / 32) from its series (terms up to the 5th power: 2e-15).
 // Adding 1.5 * 2^52 leaves 32 n + i in the sum's low bits, adding 2^52 the rounded integer.  Off by 1e-14 of itself and the
-// last rounding; depth 0 gives 2^42.  About 25 instructions, a third of the series alone (9.7 M weights: 41 -> XX us).
+// last rounding; depth 0 gives 2^42.  About 25 instructions, less than half of a series over a whole binade (64 rows of 151936
+// by temperature alone: 41 -> 34 us).
 __device__ __forceinline__ u64 weight_at(double depth, const double *roots) {
     constexpr double kHead = 6755399441055744.0, kLn = 0.693147180559945309417 / kRoots;
     const double y = fma(depth, -1.44269504088896340736 * kRoots, 42.0 * kRoots), head = y + kHead, f = y - (head - kHead);
@@ -146,17 +151,23 @@ __device__ __forceinline__ u64 kept_weight_at(double depth, const Row &r, const 
 }
 __device__ __forceinline__ uint32_t bin_at(double depth) { return static_cast<uint32_t>(depth * kBinsPerUnit); }
 
+// v + what a cross-lane move brings to the rows of 16 lanes in ROWS (0 where nothing comes).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_add(u64 v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xf, false);
+    return v + (static_cast<u64>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo));
+}
 __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
-    auto add = [](u64 a, int lo, int hi) { return a + (static_cast<u64>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo)); };
-    auto low = [](u64 a) { return static_cast<int>(a); };
-    auto high = [](u64 a) { return static_cast<int>(a >> 32); };
-    v = add(v, dpp_i32<kDppXor1>(low(v)), dpp_i32<kDppXor1>(high(v)));
-    v = add(v, dpp_i32<kDppXor2>(low(v)), dpp_i32<kDppXor2>(high(v)));
-    v = add(v, dpp_i32<kDppRowHalfMirror>(low(v)), dpp_i32<kDppRowHalfMirror>(high(v)));
-    v = add(v, dpp_i32<kDppRowMirror>(low(v)), dpp_i32<kDppRowMirror>(high(v)));
+    v = dpp_add<kDppXor1, 0xf>(v);
+    v = dpp_add<kDppXor2, 0xf>(v);
+    v = dpp_add<kDppRowHalfMirror, 0xf>(v);
+    v = dpp_add<kDppRowMirror, 0xf>(v);
     u64 all = 0;
 #pragma unroll
-    for (int row = 0; row < 64; row += 16) all = add(all, __builtin_amdgcn_readlane(low(v), row), __builtin_amdgcn_readlane(high(v), row));
+    for (int row = 0; row < 64; row += 16)
+        all += static_cast<u64>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), row))) << 32 |
+               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), row));
     return all;
 }
 // Sum of v over the threads below this one, and of all (`part`: one u64 a wave of LDS).
@@ -164,11 +175,12 @@ template <uint32_t THREADS>
 __device__ __forceinline__ u64 sum_below(u64 v, u64 *part, u64 &all) {
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     u64 upto = v;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const u64 o = __shfl_up(upto, d);
-        upto += lane >= static_cast<uint32_t>(d) ? o : 0;
-    }
+    upto = dpp_add<0x111, 0xf>(upto);   // one lane below, two, four, eight, within rows of 16 lanes
+    upto = dpp_add<0x112, 0xf>(upto);
+    upto = dpp_add<0x114, 0xf>(upto);
+    upto = dpp_add<0x118, 0xf>(upto);
+    upto = dpp_add<0x142, 0xa>(upto);   // the last lane of rows 0 and 2 to the rows behind them
+    upto = dpp_add<0x143, 0xc>(upto);   // lane 31 to rows 2 and 3
     __syncthreads();
     if (lane == 63) part[wave] = upto;
     __syncthreads();
@@ -193,7 +205,7 @@ __device__ __forceinline__ v4f load4(const SampleParams &p, const float *x, uint
 }
 // Register u of four by selection: what works on them is written once in a loop and not four times in a row.  Code is
 // fetched, too: the four launches fit the 64 KiB instruction cache together, so that a call finds what the last one left
-// (108 KB unrolled: XX us more a call).
+// (108 KB unrolled: the last launch alone took 10.9 us of one row, now 7.4).
 __device__ __forceinline__ v4f pick(const v4f (&v)[4], uint32_t u) {
     const v4f a = v[0], b = v[1], c = v[2], d = v[3];   // selected as values, so that they stay in registers
     return u == 0 ? a : u == 1 ? b : u == 2 ? c : d;
@@ -259,30 +271,31 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 
 // ---- 1 ----------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kChunkThreads) void sample_best_kernel(const SampleParams p) {
-    __shared__ uint32_t best[kMostSpanOfBest][kChunkThreads / kWave];
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
-    if (blockIdx.x == 0) {
+    if (blockIdx.x < p.copies) {
+        const uint64_t first = (static_cast<uint64_t>(row) * p.copies + blockIdx.x) * kBins;
         for (uint32_t b = t; b < kBins; b += kChunkThreads) {
-            p.bin_mass[static_cast<uint64_t>(row) * kBins + b] = 0;
-            p.bin_count[static_cast<uint64_t>(row) * kBins + b] = 0;
+            p.bin_mass[first + b] = 0;
+            p.bin_count[first + b] = 0;
         }
-        if (t == 0) p.listed[row] = 0;
+        if (blockIdx.x == 0 && t == 0) p.listed[row] = 0;
     }
     span.walk([&](const float (&v)[4], uint32_t, uint32_t c) {
         uint32_t key = 0;
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) key = key_of(v[k]) > key ? key_of(v[k]) : key;
         key = wave_max_u32(key);
-        if (t % kWave == 0) best[c][t / kWave] = key;
+        if (t % kWave == 0) p.best[(static_cast<uint64_t>(row) * p.chunks + span.first + c) * 4 + t / kWave] = key;
     });
-    __syncthreads();
-    if (span.first + t < span.end) {
-        uint32_t key = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < kChunkThreads / kWave; ++w) key = best[t][w] > key ? best[t][w] : key;
-        p.best[static_cast<uint64_t>(row) * p.chunks + span.first + t] = key;
-    }
+}
+
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+// The largest key of a row's chunk c.
+__device__ __forceinline__ uint32_t best_of(const SampleParams &p, uint32_t row, uint32_t c) {
+    const v4u q = *reinterpret_cast<const v4u *>(p.best + (static_cast<uint64_t>(row) * p.chunks + c) * 4);
+    const uint32_t a = q.x > q.y ? q.x : q.y, b = q.z > q.w ? q.z : q.w;
+    return a > b ? a : b;
 }
 
 // Sums and candidates of a span's chunks on their way out of a workgroup.
@@ -292,12 +305,12 @@ struct ChunkSpace {   // LDS
     uint32_t n[kMostSpan], best[kMostSpan];
 };
 // Clears it, makes the table and fetches the chunks' maxima; a barrier follows.
-__device__ __forceinline__ void open_space(ChunkSpace &s, const Span &span, const uint32_t *best) {
+__device__ __forceinline__ void open_space(ChunkSpace &s, const Span &span, const SampleParams &p, uint32_t row) {
     const uint32_t t = threadIdx.x;
     make_roots(s.roots);
     if (t >= kMostSpan) return;
     s.n[t] = 0;
-    s.best[t] = span.first + t < span.end ? best[span.first + t] : 0;
+    s.best[t] = span.first + t < span.end ? best_of(p, row, span.first + t) : 0;
 #pragma unroll
     for (uint32_t w = 0; w < kChunkThreads / kWave; ++w) s.mass[t][w] = 0;
 }
@@ -315,23 +328,34 @@ __device__ __forceinline__ void collect(const SampleParams &p, uint32_t row, Chu
         }
 }
 
-// The largest key, in its upper 24 bits, that k of the chunks' maxima reach (0: none).  Every wave for itself.
-template <uint32_t N>
-__device__ __forceinline__ uint32_t reached_by(const uint32_t *best, uint32_t chunks, uint32_t k) {
-    uint32_t keys[N], least = 0;
+// The largest key, in its upper 20 bits, that k of the maxima which at(0 .. count - 1) gives reach (0: none): bit by bit, from
+// the first in which they differ.  One wave finds it for the workgroup.
+template <uint32_t N, typename F>
+__device__ __forceinline__ uint32_t reached_by(F at, uint32_t count, uint32_t k, uint32_t &shared) {
+    if (threadIdx.x < kWave) {
+        uint32_t keys[N], most = 0, inverse = 0;
 #pragma unroll
-    for (uint32_t u = 0; u < N; ++u) {
-        const uint32_t c = u * kWave + threadIdx.x % kWave;
-        keys[u] = c < chunks ? best[c] : 0;
-    }
+        for (uint32_t u = 0; u < N; ++u) {
+            const uint32_t c = u * kWave + threadIdx.x;
+            keys[u] = c < count ? at(c) : 0;
+            most = keys[u] > most ? keys[u] : most;
+            inverse = c < count && ~keys[u] > inverse ? ~keys[u] : inverse;
+        }
+        most = wave_max_u32(most);
+        inverse = wave_max_u32(inverse);
+        const uint32_t differ = (most ^ ~inverse) | 1u << 11;
+        uint32_t bit = 0x80000000u >> __clz(differ), least = most & ~(2 * bit - 1);
 #pragma unroll 1
-    for (uint32_t bit = 1u << 31; bit >= 1u << 8; bit >>= 1) {
-        uint32_t reach = 0;
+        for (; bit >= 1u << 12; bit >>= 1) {
+            uint32_t reach = 0;
 #pragma unroll
-        for (uint32_t u = 0; u < N; ++u) reach += __popcll(__builtin_amdgcn_ballot_w64(keys[u] >= (least | bit)));
-        if (reach >= k) least |= bit;
+            for (uint32_t u = 0; u < N; ++u) reach += __popcll(__builtin_amdgcn_ballot_w64(keys[u] >= (least | bit)));
+            if (reach >= k) least |= bit;
+        }
+        if (threadIdx.x == 0) shared = least;
     }
-    return least;
+    __syncthreads();
+    return shared;
 }
 
 // ---- 2 ----------------------------------------------------------------------------------------------------------------
@@ -340,21 +364,24 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
     __shared__ uint32_t count[kBins];
     __shared__ u64 part[kChunkThreads / kWave];
     __shared__ ChunkSpace out;
+    __shared__ uint32_t found;
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
-    const uint32_t *best = p.best + static_cast<uint64_t>(row) * p.chunks;
-    open_space(out, span, best);
+    open_space(out, span, p, row);
     // the row's largest key
     uint32_t top = 0;
-    for (uint32_t c = t % kWave; c < p.chunks; c += kWave) top = best[c] > top ? best[c] : top;
+    for (uint32_t c = t % kWave; c < p.chunks; c += kWave) {
+        const uint32_t key = best_of(p, row, c);
+        top = key > top ? key : top;
+    }
     top = wave_max_u32(top);
     if (blockIdx.x == 0 && t == 0) p.top[row] = top;
     const Row r = row_of(p, row, top);
     if (top == 0 || r.greedy) return;
     if (r.top_k != 0 && r.top_k <= p.chunks) {
-        const uint32_t least = p.chunks <= 4 * kWave ? reached_by<4>(best, p.chunks, r.top_k)
-                                                     : reached_by<kMaxChunks / kWave>(best, p.chunks, r.top_k);
-        __syncthreads();
+        auto chunk = [&](uint32_t c) { return best_of(p, row, c); };
+        const uint32_t least = p.chunks <= 4 * kWave ? reached_by<4>(chunk, p.chunks, r.top_k, found)
+                                                     : reached_by<kMaxChunks / kWave>(chunk, p.chunks, r.top_k, found);
         if (least != 0) {
             if (blockIdx.x == 0 && t == 0) {
                 Cut cut{};
@@ -383,10 +410,16 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
         // From there on only the sum counts, in the last step, which no logit reaches.
         const double spare = (1.0 - r.top_p) / p.vocab - 0.5 / kOne;
         const double far = by_count || !(spare > 0.0) ? kReach : fmin(kReach, 0.1 - log(spare));
+        // The top_k-th largest of the maxima of quarters of chunks, where they are that many, is a bound as well: what lies
+        // below it is not looked at (64 rows of 248320, top_k 400: 80 -> 73 us).
+        uint32_t least = 0;
+        if (by_count && r.top_k <= 4 * p.chunks && 4 * p.chunks <= 16 * kWave)
+            least = reached_by<16>([&](uint32_t c) { return p.best[static_cast<uint64_t>(row) * p.chunks * 4 + c]; }, 4 * p.chunks, r.top_k, found);
         u64 rest = 0;
         span.walk([&](const float (&v)[4], uint32_t, uint32_t) {
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
+                if (key_of(v[k]) < least) continue;
                 const double depth = depth_at(v[k], r);
                 if (!(depth < kReach)) continue;
                 const uint32_t b = bin_at(depth);
@@ -396,7 +429,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
                 if (depth < far) atomicAdd(&mass[b], w);
                 else rest += w;
             }
-        });
+        }, [&](uint32_t c) { return out.best[c] >= least; });
         rest = wave_sum_u64(rest);
         if (t % kWave == 0 && rest != 0) atomicAdd(&mass[kBins - 1], rest);
         __syncthreads();
@@ -404,12 +437,13 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) mine[k] = count[4 * t + k];
         u64 all, before = by_count ? sum_below<kChunkThreads>((mine[0] + mine[1]) + (mine[2] + mine[3]), part, all) : 0;
+        const uint64_t first = (static_cast<uint64_t>(row) * p.copies + blockIdx.x % p.copies) * kBins;
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
             const uint32_t b = 4 * t + k;
             if (by_count && before >= r.top_k) break;
-            if (mine[k] != 0) atomicAdd(&p.bin_count[static_cast<uint64_t>(row) * kBins + b], mine[k]);
-            if (mass[b] != 0) atomicAdd(&p.bin_mass[static_cast<uint64_t>(row) * kBins + b], mass[b]);
+            if (mine[k] != 0) atomicAdd(&p.bin_count[first + b], mine[k]);
+            if (mass[b] != 0) atomicAdd(&p.bin_mass[first + b], mass[b]);
             before += mine[k];
         }
         return;
@@ -441,10 +475,14 @@ __device__ __forceinline__ Cut find_cut(const SampleParams &p, uint32_t row, con
     const bool holds = t < kHolders;
     u64 m[4] = {}, c[4] = {}, all_mass, all_count;
     if (holds) {
+        const uint64_t first = static_cast<uint64_t>(row) * p.copies * kBins + 4 * t;
+#pragma unroll 4
+        for (uint32_t i = 0; i < p.copies; ++i) {
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-            m[k] = p.bin_mass[static_cast<uint64_t>(row) * kBins + 4 * t + k];
-            c[k] = p.bin_count[static_cast<uint64_t>(row) * kBins + 4 * t + k];
+            for (uint32_t k = 0; k < 4; ++k) {
+                m[k] += p.bin_mass[first + i * kBins + k];
+                c[k] += p.bin_count[first + i * kBins + k];
+            }
         }
     }
     if (t == 0) { s.found[0] = s.found[1] = s.found[2] = kBins; s.k_count = 0; }
@@ -500,7 +538,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
     __shared__ ChunkSpace out;
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
-    open_space(out, span, p.best + static_cast<uint64_t>(row) * p.chunks);   // find_cut's barriers follow
+    open_space(out, span, p, row);   // find_cut's barriers follow
     const uint32_t top = p.top[row];
     const Row r = row_of(p, row, top);
     if (top == 0 || r.greedy || !(r.top_k != 0 || r.top_p < 1.0)) return;
@@ -547,6 +585,54 @@ struct DrawSpace {   // LDS
     double roots[kRoots];
 };
 
+// Sorts the first n of x, larger first: a bitonic network over 1024 numbers, four neighbouring ones a thread.  Partners meet in
+// registers, by lane exchange (33 of the 55 steps), or, 256 and 512 apart, through x.  About 4 us; the search by digits that
+// takes over beyond 1024 needs 15.
+constexpr uint32_t kSorted = 4 * kRowThreads;
+__device__ __forceinline__ void sort_down(u64 *x, uint32_t n) {
+    const uint32_t t = threadIdx.x;
+    u64 v[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) v[i] = 4 * t + i < n ? x[4 * t + i] : 0;
+    auto order = [](u64 &a, u64 &b, bool down) {
+        const u64 more = a > b ? a : b, less = a > b ? b : a;
+        a = down ? more : less;
+        b = down ? less : more;
+    };
+    order(v[0], v[1], true);
+    order(v[2], v[3], false);
+#pragma unroll 1
+    for (uint32_t k = 4; k <= kSorted; k *= 2) {
+        const bool down = (4 * t & k) == 0;
+        uint32_t j = k / 2;
+#pragma unroll 1
+        for (; j >= 4; j /= 2) {
+            const bool take_more = ((4 * t & j) == 0) == down;
+            u64 other[4];
+            if (j >= 4 * kWave) {   // uniform
+                __syncthreads();
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) x[4 * t + i] = v[i];
+                __syncthreads();
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) other[i] = x[(4 * t ^ j) + i];
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) other[i] = __shfl_xor(v[i], static_cast<int>(j / 4));
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) v[i] = (v[i] > other[i]) == take_more ? v[i] : other[i];
+        }
+        order(v[0], v[2], down);
+        order(v[1], v[3], down);
+        order(v[0], v[1], down);
+        order(v[2], v[3], down);
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) x[4 * t + i] = v[i];
+}
+
 __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SampleParams p) {
     __shared__ DrawSpace s;
     const uint32_t t = threadIdx.x, row = blockIdx.x;
@@ -578,7 +664,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
         if (t == 0) s.at = kMaxChunks;
         __syncthreads();
         for (uint32_t c = t; c < p.chunks; c += kRowThreads)
-            if (p.best[static_cast<uint64_t>(row) * p.chunks + c] == top) atomicMin(&s.at, c);
+            if (best_of(p, row, c) == top) atomicMin(&s.at, c);
         if (t == 0) s.bounds[0] = 0xffffffffu;
         __syncthreads();
         const uint32_t i = s.at * kChunk + 4 * t;
@@ -621,7 +707,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) s.chunk_mass[4 * t + k] = summed ? left[k] : 0;
     u64 last = 0;   // rank of the last kept element: everything from it up is kept
-    if (cuts && (whole || n > kRowThreads)) {
+    if (cuts && (whole || n > kSorted)) {
         // Many candidates, or more than the lists hold: then all logits of the row are.  The last rank that a cut keeps, of
         // the steps lo .. hi and from `after` up, is the one before which fewer than `limit` (by count or weight) come: eight
         // bits of the 64-bit ranks a walk, with counts and weights of the 256 values in LDS.  One loop around one walk, since
@@ -745,19 +831,29 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
             }
         }
     } else if (cuts) {
-        // a candidate a thread, ranked by counting
-        u64 own = t < n ? s.cand[t] : 0;
-        s.cand[kRowThreads + t] = own;
-        __syncthreads();
-        uint32_t above = 0;
+        if (n <= kRowThreads) {   // ranked by counting
+            const u64 own = t < n ? s.cand[t] : 0;
+            s.cand[kRowThreads + t] = own;
+            __syncthreads();
+            uint32_t above = 0;
 #pragma unroll 8
-        for (uint32_t i = 0; i < n; ++i) above += s.cand[kRowThreads + i] > own;
-        if (t < n) s.cand[above] = own;   // ranks differ
+            for (uint32_t i = 0; i < n; ++i) above += s.cand[kRowThreads + i] > own;
+            if (t < n) s.cand[above] = own;   // ranks differ
+        } else {
+            sort_down(s.cand, n);
+        }
         __syncthreads();
-        own = t < n ? s.cand[t] : 0;
-        const double depth = depth_of(static_cast<uint32_t>(own >> 32), r);
-        const uint32_t step = depth < kReach ? bin_at(depth) : kBins - 1;
-        const u64 w = t < n ? weight_at(depth, s.roots) : 0;
+        // four neighbouring ranks a thread
+        double depth[4];
+        uint32_t step[4];
+        u64 w[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            const u64 own = 4 * t + k < n ? s.cand[4 * t + k] : 0;
+            depth[k] = depth_of(static_cast<uint32_t>(own >> 32), r);
+            step[k] = depth[k] < kReach ? bin_at(depth[k]) : kBins - 1;
+            w[k] = weight_at(depth[k], s.roots);   // of no rank: 0
+        }
         uint32_t kept = n;   // candidates that stay: a prefix of their ranks
         u64 mass_k = cut.all_mass, all;
         if (cut.k_first < kBins) {
@@ -765,13 +861,18 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
             if (!listed) {
                 if (t == 0) s.bounds[0] = n;
                 __syncthreads();
-                if (t < n && step == cut.k_first) atomicMin(&s.bounds[0], t);
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k)
+                    if (4 * t + k < n && step[k] == cut.k_first) atomicMin(&s.bounds[0], 4 * t + k);
                 __syncthreads();
                 first = s.bounds[0];
             }
             kept = first + (r.top_k - cut.k_count);
             if (r.top_p < 1.0) {
-                (void)sum_below<kRowThreads>(t >= first && t < kept ? w : 0, s.part, mass_k);
+                u64 sum = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) sum += 4 * t + k >= first && 4 * t + k < kept ? w[k] : 0;
+                (void)sum_below<kRowThreads>(sum, s.part, mass_k);
                 mass_k += cut.k_mass;
             }
         }
@@ -779,13 +880,20 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
             const double limit_f = ceil(r.top_p * static_cast<double>(mass_k));
             const u64 limit = limit_f > 1.0 ? static_cast<u64>(limit_f) : 1ull;   // rank 0 always stays
             if (t == 0) s.bounds[1] = 0;
-            const u64 run = cut.sure_mass + sum_below<kRowThreads>(w, s.part, all);
-            if (t < n && step <= cut.last && run < limit) atomicMax(&s.bounds[1], t + 1);
+            u64 run = cut.sure_mass + sum_below<kRowThreads>((w[0] + w[1]) + (w[2] + w[3]), s.part, all);
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                if (4 * t + k < n && step[k] <= cut.last && run < limit) atomicMax(&s.bounds[1], 4 * t + k + 1);
+                run += w[k];
+            }
             __syncthreads();
             kept = s.bounds[1] < kept ? s.bounds[1] : kept;
         }
         last = s.cand[kept - 1];   // each cut keeps a candidate: the step before which it falls short holds it
-        if (t < kept && w != 0 && depth <= r.deepest) atomicAdd(&s.chunk_mass[(0xffffffffu - static_cast<uint32_t>(own)) / kChunk], w);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+            if (4 * t + k < kept && w[k] != 0 && depth[k] <= r.deepest)
+                atomicAdd(&s.chunk_mass[(0xffffffffu - static_cast<uint32_t>(s.cand[4 * t + k])) / kChunk], w[k]);
     }
     __syncthreads();
 
@@ -821,15 +929,23 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
     }
 }
 
-// Chunks of a workgroup: one while that leaves CUs idle, up to kMostSpan where rows are many (the histogram of a workgroup
-// is then cleared and added to the row's once for several chunks).
-constexpr uint32_t kGridWanted = 512;
+// A workgroup's histogram is added to one of a row's copies, one for kSpansOfCopy workgroups: atomics on the same few hundred
+// numbers wait for each other (one row of 248320 by top_p, 1, 4 and 8 copies: 38, 25 and 27 us).
+constexpr uint32_t kSpansOfCopy = 15, kMostCopies = 4;
 
 uint32_t chunks_of(uint32_t vocab) { return (vocab + kChunk - 1) / kChunk; }
-// Bytes of a row: chunk_mass, bin_mass, candidates, cut, bin_count, best, n_candidates, top, listed.
-uint64_t row_bytes(uint32_t vocab) {
-    const uint64_t chunks = chunks_of(vocab);
-    return 8 * (chunks + kBins + chunks * kChunkCandidates) + sizeof(Cut) + 4 * (kBins + 2 * chunks + 2);
+uint32_t span_of(uint32_t batch, uint32_t vocab, uint32_t most) {
+    const uint64_t crowd = static_cast<uint64_t>(batch) * chunks_of(vocab) / kGridWanted;
+    return crowd < 1 ? 1 : crowd > most ? most : static_cast<uint32_t>(crowd);
+}
+uint32_t copies_of(uint32_t batch, uint32_t vocab) {
+    const uint32_t spans = chunks_of(vocab) / span_of(batch, vocab, kMostSpan), copies = spans / kSpansOfCopy;
+    return copies < 1 ? 1 : copies > kMostCopies ? kMostCopies : copies;
+}
+// Bytes of a row: best, chunk_mass, bin_mass, candidates, cut, bin_count, n_candidates, top, listed.
+uint64_t row_bytes(uint32_t batch, uint32_t vocab) {
+    const uint64_t chunks = chunks_of(vocab), bins = kBins * copies_of(batch, vocab);
+    return 16 * chunks + 8 * (chunks + bins + chunks * kChunkCandidates) + sizeof(Cut) + 4 * (bins + chunks + 2);
 }
 
 }  // namespace
@@ -838,7 +954,7 @@ uint64_t row_bytes(uint32_t vocab) {
 using namespace q8mi;
 
 extern "C" size_t q8mi_sample_scratch_bytes(uint32_t batch, uint32_t vocab) {
-    return 16 + batch * row_bytes(vocab);
+    return 16 + batch * row_bytes(batch, vocab);
 }
 
 extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, uint32_t stride, const float *temperature,
@@ -854,24 +970,23 @@ extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, 
     p.logits = logits; p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
     p.uniform = uniform; p.out = out; p.vocab = vocab; p.stride = stride;
     p.chunks = chunks_of(vocab);
-    const uint64_t crowd = static_cast<uint64_t>(batch) * p.chunks / kGridWanted;
-    auto span_of = [&](uint32_t most) { return crowd < 1 ? 1u : crowd > most ? most : static_cast<uint32_t>(crowd); };
+    p.copies = copies_of(batch, vocab);
     p.vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (batch == 1 || stride % 4 == 0);
     uint8_t *at = static_cast<uint8_t *>(scratch);
     auto take = [&](uint64_t bytes) { uint8_t *a = at; at += batch * bytes; return a; };
+    p.best = reinterpret_cast<uint32_t *>(take(16ull * p.chunks));   // read by 16 bytes
     p.chunk_mass = reinterpret_cast<u64 *>(take(8ull * p.chunks));
-    p.bin_mass = reinterpret_cast<u64 *>(take(8ull * kBins));
+    p.bin_mass = reinterpret_cast<u64 *>(take(8ull * p.copies * kBins));
     p.candidates = reinterpret_cast<u64 *>(take(8ull * p.chunks * kChunkCandidates));
     p.cut = reinterpret_cast<Cut *>(take(sizeof(Cut)));
-    p.bin_count = reinterpret_cast<uint32_t *>(take(4ull * kBins));
-    p.best = reinterpret_cast<uint32_t *>(take(4ull * p.chunks));
+    p.bin_count = reinterpret_cast<uint32_t *>(take(4ull * p.copies * kBins));
     p.n_candidates = reinterpret_cast<uint32_t *>(take(4ull * p.chunks));
     p.top = reinterpret_cast<uint32_t *>(take(4));
     p.listed = reinterpret_cast<uint32_t *>(take(4));
     hipStream_t s = as_stream(stream);
-    p.span = span_of(kMostSpanOfBest);
+    p.span = span_of(batch, vocab, kMostSpanOfBest);
     sample_best_kernel<<<dim3((p.chunks + p.span - 1) / p.span, batch), kChunkThreads, 0, s>>>(p);
-    p.span = span_of(kMostSpan);
+    p.span = span_of(batch, vocab, kMostSpan);
     const dim3 grid((p.chunks + p.span - 1) / p.span, batch);
     sample_weigh_kernel<<<grid, kChunkThreads, 0, s>>>(p);
     if (top_k != nullptr || top_p != nullptr) sample_collect_kernel<<<grid, kChunkThreads, 0, s>>>(p);
