@@ -27,7 +27,6 @@ constexpr uint32_t kAttnThreads = 256;
 constexpr uint32_t kTile = 32;         // tokens of a step and wave
 constexpr uint32_t kMaxChunk = 2048;   // tokens of a workgroup: their page ids are held in LDS
 constexpr uint32_t kRowTile = 16;      // query rows of a wave
-constexpr uint32_t kJoinThreads = 256;
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -230,6 +229,7 @@ struct Layout {
     // Waves that share a tile meet at barriers: a second stage hides what a load takes longer than a step.  Waves on tiles of
     // their own are hidden by each other and by the second workgroup of the CU, which a second stage would not leave room for.
     static constexpr uint32_t kStages = WR > 1 && kGroups * 4 * kTileBytes <= 64 * 1024 ? 2 : 1;
+    static_assert(WR < 4 || kStages == 2, "a wave without rows passes no barrier but the first of a step");
     static constexpr uint32_t kTiles = 0;                              // [group][stage][K, V][tile]
     static constexpr uint32_t kPages = kGroups * kStages * 2 * kTileBytes;   // page ids of the chunk
     static constexpr uint32_t kMergeBytes = kGroups > 1 ? 4 * kRowTile * (D + 4) * 4 + 4 * kRowTile * 8 : 0;
@@ -433,13 +433,10 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
     uint32_t odd_tokens = 0;                               // bit i: token first_last + 1 + i holds values that are not finite
     uint32_t n_steps = (t1 - t0 + L::kUnit - 1) / L::kUnit;
     auto load_first = [&]() {
-#pragma unroll
-    for (uint32_t st = 0; st < L::kStages; ++st) {
-        if (st >= n_steps) break;   // uniform
-        const uint32_t where = locate(t0 + (st * L::kGroups + wg) * kTile);
-        load_tile(k_pool, k_tile ^ st * 2 * L::kTileBytes, where);
-        load_tile(v_pool, v_tile ^ st * 2 * L::kTileBytes, where);
-    }
+    if (n_steps == 0) return;   // uniform
+    const uint32_t where = locate(t0 + wg * kTile);
+    load_tile(k_pool, k_tile, where);
+    load_tile(v_pool, v_tile, where);
     };
     load_first();
     __builtin_amdgcn_sched_barrier(0);
@@ -480,6 +477,13 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
     }
     const float to_log2 = p.scale_log2 / row_scale;
 
+    auto turn = [&]() {   // to the other stage
+        k_tile ^= 2 * L::kTileBytes; v_tile ^= 2 * L::kTileBytes;
+        k_at ^= 2 * L::kTileBytes; v_at ^= 2 * L::kTileBytes;
+    };
+    // a wave of the tile's end without a query row only loads: its LDS reads and products would slow the others (48 rows in
+    // tiles of 64: 86 -> 78 us)
+    const bool idle = row0 + wr * kRowTile >= n_rows;   // uniform
     for (uint32_t step = 0; n_steps != 0; ++step) {
         if (step == n_steps) {   // the next chunk of the piece
             if (t1 == t_end) break;
@@ -493,14 +497,29 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
             load_first();
         }
         const uint32_t first = t0 + (step * L::kGroups + wg) * kTile;
-        const uint32_t next = locate(first + L::kStages * L::kGroups * kTile);
-        const bool more = step + L::kStages < n_steps;         // this step's stage gets another tile
-        const bool behind_one = L::kStages > 1 && step + 1 < n_steps;
-
-        // the keys are here; this step's values, and the next step's tile, may still travel
-        if (behind_one) wait_loads<3 * L::kLoadsPerWave>();
-        else wait_loads<L::kLoadsPerWave>();
-        if constexpr (WR > 1) __syncthreads();
+        const uint32_t next = locate(first + L::kGroups * kTile);
+        const bool more = step + 1 < n_steps;
+        if constexpr (L::kStages == 2) {   // this step's tile is here, and every wave has left the one before: its place takes the next
+            wait_loads<0>();
+            __syncthreads();
+            if (more) {
+                load_tile(k_pool, k_tile ^ 2 * L::kTileBytes, next);
+                load_tile(v_pool, v_tile ^ 2 * L::kTileBytes, next);
+            }
+        } else {   // the keys are here; the values may still travel
+            wait_loads<L::kLoadsPerWave>();
+            if constexpr (WR > 1) __syncthreads();
+        }
+        // whole: every row sees the whole tile (with several waves on a tile: all tiles of the step, so that the barriers below
+        // are met by all)
+        const uint32_t behind = WR > 1 ? t0 + (step + 1) * L::kGroups * kTile : first + kTile;
+        const bool whole = !any_bad && behind <= t1 && static_cast<int64_t>(behind) - 1 <= first_last;   // uniform
+        if constexpr (WR == 4) {   // two stages: no barrier before the next step's
+            if (idle && whole) {
+                turn();
+                continue;
+            }
+        }
         asm volatile("" : "+v"(k_at), "+v"(v_at));   // their variants are made anew each step: held, they cost 32 registers
         v4f s[2][Op::kTerms];
 #pragma unroll
@@ -531,15 +550,13 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
                 for (uint32_t h = 0; h < 2; ++h) s[h][k] = Op::mma(a[h], qf[j][k], s[h][k]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        wait_lds_reads();
-        if constexpr (WR > 1) __syncthreads();
-        if (more) load_tile(k_pool, k_tile, next);
+        if constexpr (L::kStages == 1) {
+            wait_lds_reads();
+            if constexpr (WR > 1) __syncthreads();
+            if (more) load_tile(k_pool, k_tile, next);
+        }
 
-        // a lane's eight tokens: first + h * 16 + g * 4 + i.  whole: every row sees the whole tile (with several waves on
-        // a tile: all tiles of the step, so that the barriers below are met by all)
-        const uint32_t behind = WR > 1 ? t0 + (step + 1) * L::kGroups * kTile : first + kTile;
-        const bool whole = !any_bad && behind <= t1 && static_cast<int64_t>(behind) - 1 <= first_last;   // uniform
-        float w[8];
+        float w[8];   // of a lane's eight tokens: first + h * 16 + g * 4 + i
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -581,10 +598,11 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
         Op::split(w, pf);
 
         // the values are here; what was asked for after them may still travel
-        if (more) wait_loads<(2 * L::kStages - 1) * L::kLoadsPerWave>();
-        else if (behind_one) wait_loads<2 * L::kLoadsPerWave>();
-        else wait_loads<0>();
-        if constexpr (WR > 1) __syncthreads();
+        if constexpr (L::kStages == 1) {
+            if (more) wait_loads<L::kLoadsPerWave>();
+            else wait_loads<0>();
+            if constexpr (WR > 1) __syncthreads();
+        }
         // V^T operand of 16 outputs: the transposing read gives lane i of a group of 16 column i of the rows that the
         // group's lanes point to, here its tokens g * 4 .. + 3 and 16 + g * 4 .. + 3
         auto values = [&](uint32_t d) -> typename Op::Raw {
@@ -656,12 +674,12 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
                 for (uint32_t d = 0; d < kBlock; ++d) o[b * kBlock + d] = Op::mma(a[d], pf[k], o[b * kBlock + d]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        wait_lds_reads();
-        if constexpr (WR > 1) __syncthreads();
-        if (more) load_tile(v_pool, v_tile, next);
-        if constexpr (L::kStages == 2) {
-            k_tile ^= 2 * L::kTileBytes; v_tile ^= 2 * L::kTileBytes;
-            k_at ^= 2 * L::kTileBytes; v_at ^= 2 * L::kTileBytes;
+        if constexpr (L::kStages == 1) {
+            wait_lds_reads();
+            if constexpr (WR > 1) __syncthreads();
+            if (more) load_tile(v_pool, v_tile, next);
+        } else {
+            turn();
         }
     }
     l = rows_sum(l);
@@ -742,7 +760,7 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
 }
 
 // Joins the pieces of one query row and head, in their order: kGroups threads share a column and meet in LDS.
-template <uint32_t D, int KV>
+template <uint32_t D, int KV, uint32_t kJoinThreads>
 __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const AttnParams p) {
     constexpr uint32_t kGroups = kJoinThreads / (D / 4);
     __shared__ float tops[kJoinThreads / kWave], sums[kGroups];
@@ -833,6 +851,10 @@ Plan plan_of(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_
     return r;
 }
 
+// Rows of queries and heads from which a wave, and not four, joins the pieces of one: they fill the chip, each has few pieces, and
+// four waves would mostly meet (128 x 32 rows: 9.2 -> 5.2 us; below, 24 rows of 128 pieces: 5.4 and not 9.8 us).
+constexpr uint32_t kManyJoined = 1024;
+
 template <uint32_t D, int KV, uint32_t WR>
 int launch_waves(AttnParams &p, hipStream_t s) {
     using L = Layout<D, KV, WR>;
@@ -853,7 +875,11 @@ int launch_waves(AttnParams &p, hipStream_t s) {
     const uint32_t resident = kChipCus * L::kResident;
     if (p.groups > resident) p.groups = resident;
     attention_kernel<D, KV, WR><<<p.groups, kAttnThreads, L::kBytes, s>>>(p);
-    if (p.max_kv_len > L::kUnit) attention_join_kernel<D, KV><<<dim3(p.n_seqs * p.max_q_len, p.q_heads), kJoinThreads, 0, s>>>(p);
+    if (p.max_kv_len > L::kUnit) {
+        const dim3 rows(p.n_seqs * p.max_q_len, p.q_heads);
+        if (static_cast<uint64_t>(rows.x) * rows.y >= kManyJoined) attention_join_kernel<D, KV, 64><<<rows, 64, 0, s>>>(p);
+        else attention_join_kernel<D, KV, 256><<<rows, 256, 0, s>>>(p);
+    }
     return check_launch("paged_attention");
 }
 template <uint32_t D, int KV>
