@@ -831,9 +831,13 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Attn
         store_out(p, static_cast<uint64_t>(q_row) * p.stride_out + head * D + d * 4 + i, sum == 0.0f ? 0.0f : out[i] / sum * norm);
 }
 
+constexpr uint32_t kChipCus = 256;
+// Where units of fewer tokens still leave CUs idle, waves without rows help to load: a workgroup then takes 32 tokens instead of
+// 128 through its one CU's path to memory (4 key heads of 256, 500 tokens: 14.6 -> 13.6 us; with 250 units, 2000 tokens, the
+// join of so many pieces takes more than that: 14.8 and 15.8 us).
+constexpr uint32_t kFewUnits = 192;
 // How a call is cut: waves side by side on rows, and workgroups: as many as a chip of 256 CUs holds at once (one to three a CU,
 // by registers and LDS), so that equal runs of the work end together, or one a unit.  Sizes alone decide, for every device.
-constexpr uint32_t kChipCus = 256;
 struct Plan {
     uint32_t waves_on_rows, groups;
 };
@@ -842,9 +846,13 @@ Plan plan_of(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_
     Plan r;
     const uint32_t rows = max_q_len * (kv_heads ? q_heads / kv_heads : 0);
     r.waves_on_rows = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    const uint64_t tiles = (rows + kRowTile * r.waves_on_rows - 1) / (kRowTile * r.waves_on_rows);
-    const uint32_t unit = kTile * 4 / r.waves_on_rows;
-    const uint64_t most = n_seqs * static_cast<uint64_t>(kv_heads) * tiles * (max_kv_len ? (max_kv_len + unit - 1) / unit : 1);
+    auto units_by = [&](uint32_t waves) {
+        const uint64_t tiles = (rows + kRowTile * waves - 1) / (kRowTile * waves);
+        const uint32_t unit = kTile * 4 / waves;
+        return n_seqs * static_cast<uint64_t>(kv_heads) * tiles * (max_kv_len ? (max_kv_len + unit - 1) / unit : 1);
+    };
+    if (units_by(4) <= kFewUnits) r.waves_on_rows = 4;
+    const uint64_t most = units_by(r.waves_on_rows);
     const uint32_t resident = kChipCus * (head_dim == 64 ? 3 : 2);
     r.groups = static_cast<uint32_t>(most < resident ? most : resident);
     if (units) *units = most;

@@ -17,7 +17,7 @@ pytestmark = pytest.mark.gpu
 
 class Case:
     def __init__(self, lens, rows, heads, kv_heads, dim, kind="bf16", act="f32", out_act=None, page=16, order="htd", gap=0, pad=0,
-                 max_q=None, starts=True, max_kv=None, seed=0, q_scale=2.0, scale=None, spare_rows=2, table_pad=1):
+                 max_q=None, starts=True, max_kv=None, far=False, seed=0, q_scale=2.0, scale=None, spare_rows=2, table_pad=1):
         rng = np.random.default_rng(seed)
         self.rng = rng
         self.lens, self.rows = list(lens), list(rows)
@@ -31,6 +31,8 @@ class Case:
         need = [max(0, (n + page - 1) // page) for n in self.lens]
         self.wide = max(need + [1]) + table_pad
         self.max_kv = max(max(self.lens), 1) if max_kv is None else max_kv
+        if far:   # bounds of a long context: the cut of a large call, on the lengths of a small one
+            self.wide, self.max_kv = 70000 // page + 1, 70000
         pages = sum(need) + 2
         ks, vs = (1 / 16, 1 / 8) if kind == "e4m3" else (1.0, 1.0)
         self.pools = R.Pools(kind, pages, page, kv_heads, dim, order, gap, ks, vs)     # unwritten rows are NaN in every type
@@ -109,23 +111,29 @@ def run(*a, **k):
     return c
 
 
+FAR = pytest.mark.parametrize("far", [False, True], ids=["near", "far"])
+
+
+@FAR
 @pytest.mark.parametrize("act", ["f32", "bf16"])
 @pytest.mark.parametrize("kind", ["bf16", "f16", "e4m3"])
 @pytest.mark.parametrize("dim,heads,kv_heads", [(256, 24, 4), (256, 2, 2), (128, 8, 1), (128, 10, 2), (64, 12, 12), (64, 20, 1)])
-def test_types_and_heads(gpu, dim, heads, kv_heads, kind, act):
-    run([37, 150], [1, 1], heads, kv_heads, dim, kind, act, seed=dim + heads)
+def test_types_and_heads(gpu, dim, heads, kv_heads, kind, act, far):
+    run([37, 150], [1, 1], heads, kv_heads, dim, kind, act, seed=dim + heads, far=far)
 
 
+@FAR
 @pytest.mark.parametrize("kind", ["bf16", "f16", "e4m3"])
 @pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 500, 1023, 1025, 3001])
-def test_lengths(gpu, n, kind):
-    run([n], [1], 6, 1, 256, kind, seed=n)
+def test_lengths(gpu, n, kind, far):
+    run([n], [1], 6, 1, 256, kind, seed=n, far=far)
 
 
+@FAR
 @pytest.mark.parametrize("rows", [2, 3, 5, 8, 11, 16])
 @pytest.mark.parametrize("dim,heads,kv_heads", [(256, 12, 2), (128, 40, 8), (64, 7, 7)])
-def test_several_rows(gpu, rows, dim, heads, kv_heads):
-    run([rows, 3, 130, 700], [rows, min(3, rows), rows, 1], heads, kv_heads, dim, seed=rows)
+def test_several_rows(gpu, rows, dim, heads, kv_heads, far):
+    run([rows, 3, 130, 700], [rows, min(3, rows), rows, 1], heads, kv_heads, dim, seed=rows, far=far)
 
 
 def test_wide_group(gpu):
@@ -133,22 +141,25 @@ def test_wide_group(gpu):
     run([100, 40], [16, 7], 80, 1, 64, seed=8)
 
 
+@FAR
 @pytest.mark.parametrize("page", [1, 3, 8, 20, 48, 256, 1000])
-def test_page_sizes(gpu, page):
-    run([333, 1, 64], [1, 1, 2], 8, 2, 128, "f16", page=page, seed=page)
+def test_page_sizes(gpu, page, far):
+    run([333, 1, 64], [1, 1, 2], 8, 2, 128, "f16", page=page, seed=page, far=far)
 
 
+@FAR
 @pytest.mark.parametrize("case", [dict(order="thd"), dict(gap=8), dict(pad=8), dict(act="bf16", out_act="f32"),
                                   dict(act="f32", out_act="bf16"), dict(starts=False), dict(starts=False, spare_rows=0), dict(scale=0.0),
                                   dict(scale=-0.3), dict(q_scale=40.0)], ids=str)
-def test_strides_and_forms(gpu, case):
-    run([90, 33], [2, 2], 8, 4, 128, seed=12, **case)
+def test_strides_and_forms(gpu, case, far):
+    run([90, 33], [2, 2], 8, 4, 128, seed=12, far=far, **case)
 
 
-def test_empty_and_idle(gpu):
+@FAR
+def test_empty_and_idle(gpu, far):
     """Sequences without tokens, without rows, with fewer tokens than rows (their first rows see nothing: zeros) and a
     negative length."""
-    run([0, 70, 2, -3, 5, 0], [1, 0, 4, 1, 5, 2], 4, 2, 128, seed=13)
+    run([0, 70, 2, -3, 5, 0], [1, 0, 4, 1, 5, 2], 4, 2, 128, seed=13, far=far)
 
 
 def test_every_sequence_empty(gpu):
@@ -167,9 +178,10 @@ def test_bounds_of_the_host(gpu):
     c.check()
 
 
-def test_bad_pages_hide_their_tokens(gpu):
+@FAR
+def test_bad_pages_hide_their_tokens(gpu, far):
     """Page ids below zero and beyond the pool: nothing is read, the other tokens count."""
-    c = Case([100, 50], [1, 2], 4, 2, 128, page=16, seed=16)
+    c = Case([100, 50], [1, 2], 4, 2, 128, page=16, seed=16, far=far)
     bad = {(0, 1): -1, (0, 4): c.pools.pages, (1, 0): 2 ** 31 - 1, (1, 3): -2 ** 31}
     for (s, p), v in bad.items():
         c.table[s, p] = v
@@ -179,10 +191,11 @@ def test_bad_pages_hide_their_tokens(gpu):
     c.check(hidden=lambda s, t: (s, t // 16) in bad)
 
 
+@FAR
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
-def test_later_tokens_do_not_leak(gpu, kind):
+def test_later_tokens_do_not_leak(gpu, kind, far):
     """A draft's key or value that holds infinities or NaN reaches its own and later rows only."""
-    c = Case([40], [4], 6, 2, 128, kind, seed=17)
+    c = Case([40], [4], 6, 2, 128, kind, seed=17, far=far)
     inf, nan = {"bf16": (0x7f80, 0x7fc0), "f16": (0x7c00, 0x7e00)}[kind]
     t = 38                                      # seen by rows 2 and 3
     for name, bits in (("v", inf), ("v", nan)):
@@ -267,9 +280,10 @@ def test_results_repeat(gpu):
                                                      (256, 12, 2, "e4m3")])
 @pytest.mark.parametrize("page", [1, 4, 5, 16, 24, 64])
 @pytest.mark.parametrize("rows", [1, 5])
-def test_page_sizes_of_every_type(gpu, page, dim, heads, kv_heads, kind, rows):
+@FAR
+def test_page_sizes_of_every_type(gpu, page, dim, heads, kv_heads, kind, rows, far):
     """Pages that a transfer of several tokens fits into, and pages it does not."""
-    run([203, 64, 9], [rows, 1, rows], heads, kv_heads, dim, kind, page=page, seed=page + rows)
+    run([203, 64, 9], [rows, 1, rows], heads, kv_heads, dim, kind, page=page, seed=page + rows, far=far)
 
 
 @pytest.mark.parametrize("n", [63, 64, 65, 200])
@@ -304,8 +318,9 @@ def test_runs_beyond_one_chunk(gpu, page, dim, kind, rows):
 
 
 @pytest.mark.parametrize("dim,heads,kv_heads,rows", [(128, 6, 1, 4), (256, 12, 1, 2), (64, 40, 1, 2), (256, 20, 1, 16)])
-def test_bad_pages_with_rows_side_by_side(gpu, dim, heads, kv_heads, rows):
-    c = Case([300, 70], [rows, rows], heads, kv_heads, dim, "f16", page=16, seed=40 + rows)
+@FAR
+def test_bad_pages_with_rows_side_by_side(gpu, dim, heads, kv_heads, rows, far):
+    c = Case([300, 70], [rows, rows], heads, kv_heads, dim, "f16", page=16, seed=40 + rows, far=far)
     bad = {(0, 1): -1, (0, 9): c.pools.pages, (1, 0): 2 ** 31 - 1}
     for (s, p), v in bad.items():
         c.table[s, p] = v
@@ -317,11 +332,12 @@ def test_bad_pages_with_rows_side_by_side(gpu, dim, heads, kv_heads, rows):
 
 @pytest.mark.parametrize("kind", ["bf16", "f16", "e4m3"])
 @pytest.mark.parametrize("dim,heads,kv_heads,rows", [(128, 2, 2, 8), (128, 6, 2, 8), (256, 6, 1, 16), (64, 40, 1, 5)])
-def test_later_tokens_of_several_rows(gpu, dim, heads, kv_heads, rows, kind):
+@FAR
+def test_later_tokens_of_several_rows(gpu, dim, heads, kv_heads, rows, kind, far):
     """Every other new token holds NaN in some elements of key and value: each row is not finite exactly where a token it sees makes
     it so."""
     n = 90
-    c = Case([n], [rows], heads, kv_heads, dim, kind, page=32, seed=50 + rows)
+    c = Case([n], [rows], heads, kv_heads, dim, kind, page=32, seed=50 + rows, far=far)
     nan = {"bf16": 0x7fc0, "f16": 0x7e00, "e4m3": 0x7f}[kind]
     for t in range(n - rows + 2, n, 2):        # value elements: those columns of rows from t's own on
         at = c.pools.at(c.table[0, t // 32], t % 32)
@@ -357,10 +373,11 @@ def test_rows_beyond_the_bound_hold_nothing_back(gpu, kind):
     c.check()
 
 
+@FAR
 @pytest.mark.parametrize("page", [16, 3])
-def test_a_context_behind_4_gib(gpu, page):
+def test_a_context_behind_4_gib(gpu, page, far):
     """Pages whose bytes lie beyond 32-bit offsets of the pools, through both ways of addressing."""
-    c = Case([70], [1], 4, 2, 128, "f16", page=page, seed=70)
+    c = Case([70], [1], 4, 2, 128, "f16", page=page, seed=70, far=far)
     pages, stride = 40, (1 << 26) + 512 * page       # elements: 128 MiB a page and a little
     values = stride // 16 * 8                        # they lie half a page stride behind the keys
     big = hip.DeviceBuffer(2 * stride * pages)
