@@ -17,8 +17,12 @@ namespace {
 constexpr uint32_t kAppendThreads = 256;
 constexpr uint32_t kAppendWaves = kAppendThreads / kWave;
 // Few tokens: a wave per head (or two, or four, that fit its lanes), so that one token occupies several CUs.  From kManyWaves
-// heads on, a workgroup per token, several heads a wave: the angles of a token are worked out once for all of them.
-constexpr uint32_t kManyHeads = 4, kManyWaves = 4096;
+// such waves on, a workgroup per token, kManyHeads times as many heads a wave at a time: the angles of a token are worked out
+// once for all of them (32 heads of 256: 128 tokens 5.7 and not 6.8 us, 192 both 8.2, 256 8.5 and not 9.7, 512 8.9 and not
+// 13.9).  Many tokens run at the rate of a copy (2048 of 32 heads of 256 in fp32, 126 MB: 27.7 us) or, in bf16, three quarters
+// of it (8191 of 48 heads of 128, 201 MB: 53.6 us; four heads at a time 59, the next ones already on their way 54.5, 16 bytes
+// a lane 82: waves in flight count for more than bytes of each).
+constexpr uint32_t kManyHeads = 2, kManyWaves = 6144;
 
 struct AppendParams {
     const void *q, *k, *v;
