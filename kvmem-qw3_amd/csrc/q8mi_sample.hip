@@ -54,6 +54,7 @@ struct Cut {
     u64 sure_mass, k_mass, all_mass;
 };
 
+struct Row;
 struct SampleParams {
     const float *logits;
     const float *temperature, *top_p, *min_p, *uniform;
@@ -63,6 +64,7 @@ struct SampleParams {
     u64 *bin_mass;      // [row][copy][kBins]
     u64 *candidates;    // [row][chunk][kChunkCandidates]: key << 32 | ~index, in any order
     Cut *cut;           // [row] (launch 2 or 3)
+    Row *rows;          // [row]
     uint32_t *best;     // [row][chunk][quarter]: largest key
     uint32_t *top;      // [row]: largest key (launch 2)
     uint32_t *listed;   // [row]: launch 2 has collected everything from rank 0 to the cuts
@@ -87,17 +89,18 @@ __device__ __forceinline__ u64 rank_of(uint32_t key, uint32_t index) {   // larg
     return static_cast<u64>(key) << 32 | (0xffffffffu - index);
 }
 
+// A row's settings as the launches use them; worked out once, by launch 1.
 struct Row {
-    double max;
+    double max;        // launches 2 to 4
     double per_unit;   // 1 / temperature, above zero
     double deepest;    // what min_p keeps lies no deeper: p >= min_p <=> depth <= -log(min_p)
-    uint32_t top_k;    // 0: off
     double top_p;      // 1: off
-    bool greedy;
+    double far;        // a cut by weight alone lies above this depth
+    uint32_t top_k;    // 0: off
+    uint32_t greedy;
 };
-__device__ __forceinline__ Row row_of(const SampleParams &p, uint32_t row, uint32_t top_key) {
-    Row r;
-    r.max = logit_of(top_key);
+__device__ __forceinline__ Row settings_of(const SampleParams &p, uint32_t row) {
+    Row r{};
     const float t = p.temperature ? p.temperature[row] : 1.0f;
     r.greedy = !(t > 0.0f);
     // an infinite temperature: depths below 1e-250, which no other one gives, where p is 1 and -inf still lies at the bottom
@@ -108,6 +111,15 @@ __device__ __forceinline__ Row row_of(const SampleParams &p, uint32_t row, uint3
     r.top_k = k > 0 && static_cast<uint32_t>(k) < p.vocab ? k : 0;
     const float top_p = p.top_p ? p.top_p[row] : 1.0f;
     r.top_p = top_p < 1.0f ? top_p : 1.0;
+    // the largest weighs 1, so 1 - top_p may always be dropped, and `vocab` logits below a depth whose weight is
+    // (1 - top_p) / vocab, less the half step that rounding may add to it, cannot hold the cut
+    const double spare = (1.0 - r.top_p) / p.vocab - 0.5 / kOne;
+    r.far = spare > 0.0 ? fmin(kReach, 0.1 - log(spare)) : kReach;
+    return r;
+}
+__device__ __forceinline__ Row row_of(const SampleParams &p, uint32_t row, uint32_t top_key) {
+    Row r = p.rows[row];
+    r.max = logit_of(top_key);
     return r;
 }
 // How far below the maximum, in temperatures, 0 .. kBottom.  NaN and -inf lie at the bottom; below +inf, it itself is the only
@@ -279,7 +291,10 @@ __global__ __launch_bounds__(kChunkThreads) void sample_best_kernel(const Sample
             p.bin_mass[first + b] = 0;
             p.bin_count[first + b] = 0;
         }
-        if (blockIdx.x == 0 && t == 0) p.listed[row] = 0;
+        if (blockIdx.x == 0 && t == 0) {
+            p.listed[row] = 0;
+            p.rows[row] = settings_of(p, row);
+        }
     }
     span.walk([&](const float (&v)[4], uint32_t, uint32_t c) {
         uint32_t key = 0;
@@ -304,10 +319,9 @@ struct ChunkSpace {   // LDS
     double roots[kRoots];
     uint32_t n[kMostSpan], best[kMostSpan];
 };
-// Clears it, makes the table and fetches the chunks' maxima; a barrier follows.
+// Clears it and fetches the chunks' maxima; a barrier follows.
 __device__ __forceinline__ void open_space(ChunkSpace &s, const Span &span, const SampleParams &p, uint32_t row) {
     const uint32_t t = threadIdx.x;
-    make_roots(s.roots);
     if (t >= kMostSpan) return;
     s.n[t] = 0;
     s.best[t] = span.first + t < span.end ? best_of(p, row, span.first + t) : 0;
@@ -364,17 +378,21 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
     __shared__ uint32_t count[kBins];
     __shared__ u64 part[kChunkThreads / kWave];
     __shared__ ChunkSpace out;
-    __shared__ uint32_t found;
+    __shared__ uint32_t found, tops[kChunkThreads / kWave];
     const uint32_t t = threadIdx.x, row = blockIdx.y;
     Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
     open_space(out, span, p, row);
     // the row's largest key
     uint32_t top = 0;
-    for (uint32_t c = t % kWave; c < p.chunks; c += kWave) {
+    for (uint32_t c = t; c < p.chunks; c += kChunkThreads) {
         const uint32_t key = best_of(p, row, c);
         top = key > top ? key : top;
     }
     top = wave_max_u32(top);
+    if (t % kWave == 0) tops[t / kWave] = top;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kChunkThreads / kWave; ++w) top = tops[w] > top ? tops[w] : top;
     if (blockIdx.x == 0 && t == 0) p.top[row] = top;
     const Row r = row_of(p, row, top);
     if (top == 0 || r.greedy) return;
@@ -403,13 +421,12 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
     const bool by_count = r.top_k != 0, by_mass = r.top_p < 1.0;   // each needs its half of the histogram
     if (by_count || by_mass) {
         for (uint32_t b = t; b < kBins; b += kChunkThreads) { mass[b] = 0; count[b] = 0; }
+        make_roots(out.roots);
         __syncthreads();
         // The row's steps are added up by atomics, so few are sent.  Where this span alone has top_k above a step, the cut
-        // lies above it, too.  Without top_k: the largest weighs 1, so 1 - top_p may always be dropped, and `vocab` logits below
-        // a depth whose weight is (1 - top_p) / vocab, less the half step that rounding may add to it, cannot hold the cut.
-        // From there on only the sum counts, in the last step, which no logit reaches.
-        const double spare = (1.0 - r.top_p) / p.vocab - 0.5 / kOne;
-        const double far = by_count || !(spare > 0.0) ? kReach : fmin(kReach, 0.1 - log(spare));
+        // lies above it, too.  Without top_k, it does not lie below r.far: from there on only the sum counts, in the last
+        // step, which no logit reaches.
+        const double far = by_count ? kReach : r.far;
         // The top_k-th largest of the maxima of quarters of chunks, where they are that many, is a bound as well: what lies
         // below it is not looked at (64 rows of 248320, top_k 400: 80 -> 73 us).
         uint32_t least = 0;
@@ -448,6 +465,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
         }
         return;
     }
+    make_roots(out.roots);
     __syncthreads();
     span.walk([&](const float (&v)[4], uint32_t, uint32_t c) {
         u64 sum = 0;
@@ -543,6 +561,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
     const Row r = row_of(p, row, top);
     if (top == 0 || r.greedy || !(r.top_k != 0 || r.top_p < 1.0)) return;
     if (p.listed[row]) return;
+    make_roots(out.roots);
     const Cut cut = find_cut<kChunkThreads>(p, row, r, space);
     if (blockIdx.x == 0 && t == 0) p.cut[row] = cut;
     // logits well below the last step of interest need no 64-bit depth
@@ -942,10 +961,10 @@ uint32_t copies_of(uint32_t batch, uint32_t vocab) {
     const uint32_t spans = chunks_of(vocab) / span_of(batch, vocab, kMostSpan), copies = spans / kSpansOfCopy;
     return copies < 1 ? 1 : copies > kMostCopies ? kMostCopies : copies;
 }
-// Bytes of a row: best, chunk_mass, bin_mass, candidates, cut, bin_count, n_candidates, top, listed.
+// Bytes of a row: best, chunk_mass, bin_mass, candidates, cut, rows, bin_count, n_candidates, top, listed.
 uint64_t row_bytes(uint32_t batch, uint32_t vocab) {
     const uint64_t chunks = chunks_of(vocab), bins = kBins * copies_of(batch, vocab);
-    return 16 * chunks + 8 * (chunks + bins + chunks * kChunkCandidates) + sizeof(Cut) + 4 * (bins + chunks + 2);
+    return 16 * chunks + 8 * (chunks + bins + chunks * kChunkCandidates) + sizeof(Cut) + sizeof(Row) + 4 * (bins + chunks + 2);
 }
 
 }  // namespace
@@ -979,6 +998,7 @@ extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, 
     p.bin_mass = reinterpret_cast<u64 *>(take(8ull * p.copies * kBins));
     p.candidates = reinterpret_cast<u64 *>(take(8ull * p.chunks * kChunkCandidates));
     p.cut = reinterpret_cast<Cut *>(take(sizeof(Cut)));
+    p.rows = reinterpret_cast<Row *>(take(sizeof(Row)));
     p.bin_count = reinterpret_cast<uint32_t *>(take(4ull * p.copies * kBins));
     p.n_candidates = reinterpret_cast<uint32_t *>(take(4ull * p.chunks));
     p.top = reinterpret_cast<uint32_t *>(take(4));
