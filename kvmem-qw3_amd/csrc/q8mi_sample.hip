@@ -182,6 +182,14 @@ __device__ __forceinline__ u64 wave_sum_u64(u64 v) {
                static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), row));
     return all;
 }
+__device__ __forceinline__ u64 wave_max_u64(u64 v) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const u64 o = __shfl_xor(v, d);
+        v = o > v ? o : v;
+    }
+    return v;
+}
 // Sum of v over the threads below this one, and of all (`part`: one u64 a wave of LDS).
 template <uint32_t THREADS>
 __device__ __forceinline__ u64 sum_below(u64 v, u64 *part, u64 &all) {
@@ -217,7 +225,7 @@ __device__ __forceinline__ v4f load4(const SampleParams &p, const float *x, uint
 }
 // Register u of four by selection: what works on them is written once in a loop and not four times in a row.  Code is
 // fetched, too: the four launches fit the 64 KiB instruction cache together, so that a call finds what the last one left
-// (108 KB unrolled: the last launch alone took 10.9 us of one row, now 7.4).
+// (108 KB unrolled: the last launch alone took 10.9 us of one row, now 6.9).
 __device__ __forceinline__ v4f pick(const v4f (&v)[4], uint32_t u) {
     const v4f a = v[0], b = v[1], c = v[2], d = v[3];   // selected as values, so that they stay in registers
     return u == 0 ? a : u == 1 ? b : u == 2 ? c : d;
@@ -428,7 +436,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
         // step, which no logit reaches.
         const double far = by_count ? kReach : r.far;
         // The top_k-th largest of the maxima of quarters of chunks, where they are that many, is a bound as well: what lies
-        // below it is not looked at (64 rows of 248320, top_k 400: 80 -> 73 us).
+        // below it is not looked at (64 rows of 248320, top_k 400: 80 -> 72 us).
         uint32_t least = 0;
         if (by_count && r.top_k <= 4 * p.chunks && 4 * p.chunks <= 16 * kWave)
             least = reached_by<16>([&](uint32_t c) { return p.best[static_cast<uint64_t>(row) * p.chunks * 4 + c]; }, 4 * p.chunks, r.top_k, found);
@@ -606,7 +614,7 @@ struct DrawSpace {   // LDS
 
 // Sorts the first n of x, larger first: a bitonic network over 1024 numbers, four neighbouring ones a thread.  Partners meet in
 // registers, by lane exchange (33 of the 55 steps), or, 256 and 512 apart, through x.  About 4 us; the search by digits that
-// takes over beyond 1024 needs 15.
+// takes over beyond 1024 needs about 12.
 constexpr uint32_t kSorted = 4 * kRowThreads;
 __device__ __forceinline__ void sort_down(u64 *x, uint32_t n) {
     const uint32_t t = threadIdx.x;
@@ -704,20 +712,44 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
     bool whole = false;
     if (cuts) {
         u64 sum = 0, all;
-        bool full = false;
+        bool full = false, more = false;
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
             full |= of[k] > kChunkCandidates;
+            more |= of[k] > 2;
             sum += of[k];
         }
         uint32_t at = static_cast<uint32_t>(sum_below<kRowThreads>(sum, s.part, all));
-        n = static_cast<uint32_t>(all);
+        n = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(all));   // loops to it are scalar
         whole = __syncthreads_or(full) || n > kMaxCandidates;
         if (!whole) {
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
-                const u64 *list = p.candidates + (static_cast<uint64_t>(row) * p.chunks + 4 * t + k) * kChunkCandidates;
-                for (uint32_t i = 0; i < of[k]; ++i) s.cand[at++] = i == 0 ? two[k][0] : i == 1 ? two[k][1] : list[i];
+                s.chunk_mass[4 * t + k] = static_cast<u64>(of[k]) << 32 | at;   // for what follows here alone
+                if (of[k] > 0) s.cand[at] = two[k][0];
+                if (of[k] > 1) s.cand[at + 1] = two[k][1];
+                at += of[k];
+            }
+            if (__syncthreads_or(more)) {   // the others: sixteen lanes a chunk, four chunks of theirs asked for at once
+                const uint32_t lane = threadIdx.x % 16;
+#pragma unroll 1
+                for (uint32_t c0 = t / 16; c0 < p.chunks; c0 += 4 * (kRowThreads / 16)) {
+                    u64 place[4], got[4];
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u) {
+                        const uint32_t c = c0 + u * (kRowThreads / 16);
+                        place[u] = c < p.chunks ? s.chunk_mass[c] : 0;
+                        if (2 + lane < place[u] >> 32)
+                            got[u] = p.candidates[(static_cast<uint64_t>(row) * p.chunks + c) * kChunkCandidates + 2 + lane];
+                    }
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u) {
+                        const uint32_t c = c0 + u * (kRowThreads / 16), count = place[u] >> 32, to = static_cast<uint32_t>(place[u]);
+                        if (2 + lane < count) s.cand[to + 2 + lane] = got[u];
+                        for (uint32_t i = 18 + lane; i < count; i += 16)
+                            s.cand[to + i] = p.candidates[(static_cast<uint64_t>(row) * p.chunks + c) * kChunkCandidates + i];
+                    }
+                }
             }
         }
         __syncthreads();
@@ -731,29 +763,32 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
         // the steps lo .. hi and from `after` up, is the one before which fewer than `limit` (by count or weight) come: eight
         // bits of the 64-bit ranks a walk, with counts and weights of the 256 values in LDS.  One loop around one walk, since
         // the code of a walk is long.
-        uint32_t width = 64;   // bits in which the ranks differ
-        u64 prefix = 0;        // the others
+        uint32_t width = 64;   // digits are of rank - low: among the candidates, no more than their range has
+        u64 low = 0;
         if (!whole) {
-            if (t == 0) { s.result[0] = 0; s.result[1] = ~0ull; }
-            __syncthreads();
-            u64 any = 0, every = ~0ull;
+            u64 high = 0, inverse = 0;
             for (uint32_t c = t; c < n; c += kRowThreads) {
-                const u64 rank = s.cand[c];
-                any |= rank;
-                every &= rank;
+                high = s.cand[c] > high ? s.cand[c] : high;
+                inverse = ~s.cand[c] > inverse ? ~s.cand[c] : inverse;
             }
-            atomicOr(&s.result[0], any);
-            atomicAnd(&s.result[1], every);
+            high = wave_max_u64(high);
+            inverse = wave_max_u64(inverse);
+            if (t % kWave == 0) { s.part[t / kWave] = high; s.mass[t / kWave] = inverse; }
             __syncthreads();
-            width = 64 - __clzll(s.result[0] ^ s.result[1]);   // candidates are more than one, and differ
-            prefix = width < 64 ? s.result[0] >> width : 0;
+#pragma unroll
+            for (uint32_t w = 0; w < kRowThreads / kWave; ++w) {
+                high = s.part[w] > high ? s.part[w] : high;
+                inverse = s.mass[w] > inverse ? s.mass[w] : inverse;
+            }
+            low = ~inverse;
+            width = 64 - __clzll(high - low);   // candidates are more than one, and differ
             __syncthreads();
         }
         enum { kByCount, kSum, kByMass, kKeep };
         uint32_t stage = cut.k_first < kBins ? kByCount : r.top_p < 1.0 ? kByMass : kKeep;
         bool alone = false;        // one rank has the digits found so far: the rest of it at once
-        uint32_t shift = width;    // found: the bits from `shift` on
-        u64 found = prefix, before = 0, after = 0, sum = 0;
+        uint32_t shift = width;    // found: the bits of rank - low from `shift` on
+        u64 found = 0, before = 0, after = 0, sum = 0;
         u64 limit = r.top_k - cut.k_count;
         auto mass_limit = [&](u64 kept) {   // of a cut by weight, when top_k keeps `kept`
             const double limit_f = ceil(r.top_p * static_cast<double>(kept));
@@ -774,12 +809,13 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
                 const double depth = depth_of(static_cast<uint32_t>(rank >> 32), r);
                 const uint32_t b = depth < kReach ? bin_at(depth) : kBins - 1;
                 if (digits) {
-                    if (rank < after || (shift < 64 && rank >> shift != found) || b < lo || b > hi) return;
+                    const u64 v = rank - low;
+                    if (rank < after || (shift < 64 && v >> shift != found) || b < lo || b > hi) return;
                     if (alone) {
-                        s.result[0] = rank;
+                        s.result[0] = v;
                         return;
                     }
-                    const uint32_t digit = static_cast<uint32_t>(rank >> next) & ((1u << bits) - 1);
+                    const uint32_t digit = static_cast<uint32_t>(v >> next) & ((1u << bits) - 1);
                     atomicAdd(&s.count[digit], 1u);
                     if (stage == kByMass) atomicAdd(&s.mass[digit], weight_at(depth, s.roots));
                 } else if (rank >= last) {
@@ -790,7 +826,14 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
             };
             if (!whole) {
 #pragma unroll 1
-                for (uint32_t c = t; c < n; c += kRowThreads) visit(s.cand[c]);
+                for (uint32_t c = t; c < n; c += 4 * kRowThreads) {   // one wave a SIMD: four at a time hide each other's latency
+                    u64 rank[4];
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u) rank[u] = c + u * kRowThreads < n ? s.cand[c + u * kRowThreads] : 0;
+#pragma unroll
+                    for (uint32_t u = 0; u < 4; ++u)
+                        if (rank[u] != 0) visit(rank[u]);
+                }
             } else {
 #pragma unroll 1
                 for (uint32_t i0 = 4 * t; i0 < p.vocab; i0 += 16 * kRowThreads) {
@@ -819,7 +862,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
                     const u64 v = stage == kByMass ? s.mass[mine] : of;
                     u64 all;
                     const u64 upto = before + sum_below<kRowThreads>(v, s.part, all);
-                    if (of != 0) atomicMax(&s.at, t);   // where the limit is beyond all: the last value that occurs
+                    // where the limit is beyond all: the last value that occurs (atomics of a whole wave on one address would
+                    // take 40 cycles a lane)
+                    const u64 occurs = __builtin_amdgcn_ballot_w64(of != 0);
+                    if (t % kWave == 0 && occurs != 0) atomicMax(&s.at, t + 63u - static_cast<uint32_t>(__builtin_clzll(occurs)));
                     if (upto < limit && upto + v >= limit) { s.result[0] = mine; s.result[1] = upto; }
                     __syncthreads();
                     if (s.result[0] == ~0ull && t == s.at) { s.result[0] = mine; s.result[1] = upto; }
@@ -834,7 +880,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
                     found = s.result[0];
                     __syncthreads();
                 }
-                last = after = found;
+                last = after = found + low;
                 stage = stage == kByCount && r.top_p < 1.0 ? kSum : kKeep;
             } else if (stage == kSum) {
                 u64 kept;
@@ -843,7 +889,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
                 stage = kByMass;
                 alone = false;
                 shift = width;
-                found = prefix;
+                found = 0;
                 before = 0;
             } else {
                 break;
@@ -878,13 +924,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
         if (cut.k_first < kBins) {
             uint32_t first = 0;   // the first candidate of top_k's step
             if (!listed) {
-                if (t == 0) s.bounds[0] = n;
-                __syncthreads();
+                uint32_t above = 0;   // steps never fall along the ranks
 #pragma unroll
-                for (uint32_t k = 0; k < 4; ++k)
-                    if (4 * t + k < n && step[k] == cut.k_first) atomicMin(&s.bounds[0], 4 * t + k);
-                __syncthreads();
-                first = s.bounds[0];
+                for (uint32_t k = 0; k < 4; ++k) above += 4 * t + k < n && step[k] < cut.k_first;
+                (void)sum_below<kRowThreads>(above, s.part, all);
+                first = static_cast<uint32_t>(all);
             }
             kept = first + (r.top_k - cut.k_count);
             if (r.top_p < 1.0) {
@@ -898,15 +942,15 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
         if (r.top_p < 1.0) {
             const double limit_f = ceil(r.top_p * static_cast<double>(mass_k));
             const u64 limit = limit_f > 1.0 ? static_cast<u64>(limit_f) : 1ull;   // rank 0 always stays
-            if (t == 0) s.bounds[1] = 0;
             u64 run = cut.sure_mass + sum_below<kRowThreads>((w[0] + w[1]) + (w[2] + w[3]), s.part, all);
+            uint32_t within = 0;   // nor do sums
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
-                if (4 * t + k < n && step[k] <= cut.last && run < limit) atomicMax(&s.bounds[1], 4 * t + k + 1);
+                within += 4 * t + k < n && step[k] <= cut.last && run < limit;
                 run += w[k];
             }
-            __syncthreads();
-            kept = s.bounds[1] < kept ? s.bounds[1] : kept;
+            (void)sum_below<kRowThreads>(within, s.part, all);
+            kept = all < kept ? static_cast<uint32_t>(all) : kept;
         }
         last = s.cand[kept - 1];   // each cut keeps a candidate: the step before which it falls short holds it
 #pragma unroll
