@@ -297,7 +297,8 @@ typedef struct q8mi_kv_cache {
 
 /* What lies between the Q/K/V projections and the attention, in one launch: RMS norm of every query and key
  * head, position rotation of the normalised heads, and the append of keys and values to the cache.
- *   norm      y[i] = x[i] / sqrt(mean_i x[i]^2 + eps) * weight[i] over a head's head_dim elements;
+ *   norm      y[i] = x[i] / sqrt(mean_i x[i]^2 + eps) * weight[i] over a head's head_dim elements (squares are
+ *             summed in fp32: what is under the root must lie within 2^-126 .. 2^127);
  *             q_norm_weight / k_norm_weight (head_dim floats) may be NULL: those heads are not normalised
  *   rotation  of the first rotary_dim elements (a multiple of 8, at most head_dim; 0 = none):
  *             (a, b) -> (a cos t - b sin t, b cos t + a sin t), t = positions[token] * freqs[i] radians,
@@ -339,7 +340,7 @@ int q8mi_qk_norm_rope_append(const void *q, const void *k, const void *v, void *
  * scratch: q8mi_paged_attention_scratch_bytes() device bytes, 16-byte aligned; calls that may overlap need
  * one each.  Nothing in it needs clearing.  Results repeat bit by bit.  Q8MI_REJECTED: q_heads not a multiple of
  * kv_heads or above 65535, the bounds above, q, out or their strides in bytes not multiples of 16, a scale that
- * is not finite, a pool of 64 GiB and more, 2^22 rows and more. */
+ * is not finite or beyond 2^127, a pool of 64 GiB and more, 2^22 rows and more. */
 size_t q8mi_paged_attention_scratch_bytes(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads,
                                           uint32_t head_dim, uint32_t max_kv_len);
 int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_rows, uint32_t stride_q_row,

@@ -931,7 +931,8 @@ extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_row
     if (max_q_len == 0 || max_q_len > kMaxRows) return fail(Q8MI_REJECTED, "%s: %u rows a sequence (1..%u)", what, max_q_len, kMaxRows);
     if (max_kv_len > 0x7fffffffu || max_kv_len > static_cast<uint64_t>(stride_page_table) * cache->page_size)
         return fail(Q8MI_REJECTED, "%s: max_kv_len %u is beyond a page table row of %u", what, max_kv_len, stride_page_table);
-    if (!isfinite(scale)) return fail(Q8MI_REJECTED, "%s: scale is not finite", what);
+    const float scale_log2 = scale * 1.44269504088896340736f * (cache->dtype == Q8MI_KV_E4M3 ? cache->k_scale : 1.0f);
+    if (!isfinite(scale_log2)) return fail(Q8MI_REJECTED, "%s: scale %g is not finite, or too large", what, static_cast<double>(scale));
     const uint64_t q_es = q_is_bf16 ? 2 : 4, o_es = out_is_bf16 ? 2 : 4, width = static_cast<uint64_t>(q_heads) * cache->head_dim;
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(scratch)) % 16 != 0 ||
         stride_q_row * q_es % 16 != 0 || stride_out_row * o_es % 16 != 0)
@@ -961,7 +962,7 @@ extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_row
     p.q_rows = q_rows; p.stride_q = stride_q_row; p.stride_out = stride_out_row; p.stride_page_table = stride_page_table;
     p.n_seqs = n_seqs; p.max_q_len = max_q_len; p.q_heads = q_heads; p.group = q_heads / cache->kv_heads;
     p.max_kv_len = max_kv_len; p.groups = plan.groups;
-    p.scale_log2 = scale * 1.44269504088896340736f * (cache->dtype == Q8MI_KV_E4M3 ? cache->k_scale : 1.0f);
+    p.scale_log2 = scale_log2;
     p.q_is_bf16 = q_is_bf16; p.out_is_bf16 = out_is_bf16;
     hipStream_t s = as_stream(stream);
     if (cache->dtype == Q8MI_KV_BF16) return launch_type<Q8MI_KV_BF16>(p, plan.waves_on_rows, s);

@@ -3,7 +3,9 @@
 // Q/K/V projections, head norms + rotation + cache append, attention over the paged cache, O, FFN, logits, sampling.
 //   attention  every attention output against a CPU double computation from the projections the device made
 //   tokens     every sampled token against a CPU sampler on the device's logits
-//   graph      the same loop with the step captured once and replayed: the same tokens
+//   graph      the same loop with the step captured once and replayed: the same tokens, also after larger calls have outgrown the
+//              scratch that the graph names
+//   refusals   what the operators answer to tensors that are too small or of another type
 // Prints one line per case; exit code 0 only if all pass.
 #include <algorithm>
 #include <cmath>
@@ -284,8 +286,52 @@ int main(int argc, char **argv) {
                 good = run.ok(run.b.replay_graph(), "replay");
             }
             if (good) got.push_back(run.token());
+            if (good && i == 4) {   // larger calls: their scratch takes the place of the one that the graph names
+                auto many = m.backend.tensor_f32(9 * kVocab, "logits"), us9 = m.backend.tensor_f32(9, "u");
+                auto toks = m.backend.argmax_buffer(9);
+                auto lens = m.backend.tensor_i32(40, "lens"), pages = m.backend.tensor_i32(40 * kWide, "pages");
+                auto rows = m.backend.tensor_f32(40 * kQ, "q"), out = m.backend.tensor_f32(40 * kQ, "out");
+                run.put(*many, std::vector<float>(9 * kVocab, 0.5f));
+                run.put(*us9, std::vector<float>(9, 0.5f));
+                run.put(*lens, std::vector<int32_t>(40, 9));
+                run.put(*pages, std::vector<int32_t>(40 * kWide, 1));
+                run.put(*rows, std::vector<float>(40 * kQ, 1.0f));
+                good = run.ok(m.backend.sample_rows(*many, 9, kVocab, kVocab, nullptr, nullptr, nullptr, nullptr, *us9, *toks), "large sample") &&
+                       run.ok(m.backend.paged_attention(*out, *rows, *run.cache, *pages, kWide, *lens, nullptr, 40, 40, 1, kHeads, kMaxKv, 0.1f, kQ, kQ),
+                              "large attention") &&
+                       run.ok(m.backend.synchronize(), "synchronize");
+            }
         }
         report("graph", good && got == eager, run.error);
+    }
+    {
+        Run run(m);
+        auto refused = [&](const qw3::DeviceStatus &st) { return !st.ok && st.message && *st.message; };
+        auto half = m.backend.tensor_bf16(kPrompt * kQ, "bf16");
+        auto append = [&](const qw3::DeviceTensor &q, const qw3::DeviceTensor &k, const qw3::DeviceWeight *n, const qw3::DeviceWeight *f,
+                          uint32_t rot, const qw3::DeviceTensor &slots, uint32_t tokens) {
+            return m.backend.qk_norm_rope_append(*run.qr, q, k, *run.v, n, m.kn.get(), kEps, f, rot, false, *run.pos, slots, tokens, kHeads,
+                                                 kQ, kDim, kKv, kKv, kQ, *run.cache);
+        };
+        auto attend = [&](const qw3::DeviceTensor &q, const qw3::DeviceTensor &table, const qw3::DeviceTensor &lens, uint32_t rows, uint32_t max_kv) {
+            return m.backend.paged_attention(*run.attn, q, *run.cache, table, kWide, lens, nullptr, 1, rows, 1, kHeads, max_kv, 1.0f, kQ, kQ);
+        };
+        auto sample = [&](const qw3::DeviceTensor &x, uint32_t batch, const qw3::DeviceTensor *k) {
+            return m.backend.sample_rows(x, batch, kVocab, kVocab, run.temp.get(), k, nullptr, nullptr, *run.u, *run.tok);
+        };
+        auto &q = *run.q, &k = *run.k;
+        const bool good =
+            refused(append(*half, k, nullptr, m.freqs.get(), kRot, *run.slots, 1)) && refused(append(q, *run.u, nullptr, m.freqs.get(), kRot, *run.slots, 1)) &&
+            refused(append(q, k, m.freqs.get(), m.freqs.get(), kRot, *run.slots, 1)) && refused(append(q, k, nullptr, m.qn.get(), kRot, *run.slots, 1)) &&
+            refused(append(q, k, nullptr, m.freqs.get(), 2 * kRot, *run.slots, 1)) && refused(append(q, k, nullptr, m.freqs.get(), kRot, *run.pos, 1)) &&
+            refused(append(q, k, nullptr, m.freqs.get(), kRot, *run.slots, kPrompt + 1)) && refused(append(q, k, nullptr, m.freqs.get(), kRot - 4, *run.slots, 1)) &&
+            refused(attend(*run.u, *run.table, *run.lens, 1, kMaxKv)) && refused(attend(q, *run.lens, *run.lens, 1, kMaxKv)) &&
+            refused(attend(q, *run.table, *run.u, 1, kMaxKv)) && refused(attend(q, *run.table, *run.lens, kPrompt + 1, kMaxKv)) &&
+            refused(attend(q, *run.table, *run.lens, 1, kMaxKv + 1)) && refused(sample(*run.u, 1, nullptr)) && refused(sample(*half, 1, nullptr)) &&
+            refused(sample(*run.logits, 2, nullptr)) && refused(sample(*run.logits, 1, run.u.get())) &&
+            !m.backend.kv_cache(qw3::DeviceTensorDType::F32, 4, 8, 2, 64, 1.0f, 1.0f, "x") &&
+            !m.backend.kv_cache(qw3::DeviceTensorDType::F16, 4, 8, 2, 96, 1.0f, 1.0f, "x");
+        report("refusals", good);
     }
     std::printf("%d failed\n", g_failed);
     std::fflush(stdout);

@@ -16,7 +16,7 @@ def test_decode_loop():
     print(r.stdout)
     print(r.stderr)
     assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
-    assert [line.split(":")[0] for line in r.stdout.splitlines() if line.startswith("PASS")] == ["PASS attention", "PASS tokens", "PASS graph"]
+    assert [line.split(":")[0] for line in r.stdout.splitlines() if line.startswith("PASS")] == ["PASS attention", "PASS tokens", "PASS graph", "PASS refusals"]
 
 
 def test_host_library_exports_the_operators():

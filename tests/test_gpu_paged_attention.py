@@ -166,6 +166,11 @@ def test_every_sequence_empty(gpu):
     run([0, 0], [1, 2], 4, 2, 256, seed=13)
 
 
+def test_no_tokens_at_all(gpu):
+    """A bound of no tokens: every row is zero, the cached tokens are not looked at."""
+    run([5, 0], [1, 2], 4, 2, 128, max_kv=0, seed=13)
+
+
 def test_bounds_of_the_host(gpu):
     """Rows beyond max_q_len and beyond q_rows are not computed, tokens from max_kv_len on not read."""
     c = Case([80, 60], [5, 2], 4, 2, 128, max_q=3, max_kv=64, seed=14, spare_rows=0)
