@@ -711,17 +711,13 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
     uint32_t n = 0;
     bool whole = false;
     if (cuts) {
-        u64 sum = 0, all;
-        bool full = false, more = false;
+        u64 sum = 0, all;   // candidates; from bit 32 on, chunks with more than two; from bit 48 on, with more than their list holds
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) {
-            full |= of[k] > kChunkCandidates;
-            more |= of[k] > 2;
-            sum += of[k];
-        }
+        for (uint32_t k = 0; k < 4; ++k) sum += of[k] + (of[k] > 2 ? 1ull << 32 : 0) + (of[k] > kChunkCandidates ? 1ull << 48 : 0);
         uint32_t at = static_cast<uint32_t>(sum_below<kRowThreads>(sum, s.part, all));
         n = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(all));   // loops to it are scalar
-        whole = __syncthreads_or(full) || n > kMaxCandidates;
+        const uint32_t flags = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(all >> 32));
+        whole = flags >> 16 != 0 || n > kMaxCandidates;
         if (!whole) {
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
@@ -730,7 +726,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
                 if (of[k] > 1) s.cand[at + 1] = two[k][1];
                 at += of[k];
             }
-            if (__syncthreads_or(more)) {   // the others: sixteen lanes a chunk, four chunks of theirs asked for at once
+            if (flags != 0) {   // the others: sixteen lanes a chunk, four chunks of theirs asked for at once
+                __syncthreads();
                 const uint32_t lane = threadIdx.x % 16;
 #pragma unroll 1
                 for (uint32_t c0 = t / 16; c0 < p.chunks; c0 += 4 * (kRowThreads / 16)) {
