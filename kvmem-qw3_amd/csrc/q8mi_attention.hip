@@ -763,7 +763,7 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
 template <uint32_t D, int KV, uint32_t kJoinThreads>
 __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const AttnParams p) {
     constexpr uint32_t kGroups = kJoinThreads / (D / 4);
-    __shared__ float tops[kJoinThreads / kWave], sums[kGroups];
+    __shared__ float2 sums[kGroups];
     __shared__ uint32_t units[kJoinThreads / kWave][2];
     __shared__ v4f parts[kGroups][D / 4];
     const uint32_t seq = blockIdx.x / p.max_q_len, token = blockIdx.x % p.max_q_len, head = blockIdx.y;
@@ -798,32 +798,37 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Attn
         const uint64_t slot = static_cast<uint64_t>(w0 + s) * 2 + (s == 0 && begin > w0 * share ? 1 : 0);
         return (slot << tile_log2) + (row & ((1u << tile_log2) - 1));
     };
-    float top = -INFINITY;
-    for (uint32_t s = threadIdx.x; s < n; s += kJoinThreads) top = fmaxf(top, p.part_ml[place(s)].x);
-    top = fmaxf(top, lane_xor<1>(top)); top = fmaxf(top, lane_xor<2>(top)); top = fmaxf(top, lane_xor<4>(top));
-    top = fmaxf(top, lane_xor<8>(top)); top = fmaxf(top, lane_xor<16>(top)); top = fmaxf(top, lane_xor<32>(top));
-    if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < kJoinThreads / kWave; ++i) top = fmaxf(top, tops[i]);
-    float sum = 0.0f;
+    // one pass: a piece's maximum and sum are asked for together with its outputs
+    float top = -INFINITY, sum = 0.0f;
     v4f out = v4f{0, 0, 0, 0};
 #pragma unroll 4
     for (uint32_t s = group; s < n; s += kGroups) {
         const uint64_t at = place(s);
         const float2 ml = p.part_ml[at];
-        const float f = ml.x == top ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
-        sum += f * ml.y;
-        out += f * *reinterpret_cast<const v4f *>(p.part + at * D + d * 4);
+        const v4f x = *reinterpret_cast<const v4f *>(p.part + at * D + d * 4);
+        const float all = fmaxf(top, ml.x);
+        const float keep = top == all ? 1.0f : __builtin_amdgcn_exp2f(top - all), f = ml.x == all ? 1.0f : __builtin_amdgcn_exp2f(ml.x - all);
+        sum = sum * keep + f * ml.y;
+        out = out * keep + f * x;
+        top = all;
     }
-    parts[group][d] = out;
-    if (d == 0) sums[group] = sum;
-    __syncthreads();
-    if (group != 0) return;
+    if constexpr (kGroups > 1) {
+        parts[group][d] = out;
+        if (d == 0) sums[group] = make_float2(top, sum);
+        __syncthreads();
+        if (group != 0) return;
+        float all = top;
 #pragma unroll
-    for (uint32_t i = 1; i < kGroups; ++i) {
-        sum += sums[i];
-        out += parts[i][d];
+        for (uint32_t i = 1; i < kGroups; ++i) all = fmaxf(all, sums[i].x);
+        const float keep = top == all ? 1.0f : __builtin_amdgcn_exp2f(top - all);
+        sum *= keep;
+        out *= keep;
+#pragma unroll
+        for (uint32_t i = 1; i < kGroups; ++i) {
+            const float f = sums[i].x == all ? 1.0f : __builtin_amdgcn_exp2f(sums[i].x - all);
+            sum += f * sums[i].y;
+            out += f * parts[i][d];
+        }
     }
     const float norm = (KV == Q8MI_KV_E4M3 ? p.cache.v_scale : 1.0f) / Operand<KV>::kWeightScale;
 #pragma unroll
