@@ -232,27 +232,33 @@ __device__ __forceinline__ v4f pick(const v4f (&v)[4], uint32_t u) {
 }
 __device__ __forceinline__ void unpack(v4f t, float (&v)[4]) { v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w; }
 
-// A workgroup's span of chunks, kAhead chunks in registers: asked for when the object is made, and the next ones before
-// those in hand are looked at.
+// A workgroup's span of chunks, kAhead chunks in registers and the next ones asked for before those in hand are looked at.
+// `early`: the first are asked for when the object is made, before it is known what the row wants of them.
 struct Span {
     const SampleParams &p;
     const float *x;
     uint32_t first, end;
+    bool early;
     v4f v[kAhead];
 
-    __device__ __forceinline__ Span(const SampleParams &params, const float *row) : p(params), x(row) {
+    __device__ __forceinline__ Span(const SampleParams &params, const float *row, bool at_once) : p(params), x(row), early(at_once) {
         first = blockIdx.x * p.span;
         end = first + p.span < p.chunks ? first + p.span : p.chunks;
 #pragma unroll
         for (uint32_t u = 0; u < kAhead; ++u) {
             v[u] = v4f{0, 0, 0, 0};
-            if (first + u < end) v[u] = load4(p, x, (first + u) * kChunk + threadIdx.x * 4);
+            if (early && first + u < end) v[u] = load4(p, x, (first + u) * kChunk + threadIdx.x * 4);
         }
     }
     // f(v, i, c) for every four logits v, from element i, that this thread has of the span's chunk c (counted from 0), of
-    // the chunks that want(c): only the first kAhead of the others are read
+    // the chunks that want(c); no others are read from here on
     template <typename F, typename W>
     __device__ __forceinline__ void walk(F f, W want) {
+        if (!early) {   // uniform
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u)
+                if (first + u < end && want(u)) v[u] = load4(p, x, (first + u) * kChunk + threadIdx.x * 4);
+        }
 #pragma unroll 1
         for (uint32_t c = first; c < end; c += kAhead) {
             v4f next[kAhead] = {};
@@ -292,7 +298,7 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 // ---- 1 ----------------------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kChunkThreads) void sample_best_kernel(const SampleParams p) {
     const uint32_t t = threadIdx.x, row = blockIdx.y;
-    Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
+    Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride, true);
     if (blockIdx.x < p.copies) {
         const uint64_t first = (static_cast<uint64_t>(row) * p.copies + blockIdx.x) * kBins;
         for (uint32_t b = t; b < kBins; b += kChunkThreads) {
@@ -388,7 +394,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
     __shared__ ChunkSpace out;
     __shared__ uint32_t found, tops[kChunkThreads / kWave];
     const uint32_t t = threadIdx.x, row = blockIdx.y;
-    Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
+    Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride, p.span == 1);
     open_space(out, span, p, row);
     // the row's largest key
     uint32_t top = 0;
@@ -563,7 +569,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_collect_kernel(const Sam
     __shared__ CutSpace space;
     __shared__ ChunkSpace out;
     const uint32_t t = threadIdx.x, row = blockIdx.y;
-    Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride);
+    Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride, p.span == 1);
     open_space(out, span, p, row);   // find_cut's barriers follow
     const uint32_t top = p.top[row];
     const Row r = row_of(p, row, top);
