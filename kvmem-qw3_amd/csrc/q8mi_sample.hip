@@ -28,7 +28,8 @@ constexpr uint32_t kChunk = 1024;                     // logits
 constexpr uint32_t kMaxChunks = kMaxVocab / kChunk;
 // Chunks of a workgroup: one while that leaves CUs idle, up to these where rows are many.  In launches 2 and 3 a span clears a
 // histogram and sends it off, or adds one up, once for all its chunks, while long spans leave the chip unevenly loaded by rows
-// of unlike settings (64 rows of 248320, spans of 4, 8, 16: 83, 71, 75 us); launch 1 holds nothing (spans of 2, 8: 2 us apart).
+// of unlike settings (64 rows of 248320 by top_p, spans of 4, 8, 12: 81, 77, 81 us); launch 1 holds nothing (spans of 2, 4: 1 us
+// apart).
 constexpr uint32_t kMostSpan = 8, kMostSpanOfBest = 2;
 constexpr uint32_t kGridWanted = 512;                 // spans above one begin at twice this many workgroups
 constexpr uint32_t kAhead = 4;                        // chunks that a workgroup of launches 1 to 3 loads at a time
@@ -311,10 +312,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_best_kernel(const Sample
         }
     }
     span.walk([&](const float (&v)[4], uint32_t, uint32_t c) {
-        uint32_t key = 0;
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) key = key_of(v[k]) > key ? key_of(v[k]) : key;
-        key = wave_max_u32(key);
+        const uint32_t key = wave_max_u32(key_of(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))));   // of a number and NaN, the number
         if (t % kWave == 0) p.best[(static_cast<uint64_t>(row) * p.chunks + span.first + c) * 4 + t / kWave] = key;
     });
 }
@@ -421,10 +419,11 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
                 p.cut[row] = cut;
                 p.listed[row] = 1;
             }
+            const float least_logit = logit_of(least);
             span.walk([&](const float (&v)[4], uint32_t i, uint32_t c) {
                 uint32_t mine = 0;
 #pragma unroll
-                for (uint32_t k = 0; k < 4; ++k) mine |= key_of(v[k]) >= least ? 1u << k : 0;
+                for (uint32_t k = 0; k < 4; ++k) mine |= v[k] >= least_logit ? 1u << k : 0;
                 collect(p, row, out, v, i, c, mine);
             }, [&](uint32_t c) { return out.best[c] >= least; });
             __syncthreads();
@@ -446,11 +445,12 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
         uint32_t least = 0;
         if (by_count && r.top_k <= 4 * p.chunks && 4 * p.chunks <= 16 * kWave)
             least = reached_by<16>([&](uint32_t c) { return p.best[static_cast<uint64_t>(row) * p.chunks * 4 + c]; }, 4 * p.chunks, r.top_k, found);
+        const float least_logit = least ? logit_of(least) : -INFINITY;
         u64 rest = 0;
         span.walk([&](const float (&v)[4], uint32_t, uint32_t) {
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) {
-                if (key_of(v[k]) < least) continue;
+                if (!(v[k] >= least_logit)) continue;
                 const double depth = depth_at(v[k], r);
                 if (!(depth < kReach)) continue;
                 const uint32_t b = bin_at(depth);
