@@ -2,9 +2,10 @@
 //
 //   out = sum_t p_t v_t,  p = softmax_t(scale * q . k_t),  t <= kv_len - rows + i
 //
-// One pass over the cache with a running maximum and sum per query row.  A workgroup takes a chunk of a sequence's tokens
-// for one key head and all the query rows that read it (rows of the sequence x query heads of the group, in tiles of 16 a
-// wave); the chunks' (maximum, sum, output) meet in a second small launch, chunk by chunk in order, so results repeat.
+// One pass over the cache with a running maximum and sum per query row.  An item is one key head of a sequence and a tile of the
+// query rows that read it (rows of the sequence x query heads of the group, 16 a wave); every workgroup takes an equal run of
+// all items' tokens, and the pieces' (maximum, sum, output) of an item that several share meet in a second small launch, in
+// order, so results repeat.
 //
 // A step is a tile of 32 tokens, held in LDS exactly as in memory, each row's 16-byte pieces permuted by an exclusive or
 // with the token so that the reads below meet different banks.  Tiles travel global -> LDS without passing through
@@ -17,6 +18,9 @@
 // Precision: cache elements are exact operands (bf16, or fp16 for fp16 and e4m3).  The fp32 side, q and the weights, is
 // split into operands that add up to it: three bf16 terms (all 24 bits), or two fp16 terms (22 bits) after scaling by a
 // power of two that keeps the second term clear of fp16's subnormals.  Sums are fp32 throughout.
+// Bound by HBM where a key head has few query rows (128 x 4096 tokens of fp16, 8 heads of 128: 2.1 GB in 324 us, 6.6 TB/s; one
+// sequence of 131072 tokens of bf16, 4 heads of 256: 537 MB in 92 us), by the matrix cores and VALUs in turn where it has many
+// (48 rows, 298 MB: 74 us), by latency where there is little to read (2000 tokens: 14 us for the two launches).
 #include "q8mi_kv.hpp"
 
 namespace q8mi {
@@ -226,8 +230,10 @@ struct Layout {
     static constexpr uint32_t kTileBytes = kTile * kRowBytes;
     static constexpr uint32_t kGroups = 4 / WR;
     static constexpr uint32_t kUnit = kGroups * kTile;                 // tokens of a step
-    // Waves that share a tile meet at barriers: a second stage hides what a load takes longer than a step.  Waves on tiles of
-    // their own are hidden by each other and by the second workgroup of the CU, which a second stage would not leave room for.
+    // Waves that share a tile meet at barriers, of which two stages need one a step instead of four (16 sequences of 8 rows, heads
+    // of 256: 91 -> 78 us, together with waves that only load).  Waves on tiles of their own are hidden by each other and by the
+    // other workgroups of the CU, for which a second stage leaves less room (heads of 64, 64 sequences of 4096 tokens: 90 and 85 us,
+    // one of 6000: 12.8 and 14.6).
     static constexpr uint32_t kStages = WR > 1 && kGroups * 4 * kTileBytes <= 64 * 1024 ? 2 : 1;
     static_assert(WR < 4 || kStages == 2, "a wave without rows passes no barrier but the first of a step");
     static constexpr uint32_t kTiles = 0;                              // [group][stage][K, V][tile]
