@@ -395,6 +395,7 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
     __shared__ ChunkSpace out;
     __shared__ uint32_t found, tops[kChunkThreads / kWave];
     const uint32_t t = threadIdx.x, row = blockIdx.y;
+    Row r = p.rows[row];
     Span span(p, p.logits + static_cast<uint64_t>(row) * p.stride, p.span == 1);
     open_space(out, span, p, row);
     // the row's largest key
@@ -409,8 +410,8 @@ __global__ __launch_bounds__(kChunkThreads) void sample_weigh_kernel(const Sampl
 #pragma unroll
     for (uint32_t w = 0; w < kChunkThreads / kWave; ++w) top = tops[w] > top ? tops[w] : top;
     if (blockIdx.x == 0 && t == 0) p.top[row] = top;
-    const Row r = row_of(p, row, top);
-    if (top == 0 || r.greedy) return;
+    r.max = logit_of(top);
+    if ((top == 0) | (r.greedy != 0)) return;
     if (r.top_k != 0 && r.top_k <= p.chunks) {
         auto chunk = [&](uint32_t c) { return best_of(p, row, c); };
         const uint32_t least = p.chunks <= 4 * kWave ? reached_by<4>(chunk, p.chunks, r.top_k, found)
@@ -691,12 +692,14 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
     }
     const Cut cut = p.cut[row];
     float u = p.uniform[row];
-    if (top == 0) {
-        if (t == 0) p.out[row] = q8mi_argmax_pair{-INFINITY, -1};
-        return;
-    }
     const Row r = row_of(p, row, top);
-    if (r.greedy) {   // the first chunk with that key, its first such element
+    const uint32_t is_listed = p.listed[row];
+    if ((top == 0) | (r.greedy != 0)) {   // both are asked for before either is looked at
+        if (top == 0) {
+            if (t == 0) p.out[row] = q8mi_argmax_pair{-INFINITY, -1};
+            return;
+        }
+        // the first chunk with that key, its first such element
         if (t == 0) s.at = kMaxChunks;
         __syncthreads();
         for (uint32_t c = t; c < p.chunks; c += kRowThreads)
@@ -715,7 +718,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
     }
     make_roots(s.roots);   // sum_below's barriers follow
     const bool cuts = r.top_k != 0 || r.top_p < 1.0;
-    const bool listed = cuts && p.listed[row] != 0;
+    const bool listed = cuts && is_listed != 0;
     // the candidates of the chunks, one list after the other; `whole`: more than their places hold
     uint32_t n = 0;
     bool whole = false;
