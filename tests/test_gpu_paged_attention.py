@@ -413,3 +413,29 @@ def test_two_calls_at_once(gpu):
     b.synchronize()
     c.check()
     d.check()
+
+
+def test_graphs_share_a_scratch(gpu):
+    """Two captured calls on one scratch, replayed in turn on one stream."""
+    s = hip.Stream()
+    c, d = Case([3000, 100], [1, 1], 6, 1, 256, seed=90), Case([500, 1800], [4, 2], 6, 1, 256, seed=91)
+    big = max(c, d, key=lambda x: x.scratch_bytes)
+    c.scratch = d.scratch = big.scratch
+    c.scratch_bytes = d.scratch_bytes = big.scratch_bytes
+    graphs = []
+    for case in (c, d):
+        case.launch(s.handle)
+        s.synchronize()
+        g = hip.Graph(s)
+        with g:
+            case.launch(s.handle)
+        graphs.append(g)
+    for _ in range(3):
+        for case in (c, d):
+            case.dout.fill(0x5a)
+        hip.synchronize()
+        for g in graphs:
+            g.launch()
+        s.synchronize()
+        c.check()
+        d.check()

@@ -229,3 +229,34 @@ def test_two_calls_at_once(gpu):
 def test_many_rows(gpu):
     """A row each for many sequences, several chunks to a workgroup."""
     run(logits(300, 9001, 30), temperature=0.8, top_k=[5, 0, 700] * 100, top_p=[0.9, 0.95, 0.8] * 100, seed=31)
+
+
+@pytest.mark.parametrize("vocab,k", [(32000, 40), (32003, 64), (32003, 65), (2000, 4), (1025, 3), (131072, 128), (65536, 128), (65536, 129)])
+def test_counts_about_the_chunks(gpu, vocab, k):
+    """top_k about the number of chunks of a row, and about twice that."""
+    run(logits(4, vocab, vocab + k), temperature=0.9, top_k=[k - 1, k, k + 1, k], top_p=[0.95, 1.0, 0.9, 0.5], seed=k)
+
+
+def test_graphs_share_a_scratch(gpu):
+    """Two captured calls on one scratch, replayed in turn on one stream."""
+    s = hip.Stream()
+    c, d = Case(logits(3, 40000, 40), top_k=30, seed=41), Case(logits(3, 40000, 42), temperature=0.7, top_p=0.9, seed=43)
+    d.scratch = c.scratch
+    graphs = []
+    for case in (c, d):
+        case.launch(s.handle)
+        g = hip.Graph(s)
+        with g:
+            case.launch(s.handle)
+        graphs.append(g)
+    for rep in range(3):
+        for case in (c, d):
+            case.u = np.random.default_rng(50 + rep).random(3).astype(np.float32)
+            case.dev[5].upload(case.u)
+            case.out.fill(0xff)
+        hip.synchronize()
+        for g in graphs:
+            g.launch()
+        s.synchronize()
+        c.check()
+        d.check()
