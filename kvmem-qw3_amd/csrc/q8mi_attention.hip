@@ -257,6 +257,7 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
     extern __shared__ __align__(16) uint8_t lds[];
     int32_t *pages = reinterpret_cast<int32_t *>(lds + L::kPages);
     float *kept_scores = reinterpret_cast<float *>(lds + L::kScores);
+    __shared__ uint32_t bad_pages[kAttnThreads / kWave];
 
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -368,7 +369,13 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
         }
         // Everything requested so far is here before the first tile is asked for: a later wait for it would wait for the tile.
         __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
-        any_bad = __syncthreads_or(bad);
+        const bool wave_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+        if (lane == 0) bad_pages[wave] = wave_bad;
+        __syncthreads();
+        any_bad = false;
+#pragma unroll
+        for (uint32_t w = 0; w < kAttnThreads / kWave; ++w) any_bad |= bad_pages[w] != 0;
+        any_bad = __builtin_amdgcn_readfirstlane(any_bad);
     };
     if (piece > 1) __syncthreads();   // the piece before has left LDS
     load_pages();
@@ -729,14 +736,17 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
         const float f = m == all ? 1.0f : __builtin_amdgcn_exp2f(m - all);
         m = all;
         l = sum;
+        if (live) {   // few of the tile's rows may be
 #pragma unroll
-        for (uint32_t d = 0; d < kOuts; ++d) {
-            const v4f x = o[d] * f;
-            *reinterpret_cast<v4f *>(mo + (wave * kRowTile + lane % 16) * (D + 4) + d * 16 + g * 4) = x;
+            for (uint32_t d = 0; d < kOuts; ++d) {
+                const v4f x = o[d] * f;
+                *reinterpret_cast<v4f *>(mo + (wave * kRowTile + lane % 16) * (D + 4) + d * 16 + g * 4) = x;
+            }
         }
         __syncthreads();
         // every wave adds a share of the columns of its rows
         constexpr uint32_t kShare = kOuts / L::kGroups;
+        if (live) {
 #pragma unroll
         for (uint32_t u = 0; u < kShare; ++u) {
             const uint32_t d = wg * kShare + u;
@@ -745,6 +755,7 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
             for (uint32_t k = 0; k < L::kGroups; ++k)
                 x += *reinterpret_cast<const v4f *>(mo + ((k * WR + wr) * kRowTile + lane % 16) * (D + 4) + d * 16 + g * 4);
             o[u] = x;
+        }
         }
     }
     constexpr uint32_t kOwn = kOuts / L::kGroups;
