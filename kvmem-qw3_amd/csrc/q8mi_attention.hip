@@ -17,7 +17,8 @@
 //            same row as its weights: rescaling by a new maximum is one factor per lane.
 // Precision: cache elements are exact operands (bf16, or fp16 for fp16 and e4m3).  The fp32 side, q and the weights, is
 // split into operands that add up to it: three bf16 terms (all 24 bits), or two fp16 terms (22 bits) after scaling by a
-// power of two that keeps the second term clear of fp16's subnormals.  Sums are fp32 throughout.
+// power of two that keeps the second term clear of fp16's subnormals (of weights from 2^-17 of the largest on; smaller ones are
+// off by up to 2^-39 of it).  Sums are fp32 throughout.
 // Bound by HBM where a key head has few query rows (128 x 4096 tokens of fp16, 8 heads of 128: 2.1 GB in 324 us, 6.6 TB/s; one
 // sequence of 131072 tokens of bf16, 4 heads of 256: 537 MB in 92 us), by the matrix cores and VALUs in turn where it has many
 // (48 rows, 298 MB: 74 us), by latency where there is little to read (2000 tokens: 14 us for the two launches).
@@ -161,7 +162,7 @@ struct Operand<Q8MI_KV_F16> {
     using Raw = v8s;
     static __device__ __forceinline__ v8s operand(Raw x) { return x; }
     static constexpr int kTerms = 2;
-    static constexpr float kWeightScale = 16384.0f;   // weights are at most 1: the second term ends at 2^-38
+    static constexpr float kWeightScale = 16384.0f;   // weights are at most 1: the terms' last step is 2^-24 / 2^14
     static __device__ __forceinline__ v4f mma(v8s a, v8s b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
     }

@@ -3,7 +3,13 @@
 Bounds (u = 2^-24): a score is a sum of D products and a few more roundings, off by at most d = (6 sqrt(D) + 8) u of
 scale * sum |q k| (probabilistic bound of D random roundings); every weight then changes by a factor within exp(+-d), their sum
 likewise, the exponential and the split of a weight over matrix operands add 8 u, and n weights times values are added with
-6 sqrt(n) u: below (2 d size + (6 sqrt(n) + 16) u) of sum p |v|.  bf16 outputs add half a step."""
+6 sqrt(n) u: below (2 d size + (6 sqrt(n) + 16) u) of sum p |v|.  bf16 outputs add half a step.
+
+fp16 and e4m3 caches: a weight, at most 1 before the division by the sum (which is at least 1), enters the products times 2^14
+as two fp16 numbers.  Its first term is off by half a step, at most 2^-11 of itself, and the second, the rest, by 2^-11 of that, 2^-22
+= 4 u of the weight (part of the 8 u above), as long as their steps follow their size; fp16's smallest step is 2^-24, so that below
+it a weight is off by half of that, 2^-25 / 2^14 = 2^-39 of the row's largest: where the tokens of large weight hold zeros, their sum
+2^-39 sum |v| is what counts."""
 import numpy as np
 import pytest
 
@@ -93,6 +99,8 @@ class Case:
                 want, mag, size = R.attention(q, self.k[s][ts], self.v[s][ts], np.float64(np.float32(self.scale)), len(ts))
                 u = R.U
                 tol = (2 * (6 * self.dim ** 0.5 + 8) * u * size[:, None] + (6 * max(1, len(ts)) ** 0.5 + 16) * u) * mag
+                if self.kind != "bf16" and ts:
+                    tol = tol + 2.0 ** -39 * np.abs(self.v[s][ts]).sum(0).repeat(self.heads // self.kv_heads, 0)
                 if self.out_act == "bf16":
                     tol = tol + R.HALF_STEP["bf16"] * (np.abs(want) + tol)
                 g = R.act_value(got[r, :self.width], self.out_act).reshape(self.heads, self.dim)
@@ -439,3 +447,20 @@ def test_graphs_share_a_scratch(gpu):
         s.synchronize()
         c.check()
         d.check()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "e4m3"])
+def test_small_weights(gpu, kind):
+    """Outputs that tokens of very small weight make alone: those of large weight hold zeros there."""
+    c = Case([300], [1], 4, 4, 64, kind, seed=100, q_scale=8.0)
+    for t in range(300):
+        at = c.pools.at(c.table[0, t // 16], t % 16)
+        q = R.act_value(c.q[0, :c.width], c.act).reshape(4, 64)
+        for h in range(4):
+            if c.scale * (c.k[0][:, h] @ q[h]).max() - c.scale * c.k[0][t, h] @ q[h] < 15:
+                c.pools.host["v"][at[h, ::2]] = 0
+                c.v[0][t, h, ::2] = 0
+    c.pools.upload()
+    c.launch()
+    hip.synchronize()
+    c.check()
