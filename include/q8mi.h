@@ -341,8 +341,8 @@ int q8mi_qk_norm_rope_append(const void *q, const void *k, const void *v, void *
  * and number of rows asks the runtime for its LDS: make it outside a graph capture.
  * scratch: q8mi_paged_attention_scratch_bytes() device bytes, 16-byte aligned; calls that may overlap need
  * one each.  Nothing in it needs clearing.  Results repeat bit by bit.  Q8MI_REJECTED: q_heads not a multiple of
- * kv_heads or above 65535, the bounds above, q, out or their strides in bytes not multiples of 16, a scale that
- * is not finite or beyond 2^127, a pool of 64 GiB and more, 2^22 rows and more. */
+ * kv_heads or above 65535, the bounds above, out the same as q, q, out or their strides in bytes not multiples
+ * of 16, a scale that is not finite or beyond 2^127, a pool of 64 GiB and more, 2^22 rows and more. */
 size_t q8mi_paged_attention_scratch_bytes(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads,
                                           uint32_t head_dim, uint32_t max_kv_len);
 int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_rows, uint32_t stride_q_row,

@@ -949,6 +949,7 @@ extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_row
     if (n_seqs == 0 || q_rows == 0) return Q8MI_OK;
     if (q == nullptr || out == nullptr || page_table == nullptr || kv_lens == nullptr || scratch == nullptr)
         return fail(Q8MI_REJECTED, "%s: null pointer", what);
+    if (out == q) return fail(Q8MI_REJECTED, "%s: out is q", what);   // a row's outputs are stored while others still read it
     if (q_heads == 0 || q_heads > 65535 || q_heads % cache->kv_heads != 0)
         return fail(Q8MI_REJECTED, "%s: %u query heads over %u", what, q_heads, cache->kv_heads);
     if (max_q_len == 0 || max_q_len > kMaxRows) return fail(Q8MI_REJECTED, "%s: %u rows a sequence (1..%u)", what, max_q_len, kMaxRows);

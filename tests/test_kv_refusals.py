@@ -32,7 +32,7 @@ def append(c=None, **changed):
 
 
 def attend(c=None, **changed):
-    a = dict(q=P, q_is_bf16=0, q_rows=4, sq=512, cache=cache() if c is None else c, table=P, stable=4, lens=P, starts=None, n=2, new=2, heads=4,
+    a = dict(q=2 * P, q_is_bf16=0, q_rows=4, sq=512, cache=cache() if c is None else c, table=P, stable=4, lens=P, starts=None, n=2, new=2, heads=4,
              max_kv=64, scale=1.0, out=P, out_is_bf16=0, so=512, scratch=P)
     a.update(changed)
     return q8mi.lib().q8mi_paged_attention(*a.values(), None)
@@ -68,7 +68,7 @@ def test_append(bad):
 @pytest.mark.parametrize("bad", [dict(q=0), dict(out=0), dict(table=0), dict(lens=0), dict(scratch=0), dict(heads=0), dict(heads=5),
                                  dict(new=0), dict(new=17), dict(max_kv=65), dict(scale=NAN), dict(scale=INF), dict(q=P + 4),
                                  dict(out=P + 8), dict(scratch=P + 4), dict(sq=514), dict(so=510), dict(sq=256), dict(so=508),
-                                 dict(q_is_bf16=1, sq=516), dict(n=1 << 22), dict(scale=3e38), dict(heads=65538, sq=1 << 24, so=1 << 24)], ids=str)
+                                 dict(q_is_bf16=1, sq=516), dict(n=1 << 22), dict(scale=3e38), dict(out=2 * P), dict(heads=65538, sq=1 << 24, so=1 << 24)], ids=str)
 def test_attention(bad):
     assert attend(**bad) == q8mi.REJECTED
     assert q8mi.last_error()
