@@ -41,6 +41,18 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
+// Division of numbers below 2^31 by one that the host knows: mulhi(t, magic) >> shift; magic 0: by 1.
+struct Divisor {
+    uint32_t magic, shift;
+};
+__device__ __forceinline__ uint32_t operator/(uint32_t t, Divisor d) { return d.magic ? __umulhi(t, d.magic) >> d.shift : t; }
+Divisor divisor(uint32_t by) {   // the error of magic, below 2^-31 relative, stays below 1 for every such t
+    if (by == 1) return {0, 0};
+    uint32_t bits = 1;
+    while ((1u << bits) < by) ++bits;
+    return {static_cast<uint32_t>((1ull << (31 + bits)) / by + 1), bits - 1};
+}
+
 struct AttnParams {
     const void *q;
     void *out;
@@ -51,7 +63,7 @@ struct AttnParams {
     uint32_t q_rows, stride_q, stride_out, stride_page_table;
     uint32_t n_seqs, max_q_len, q_heads, group, max_kv_len;
     uint32_t groups;   // workgroups
-    uint32_t page_magic, page_shift;   // t / page_size = mulhi(t, page_magic) >> page_shift; magic 0: page_size 1
+    Divisor by_page, by_group, by_groups;   // page_size, group, groups
     uint32_t unit_page, unit_token;    // cache strides in units of 16 bytes
     uint32_t waves_log2;               // waves side by side on rows: tiles of 16 << waves_log2 rows, units of 128 >> it tokens
     int whole_loads;                   // the tokens of one transfer instruction never straddle pages
@@ -97,7 +109,7 @@ __device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
 }
 
 __device__ __forceinline__ uint32_t page_of(const AttnParams &p, uint32_t t) {
-    return p.page_magic ? __umulhi(t, p.page_magic) >> p.page_shift : t;
+    return t / p.by_page;
 }
 
 __device__ __forceinline__ void store_out(const AttnParams &p, uint64_t at, float v) {
@@ -287,7 +299,7 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
             if (at == 0) break;
         }
     }
-    const uint32_t share = __builtin_amdgcn_readfirstlane((total + p.groups - 1) / p.groups);
+    const uint32_t share = __builtin_amdgcn_readfirstlane((total + p.groups - 1) / p.by_groups);
     uint32_t begin = blockIdx.x * share;
     if (begin >= total) return;
     const uint32_t end = __builtin_amdgcn_readfirstlane(begin + share < total ? begin + share : total);
@@ -337,7 +349,7 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
 
     // this lane's query row
     const uint32_t row = row0 + wr * kRowTile + lane % 16;
-    const uint32_t token = row / p.group, head = kv_head * p.group + row % p.group;
+    const uint32_t token = row / p.by_group, head = kv_head * p.group + row - token * p.group;
     const int64_t q_row = rows.start + token;
     const bool live = row < n_rows && q_row >= 0 && q_row < p.q_rows;
     const int64_t last64 = rows.kv_len - rows.count + token;                   // the last token it sees
@@ -806,10 +818,10 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Attn
 #pragma unroll
         for (uint32_t i = 0; i < kJoinThreads / kWave; ++i) { total += units[i][0]; before += units[i][1]; }
     }
-    const uint32_t share = (total + p.groups - 1) / p.groups;
-    const uint32_t tile_log2 = 4 + p.waves_log2, row = token * p.group + head % p.group, tile = row >> tile_log2;
+    const uint32_t share = (total + p.groups - 1) / p.by_groups, kv_head = head / p.by_group;
+    const uint32_t tile_log2 = 4 + p.waves_log2, row = token * p.group + head - kv_head * p.group, tile = row >> tile_log2;
     const uint32_t tiles = (rows.used * p.group + (1u << tile_log2) - 1) >> tile_log2, item_units = units_of_item(p.waves_log2, rows);
-    const uint32_t begin = before + (head / p.group * tiles + tile) * item_units, end = begin + item_units;
+    const uint32_t begin = before + (kv_head * tiles + tile) * item_units, end = begin + item_units;
     const uint32_t w0 = begin / share, n = (end - 1) / share - w0 + 1;   // the workgroups that share the item
     if (n == 1) return;
     auto place = [&](uint32_t s) -> uint64_t {   // of the row in piece s
@@ -905,6 +917,7 @@ int launch_waves(AttnParams &p, hipStream_t s) {
     p.waves_log2 = WR == 1 ? 0 : WR == 2 ? 1 : 2;
     const uint32_t resident = kChipCus * L::kResident;
     if (p.groups > resident) p.groups = resident;
+    p.by_groups = divisor(p.groups);
     attention_kernel<D, KV, WR><<<p.groups, kAttnThreads, L::kBytes, s>>>(p);
     if (p.max_kv_len > L::kUnit) {
         const dim3 rows(p.n_seqs * p.max_q_len, p.q_heads);
@@ -974,17 +987,13 @@ extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_row
         return fail(Q8MI_REJECTED, "%s: a pool of 64 GiB and more", what);
     AttnParams p{};
     p.unit_page = static_cast<uint32_t>(unit_page); p.unit_token = static_cast<uint32_t>(unit_token);
-    if (cache->page_size > 1) {   // exact for every t below 2^31
-        uint32_t bits = 1;
-        while ((1u << bits) < cache->page_size) ++bits;
-        p.page_magic = static_cast<uint32_t>((1ull << (31 + bits)) / cache->page_size + 1);
-        p.page_shift = bits - 1;
-    }
+    p.by_page = divisor(cache->page_size);
     p.q = q; p.out = out; p.page_table = page_table; p.kv_lens = kv_lens; p.q_starts = q_starts; p.cache = *cache;
     p.part = static_cast<float *>(scratch);
     p.part_ml = reinterpret_cast<float2 *>(p.part + partial_rows(plan) * cache->head_dim);
     p.q_rows = q_rows; p.stride_q = stride_q_row; p.stride_out = stride_out_row; p.stride_page_table = stride_page_table;
     p.n_seqs = n_seqs; p.max_q_len = max_q_len; p.q_heads = q_heads; p.group = q_heads / cache->kv_heads;
+    p.by_group = divisor(p.group);
     p.max_kv_len = max_kv_len; p.groups = plan.groups;
     p.scale_log2 = scale_log2;
     p.q_is_bf16 = q_is_bf16; p.out_is_bf16 = out_is_bf16;
