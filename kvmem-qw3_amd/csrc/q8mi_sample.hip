@@ -967,7 +967,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(const SamplePa
             (void)sum_below<kRowThreads>(within, s.part, all);
             kept = all < kept ? static_cast<uint32_t>(all) : kept;
         }
-        last = s.cand[kept - 1];   // each cut keeps a candidate: the step before which it falls short holds it
+        // Each cut that falls within reach keeps a candidate: the step before which it falls short holds it.  There are none where
+        // top_k wants more logits than lie within reach, and nothing else cuts: all of those stay.
+        last = kept != 0 ? s.cand[kept - 1] : 0;
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k)
             if (4 * t + k < kept && w[k] != 0 && depth[k] <= r.deepest)
