@@ -12,7 +12,7 @@ def within(z, temperature):
     return ((z.max(1, keepdims=True) - z) / temperature < 30).sum(1)
 
 
-@pytest.mark.parametrize("vocab,k,temperature", [(100000, 400, 0.3), (248320, 1000, 0.3), (3000, 200, 0.1), (32003, 129, 0.05), (1 << 20, 1025, 0.2)])
+@pytest.mark.parametrize("vocab,k,temperature", [(100000, 400, 0.3), (248320, 1000, 0.3), (3000, 200, 0.1), (32003, 129, 0.05), (300000, 1172, 0.2)])
 def test_fewer_within_reach_than_top_k(gpu, vocab, k, temperature):
     z = logits(6, vocab, vocab)
     assert (within(z, temperature) < k).all()
