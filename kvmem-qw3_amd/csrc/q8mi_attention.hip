@@ -876,19 +876,23 @@ constexpr uint32_t kFewUnits = 192;
 struct Plan {
     uint32_t waves_on_rows, groups;
 };
+uint32_t resident_groups(uint32_t head_dim) { return kChipCus * (head_dim == 64 ? 3 : 2); }
+uint64_t row_tiles(uint64_t rows, uint32_t waves) { return (rows + kRowTile * waves - 1) / (kRowTile * waves); }
+uint64_t token_units(uint32_t max_kv_len, uint32_t waves) {
+    const uint64_t unit = kTile * 4 / waves;
+    return max_kv_len ? (max_kv_len + unit - 1) / unit : 1;
+}
 Plan plan_of(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_kv_len,
              uint64_t *units = nullptr) {
     Plan r;
     const uint32_t rows = max_q_len * (kv_heads ? q_heads / kv_heads : 0);
     r.waves_on_rows = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     auto units_by = [&](uint32_t waves) {
-        const uint64_t tiles = (rows + kRowTile * waves - 1) / (kRowTile * waves);
-        const uint32_t unit = kTile * 4 / waves;
-        return n_seqs * static_cast<uint64_t>(kv_heads) * tiles * (max_kv_len ? (max_kv_len + unit - 1) / unit : 1);
+        return n_seqs * static_cast<uint64_t>(kv_heads) * row_tiles(rows, waves) * token_units(max_kv_len, waves);
     };
     if (units_by(4) <= kFewUnits) r.waves_on_rows = 4;
     const uint64_t most = units_by(r.waves_on_rows);
-    const uint32_t resident = kChipCus * (head_dim == 64 ? 3 : 2);
+    const uint32_t resident = resident_groups(head_dim);
     r.groups = static_cast<uint32_t>(most < resident ? most : resident);
     if (units) *units = most;
     return r;
@@ -941,6 +945,22 @@ int launch_type(AttnParams &p, uint32_t waves_on_rows, hipStream_t s) {
 
 uint64_t partial_rows(const Plan &plan) { return 2ull * plan.groups * plan.waves_on_rows * kRowTile; }
 
+// No call of these heads with no more sequences, rows and tokens takes more partial rows.  A smaller call may take more than the
+// largest one does: below kFewUnits a workgroup's tile has four waves of rows, and a wave for each of them costs as many workgroups.
+// So every arrangement that a smaller call can get counts, with the most units that it can have.
+uint64_t most_partial_rows(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_kv_len) {
+    const uint64_t rows = static_cast<uint64_t>(max_q_len) * (kv_heads ? q_heads / kv_heads : 0);
+    const uint64_t resident = resident_groups(head_dim), items = static_cast<uint64_t>(n_seqs) * kv_heads;
+    auto partial = [&](uint32_t waves, uint64_t most_rows, uint64_t most_groups) {
+        const uint64_t units = items * row_tiles(most_rows < rows ? most_rows : rows, waves) * token_units(max_kv_len, waves);
+        return 2 * (units < most_groups ? units : most_groups) * waves * kRowTile;
+    };
+    uint64_t most = partial(4, rows, rows > 32 ? resident : kFewUnits);
+    if (const uint64_t one = partial(1, 16, resident); one > most) most = one;
+    if (const uint64_t two = rows > 16 ? partial(2, 32, resident) : 0; two > most) most = two;
+    return most;
+}
+
 }  // namespace
 }  // namespace q8mi
 
@@ -948,8 +968,7 @@ using namespace q8mi;
 
 extern "C" size_t q8mi_paged_attention_scratch_bytes(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads,
                                                      uint32_t head_dim, uint32_t max_kv_len) {
-    const Plan plan = plan_of(n_seqs, max_q_len, q_heads, kv_heads, head_dim, max_kv_len);
-    return 16 + partial_rows(plan) * (head_dim + 2) * sizeof(float);
+    return 16 + most_partial_rows(n_seqs, max_q_len, q_heads, kv_heads, head_dim, max_kv_len) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_rows, uint32_t stride_q_row,
