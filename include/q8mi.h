@@ -369,8 +369,8 @@ int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_rows, uint32_t
  * drawn either; +inf logits share the whole mass.  uniform is clamped to [0, 1), NaN counts as 0.
  *   out[j] = {the token's logit, the token}: what q8mi_get_row_from_argmax reads; {-inf, -1} when every
  *            logit of the row is NaN or -inf.
- * vocab: 1 .. 2^20, batch up to 65535.  scratch: q8mi_sample_scratch_bytes() device bytes, 16-byte aligned; calls that may overlap
- * need one each, nothing in it needs clearing. */
+ * vocab: 1 .. 2^20, batch up to 65535.  scratch: q8mi_sample_scratch_bytes() device bytes, 16-byte aligned, which are enough for
+ * every call with no larger batch and vocab; calls that may overlap need one each, nothing in it needs clearing. */
 size_t q8mi_sample_scratch_bytes(uint32_t batch, uint32_t vocab);
 int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, uint32_t stride, const float *temperature,
                 const int32_t *top_k, const float *top_p, const float *min_p, const float *uniform,

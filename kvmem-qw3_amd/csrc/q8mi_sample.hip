@@ -1022,9 +1022,11 @@ uint32_t copies_of(uint32_t batch, uint32_t vocab) {
     const uint32_t spans = chunks_of(vocab) / span_of(batch, vocab, kMostSpan), copies = spans / kSpansOfCopy;
     return copies < 1 ? 1 : copies > kMostCopies ? kMostCopies : copies;
 }
-// Bytes of a row: best, chunk_mass, bin_mass, candidates, cut, rows, bin_count, n_candidates, top, listed.
-uint64_t row_bytes(uint32_t batch, uint32_t vocab) {
-    const uint64_t chunks = chunks_of(vocab), bins = kBins * copies_of(batch, vocab);
+// Bytes of a row: best, chunk_mass, bin_mass, candidates, cut, rows, bin_count, n_candidates, top, listed.  With the most copies
+// that a row of such a vocabulary can have, those of a single row: fewer rows may have more copies than many, and a scratch for
+// many must serve them.
+uint64_t row_bytes(uint32_t vocab) {
+    const uint64_t chunks = chunks_of(vocab), bins = kBins * copies_of(1, vocab);
     return 16 * chunks + 8 * (chunks + bins + chunks * kChunkCandidates) + sizeof(Cut) + sizeof(Row) + 4 * (bins + chunks + 2);
 }
 
@@ -1034,7 +1036,7 @@ uint64_t row_bytes(uint32_t batch, uint32_t vocab) {
 using namespace q8mi;
 
 extern "C" size_t q8mi_sample_scratch_bytes(uint32_t batch, uint32_t vocab) {
-    return 16 + batch * row_bytes(batch, vocab);
+    return 16 + batch * row_bytes(vocab);
 }
 
 extern "C" int q8mi_sample(const float *logits, uint32_t batch, uint32_t vocab, uint32_t stride, const float *temperature,

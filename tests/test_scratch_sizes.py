@@ -1,4 +1,4 @@
-"""The scratch sizes of the paged attention: what the largest call needs is enough for every smaller one.  No GPU needed."""
+"""The scratch sizes of the paged attention and the sampler: what the largest call needs is enough for every smaller one.  No GPU needed."""
 import itertools
 
 import pytest
@@ -33,3 +33,19 @@ def test_attention_stays_moderate():
     """No more than what 768 workgroups of four waves of rows leave, whatever the bounds."""
     assert attention(1 << 16, 16, (1 << 31) - 1, (80, 1, 64)) <= 16 + 2 * 768 * 64 * 66 * 4
     assert attention(128, 1, 131072, (24, 4, 256)) <= 16 + 2 * 192 * 64 * 258 * 4
+
+
+def sampling(batch, vocab):
+    return q8mi.lib().q8mi_sample_scratch_bytes(batch, vocab)
+
+
+@pytest.mark.parametrize("vocab", [1, 1000, 1024, 1025, 15360, 15361, 32000, 50257, 61440, 65536, 151936, 248320, 1 << 20])
+def test_sampling_grows_with_the_batch(vocab):
+    sizes = [sampling(b, vocab) for b in list(range(1, 600)) + [1000, 4096, 65535]]
+    assert sizes == sorted(sizes)
+
+
+@pytest.mark.parametrize("batch", [1, 2, 7, 16, 17, 64, 300, 1000, 65535])
+def test_sampling_grows_with_the_vocabulary(batch):
+    sizes = [sampling(batch, v) for v in range(1, (1 << 20) + 1, 511)] + [sampling(batch, 1 << 20)]
+    assert sizes == sorted(sizes)
