@@ -337,8 +337,8 @@ int q8mi_qk_norm_rope_append(const void *q, const void *k, const void *v, void *
  * the host gives their bounds: n_seqs, q_rows (rows of q and out), max_q_len (1..16) and max_kv_len (at most
  * stride_page_table * page_size).  Tokens from max_kv_len on are not read, rows of a sequence from
  * max_q_len on and rows from q_rows on not computed, and a page id outside the pool hides its tokens.  A row
- * of q must not belong to two sequences, and out must not overlap q.  The first call of a head_dim, cache type
- * and number of rows asks the runtime for its LDS: make it outside a graph capture.
+ * of q must not belong to two sequences, and out must not overlap q.  The first call of a head_dim and cache
+ * type on a device asks the runtime for LDS, for calls of all sizes: make it outside a graph capture.
  * scratch: q8mi_paged_attention_scratch_bytes() device bytes, 16-byte aligned, which are enough for every call of the
  * same q_heads, kv_heads and head_dim whose n_seqs, max_q_len and max_kv_len are no larger; calls that may overlap need
  * one each.  Nothing in it needs clearing.  Results repeat bit by bit.  Q8MI_REJECTED: q_heads not a multiple of

@@ -22,6 +22,8 @@
 // Bound by HBM where a key head has few query rows (128 x 4096 tokens of fp16, 8 heads of 128: 2.1 GB in 324 us, 6.6 TB/s; one
 // sequence of 131072 tokens of bf16, 4 heads of 256: 537 MB in 92 us), by the matrix cores and VALUs in turn where it has many
 // (48 rows, 298 MB: 74 us), by latency where there is little to read (2000 tokens: 14 us for the two launches).
+#include <atomic>
+
 #include "q8mi_kv.hpp"
 
 namespace q8mi {
@@ -902,22 +904,33 @@ Plan plan_of(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_
 // four waves would mostly meet (128 x 32 rows: 9.2 -> 5.2 us; below, 24 rows of 128 pieces: 5.4 and not 9.8 us).
 constexpr uint32_t kManyJoined = 1024;
 
+// More LDS than the default grant is asked for once per head_dim, cache type and device, for every arrangement of waves: which of
+// them a call takes depends on all its sizes, and a later one may be under capture.
+template <uint32_t D, int KV, uint32_t WR>
+bool grant() {
+    constexpr uint32_t kBytes = Layout<D, KV, WR>::kBytes;
+    return kBytes <= 64 * 1024 || hipFuncSetAttribute(reinterpret_cast<const void *>(attention_kernel<D, KV, WR>),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kBytes) == hipSuccess;
+}
+template <uint32_t D, int KV>
+int grant_lds() {
+    static std::atomic<uint64_t> granted{0};   // a bit a device; two threads may both get here first: the grant is idempotent
+    int dev = 0;
+    if (const hipError_t e = hipGetDevice(&dev); e != hipSuccess) return fail(Q8MI_LAUNCH_ERROR, "paged_attention: %s", hipGetErrorString(e));
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;   // devices beyond are asked for every time
+    if (granted & bit) return Q8MI_OK;
+    if (!grant<D, KV, 1>() || !grant<D, KV, 2>() || !grant<D, KV, 4>()) {
+        (void)hipGetLastError();
+        return fail(Q8MI_LAUNCH_ERROR, "paged_attention: cannot reserve LDS");
+    }
+    granted |= bit;
+    return Q8MI_OK;
+}
+
 template <uint32_t D, int KV, uint32_t WR>
 int launch_waves(AttnParams &p, hipStream_t s) {
     using L = Layout<D, KV, WR>;
     p.whole_loads = p.cache.page_size % L::kRowsPerLoad == 0 && static_cast<uint64_t>(L::kRowsPerLoad) * p.unit_token < 1u << 28;
-    if (L::kBytes > 64 * 1024) {
-        // more than the default grant: asked for once per instantiation and device
-        static thread_local int granted = -1;
-        int dev = 0;
-        if (hipGetDevice(&dev) != hipSuccess) return check_launch("paged_attention");
-        if (dev != granted) {
-            if (hipFuncSetAttribute(reinterpret_cast<const void *>(attention_kernel<D, KV, WR>),
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != hipSuccess)
-                return check_launch("paged_attention");
-            granted = dev;
-        }
-    }
     p.waves_log2 = WR == 1 ? 0 : WR == 2 ? 1 : 2;
     const uint32_t resident = kChipCus * L::kResident;
     if (p.groups > resident) p.groups = resident;
@@ -932,6 +945,7 @@ int launch_waves(AttnParams &p, hipStream_t s) {
 }
 template <uint32_t D, int KV>
 int launch_dim(AttnParams &p, uint32_t waves_on_rows, hipStream_t s) {
+    if (const int rc = grant_lds<D, KV>(); rc != Q8MI_OK) return rc;
     if (waves_on_rows == 1) return launch_waves<D, KV, 1>(p, s);
     if (waves_on_rows == 2) return launch_waves<D, KV, 2>(p, s);
     return launch_waves<D, KV, 4>(p, s);
