@@ -17,7 +17,7 @@
 //            same row as its weights: rescaling by a new maximum is one factor per lane.
 // Precision: cache elements are exact operands (bf16, or fp16 for fp16 and e4m3).  The fp32 side, q and the weights, is
 // split into operands that add up to it: three bf16 terms (all 24 bits), or two fp16 terms (22 bits) after scaling by a
-// power of two that keeps the second term clear of fp16's subnormals (of weights from 2^-17 of the largest on; smaller ones are
+// power of two that keeps the second term clear of fp16's subnormals (of those from 2^-17 of the row's largest on; smaller ones are
 // off by up to 2^-39 of it).  Sums are fp32 throughout.
 // Bound by HBM where a key head has few query rows (128 x 4096 tokens of fp16, 8 heads of 128: 2.1 GB in 324 us, 6.6 TB/s; one
 // sequence of 131072 tokens of bf16, 4 heads of 256: 537 MB in 92 us), by the matrix cores and VALUs in turn where it has many
@@ -478,7 +478,7 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
         for (int i = 0; i < 8; ++i)
             qv[j][i] = as_f32(!p.q_is_bf16 ? ws[i] : i % 2 ? ws[i / 2] & static_cast<int>(0xffff0000u) : ws[i / 2] << 16);
     }
-    float row_scale = 1.0f;   // fp16 operands: the row's largest |q| goes to 2^13 .. 2^14
+    int row_shift = 0;   // fp16 operands: the row's largest |q| goes to 2^14 .. 2^15, so that the second term's last step is 2^-38 of it
     if constexpr (KV != Q8MI_KV_BF16) {
         float top = 0.0f;
 #pragma unroll
@@ -486,24 +486,21 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(qv[j][i]));
         top = rows_max(top);
-        int e = 0;
         if (top > 0.0f && top < INFINITY) {
-            (void)frexpf(top, &e);
-            e = 14 - e;
-            e = e > 100 ? 100 : e;
+            (void)frexpf(top, &row_shift);
+            row_shift = 15 - row_shift;   // up to 163: applied by ldexp, since as a factor it would leave fp32
         }
-        row_scale = ldexpf(1.0f, e);
     }
     v8s qf[kSteps][Op::kTerms];
 #pragma unroll
     for (uint32_t j = 0; j < kSteps; ++j) {
         if constexpr (KV != Q8MI_KV_BF16) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) qv[j][i] *= row_scale;
+            for (int i = 0; i < 8; ++i) qv[j][i] = ldexpf(qv[j][i], row_shift);
         }
         Op::split(qv[j], qf[j]);
     }
-    const float to_log2 = p.scale_log2 / row_scale;
+    const float to_log2 = KV == Q8MI_KV_BF16 ? p.scale_log2 : ldexpf(p.scale_log2, -row_shift);
 
     auto turn = [&]() {   // to the other stage
         k_tile ^= 2 * L::kTileBytes; v_tile ^= 2 * L::kTileBytes;
