@@ -772,13 +772,15 @@ __global__ __launch_bounds__(kAttnThreads, (Layout<D, KV, WR>::kResident)) void 
     }
     constexpr uint32_t kOwn = kOuts / L::kGroups;
     const uint32_t d0 = wg * kOwn;
+    const float v_scale = KV == Q8MI_KV_E4M3 ? p.cache.v_scale : 1.0f;
     if (live && whole_item) {
-        const float norm = l > 0.0f || l != l ? (KV == Q8MI_KV_E4M3 ? p.cache.v_scale : 1.0f) / Op::kWeightScale / l : 0.0f;
+        // the cache's scale comes last: it may be so small that its quotient by the sum would be a subnormal
+        const float norm = l > 0.0f || l != l ? 1.0f / Op::kWeightScale / l : 0.0f;
         const uint64_t at = static_cast<uint64_t>(q_row) * p.stride_out + head * D + g * 4;
 #pragma unroll
         for (uint32_t u = 0; u < kOwn; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) store_out(p, at + (d0 + u) * 16 + i, norm == 0.0f ? 0.0f : o[u][i] * norm);
+            for (int i = 0; i < 4; ++i) store_out(p, at + (d0 + u) * 16 + i, norm == 0.0f ? 0.0f : o[u][i] * norm * v_scale);
     } else if (live) {
         const uint64_t at = static_cast<uint64_t>(slot_of_piece) * (WR * kRowTile) + wr * kRowTile + lane % 16;
 #pragma unroll
@@ -859,10 +861,11 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Attn
             out += f * parts[i][d];
         }
     }
-    const float norm = (KV == Q8MI_KV_E4M3 ? p.cache.v_scale : 1.0f) / Operand<KV>::kWeightScale;
+    constexpr float kNorm = 1.0f / Operand<KV>::kWeightScale;
+    const float v_scale = KV == Q8MI_KV_E4M3 ? p.cache.v_scale : 1.0f;   // last, as above
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        store_out(p, static_cast<uint64_t>(q_row) * p.stride_out + head * D + d * 4 + i, sum == 0.0f ? 0.0f : out[i] / sum * norm);
+        store_out(p, static_cast<uint64_t>(q_row) * p.stride_out + head * D + d * 4 + i, sum == 0.0f ? 0.0f : out[i] / sum * kNorm * v_scale);
 }
 
 constexpr uint32_t kChipCus = 256;

@@ -62,3 +62,22 @@ def test_subnormal_queries(gpu, kind, k, exponent):
     p = attend(pools, q, 2, scale)[0, 0].astype(np.float64)
     want = 1 / (1 + np.exp(-score))
     assert np.abs(p - want).max() <= (8 * score + 16) * R.U
+
+
+@pytest.mark.parametrize("v_scale", [1.3 * 2.0 ** -124, 1.3 * 2.0 ** -100, 1.3 * 2.0 ** 120])
+@pytest.mark.parametrize("n", [1, 50, 3000])
+def test_value_scales_near_the_ends(gpu, n, v_scale):
+    """Zero queries weigh all tokens alike; the mean is good to fp32's roundings of the sum, however small the scale (outputs that
+    are subnormal: to half their step)."""
+    rng = np.random.default_rng(n)
+    v_scale = float(np.float32(v_scale))
+    pages = (n + 15) // 16
+    pools = R.Pools("e4m3", pages, 16, 2, 64, v_scale=v_scale, fill=0)
+    v = np.zeros((n, 2, 64))
+    for t in range(n):
+        bits = R.e4m3_bits(4 * rng.standard_normal((2, 64)))
+        pools.put("v", t // 16, t % 16, bits)
+        v[t] = R.E4M3[bits] * v_scale
+    got = attend(pools, np.zeros((1, 4, 64)), n, 1.0)[0].astype(np.float64)
+    want, mag = v.mean(0).repeat(2, 0), np.abs(v).mean(0).repeat(2, 0)
+    assert (np.abs(got - want) <= (6 * n ** 0.5 + 16) * R.U * mag + 2.0 ** -150).all()
