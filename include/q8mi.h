@@ -311,8 +311,9 @@ typedef struct q8mi_kv_cache {
  * Activations (q, k, v, q_out) are fp32, or bf16 when is_bf16 != 0.  Head h of token j of q begins at
  * j*stride_q_row + h*stride_q_head (queries may lie between other things, e.g. their gates); heads of k, v and
  * q_out follow one another, rows stride_k_row, stride_v_row and stride_q_out_row elements apart.  q_out may be
- * q when the strides agree (stride_q_head == head_dim), and must not overlap it otherwise.  All array
- * arguments are device memory; any alignment, 16-byte aligned rows take vector accesses. */
+ * q when the strides agree (stride_q_head == head_dim); any other overlap of q_out with q, k or v is
+ * Q8MI_REJECTED (rows side by side in one buffer are none).  All array arguments are device memory; any
+ * alignment, 16-byte aligned rows take vector accesses. */
 int q8mi_qk_norm_rope_append(const void *q, const void *k, const void *v, void *q_out, int is_bf16, uint32_t tokens,
                              uint32_t q_heads, uint32_t stride_q_row, uint32_t stride_q_head, uint32_t stride_k_row,
                              uint32_t stride_v_row, uint32_t stride_q_out_row, const float *q_norm_weight,
@@ -337,13 +338,14 @@ int q8mi_qk_norm_rope_append(const void *q, const void *k, const void *v, void *
  * the host gives their bounds: n_seqs, q_rows (rows of q and out), max_q_len (1..16) and max_kv_len (at most
  * stride_page_table * page_size).  Tokens from max_kv_len on are not read, rows of a sequence from
  * max_q_len on and rows from q_rows on not computed, and a page id outside the pool hides its tokens.  A row
- * of q must not belong to two sequences, and out must not overlap q.  The first call of a head_dim and cache
- * type on a device asks the runtime for LDS, for calls of all sizes: make it outside a graph capture.
- * scratch: q8mi_paged_attention_scratch_bytes() device bytes, 16-byte aligned, which are enough for every call of the
- * same q_heads, kv_heads and head_dim whose n_seqs, max_q_len and max_kv_len are no larger; calls that may overlap need
- * one each.  Nothing in it needs clearing.  Results repeat bit by bit.  Q8MI_REJECTED: q_heads not a multiple of
- * kv_heads or above 65535, the bounds above, out the same as q, q, out or their strides in bytes not multiples
- * of 16, a scale that is not finite or beyond 2^127, a pool of 64 GiB and more, 2^22 rows and more. */
+ * of q must not belong to two sequences.  The first call of a head_dim and cache type on a device asks the
+ * runtime for LDS, for calls of all sizes: make it outside a graph capture.
+ * scratch: q8mi_paged_attention_scratch_bytes() device bytes, 16-byte aligned, which are enough for every call
+ * of the same q_heads, kv_heads and head_dim whose n_seqs, max_q_len and max_kv_len are no larger; calls that
+ * may overlap need one each.  Nothing in it needs clearing.  Results repeat bit by bit.
+ * Q8MI_REJECTED: q_heads not a multiple of kv_heads or above 65535, the bounds above, out overlapping q (rows
+ * side by side in one buffer do not), q, out or their strides in bytes not multiples of 16, a scale that is not
+ * finite or beyond 2^127, a pool of 64 GiB and more, 2^22 rows and more. */
 size_t q8mi_paged_attention_scratch_bytes(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads,
                                           uint32_t head_dim, uint32_t max_kv_len);
 int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_rows, uint32_t stride_q_row,

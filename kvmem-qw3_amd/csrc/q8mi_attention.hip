@@ -1008,6 +1008,9 @@ extern "C" int q8mi_paged_attention(const void *q, int q_is_bf16, uint32_t q_row
         stride_q_row * q_es % 16 != 0 || stride_out_row * o_es % 16 != 0)
         return fail(Q8MI_REJECTED, "%s: rows of q and out must begin on 16-byte boundaries", what);
     if (q_rows > 1 && (stride_q_row < width || stride_out_row < width)) return fail(Q8MI_REJECTED, "%s: rows overlap", what);
+    if (rows_meet({reinterpret_cast<uintptr_t>(q), q_rows, stride_q_row * q_es, width * q_es},
+                  {reinterpret_cast<uintptr_t>(out), q_rows, stride_out_row * o_es, width * o_es}))
+        return fail(Q8MI_REJECTED, "%s: out overlaps q", what);
 
     uint64_t units = 0;
     const Plan plan = plan_of(n_seqs, max_q_len, q_heads, cache->kv_heads, cache->head_dim, max_kv_len, &units);

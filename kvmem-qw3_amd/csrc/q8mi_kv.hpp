@@ -32,6 +32,28 @@ inline int check_kv_cache(const char *what, const q8mi_kv_cache *c) {
     return Q8MI_OK;
 }
 
+// Rows of activations in memory, in bytes: `count` rows of `width`, `stride` apart (no less than width where there are several).
+struct RowSet {
+    uintptr_t base;
+    uint64_t count, stride, width;
+    uintptr_t end() const { return base + (count - 1) * stride + width; }
+};
+// Whether two sets of rows share a byte.  Sets that lie side by side in one buffer (one row's queries beside its outputs) do not.
+inline bool rows_meet(const RowSet &a, const RowSet &b) {
+    if (a.end() <= b.base || b.end() <= a.base) return false;
+    if (a.count > 1 && a.stride == b.stride) {   // one answer for all rows: where b's row lies behind the a row before it
+        const uint64_t s = a.stride;
+        const uint64_t behind = b.base >= a.base ? (b.base - a.base) % s : (s - (a.base - b.base) % s) % s;
+        return behind < a.width || behind + b.width > s;
+    }
+    for (uint64_t i = 0; i < a.count; ++i) {
+        const uintptr_t lo = a.base + i * a.stride, hi = lo + a.width;
+        const uint64_t k = lo < b.base + b.width ? 0 : (lo - b.base - b.width) / b.stride + 1;   // the first of b's that ends behind lo
+        if (k < b.count && b.base + k * b.stride < hi) return true;
+    }
+    return false;
+}
+
 // Two floats as bf16, nearest even (v_cvt_pk_bf16_f32), the first in the lower half.
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     typedef __bf16 v2bf __attribute__((ext_vector_type(2)));

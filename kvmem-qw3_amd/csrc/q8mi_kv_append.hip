@@ -257,6 +257,19 @@ extern "C" int q8mi_qk_norm_rope_append(const void *q, const void *k, const void
         return fail(Q8MI_REJECTED, "%s: rows overlap", what);
     if (q_out == q && (stride_q_head != D || (tokens > 1 && stride_q_row != stride_q_out_row)))
         return fail(Q8MI_REJECTED, "%s: in place needs dense heads and one row stride", what);
+    {
+        const uint64_t es = is_bf16 ? 2 : 4;
+        auto rows_at = [&](const void *base, uint64_t first, uint64_t stride, uint64_t width) {
+            return RowSet{reinterpret_cast<uintptr_t>(base) + first * es, tokens, stride * es, width * es};
+        };
+        const RowSet to = rows_at(q_out, 0, stride_q_out_row, q_heads * D);
+        if (rows_meet(rows_at(k, 0, stride_k_row, cache->kv_heads * D), to) || rows_meet(rows_at(v, 0, stride_v_row, cache->kv_heads * D), to))
+            return fail(Q8MI_REJECTED, "%s: q_out overlaps k or v", what);
+        if (q_out != q && rows_meet(rows_at(q, 0, stride_q_row, (q_heads - 1) * static_cast<uint64_t>(stride_q_head) + D), to))
+            for (uint32_t h = 0; h < q_heads; ++h)   // it may still lie in what is between the heads
+                if (rows_meet(rows_at(q, static_cast<uint64_t>(h) * stride_q_head, stride_q_row, D), to))
+                    return fail(Q8MI_REJECTED, "%s: q_out overlaps q", what);
+    }
 
     AppendParams p{};
     p.q = q; p.k = k; p.v = v; p.q_out = q_out;
