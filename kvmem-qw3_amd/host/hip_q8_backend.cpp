@@ -61,6 +61,9 @@ struct HipWeight final : DeviceWeight {
     uint8_t *ptr = nullptr;
     uint64_t bytes = 0;
     OwnerRef owner;
+    // rope_frequencies calls itself F32, too: its elements have 8 bytes
+    bool is_f32() const { return format == DeviceWeightFormat::F32 && bytes == rows * cols * 4; }
+    bool is_f64() const { return format == DeviceWeightFormat::F32 && bytes == rows * cols * 8; }
     ~HipWeight() override {
         tell_owner(owner, ptr);
         if (ptr) (void)hipFree(ptr);
@@ -209,7 +212,7 @@ std::unique_ptr<DeviceWeight> HipQ8Backend::rope_frequencies(const double *radia
     w->owner = owner_;
     w->rows = 1;
     w->cols = count;
-    w->format = DeviceWeightFormat::F32;   // the nearest name: `bytes` tells 64-bit elements apart
+    w->format = DeviceWeightFormat::F32;   // the nearest name: is_f32 and is_f64 tell by `bytes`
     w->bytes = count * 8;
     if (hipMalloc(reinterpret_cast<void **>(&w->ptr), w->bytes ? w->bytes : 1) != hipSuccess ||
         hipMemcpy(w->ptr, radians, w->bytes, hipMemcpyHostToDevice) != hipSuccess) {
@@ -685,7 +688,7 @@ DeviceStatus HipQ8Backend::rms_norm_batch(DeviceTensor &out, const DeviceTensor 
     const auto &w = W(weight);
     if (T(out).is_bf16()) return {false, "hip rms_norm_batch BF16 output is not implemented"};
     if (T(x).is_bf16()) return {false, "hip rms_norm_batch BF16 input is outside the Q8_0 path"};
-    if (w.format != DeviceWeightFormat::F32 || w.cols < n) return {false, "rms_norm_batch: norm weight is not fp32 [n]"};
+    if (!w.is_f32() || w.cols < n) return {false, "rms_norm_batch: norm weight is not fp32 [n]"};
     if (T(x).count < static_cast<uint64_t>(batch) * n || T(out).count < static_cast<uint64_t>(batch) * n)
         return {false, "rms_norm_batch: tensor smaller than batch * n"};
     const float *xin = T(x).f32();
@@ -748,7 +751,7 @@ DeviceStatus HipQ8Backend::rms_norm_q8_0_matmul_fanout(DeviceTensor &normalized,
     const auto &nw = W(norm_weight);
     const uint32_t cols = in_stride;
     bool fast = batch <= 8 && cols % 32 == 0 && !T(x).is_bf16() && !T(normalized).is_bf16() &&
-                nw.format == DeviceWeightFormat::F32 && nw.cols == cols &&
+                nw.is_f32() && nw.cols == cols &&
                 T(x).count >= static_cast<uint64_t>(batch) * cols &&
                 T(normalized).count >= static_cast<uint64_t>(batch) * cols;
     for (uint32_t i = 0; i < fanout && fast; ++i) {
@@ -1137,9 +1140,9 @@ DeviceStatus HipQ8Backend::qk_norm_rope_append(DeviceTensor &q_out, const Device
         !fits(q_out, tokens, stride_q_out_row, q_heads * dim))
         return {false, "qk_norm_rope_append: rows outside their tensors"};
     for (const DeviceWeight *w : {q_norm, k_norm})
-        if (w && (w->format != DeviceWeightFormat::F32 || w->cols < dim || W(*w).bytes != w->cols * 4))
+        if (w && (!W(*w).is_f32() || w->cols < dim))
             return {false, "qk_norm_rope_append: a norm weight needs head_dim fp32 elements"};
-    if (rotary_dim != 0 && (!freqs || W(*freqs).bytes < rotary_dim / 2 * 8ull || W(*freqs).bytes != freqs->cols * 8))
+    if (rotary_dim != 0 && (!freqs || !W(*freqs).is_f64() || freqs->cols < rotary_dim / 2))
         return {false, "qk_norm_rope_append: too few frequencies"};
     if (!is_i32(positions) || positions.count < tokens || slots.elem_size != 8 || slots.count < tokens)
         return {false, "qk_norm_rope_append: positions (32 bits) and slots (64 bits) of every token"};
