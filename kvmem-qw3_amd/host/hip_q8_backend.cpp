@@ -30,6 +30,7 @@
 //     of its sum when that is the next call (PendingAdd).  Same bits either way.
 #include "hip_q8_backend.hpp"
 
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 
@@ -228,12 +229,16 @@ std::unique_ptr<DeviceKvCache> HipQ8Backend::kv_cache(DeviceTensorDType dtype, u
     if (capturing_) return nullptr;
     const bool fp8 = dtype == DeviceTensorDType::FP8_E4M3;
     if (!fp8 && dtype != DeviceTensorDType::F16 && dtype != DeviceTensorDType::BF16) return nullptr;
-    if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || pages == 0 || page_size == 0 || kv_heads == 0) return nullptr;
+    if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || pages == 0 || pages > 0x7fffffffu || page_size == 0 ||
+        page_size > 65536 || kv_heads == 0 || kv_heads > 65536)
+        return nullptr;   // what every operator on it would refuse
+    if (fp8 && !(std::isfinite(k_scale) && std::isfinite(v_scale) && k_scale > 0.0f && v_scale > 0.0f)) return nullptr;
     auto c = std::make_unique<HipKvCache>();
     c->dtype = dtype;
     c->pages = pages; c->page_size = page_size; c->kv_heads = kv_heads; c->head_dim = head_dim;
     c->k_scale = k_scale; c->v_scale = v_scale;
-    const uint64_t bytes = static_cast<uint64_t>(pages) * page_size * kv_heads * head_dim * (fp8 ? 1 : 2);
+    uint64_t bytes = 0;   // the first factor is below 2^56
+    if (__builtin_mul_overflow(static_cast<uint64_t>(pages) * page_size * head_dim * (fp8 ? 1 : 2), kv_heads, &bytes)) return nullptr;
     for (void **pool : {&c->k, &c->v})
         if (hipMalloc(pool, bytes) != hipSuccess || hipMemsetAsync(*pool, 0, bytes, stream_) != hipSuccess) {
             (void)hipGetLastError();

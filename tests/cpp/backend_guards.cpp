@@ -1,5 +1,6 @@
 // What HipQ8Backend answers to handles of the wrong kind and to caches that no operator would take.
 //   frequencies  64-bit rotation frequencies are no norm weight, and 32-bit ones no frequencies
+//   caches       what the cache operators would refuse is not made, nor a pool whose size leaves 64 bits
 // Prints one line per case; exit code 0 only if all pass.
 #include <cmath>
 #include <cstdint>
@@ -43,12 +44,30 @@ void frequencies(qw3::HipQ8Backend &b) {
     report("frequencies", ok);
 }
 
+void caches(qw3::HipQ8Backend &b) {
+    using D = qw3::DeviceTensorDType;
+    auto made = [&](D t, uint32_t pages, uint32_t page_size, uint32_t heads, uint32_t dim, float ks = 1.0f, float vs = 1.0f) {
+        return b.kv_cache(t, pages, page_size, heads, dim, ks, vs, "kv") != nullptr;
+    };
+    const float nan = std::nanf(""), inf = INFINITY;
+    bool ok = made(D::BF16, 1, 65536, 1, 64) && !made(D::BF16, 1, 65537, 1, 64) && !made(D::BF16, 0, 16, 1, 64) && !made(D::BF16, 1, 0, 1, 64) &&
+              !made(D::BF16, 1, 16, 0, 64);
+    for (float bad : {0.0f, -1.0f, nan, inf})
+        ok = ok && !made(D::FP8_E4M3, 2, 16, 1, 64, bad, 1.0f) && !made(D::FP8_E4M3, 2, 16, 1, 64, 1.0f, bad) && made(D::F16, 2, 16, 1, 64, bad, bad);
+    ok = ok && made(D::FP8_E4M3, 2, 16, 1, 64, 1e-30f, 1e30f);
+    // 2^64 bytes and a little more: their low bits alone are a pool of moderate size
+    ok = ok && !made(D::F16, 1u << 30, 65536, 1u << 9, 256) && !made(D::FP8_E4M3, 1u << 31, 65536, 1u << 9, 256) &&
+         !made(D::F16, 1u << 30, 65536, (1u << 9) + (1u << 11), 256) && !made(D::BF16, 0x80000001u, 65536, 1u << 16, 64);
+    report("caches", ok && b.synchronize().ok);
+}
+
 }  // namespace
 
 int main() {
     {
         qw3::HipQ8Backend b;
         frequencies(b);
+        caches(b);
     }
     std::printf("%d failed\n", g_failed);
     std::fflush(stdout);
