@@ -331,8 +331,9 @@ int q8mi_qk_norm_rope_append(const void *q, const void *k, const void *v, void *
  * for every query head h with the keys and values of head h / (q_heads / kv_heads).  What a row does not see
  * has no influence on it, whatever it holds (an infinity or NaN that it sees does, also where its weight is 0);
  * a row that sees nothing is zero; rows of q outside every sequence leave out as it was.
- * Sums are fp32; q and p are held to 22 bits or more, with fp16 and e4m3 caches no finer than 2^-39 of their
- * row's largest.
+ * Sums are fp32, and the outputs' are divided by the weights' sum (1 to the number of tokens) at the end, so that
+ * bf16 values beyond 2^127 / tokens may overflow; q and p are held to 22 bits or more, with fp16 and e4m3 caches
+ * no finer than 2^-39 of their row's largest.
  * q and out: rows stride_q_row / stride_out_row elements apart, heads dense; fp32, or bf16 per *_is_bf16.
  * kv_lens, q_starts and page_table are device memory and may change between replays of a captured call;
  * the host gives their bounds: n_seqs, q_rows (rows of q and out), max_q_len (1..16) and max_kv_len (at most

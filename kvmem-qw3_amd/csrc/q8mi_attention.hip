@@ -21,7 +21,8 @@
 // off by up to 2^-39 of it).  Sums are fp32 throughout.
 // Bound by HBM where a key head has few query rows (128 x 4096 tokens of fp16, 8 heads of 128: 2.1 GB in 324 us, 6.6 TB/s; one
 // sequence of 131072 tokens of bf16, 4 heads of 256: 537 MB in 92 us), by the matrix cores and VALUs in turn where it has many
-// (48 rows, 298 MB: 74 us), by latency where there is little to read (2000 tokens: 14 us for the two launches).
+// (48 rows, 298 MB: 71 us; the call's largest number of rows arranges the waves of all its sequences, and waves that a sequence has
+// no rows for only load), by latency where there is little to read (2000 tokens: 14 us for the two launches).
 #include <atomic>
 
 #include "q8mi_kv.hpp"

@@ -16,8 +16,8 @@
 //   4  one workgroup a row ranks the collected logits, takes the cuts in them, finds the chunk that holds the drawn element
 //      and walks it
 // Bound by the launches' latency for one row (248320 logits, top_k 20 and top_p: 2.8 + 5.2 + 2.1 + 6.8 us; top_p alone 23 us in
-// all), for many by the 64-bit weights and the histograms (64 rows: 27 us by top_k 40 of 151936, 33 us by temperature alone, 74 us by
-// top_p of 248320; reading those once takes 11).
+// all, at temperature 1), for many by the 64-bit weights and the histograms (64 rows: 26 us by top_k 40 of 151936, 33 us by
+// temperature alone, 71 us by top_p of 248320 at temperature 1; reading those once takes 11).
 // A row with more than 4096 logits to collect (thousands of equal ones, a temperature that levels all) is searched by the
 // fourth launch's workgroup alone, digit by digit of the ranks.
 #include "q8mi_device.hpp"
