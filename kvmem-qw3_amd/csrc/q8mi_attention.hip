@@ -961,7 +961,7 @@ int launch_type(AttnParams &p, uint32_t waves_on_rows, hipStream_t s) {
 uint64_t partial_rows(const Plan &plan) { return 2ull * plan.groups * plan.waves_on_rows * kRowTile; }
 
 // No call of these heads with no more sequences, rows and tokens takes more partial rows.  A smaller call may take more than the
-// largest one does: below kFewUnits a workgroup's tile has four waves of rows, and a wave for each of them costs as many workgroups.
+// largest one does: up to kFewUnits a workgroup's tile has the rows of four waves, above it, with as few query rows, those of one.
 // So every arrangement that a smaller call can get counts, with the most units that it can have.
 uint64_t most_partial_rows(uint32_t n_seqs, uint32_t max_q_len, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_kv_len) {
     const uint64_t rows = static_cast<uint64_t>(max_q_len) * (kv_heads ? q_heads / kv_heads : 0);

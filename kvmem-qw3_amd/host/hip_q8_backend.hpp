@@ -119,8 +119,8 @@ public:
     std::unique_ptr<DeviceTensor> tensor_i64(uint64_t count, const char *label);
     // rotation frequencies in radians per position, one per pair: rows = 1, cols = count, 64-bit
     std::unique_ptr<DeviceWeight> rope_frequencies(const double *radians, uint64_t count, const char *label);
-    // a cache of pages x page_size tokens, zeroed; null when the operators below would refuse it (type, head_dim, a page_size or
-    // kv_heads above 65536, FP8 scales that are not finite and above zero) or memory is short
+    // a cache of pages x page_size tokens, zeroed; null when the operators below would refuse it (type, head_dim, 2^31 pages, a page_size
+    // or kv_heads above 65536, FP8 scales that are not finite and above zero) or memory is short
     std::unique_ptr<DeviceKvCache> kv_cache(DeviceTensorDType dtype, uint32_t pages, uint32_t page_size, uint32_t kv_heads,
                                             uint32_t head_dim, float k_scale, float v_scale, const char *label);
     // fp32 vector (norm weights): rows = 1, cols = count (src/kernels_cuda.cu: weight_f32)

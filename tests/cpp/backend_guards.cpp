@@ -1,6 +1,9 @@
-// What HipQ8Backend answers to handles of the wrong kind and to caches that no operator would take.
+// What HipQ8Backend answers to handles of the wrong kind and to caches that no operator would take, and what one eager call with a
+// program's largest bounds prepares.
 //   frequencies  64-bit rotation frequencies are no norm weight, and 32-bit ones no frequencies
 //   caches       what the cache operators would refuse is not made, nor a pool whose size leaves 64 bits
+//   captured     after the largest attention and sampling have run once, smaller ones are captured without growing a scratch, and
+//                replays give the eager calls' bits
 // Prints one line per case; exit code 0 only if all pass.
 #include <cmath>
 #include <cstdint>
@@ -61,6 +64,74 @@ void caches(qw3::HipQ8Backend &b) {
     report("caches", ok && b.synchronize().ok);
 }
 
+void captured(qw3::HipQ8Backend &b) {
+    constexpr uint32_t heads = 24, kv_heads = 4, dim = 256, seqs = 3, wide = 1250, page = 16, width = heads * dim, rows = 32, vocab = 32000;
+    auto cache = b.kv_cache(qw3::DeviceTensorDType::F16, 4, page, kv_heads, dim, 1.0f, 1.0f, "kv");
+    auto q = b.tensor_f32(seqs * width, "q"), out = b.tensor_f32(seqs * width, "out"), logits = b.tensor_f32(rows * vocab, "logits"),
+         u = b.tensor_f32(rows, "u"), top_p = b.tensor_f32(rows, "top_p"), k = b.tensor_f32(40 * kv_heads * dim, "k"),
+         v = b.tensor_f32(40 * kv_heads * dim, "v"), unused = b.tensor_f32(40 * width, "q_out"), queries = b.tensor_f32(40 * width, "queries");
+    auto table = b.tensor_i32(seqs * wide, "table"), lens = b.tensor_i32(seqs, "lens"), positions = b.tensor_i32(40, "positions");
+    auto slots = b.tensor_i64(40, "slots");
+    auto tokens = b.argmax_buffer(rows);
+    bool ok = true;
+    auto put = [&](qw3::DeviceTensor &t, const auto &x) { ok = ok && b.copy_bytes_from_host(t, 0, x.data(), x.size() * sizeof(x[0])).ok; };
+    auto noise = [](size_t n, uint32_t seed) {
+        std::vector<float> x(n);
+        for (auto &f : x) f = static_cast<float>((seed = seed * 1664525u + 1013904223u) >> 8) / 8388608.0f - 1.0f;
+        return x;
+    };
+    std::vector<int32_t> pages(seqs * wide, 0), at(40);
+    std::vector<int64_t> slot(40);
+    for (uint32_t i = 0; i < 40; ++i) { at[i] = static_cast<int32_t>(i); slot[i] = i; }
+    for (uint32_t s = 0; s < seqs; ++s)
+        for (uint32_t i = 0; i < 3; ++i) pages[s * wide + i] = static_cast<int32_t>(i);
+    put(*table, pages); put(*lens, std::vector<int32_t>{40, 17, 33}); put(*positions, at); put(*slots, slot);
+    put(*q, noise(seqs * width, 1)); put(*k, noise(40 * kv_heads * dim, 2)); put(*v, noise(40 * kv_heads * dim, 3));
+    put(*queries, noise(40 * width, 4)); put(*logits, noise(rows * vocab, 5)); put(*u, std::vector<float>(rows, 0.4f));
+    put(*top_p, std::vector<float>(rows, 0.9f));
+    ok = ok && b.qk_norm_rope_append(*unused, *queries, *k, *v, nullptr, nullptr, 1e-6f, nullptr, 0, false, *positions, *slots, 40, heads, width, dim,
+                                     kv_heads * dim, kv_heads * dim, width, *cache).ok;
+    auto attend = [&](uint32_t n, uint32_t max_kv) {
+        const auto st = b.paged_attention(*out, *q, *cache, *table, wide, *lens, nullptr, n, n, 1, heads, max_kv, 0.0625f, width, width);
+        if (!st.ok) std::printf("  attention of %u, %u: %s\n", n, max_kv, st.message);
+        return st.ok;
+    };
+    auto sample = [&](uint32_t n) {
+        const auto st = b.sample_rows(*logits, n, vocab, vocab, nullptr, nullptr, top_p.get(), nullptr, *u, *tokens);
+        if (!st.ok) std::printf("  sampling of %u: %s\n", n, st.message);
+        return st.ok;
+    };
+    auto outputs = [&](uint32_t n) {
+        std::vector<float> x(n * width);
+        ok = ok && b.copy_to_host(*out, x.data(), 0, x.size()).ok;
+        return x;
+    };
+    auto drawn = [&](uint32_t n) {
+        std::vector<qw3::DeviceArgmax> x(n);
+        std::vector<int> t;
+        ok = ok && b.copy_argmax_buffer_to_host(*tokens, x.data(), n).ok;
+        for (auto &a : x) t.push_back(a.token);
+        return t;
+    };
+    ok = ok && attend(seqs, wide * page) && sample(rows);   // the largest, once
+    const uint32_t n_seqs[] = {1, 2, 3, 1, 3}, max_kv[] = {1536, 700, 700, 64, 20000}, batch[] = {31, 16, 1, 20, 32};
+    for (int i = 0; ok && i < 5; ++i) {
+        ok = b.begin_capture();
+        if (!ok) break;
+        const bool served = attend(n_seqs[i], max_kv[i]) && sample(batch[i]);
+        ok = b.end_capture().ok && served;
+        ok = ok && attend(n_seqs[i], max_kv[i]) && sample(batch[i]);
+        const auto want = outputs(n_seqs[i]);
+        const auto want_tokens = drawn(batch[i]);
+        for (int replay = 0; ok && replay < 3; ++replay) {
+            ok = b.zero_tensor(*out).ok && b.replay_graph().ok;
+            ok = ok && outputs(n_seqs[i]) == want && drawn(batch[i]) == want_tokens;
+        }
+        for (float f : want) ok = ok && std::isfinite(f);
+    }
+    report("captured", ok);
+}
+
 }  // namespace
 
 int main() {
@@ -68,6 +139,7 @@ int main() {
         qw3::HipQ8Backend b;
         frequencies(b);
         caches(b);
+        captured(b);
     }
     std::printf("%d failed\n", g_failed);
     std::fflush(stdout);

@@ -1,4 +1,5 @@
-"""Runs tests/cpp/backend_guards.cpp: what the host layer refuses of its own handles."""
+"""Runs tests/cpp/backend_guards.cpp: what the host layer refuses of its own handles, and what one eager call with the
+largest bounds prepares for captured ones."""
 import os
 import subprocess
 
@@ -12,4 +13,4 @@ def test_guards():
     assert os.path.exists(DRIVER), "the driver is not built (run __graft_entry__.build())"
     r = subprocess.run([DRIVER], capture_output=True, text=True, timeout=110)
     assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
-    assert [line for line in r.stdout.splitlines() if line.startswith("PASS")] == ["PASS frequencies", "PASS caches"]
+    assert [line for line in r.stdout.splitlines() if line.startswith("PASS")] == ["PASS frequencies", "PASS caches", "PASS captured"]
